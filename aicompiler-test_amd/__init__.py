@@ -113,6 +113,17 @@ def _declare(l):
                                          vp, vp]),
         "tmc_attention_timeline": (i32, [vp, i64]),
         "tmc_argmax_f32": (i32, [vp, vp, i64, i64, vp]),
+        "tmc_window_attention_workspace_bytes": (sz, [i64, i64, i64, i64, i64, i64, i64]),
+        "tmc_window_decode_attention": (i32, [vp, vp, vp, vp, vp, vp, vp, i32, i64, i64, i64, i64,
+                                              i64, i64, i64, i64, i64, i64, i64, vp, sz, i32, vp]),
+        "tmc_window_prefill_attention_f16": (i32, [vp, vp, vp, vp, vp, vp, i64, vp, vp, i64, i64,
+                                                   i64, i64, i64, i64, i64, i64, i64, i64, i64,
+                                                   vp]),
+        "tmc_move_pages": (i32, [vp, vp, i64, vp, i64, i32, i64, i64, i64, i64, i64, i64, vp]),
+        "tmc_check_page_moves": (i32, [vp, i64, i64, i64, i64]),
+        "tmc_rebuild_tables": (i32, [vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, vp]),
+        "tmc_logprobs_workspace_bytes": (sz, [i64, i64, i64]),
+        "tmc_logprobs": (i32, [vp, i32, i64, vp, vp, vp, vp, vp, i64, i64, i64, vp, sz, vp]),
         "tmc_lm_head_argmax_workspace_bytes": (sz, [i64, i64]),
         "tmc_rmsnorm_lm_head_partial_argmax_f16": (i32, [vp, vp, vp, vp, sz, i64, i64, f, vp, vp]),
         "tmc_lm_head_partial_argmax_packed_norm_f16": (i32, [vp, vp, vp, sz, i64, i64, i64, f, i32,
@@ -753,6 +764,206 @@ def lm_head_argmax_packed_norm(x, packed_scaled, workspace, tokens, batch, in_fe
         layout, _cfg_ref(cfg), _stream(stream)), "tmc_lm_head_partial_argmax_packed_norm_f16")
     check(lib().tmc_lm_head_final_argmax(_ptr(workspace), nbytes, _ptr(tokens), batch,
                                          vocabulary, _stream(stream)), "tmc_lm_head_final_argmax")
+
+
+# ---------------------------------------------------------------- streaming generation
+def _on_gpu(what, stream, *tensors):
+    """Refuse what a kernel on the current GPU could not read: host tensors,
+    tensors of another GPU, a stream of another GPU, gaps between elements."""
+    import torch
+    device = torch.cuda.current_device()
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda or t.device.index != device:
+            raise TmcError(f"{what}: tensors must be on the current GPU (cuda:{device}), "
+                           f"not on {t.device}")
+        if not t.is_contiguous():
+            raise TmcError(f"{what}: tensors must be contiguous")
+    if stream is not None and stream.device.index != device:
+        raise TmcError(f"{what}: the stream belongs to another GPU than the current one")
+
+
+def _typed(what, dtype, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.dtype != dtype:
+            raise TmcError(f"{what}: {name} must be {dtype}, not {t.dtype}")
+
+
+def _room(what, t, count, name):
+    if t.numel() < count:
+        raise TmcError(f"{what}: {name} holds {t.numel()} elements, {count} are needed")
+
+
+def _window_checks(what, q, k_pool, v_pool, valid_lengths, tables, row_table, active, out, rows,
+                   q_heads, kv_heads, head_dim, max_pages, page_stride, stream, pool_pages):
+    import torch
+    _on_gpu(what, stream, q, k_pool, v_pool, valid_lengths, tables, row_table, active, out)
+    _typed(what, torch.float16, q=q, k_pool=k_pool, v_pool=v_pool, out=out)
+    _typed(what, torch.int32, valid_lengths=valid_lengths, tables=tables, row_table=row_table,
+           active=active)
+    if min(rows, q_heads, kv_heads, head_dim, max_pages, page_stride) < 1:
+        raise TmcError(f"{what}: rows, heads, head_dim, pages and strides must be positive")
+    held = min(k_pool.numel(), v_pool.numel()) // page_stride
+    if pool_pages is None:
+        pool_pages = held
+    elif pool_pages > held:
+        raise TmcError(f"{what}: the pools hold {held} pages, not {pool_pages}")
+    _room(what, q, rows * q_heads * head_dim, "q")
+    _room(what, valid_lengths, rows, "valid_lengths")
+    if row_table is not None:
+        _room(what, row_table, rows, "row_table")
+    if active is not None:
+        _room(what, active, 1, "active")
+    return pool_pages
+
+
+def window_attention_workspace_bytes(batch, q_heads, kv_heads, head_dim, capacity, window,
+                                     sinks) -> int:
+    return int(lib().tmc_window_attention_workspace_bytes(batch, q_heads, kv_heads, head_dim,
+                                                          capacity, window, sinks))
+
+
+def window_decode_attention(q, k_pool, v_pool, valid_lengths, tables, active, out, max_batch,
+                            q_heads, kv_heads, head_dim, page_size, max_pages, page_stride,
+                            head_stride, window, sinks, workspace=None, stream=None,
+                            pool_pages=None, layout=0):
+    """Paged decode attention over the last `window` positions and the first
+    `sinks` ones (tmc_window_decode_attention); active may be None.  The
+    workspace must be zero before its first use."""
+    what = "tmc_window_decode_attention"
+    pool_pages = _window_checks(what, q, k_pool, v_pool, valid_lengths, tables, None, active, out,
+                                max_batch, q_heads, kv_heads, head_dim, max_pages, page_stride,
+                                stream, pool_pages)
+    _room(what, tables, max_batch * max_pages, "tables")
+    width = q_heads * head_dim
+    _room(what, out, packed_activation_elements(max_batch, width) if layout == Y_PACKED
+          else max_batch * width, "out")
+    _on_gpu(what, None, workspace)
+    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    check(lib().tmc_window_decode_attention(
+        _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(valid_lengths), _ptr(tables), _ptr(active),
+        _ptr(out), _dtype_code(q), max_batch, q_heads, kv_heads, head_dim, page_size, max_pages,
+        pool_pages, page_stride, head_stride, window, sinks, _ptr(workspace), ws_bytes, layout,
+        _stream(stream)), what)
+
+
+def window_prefill_attention(q, k_pool, v_pool, valid_lengths, tables, row_table, active, out,
+                             rows, q_heads, kv_heads, head_dim, page_size, max_pages, page_stride,
+                             head_stride, window, sinks, stream=None, pool_pages=None):
+    """The chunk form of window_decode_attention: rows of one request
+    (row_table None, one table row) or of several."""
+    what = "tmc_window_prefill_attention_f16"
+    pool_pages = _window_checks(what, q, k_pool, v_pool, valid_lengths, tables, row_table, active,
+                                out, rows, q_heads, kv_heads, head_dim, max_pages, page_stride,
+                                stream, pool_pages)
+    table_rows = 1 if row_table is None else tables.numel() // max_pages
+    _room(what, tables, max_pages, "tables")
+    _room(what, out, rows * q_heads * head_dim, "out")
+    check(lib().tmc_window_prefill_attention_f16(
+        _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(valid_lengths), _ptr(tables), _ptr(row_table),
+        table_rows, _ptr(active), _ptr(out), rows, q_heads, kv_heads, head_dim, page_size,
+        max_pages, pool_pages, page_stride, head_stride, window, sinks, _stream(stream)), what)
+
+
+def page_moves(moves, pools, pool_pages, page_size):
+    """The device array of a list of (pool, source page, destination page,
+    positions) for move_pages, checked (tmc_check_page_moves): existing pages,
+    none written twice, none both read and written."""
+    import torch
+    host_moves = torch.tensor(moves, dtype=torch.int32).reshape(-1, 4).contiguous()
+    check(lib().tmc_check_page_moves(_ptr(host_moves), host_moves.shape[0], pools, pool_pages,
+                                     page_size), "tmc_check_page_moves")
+    return host_moves.cuda()
+
+
+def move_pages(k_pools, v_pools, moves, heads, page_size, head_dim, page_stride=None,
+               head_stride=None, stream=None):
+    """Copy pages inside their pools, one K and one V pool per layer, by the
+    rows (pool, source page, destination page, positions) of `moves` (see
+    page_moves)."""
+    import torch
+    what = "tmc_move_pages"
+    if not k_pools or len(k_pools) != len(v_pools):
+        raise TmcError(f"{what}: as many K pools as V pools, and at least one")
+    _on_gpu(what, stream, *k_pools, *v_pools, moves)
+    _typed(what, torch.int32, moves=moves)
+    _typed(what, k_pools[0].dtype, **{f"pool {i}": t for i, t in enumerate([*k_pools, *v_pools])})
+    if moves.dim() != 2 or moves.shape[1] != 4:
+        raise TmcError(f"{what}: moves must be [count, 4]")
+    head_stride = page_size * head_dim if head_stride is None else head_stride
+    page_stride = heads * head_stride if page_stride is None else page_stride
+    if min(heads, page_size, head_dim, page_stride) < 1:
+        raise TmcError(f"{what}: heads, page_size, head_dim and strides must be positive")
+    if moves.shape[0] == 0:
+        return
+    pool_pages = min(t.numel() for t in [*k_pools, *v_pools]) // page_stride
+    count = len(k_pools)
+    keys = (C.c_void_p * count)(*[t.data_ptr() for t in k_pools])
+    values = (C.c_void_p * count)(*[t.data_ptr() for t in v_pools])
+    check(lib().tmc_move_pages(keys, values, count, _ptr(moves), moves.shape[0],
+                               _dtype_code(k_pools[0]), pool_pages, heads, page_size, head_dim,
+                               page_stride, head_stride, _stream(stream)), what)
+
+
+def rebuild_tables(tables, out, pool_pages, parents=None, remap=None, tail_slots=None, tails=None,
+                   stream=None):
+    """Block tables [layers, rows, max_pages] after a fork (parents, tail_slots
+    and tails [layers, rows]) or a compaction (remap [layers, pool_pages])."""
+    import torch
+    what = "tmc_rebuild_tables"
+    _on_gpu(what, stream, tables, out, parents, remap, tail_slots, tails)
+    _typed(what, torch.int32, tables=tables, out=out, parents=parents, remap=remap,
+           tail_slots=tail_slots, tails=tails)
+    if tables.dim() != 3 or out.dim() != 3 or tables.shape[0] != out.shape[0] or \
+            tables.shape[2] != out.shape[2]:
+        raise TmcError(f"{what}: tables and out must be [layers, rows, max_pages] of the same "
+                       "layers and pages")
+    layers, rows, max_pages = out.shape
+    for name, t, count in (("parents", parents, rows), ("remap", remap, layers * pool_pages),
+                           ("tail_slots", tail_slots, rows), ("tails", tails, layers * rows)):
+        if t is not None:
+            _room(what, t, count, name)
+    check(lib().tmc_rebuild_tables(_ptr(tables), _ptr(parents), _ptr(remap), _ptr(tail_slots),
+                                   _ptr(tails), _ptr(out), layers, tables.shape[1], rows,
+                                   max_pages, pool_pages, _stream(stream)), what)
+
+
+def logprobs_workspace_bytes(rows, vocabulary, top) -> int:
+    return int(lib().tmc_logprobs_workspace_bytes(rows, vocabulary, top))
+
+
+def logprobs(logits, tokens, logprob, entropy=None, top_tokens=None, top_logprobs=None,
+             workspace=None, stream=None):
+    """Log probabilities of `tokens` [rows] in logits [rows, vocabulary] (f32 or
+    f16; rows may be strided), the rows' entropy and the top_tokens.shape[1]
+    most probable tokens.  tokens and logprob may both be None.  The workspace
+    must be zero before its first use."""
+    import torch
+    what = "tmc_logprobs"
+    if logits.dim() != 2 or logits.stride(1) != 1:
+        raise TmcError(f"{what}: logits must be [rows, vocabulary] with adjacent elements")
+    if not logits.is_cuda or logits.device.index != torch.cuda.current_device():
+        raise TmcError(f"{what}: tensors must be on the current GPU, not on {logits.device}")
+    _on_gpu(what, stream, tokens, logprob, entropy, top_tokens, top_logprobs, workspace)
+    _typed(what, torch.int32, tokens=tokens, top_tokens=top_tokens)
+    _typed(what, torch.float32, logprob=logprob, entropy=entropy, top_logprobs=top_logprobs)
+    rows, vocabulary = logits.shape
+    top = 0
+    if top_tokens is not None:
+        if top_logprobs is None or top_tokens.dim() != 2 or top_tokens.shape[0] != rows or \
+                top_logprobs.shape != top_tokens.shape:
+            raise TmcError(f"{what}: top_tokens and top_logprobs must be [rows, top]")
+        top = top_tokens.shape[1]
+    for name, t in (("tokens", tokens), ("logprob", logprob), ("entropy", entropy)):
+        if t is not None:
+            _room(what, t, rows, name)
+    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    check(lib().tmc_logprobs(
+        _ptr(logits), _dtype_code(logits), logits.stride(0) if rows > 1 else vocabulary,
+        _ptr(tokens), _ptr(logprob), _ptr(entropy), _ptr(top_tokens) if top else None,
+        _ptr(top_logprobs) if top else None, rows, vocabulary, top, _ptr(workspace), ws_bytes,
+        _stream(stream)), what)
 
 
 def fill_normal(t, seed, mean=0.0, std=1.0, stream=None):

@@ -794,6 +794,112 @@ void tmc_host_free(void *ptr);
 int tmc_copy_pages(const void *src, void *dst, const int32_t *pages, int64_t count,
                    int64_t page_bytes, int scatter, void *stream);
 
+/* ------------------------------------------------- streaming generation
+ * Attention with a sliding window and sinks over the paged cache, moves of
+ * pages with the block tables that follow them, log probabilities.  No
+ * counterparts in the reference, whose attention sees every cached position,
+ * whose pages belong to one request each and whose sampling is greedy. */
+
+/* Bytes of device workspace tmc_window_decode_attention needs for these
+ * limits (capacity = page_size * max_pages; 0 when none is needed).  The
+ * workspace must be zero before its first use; every launch leaves its
+ * counters at zero, so it serves launches of any shapes, in any order, whose
+ * needs it covers.  Launches that share one workspace must not overlap. */
+size_t tmc_window_attention_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                            int64_t head_dim, int64_t capacity, int64_t window,
+                                            int64_t sinks);
+
+/* tmc_paged_decode_attention_ex with a sliding window and sinks: the token of
+ * request r, at position valid_lengths[r] - 1, attends the last `window`
+ * positions up to its own and the first `sinks` ones.  Pages that hold none of
+ * these are never looked up: their table entries may be -1, their pages given
+ * back.  A window of the capacity attends everything.  head_dim is a multiple
+ * of 8 up to 256 and q_heads any multiple of kv_heads; pool_pages, the pages
+ * each pool holds, must be given; out is 16-byte aligned.  Requests >=
+ * active_count[0] (NULL: all are active), lengths outside [1, page_size * max_pages] and
+ * requests that would see a page outside [0, pool_pages) leave their output
+ * untouched.  A NaN or infinity in the cache outside the visible positions
+ * changes nothing.  Requests may share pages. */
+int tmc_window_decode_attention(const void *q, const void *key_pool, const void *value_pool,
+                                const int32_t *valid_lengths, const int32_t *block_tables,
+                                const int32_t *active_count, void *out, int dtype,
+                                int64_t max_batch, int64_t q_heads, int64_t kv_heads,
+                                int64_t head_dim, int64_t page_size, int64_t max_pages,
+                                int64_t pool_pages, int64_t page_stride, int64_t head_stride,
+                                int64_t window, int64_t sinks, void *workspace,
+                                size_t workspace_bytes, int layout, void *stream);
+
+/* tmc_prefill_attention_rows_f16 with a sliding window and sinks: row r, at
+ * position valid_lengths[r] - 1 of the request of table row row_table[r] (row
+ * 0 when row_table is NULL; table_rows must then be 1), attends what
+ * tmc_window_decode_attention lets its token attend.  Rows of several requests
+ * may follow each other in any order; consecutive rows of one request at
+ * consecutive positions are what it is fast for.  Limits and untouched rows as
+ * there, and rows whose table row is outside [0, table_rows). */
+int tmc_window_prefill_attention_f16(const void *q, const void *key_pool, const void *value_pool,
+                                     const int32_t *valid_lengths, const int32_t *block_tables,
+                                     const int32_t *row_table, int64_t table_rows,
+                                     const int32_t *active_count, void *out, int64_t rows,
+                                     int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                     int64_t page_size, int64_t max_pages, int64_t pool_pages,
+                                     int64_t page_stride, int64_t head_stride, int64_t window,
+                                     int64_t sinks, void *stream);
+
+/* Copies pages inside their pools, K and V of any number of layers in one
+ * call: a fork gives each child a copy of the partly filled last page, a
+ * compaction moves live pages to the front.  key_pools and value_pools are
+ * host arrays of `pools` device pointers [pool_pages][heads][page_size]
+ * [head_dim] at the strides (elements; dtype f16, bf16 or f32); moves is a
+ * 16-byte aligned device array of `count` (pool, source page, destination
+ * page, positions): the first `positions` positions of every head are copied,
+ * bit for bit.  A move that names a pool or page outside its range, positions
+ * outside [1, page_size] or one page twice copies nothing.  All moves take
+ * place at once, in no order: a page that two moves write, or that one reads
+ * and another writes, ends with unspecified contents.  tmc_check_page_moves
+ * refuses such lists. */
+int tmc_move_pages(void *const *key_pools, void *const *value_pools, int64_t pools,
+                   const int32_t *moves, int64_t count, int dtype, int64_t pool_pages,
+                   int64_t heads, int64_t page_size, int64_t head_dim, int64_t page_stride,
+                   int64_t head_stride, void *stream);
+/* Host only: fails, with the reason, unless every move of the host array
+ * names existing pools and pages and 1 to page_size positions, no page is
+ * written twice and none is both read and written. */
+int tmc_check_page_moves(const int32_t *moves, int64_t count, int64_t pools, int64_t pool_pages,
+                         int64_t page_size);
+
+/* Block tables after a fork or a compaction, for all layers in one launch:
+ * entry (l, r, i) of out [layers, rows, max_pages] is entry (l, parents[r], i)
+ * of tables [layers, table_rows, max_pages] (parents NULL: r itself, rows =
+ * table_rows), through remap [layers, pool_pages] where that is given and the
+ * entry lies in [0, pool_pages), except that entry tail_slots[r] of row r is
+ * tails[l, r] where these are given (a slot outside the row: no tail).  A
+ * parent outside [0, table_rows) gives a row of -1.  out may be the tables
+ * themselves when parents is NULL, else it must not overlap them. */
+int tmc_rebuild_tables(const int32_t *tables, const int32_t *parents, const int32_t *remap,
+                       const int32_t *tail_slots, const int32_t *tails, int32_t *out,
+                       int64_t layers, int64_t table_rows, int64_t rows, int64_t max_pages,
+                       int64_t pool_pages, void *stream);
+
+/* Bytes of device workspace tmc_logprobs needs (0 when none is needed; zeroed
+ * and shared by the rules of tmc_window_attention_workspace_bytes). */
+size_t tmc_logprobs_workspace_bytes(int64_t rows, int64_t vocabulary, int64_t top);
+
+/* Log probabilities from logits [rows, vocabulary] (f32 or f16, rows
+ * row_stride elements apart):
+ *   logprob[r] = log softmax(logits[r])[tokens[r]]  (a token outside the
+ *     vocabulary leaves it untouched; tokens and logprob may both be NULL),
+ *   entropy[r] = -sum p log p in nats (may be NULL),
+ *   top_tokens, top_logprobs [rows, top]: the most probable tokens in the
+ *     order of tmc_argmax_f32 (ties to the lower index, NaN never chosen) and
+ *     their log probabilities; -1 and -inf where fewer than top are not NaN.
+ * top is at most 64 and at most the vocabulary; 0 for none.  A logit of -inf
+ * has probability 0 and adds nothing.  In a row that holds a NaN or +inf, or
+ * -inf alone, every log probability and the entropy are NaN. */
+int tmc_logprobs(const void *logits, int dtype, int64_t row_stride, const int32_t *tokens,
+                 float *logprob, float *entropy, int32_t *top_tokens, float *top_logprobs,
+                 int64_t rows, int64_t vocabulary, int64_t top, void *workspace,
+                 size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
