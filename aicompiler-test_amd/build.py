@@ -62,10 +62,10 @@ FLAGS = [
 ]
 
 
-# Per-source additions.  prefill.hip: keep MFMA accumulators in VGPRs (the
+# Per-source additions.  prefill.hip, window.hip: keep MFMA accumulators in VGPRs (the
 # online-softmax rescale multiplies them every block; from AGPRs each one is
 # a read, a multiply and a write back).
-SOURCE_FLAGS = {"prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+SOURCE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for name in ("prefill.hip", "window.hip")}
 
 
 def _compile(src: str, variant: str = "", defines: tuple = ()) -> str:

@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace tmc {
 namespace {
@@ -124,6 +125,460 @@ __global__ __launch_bounds__(kWave) void window_plain_kernel(WindowParams p) {
       p.out[window_out(p, row, head * d + lane + t * kWave)] = (half_t)(o[t] / sum);
 }
 
+// ------------------------------------------------------------ one token a request
+// D = 64 and 128, groups up to 16.  A step is 32 visible positions of one
+// (request, kv head) row.  The steps of all rows form one list, row after row,
+// that the blocks share out evenly whatever the lengths are (each block finds
+// its part from the lengths alone); a row cut by a block border is joined from
+// partials (max, sum, weighted) in the workspace by the last of its blocks to
+// arrive, in block order.
+//
+// Inside a block the waves take the steps of a part in turn.  Each wave has a
+// ring of kStages steps in LDS that only it touches, filled by 16-byte loads
+// straight to LDS: no barrier, no register holds a load in flight, and a
+// stage is reloaded as soon as its operands are in registers.  K and V rows lie
+// in LDS as in their pages, 16-byte chunks (K) and 32-byte units (V) swizzled
+// by the row so that the operand reads spread over the banks.  A position that
+// does not exist reads a zero row.  Scores S^T = K Q^T (16 positions x 16
+// heads) leave lane (head j, group g) with positions 4g .. 4g+3, the order in
+// which O^T = V^T P^T wants its weights; V^T comes from transposing LDS reads.
+constexpr int kStep = 32;
+constexpr int kDecodeWaves = 4;
+constexpr int kDecodeBlocks = 256;  // one a CU
+constexpr int kDecodeMaxRows = 2048;  // rows whose lengths a block scans
+constexpr size_t kWindowCounterBytes = 64u << 10;
+
+struct DecodePlan {
+  float* slots;    // [blocks][2][group][D + 2]
+  int* arrivals;   // [rows][kv_heads]
+  int blocks;      // blocks of the shared list; 0: one block per (row, kv head)
+  int least;       // steps a block takes at least
+};
+
+static __device__ __align__(16) unsigned s_zero_row[4];  // what absent positions read
+
+template <int N> __device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+  return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
+
+// Maximum over lanes l, l + 16, l + 32, l + 48.
+__device__ __forceinline__ float max_of_groups(float v) {
+  const unsigned x = __builtin_bit_cast(unsigned, v);
+  const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  const unsigned a0 = a[0], a1 = a[1];
+  v = fmaxf(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1));
+  const unsigned y = __builtin_bit_cast(unsigned, v);
+  const auto b = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+  const unsigned b0 = b[0], b1 = b[1];
+  return fmaxf(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
+}
+
+// The operands of one step out of LDS, waits included: the compiler would let
+// such reads wait for every load to LDS in flight.
+template <int D, int OFFSET, int PAGE_OFFSET>
+__device__ __forceinline__ void read_keys(const unsigned (&at)[D / 32], unsigned page_at,
+                                          h8 (&k)[2][D / 32], int& page) {
+  if constexpr (D == 128) {
+    asm volatile(
+        "ds_read_b32 %8, %13 offset:%16\n\t"
+        "ds_read_b128 %0, %9 offset:%14\n\tds_read_b128 %1, %10 offset:%14\n\t"
+        "ds_read_b128 %2, %11 offset:%14\n\tds_read_b128 %3, %12 offset:%14\n\t"
+        "ds_read_b128 %4, %9 offset:%15\n\tds_read_b128 %5, %10 offset:%15\n\t"
+        "ds_read_b128 %6, %11 offset:%15\n\tds_read_b128 %7, %12 offset:%15\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(k[0][0]), "=&v"(k[0][1]), "=&v"(k[0][2]), "=&v"(k[0][3]), "=&v"(k[1][0]),
+          "=&v"(k[1][1]), "=&v"(k[1][2]), "=&v"(k[1][3]), "=&v"(page)
+        : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "v"(page_at), "n"(OFFSET),
+          "n"(OFFSET + 32 * D), "n"(PAGE_OFFSET)
+        : "memory");
+  } else {
+    asm volatile(
+        "ds_read_b32 %4, %7 offset:%10\n\t"
+        "ds_read_b128 %0, %5 offset:%8\n\tds_read_b128 %1, %6 offset:%8\n\t"
+        "ds_read_b128 %2, %5 offset:%9\n\tds_read_b128 %3, %6 offset:%9\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(k[0][0]), "=&v"(k[0][1]), "=&v"(k[1][0]), "=&v"(k[1][1]), "=&v"(page)
+        : "v"(at[0]), "v"(at[1]), "v"(page_at), "n"(OFFSET), "n"(OFFSET + 32 * D),
+          "n"(PAGE_OFFSET)
+        : "memory");
+  }
+}
+
+// V^T of dims 16 t + j, t = T .. T + 3: slots 0 .. 3 hold positions 4g .. 4g+3,
+// slots 4 .. 7 positions 16 + 4g ...
+template <int D, int OFFSET>
+__device__ __forceinline__ void read_values(const unsigned* at, h8* v) {
+  h4 a0, a1, a2, a3, b0, b1, b2, b3;
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %9 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %2, %10 offset:%12\n\tds_read_b64_tr_b16 %3, %11 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %4, %8 offset:%13\n\tds_read_b64_tr_b16 %5, %9 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %6, %10 offset:%13\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(a0), "=&v"(a1), "=&v"(a2), "=&v"(a3), "=&v"(b0), "=&v"(b1), "=&v"(b2), "=&v"(b3)
+      : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(OFFSET), "n"(OFFSET + 32 * D)
+      : "memory");
+  v[0] = __builtin_shufflevector(a0, b0, 0, 1, 2, 3, 4, 5, 6, 7);
+  v[1] = __builtin_shufflevector(a1, b1, 0, 1, 2, 3, 4, 5, 6, 7);
+  v[2] = __builtin_shufflevector(a2, b2, 0, 1, 2, 3, 4, 5, 6, 7);
+  v[3] = __builtin_shufflevector(a3, b3, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// Weights are stored 2^kRaiseLog times their value in fp16 (the greatest is
+// 2^kRaiseLog itself): weights down to 2^-29 of the greatest keep their 11
+// bits, and the sum takes the rounded ones, so the factor cancels.
+constexpr float kRaiseLog = 15.0f;
+constexpr unsigned kNoUnit = 0xFFFFFFFFu;
+
+// Visible positions of a row, in steps.
+__device__ __forceinline__ int row_steps(const WindowParams& p, int row, int active) {
+  const int valid = p.valid[row];
+  if (row >= active || valid < 1 || valid > p.page_size * p.max_pages) return 0;
+  const int begin = window_begin(p, valid);
+  return (min(p.sinks, begin) + valid - begin + kStep - 1) / kStep;
+}
+
+template <int D, int STAGES>
+__global__ __launch_bounds__(kDecodeWaves * kWave) void window_decode_kernel(WindowParams p,
+                                                                             DecodePlan plan) {
+  constexpr int KS = D / 32, DT = D / 16, CH = D / 8;
+  constexpr int RPL = kWave / CH, LOADS = kStep / RPL;  // rows a load, loads of K (of V) a step
+  constexpr int STAGE = 2 * kStep * D;                  // halves
+  constexpr int THREADS = kDecodeWaves * kWave;
+  __shared__ __align__(16) half_t s_ring[kDecodeWaves * STAGES * STAGE];
+  __shared__ int s_pages[kDecodeWaves * STAGES * kWave];
+  __shared__ int s_start[kDecodeMaxRows + 1];
+  __shared__ int s_wave[kDecodeWaves];
+  __shared__ int s_last;
+  typedef __attribute__((address_space(3))) void lds_void;
+  typedef __attribute__((address_space(1))) const void global_void;
+  static_assert(sizeof(s_ring) >= kDecodeWaves * 16 * (D + 2) * sizeof(float),
+                "the waves' results fit the ring");
+
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+  const int j = lane & 15, g = lane >> 4;
+  const int active = p.active ? min(p.active[0], p.rows) : p.rows;
+
+  // ---- this block's part [at, stop) of the list
+  int row = 0, at = 0, stop = 0, per = 0, kvh = 0;
+  if (plan.blocks == 0) {
+    row = blockIdx.x / p.kv_heads;
+    kvh = blockIdx.x % p.kv_heads;
+    stop = row_steps(p, row, active);
+  } else {
+    // exclusive sums of the rows' steps
+    const int each = (p.rows + THREADS - 1) / THREADS;
+    const int from = threadIdx.x * each, to = min(p.rows, from + each);
+    int sum = 0;
+    for (int r = from; r < to; ++r) sum += row_steps(p, r, active);
+    int scan = sum;
+#pragma unroll
+    for (int off = 1; off < kWave; off <<= 1) {
+      const int below = __shfl_up(scan, off, kWave);
+      if (lane >= off) scan += below;
+    }
+    if (lane == kWave - 1) s_wave[wave] = scan;
+    __syncthreads();
+    int total = 0, before = 0;
+#pragma unroll
+    for (int w = 0; w < kDecodeWaves; ++w) {
+      if (w < wave) before += s_wave[w];
+      total += s_wave[w];
+    }
+    before += scan - sum;
+    for (int r = from; r < to; ++r) {
+      s_start[r] = before;
+      if (r + 1 < to) before += row_steps(p, r, active);
+    }
+    if (threadIdx.x == 0) s_start[p.rows] = total;
+    __syncthreads();
+    const int steps = total * p.kv_heads;
+    per = max(plan.least, (steps + plan.blocks - 1) / plan.blocks);
+    at = min(steps, (int)blockIdx.x * per);
+    stop = min(steps, at + per);
+    if (at >= stop) return;
+    // the row of the first step: the last one that starts at or before it
+    int low = 0, high = p.rows;
+    while (high - low > 1) {
+      const int mid = (low + high) / 2;
+      if (s_start[mid] * p.kv_heads <= at) low = mid; else high = mid;
+    }
+    row = low;
+  }
+  const int block_at = at;
+
+  // ---- LDS places: loads are linear (lane l: row l / CH, slot l % CH)
+  half_t* ring = s_ring + wave * STAGES * STAGE;
+  unsigned key_at[KS], value_at[DT];
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+    key_at[s] = lds_address(ring) +
+                (unsigned)(j * D * 2 + (((4 * s + g) ^ (D == 128 ? j : (j >> 1) & 7)) << 4));
+#pragma unroll
+  for (int t = 0; t < DT; ++t) {
+    const int R = 4 * g + (j >> 2), unit = t ^ (D == 128 ? R & 7 : (R >> 1) & 3);
+    value_at[t] = lds_address(ring) + (unsigned)(kStep * D * 2 + R * D * 2 + (unit << 5) + ((j & 3) << 3));
+  }
+  int* pages = s_pages + wave * STAGES * kWave;
+  const unsigned page_at = lds_address(pages + lane);
+  const char* zero = reinterpret_cast<const char*>(s_zero_row);
+
+  while (at < stop) {
+    // ---- a part of one row
+    int steps, unit_at;
+    if (plan.blocks == 0) {
+      steps = stop;
+      unit_at = 0;
+    } else {
+      while (s_start[row + 1] * p.kv_heads <= at) ++row;
+      steps = s_start[row + 1] - s_start[row];
+      kvh = (at - s_start[row] * p.kv_heads) / steps;
+      unit_at = s_start[row] * p.kv_heads + kvh * steps;
+    }
+    const int first_step = at - unit_at, last_step = min(stop - unit_at, steps);
+    const int valid = p.valid[row], begin = window_begin(p, valid), sinks = min(p.sinks, begin);
+    const int count = sinks + valid - begin;
+    const int32_t* table = p.tables + (size_t)row * p.max_pages;
+    const unsigned head_unit = (unsigned)((size_t)kvh * p.head_stride / 8);
+    h8 qb[KS];
+    {
+      const half_t* q = p.q + ((size_t)row * p.q_heads + kvh * p.group + min(j, p.group - 1)) * D;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) qb[s] = load_h8(q + 32 * s + 8 * g);
+    }
+    f4 o[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t) o[t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, lsum = 0.0f;
+    int bad = 0;
+
+    // Table slot of the position that lane (l & 31) stands for in a step (past
+    // the end: of the last one) and its row in that page.
+    auto locate = [&](int step, int& slot_row) -> const int32_t* {
+      const int u = min(step * kStep + (lane & (kStep - 1)), count - 1);
+      const int pos = u < sinks ? u : begin + u - sinks;
+      const int slot = window_page(p, pos);
+      slot_row = pos - slot * p.page_size;
+      return table + slot;
+    };
+    // 16-byte unit where that position's row starts, kNoUnit when it has none
+    auto place = [&](int step, int page, int slot_row) -> unsigned {
+      const bool ok = window_page_ok(p, page);
+      bad |= !ok;
+      return ok && step * kStep + (lane & (kStep - 1)) < count
+                 ? (unsigned)page * (unsigned)(p.page_stride / 8) + head_unit +
+                       (unsigned)(slot_row * CH)
+                 : kNoUnit;
+    };
+    // K and V rows of a step, and the pages of the step that follows it in the
+    // stage: those too by loads to LDS, so that no load the compiler could wait
+    // for mixes with the ones in flight.
+    auto issue = [&](unsigned unit, const int32_t* next, int stage) {
+      half_t* to = ring + stage * STAGE;
+      __builtin_amdgcn_global_load_lds((global_void*)next, (lds_void*)(pages + stage * kWave), 4, 0, 0);
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int R = RPL * i + lane / CH, slot = lane % CH;
+        const unsigned row_unit = (unsigned)__shfl((int)unit, R, kWave);
+        const unsigned kc = slot ^ (D == 128 ? R & 15 : (R >> 1) & 7);
+        const unsigned vc = (((slot >> 1) ^ (D == 128 ? R & 7 : (R >> 1) & 3)) << 1) | (slot & 1);
+        const bool here = row_unit != kNoUnit;
+        const char* ka = here ? reinterpret_cast<const char*>(p.k) + (size_t)(row_unit + kc) * 16 : zero;
+        const char* va = here ? reinterpret_cast<const char*>(p.v) + (size_t)(row_unit + vc) * 16 : zero;
+        __builtin_amdgcn_global_load_lds((global_void*)ka, (lds_void*)(to + RPL * i * D), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((global_void*)va, (lds_void*)(to + (kStep + RPL * i) * D),
+                                         16, 0, 0);
+      }
+    };
+    auto consume = [&](int step, const h8 (&k)[2][KS], const h8 (&v)[DT]) {
+      f4 sc[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        sc[t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+          sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][s], qb[s], sc[t], 0, 0, 0);
+      }
+      const int left = count - step * kStep;  // positions of the step that exist
+      if (left < kStep)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (16 * t + 4 * g + r >= left) sc[t][r] = -INFINITY;
+      float top = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
+                        fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+      top = max_of_groups(top) * p.scale_log2;
+      if (__builtin_amdgcn_ballot_w64(top > m) != 0) {
+        const float next = fmaxf(m, top);
+        const float alpha = next == m ? 1.0f : fast_exp2(m - next);
+        m = next;
+        lsum *= alpha;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) o[t] *= alpha;
+      }
+      const float shift = m == -INFINITY ? 0.0f : m - kRaiseLog;
+      h8 w;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          w[4 * t + r] = (half_t)fast_exp2(__fmaf_rn(sc[t][r], p.scale_log2, -shift));
+      const h8 ones = {(half_t)1.0f, (half_t)1.0f, (half_t)1.0f, (half_t)1.0f,
+                       (half_t)1.0f, (half_t)1.0f, (half_t)1.0f, (half_t)1.0f};
+      lsum = dot8(w, ones, lsum);
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+        o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[t], w, o[t], 0, 0, 0);
+    };
+
+    // ---- the wave's steps: every kDecodeWaves-th of the part
+    const int mine = first_step + wave;
+    int slot_row[STAGES];  // of the step that a stage takes next
+    {
+      int first_page[STAGES], first_row[STAGES];
+#pragma unroll
+      for (int st = 0; st < STAGES; ++st)
+        first_page[st] = *locate(mine + st * kDecodeWaves, first_row[st]);
+#pragma unroll
+      for (int st = 0; st < STAGES; ++st) {
+        const int32_t* next = locate(mine + (STAGES + st) * kDecodeWaves, slot_row[st]);
+        if (mine + st * kDecodeWaves < last_step)
+          issue(place(mine + st * kDecodeWaves, first_page[st], first_row[st]), next, st);
+      }
+    }
+    // One step out of its stage, and the stage loaded again.  BODY: every step
+    // that is waited for or loaded exists.
+    auto turn = [&](auto stage, auto body, int step) {
+      constexpr int ST = decltype(stage)::value;
+      constexpr bool BODY = decltype(body)::value;
+      const int again = step + STAGES * kDecodeWaves;
+      if (BODY || step + (STAGES - 1) * kDecodeWaves < last_step)
+        wait_loads<(2 * LOADS + 1) * (STAGES - 1)>();
+      else
+        wait_loads<0>();
+      h8 k[2][KS], v[DT];
+      int page;
+      read_keys<D, ST * STAGE * 2, ST * kWave * 4>(key_at, page_at, k, page);
+#pragma unroll
+      for (int t = 0; t < DT; t += 4) read_values<D, ST * STAGE * 2>(value_at + t, v + t);
+      if (BODY || again < last_step) {
+        const unsigned unit = place(again, page, slot_row[ST]);
+        issue(unit, locate(again + STAGES * kDecodeWaves, slot_row[ST]), ST);
+      }
+      consume(step, k, v);
+    };
+    auto round = [&](auto body, int step) {
+      constexpr bool BODY = decltype(body)::value;
+      turn(std::integral_constant<int, 0>{}, body, step);
+      if constexpr (STAGES > 1)
+        if (BODY || step + kDecodeWaves < last_step)
+          turn(std::integral_constant<int, 1>{}, body, step + kDecodeWaves);
+      if constexpr (STAGES > 2)
+        if (BODY || step + 2 * kDecodeWaves < last_step)
+          turn(std::integral_constant<int, 2>{}, body, step + 2 * kDecodeWaves);
+      if constexpr (STAGES > 3)
+        if (BODY || step + 3 * kDecodeWaves < last_step)
+          turn(std::integral_constant<int, 3>{}, body, step + 3 * kDecodeWaves);
+    };
+    int step = mine;
+    for (; step + (2 * STAGES - 1) * kDecodeWaves < last_step; step += STAGES * kDecodeWaves)
+      round(std::true_type{}, step);
+    for (; step < last_step; step += STAGES * kDecodeWaves) round(std::false_type{}, step);
+
+    // ---- the waves meet in LDS (the ring: every load into it has landed)
+    lsum = cross_sum<16>(lsum);
+    bad = __syncthreads_or(bad);
+    float* s_max = reinterpret_cast<float*>(s_ring);  // [waves][16]
+    float* s_sum = s_max + kDecodeWaves * 16;
+    float* s_out = s_sum + kDecodeWaves * 16;         // [waves][group][D]
+    if (j < p.group) {
+      if (g == 0) {
+        s_max[wave * 16 + j] = m;
+        s_sum[wave * 16 + j] = lsum;
+      }
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+        *reinterpret_cast<f4*>(s_out + (size_t)(wave * p.group + j) * D + 16 * t + 4 * g) = o[t];
+    }
+    __syncthreads();
+    const bool whole = first_step == 0 && last_step == steps;
+    const int slot = whole ? 0 : 2 * blockIdx.x + (at == block_at ? 0 : 1);
+    float* part = plan.slots + (size_t)slot * p.group * (D + 2);
+    for (int i = threadIdx.x; i < p.group * D; i += THREADS) {
+      const int head = i / D, d = i % D;
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kDecodeWaves; ++w) top = fmaxf(top, s_max[w * 16 + head]);
+      float sum = 0.0f, val = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kDecodeWaves; ++w) {
+        const float high = s_max[w * 16 + head];
+        const float scale = high == -INFINITY ? 0.0f : fast_exp2(high - top);
+        sum += scale * s_sum[w * 16 + head];
+        val += scale * s_out[(size_t)(w * p.group + head) * D + d];
+      }
+      if (whole) {
+        if (!bad)
+          p.out[window_out(p, row, (kvh * p.group + head) * D + d)] = (half_t)(val / sum);
+      } else {
+        float* to = part + (size_t)head * (D + 2);
+        __hip_atomic_store(to + d, val, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (d == 0) {
+          __hip_atomic_store(to + D, top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          __hip_atomic_store(to + D + 1, bad ? -1.0f : sum, __ATOMIC_RELAXED,
+                             __HIP_MEMORY_SCOPE_AGENT);
+        }
+      }
+    }
+    if (!whole) {
+      // the last of the row's blocks joins the partials, in block order (every
+      // word is written and read at agent scope; the stores have completed
+      // before the arrival is counted)
+      const int from = unit_at / per, to = (unit_at + steps - 1) / per;
+      int* counter = plan.arrivals + (size_t)row * p.kv_heads + kvh;
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+      if (threadIdx.x == 0)
+        s_last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+                 to - from;
+      __syncthreads();
+      if (s_last) {
+        if (threadIdx.x == 0)
+          __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        for (int i = threadIdx.x; i < p.group * D; i += THREADS) {
+          const int head = i / D, d = i % D;
+          float top = -INFINITY, sum = 0.0f, val = 0.0f;
+          bool spoiled = false;
+          for (int b = from; b <= to; ++b) {
+            const int which = 2 * b + (b == from && unit_at != b * per ? 1 : 0);
+            const float* in = plan.slots + ((size_t)which * p.group + head) * (D + 2);
+            const float x = __hip_atomic_load(in + d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const float hi = __hip_atomic_load(in + D, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const float s = __hip_atomic_load(in + D + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            spoiled |= s < 0.0f;
+            const float next = fmaxf(top, hi);
+            const float a = top == -INFINITY ? 0.0f : fast_exp2(top - next);
+            const float c = hi == -INFINITY ? 0.0f : fast_exp2(hi - next);
+            sum = sum * a + s * c;
+            val = val * a + x * c;
+            top = next;
+          }
+          if (!spoiled)
+            p.out[window_out(p, row, (kvh * p.group + head) * D + d)] = (half_t)(val / sum);
+        }
+      }
+    }
+    at = unit_at + last_step;
+    if (at < stop) __syncthreads();  // the ring is loaded again
+  }
+}
+
 // ------------------------------------------------------------------ host
 int window_params(WindowParams& p, const char* what, const void* q, const void* key_pool,
                   const void* value_pool, const int32_t* valid, const int32_t* tables, void* out,
@@ -187,11 +642,32 @@ int launch_plain(const WindowParams& p, hipStream_t stream) {
 
 using namespace tmc;
 
+namespace tmc {
+namespace {
+// The shapes window_decode_kernel takes; the others run window_plain_kernel.
+bool decode_shape(int64_t q_heads, int64_t kv_heads, int64_t head_dim) {
+  return (head_dim == 64 || head_dim == 128) && q_heads / kv_heads <= 16;
+}
+// One list of steps over all blocks, unless the rows alone are many per CU.
+bool shared_list(int64_t batch, int64_t kv_heads) {
+  return batch <= kDecodeMaxRows && batch * kv_heads < 8 * kDecodeBlocks;
+}
+size_t window_counter_bytes(int64_t batch, int64_t kv_heads) {
+  return std::max(kWindowCounterBytes, (size_t)(batch * kv_heads * 4 + 255) / 256 * 256);
+}
+}  // namespace
+}  // namespace tmc
+
 extern "C" size_t tmc_window_attention_workspace_bytes(int64_t batch, int64_t q_heads,
                                                        int64_t kv_heads, int64_t head_dim,
                                                        int64_t capacity, int64_t window,
                                                        int64_t sinks) {
-  return 0;
+  if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || capacity <= 0 || q_heads % kv_heads ||
+      window < 1 || sinks < 0 || !decode_shape(q_heads, kv_heads, head_dim) ||
+      !shared_list(batch, kv_heads))
+    return 0;
+  return window_counter_bytes(batch, kv_heads) +
+         (size_t)kDecodeBlocks * 2 * (q_heads / kv_heads) * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int tmc_window_decode_attention(
@@ -219,7 +695,27 @@ extern "C" int tmc_window_decode_attention(
   p.table_rows = p.rows;
   p.own_table = 1;
   if (layout) p.out_pass = (long)((q_heads * head_dim + 31) / 32) * 512;
-  return launch_plain(p, as_stream(stream));
+  // 16-byte units of the pools are counted in 32 bits: below 64 GiB each
+  if (!decode_shape(q_heads, kv_heads, head_dim) ||
+      (uint64_t)pool_pages * (uint64_t)page_stride / 8 >= 0xFFFFFFFFull)
+    return launch_plain(p, as_stream(stream));
+  DecodePlan plan{};
+  unsigned blocks = (unsigned)(max_batch * kv_heads);
+  if (shared_list(max_batch, kv_heads)) {
+    plan.arrivals = static_cast<int*>(workspace);
+    plan.slots = reinterpret_cast<float*>(static_cast<char*>(workspace) +
+                                          window_counter_bytes(max_batch, kv_heads));
+    plan.blocks = kDecodeBlocks;
+    plan.least = kDecodeWaves;
+    blocks = kDecodeBlocks;
+  }
+  if (head_dim == 128)
+    hipLaunchKernelGGL((window_decode_kernel<128, 2>), dim3(blocks), dim3(kDecodeWaves * kWave), 0,
+                       as_stream(stream), p, plan);
+  else
+    hipLaunchKernelGGL((window_decode_kernel<64, 4>), dim3(blocks), dim3(kDecodeWaves * kWave), 0,
+                       as_stream(stream), p, plan);
+  return check_launch("window_decode_kernel");
 }
 
 extern "C" int tmc_window_prefill_attention_f16(
