@@ -580,48 +580,49 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void window_decode_kernel(Win
 }
 
 // ------------------------------------------------------------ a chunk of rows
-// D = 64 and 128.  One block of 4 waves per (kv head, tile of query vectors =
-// tokens x query heads of that kv head); each wave holds 32 VT vectors, on
+// D = 64 and 128.  One block of 8 waves per (kv head, tile of query vectors =
+// tokens x query heads of that kv head).  A wave holds 32 vectors on
 // v_mfma_f32_32x32x16_f16: S^T = K Q^T (32 positions x 32 vectors) leaves lane
 // (vector, half) with the positions 8 (r / 4) + 4 half + r % 4, the order in
-// which O^T = V^T P^T takes its weights.  A K or V operand read from LDS feeds
-// VT products.
+// which O^T = V^T P^T takes its weights.  Two waves a SIMD: one's softmax runs
+// beside the other's products.
 //
-// SPLIT = false: the waves hold different vectors and share stages of 64
-// positions.  SPLIT = true: they hold the same vectors and take 32 positions
-// each of a stage of 128, alone in their part of it, and join at the end.  K
-// and V go through registers, loaded one stage ahead of the LDS one.
+// PG = 1: the waves hold 8 x 32 vectors and all take the 64 positions of a
+// stage.  PG = 4: they hold 2 x 32 vectors and take a quarter of the 128
+// positions of a stage each; the four partials join at the end.  K and V go
+// through registers, loaded one stage ahead of the LDS one; one barrier a
+// stage.
 //
 // A tile's positions are those that any of its tokens sees, sinks first.
 // Positions that a vector does not see are masked in the steps where that can
 // be; steps that none of a wave's vectors sees are left out.  Rows of several
 // requests in a tile are done run by run.
 typedef float f16v __attribute__((ext_vector_type(16)));
-constexpr int kChunkWaves = 4;
+constexpr int kChunkWaves = 8;
 
 // A new maximum moves the weights' scale only when it is kLag above the one in
 // use, so a wave seldom rescales its sums; weights are then at most
 // 2^(kChunkRaise + kLag) in fp16 and keep 11 bits down to 2^-24 of that scale.
 constexpr float kLag = 5.0f, kChunkRaise = 10.0f;
 
-template <int D, int VT, bool SPLIT>
-__global__ __launch_bounds__(kChunkWaves * kWave) void window_chunk_kernel(WindowParams p,
-                                                                           int tiles,
-                                                                           int tokens_per_tile) {
+template <int D, int PG>
+__global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(WindowParams p,
+                                                                              int tiles,
+                                                                              int tokens_per_tile) {
   constexpr int KS = D / 16, DT = D / 32, CH = D / 8;
-  constexpr int THREADS = kChunkWaves * kWave;
-  constexpr int SPAN = SPLIT ? 32 * kChunkWaves : 64;    // positions a stage
-  constexpr int SUBS = SPLIT ? 1 : 2;                    // steps of 32 a wave takes of it
-  constexpr int OWN = SPAN / kChunkWaves;                // rows of a stage a wave loads
-  constexpr int RPL = kWave / CH, LOADS = OWN / RPL;     // rows a load, loads of K (of V)
-  constexpr int VECTORS = 32 * VT * (SPLIT ? 1 : kChunkWaves);
-  constexpr int STAGE = 2 * SPAN * D;                    // halves: K rows, V rows
-  constexpr int BUFFERS = SPLIT ? 1 : 2;
-  __shared__ __align__(16) half_t s_kv[BUFFERS * STAGE];
+  constexpr int WAVES = kChunkWaves, THREADS = WAVES * kWave, VG = WAVES / PG;
+  constexpr int SPAN = PG == 1 ? 64 : 32 * PG;        // positions a stage
+  constexpr int OWN = SPAN / WAVES;                   // rows of a stage a wave loads
+  constexpr int RPL = kWave / CH, LOADS = OWN / RPL;  // rows a load, loads of K (of V)
+  constexpr int STAGE = 2 * SPAN * D;                 // halves: K rows, V rows
+  static_assert(LOADS >= 1 && 2 * STAGE >= WAVES * 32 * D, "results fit the stages");
+  __shared__ __align__(16) half_t s_kv[2 * STAGE];
   __shared__ int s_run, s_low, s_high;
+  __shared__ float s_max[WAVES][32], s_sum[WAVES][32];
 
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+  const int vg = wave % VG, pg = wave / VG;
   const int col = lane & 31, half = lane >> 5;
   // the tiles of one kv head stay on one XCD, whose L2 then holds its pages
   int kvh, tile;
@@ -638,6 +639,9 @@ __global__ __launch_bounds__(kChunkWaves * kWave) void window_chunk_kernel(Windo
   const char* zero = reinterpret_cast<const char*>(s_zero_row);
   const unsigned head_unit = (unsigned)((size_t)kvh * p.head_stride / 8);
   const int capacity = p.page_size * p.max_pages;
+  // this lane's vector
+  const int token = (32 * vg + col) / p.group, row = t0 + token;
+  const int head = kvh * p.group + 32 * vg + col - token * p.group;
 
   for (int run = 0; run < tokens;) {
     // ---- the run of tokens [run, run_end) of one request
@@ -657,50 +661,15 @@ __global__ __launch_bounds__(kChunkWaves * kWave) void window_chunk_kernel(Windo
     }
     const int run_end = s_run, run_at = run;
     run = run_end;
-    if (table_row < 0) {
-      __syncthreads();
-      continue;
+    int len = 0;
+    if (table_row >= 0 && token >= run_at && token < run_end) {
+      len = p.valid[row];
+      if (len < 1 || len > capacity) len = 0;
     }
-    const int32_t* table = p.tables + (size_t)table_row * p.max_pages;
-
-    // ---- this lane's vectors
-    int len[VT], from[VT], row[VT], head[VT];
-#pragma unroll
-    for (int v = 0; v < VT; ++v) {
-      const int vec = (SPLIT ? 0 : wave * 32 * VT) + 32 * v + col;
-      const int token = vec / p.group;
-      row[v] = t0 + token;
-      head[v] = kvh * p.group + vec - token * p.group;
-      len[v] = 0;
-      if (token >= run_at && token < run_end) {
-        len[v] = p.valid[row[v]];
-        if (len[v] < 1 || len[v] > capacity) len[v] = 0;
-      }
-      from[v] = len[v] > 0 ? window_begin(p, len[v]) : 0x7fffffff;
-      if (half == 0 && len[v] > 0) {
-        atomicMin(&s_low, from[v]);
-        atomicMax(&s_high, len[v]);
-      }
-    }
-    __syncthreads();
-    const int low = s_low, high = s_high;
-    if (high == 0) {
-      __syncthreads();
-      continue;
-    }
-    const int sinks = min(p.sinks, low), gap = low - sinks;
-    const int count = high - gap;  // positions of the tile: u < sinks, then u + gap
-
-    // the wave's own extremes
-    int min_len = 0x7fffffff, max_len = 0, min_from = 0x7fffffff, max_from = 0;
-#pragma unroll
-    for (int v = 0; v < VT; ++v)
-      if (len[v] > 0) {
-        min_len = min(min_len, len[v]);
-        max_len = max(max_len, len[v]);
-        min_from = min(min_from, from[v]);
-        max_from = max(max_from, from[v]);
-      }
+    const int from = len > 0 ? window_begin(p, len) : 0x7fffffff;
+    // the wave's extremes, then the tile's
+    int min_len = len > 0 ? len : 0x7fffffff, max_len = len, min_from = from,
+        max_from = len > 0 ? from : 0;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
       min_len = min(min_len, __shfl_xor(min_len, off, kWave));
@@ -712,27 +681,19 @@ __global__ __launch_bounds__(kChunkWaves * kWave) void window_chunk_kernel(Windo
     max_len = __builtin_amdgcn_readfirstlane(max_len);
     min_from = __builtin_amdgcn_readfirstlane(min_from);
     max_from = __builtin_amdgcn_readfirstlane(max_from);
-
-    const h8 nothing = {0, 0, 0, 0, 0, 0, 0, 0};
-    h8 qb[VT][KS];
-#pragma unroll
-    for (int v = 0; v < VT; ++v) {
-      const half_t* q = p.q + ((size_t)row[v] * p.q_heads + head[v]) * D;
-#pragma unroll
-      for (int s = 0; s < KS; ++s)
-        qb[v][s] = len[v] > 0 ? load_h8(q + 16 * s + 8 * half) : nothing;
+    if (lane == 0 && max_len > 0) {
+      atomicMin(&s_low, min_from);
+      atomicMax(&s_high, max_len);
     }
-    f16v o[VT][DT];
-    float m[VT], sum[VT];
-#pragma unroll
-    for (int v = 0; v < VT; ++v) {
-      m[v] = -INFINITY;
-      sum[v] = 0.0f;
-#pragma unroll
-      for (int t = 0; t < DT; ++t)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[v][t][e] = 0.0f;
+    __syncthreads();
+    const int low = s_low, high = s_high;
+    if (high == 0) {
+      __syncthreads();
+      continue;
     }
+    const int32_t* table = p.tables + (size_t)table_row * p.max_pages;
+    const int sinks = min(p.sinks, low), gap = low - sinks;
+    const int count = high - gap;  // positions of the tile: u < sinks, then u + gap
 
     // ---- loads: lane l stands for row l % OWN of the wave's part of a stage
     int bad = 0;
@@ -774,66 +735,50 @@ __global__ __launch_bounds__(kChunkWaves * kWave) void window_chunk_kernel(Windo
         *reinterpret_cast<h8*>(buf + SPAN * D + at) = vr[i];
       }
     };
+    const int stages = (count + SPAN - 1) / SPAN;
+    int slot_row, next_row;
+    const int page = locate(0, slot_row);
+    int next = locate(1, next_row);
+    load(place(0, page, slot_row));
+    // stage `at` into registers, if there is one
+    auto load_stage = [&](int at) {
+      if (at < stages) {
+        const unsigned unit = place(at, next, next_row);
+        next = locate(at + 1, next_row);
+        load(unit);
+      }
+    };
 
-    // ---- one step of 32 positions: rows R0 ... of a stage, u0 ... of the tile
-    auto step = [&](const half_t* buf, int R0, int u0) {
-      const int p0 = u0 < sinks ? u0 : u0 + gap, p1 = u0 + 31 < sinks ? u0 + 31 : u0 + 31 + gap;
-      // nothing of it in any vector's sight
-      if (p0 >= max_len || (p1 < min_from && p0 >= p.sinks)) return;
-      const bool full = p1 < min_len && (p0 >= max_from || p1 < sinks);
+    const h8 nothing = {0, 0, 0, 0, 0, 0, 0, 0};
+    h8 qb[KS];
+    {
+      const half_t* q = p.q + ((size_t)row * p.q_heads + head) * D;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) qb[s] = len > 0 ? load_h8(q + 16 * s + 8 * half) : nothing;
+    }
+    f16v o[DT];
+    float m = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[t][e] = 0.0f;
+
+    // ---- one step of 32 positions: rows R0 ... of a stage, u0 ... of the tile.
+    // V's operands are read before the weights are computed (the fences keep
+    // the reads there), into the registers that K's have left.
+    typedef __fp16 v4fp16 __attribute__((__vector_size__(8)));
+    typedef __attribute__((address_space(3))) v4fp16 lds_v4;
+    typedef const __attribute__((address_space(3))) char lds_char;
+    h8 k[KS], va[2][DT];
+    auto read_keys = [&](const half_t* buf, int R0) {
       const half_t* sk = buf + (R0 + col) * D;
-      f16v sc[VT];
 #pragma unroll
-      for (int v = 0; v < VT; ++v)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) sc[v][e] = 0.0f;
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const int c = (2 * s + half) ^ (D == 128 ? col & 15 : (col >> 1) & 7);
-        const h8 k = *reinterpret_cast<const h8*>(sk + 8 * c);
-#pragma unroll
-        for (int v = 0; v < VT; ++v)
-          sc[v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qb[v][s], sc[v], 0, 0, 0);
-      }
-      if (!full) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int u = u0 + 8 * (e >> 2) + 4 * half + (e & 3), pos = u < sinks ? u : u + gap;
-#pragma unroll
-          for (int v = 0; v < VT; ++v)
-            if (pos >= len[v] || (pos < from[v] && pos >= p.sinks)) sc[v][e] = -INFINITY;
-        }
-      }
-      h8 w[VT][2];
-#pragma unroll
-      for (int v = 0; v < VT; ++v) {
-        float top = sc[v][0];
-#pragma unroll
-        for (int e = 1; e < 16; ++e) top = fmaxf(top, sc[v][e]);
-        const unsigned x = __builtin_bit_cast(unsigned, top);
-        const auto sw = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-        const unsigned s0 = sw[0], s1 = sw[1];
-        top = fmaxf(__builtin_bit_cast(float, s0), __builtin_bit_cast(float, s1)) * p.scale_log2;
-        if (__builtin_amdgcn_ballot_w64(top > m[v] + kLag) != 0) {
-          const float next = top > m[v] + kLag ? top : m[v];
-          const float alpha = next == m[v] ? 1.0f : fast_exp2(m[v] - next);
-          m[v] = next;
-          sum[v] *= alpha;
-#pragma unroll
-          for (int t = 0; t < DT; ++t) o[v][t] *= alpha;
-        }
-        const float shift = m[v] == -INFINITY ? 0.0f : m[v] - kChunkRaise;
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          w[v][e >> 3][e & 7] = (half_t)fast_exp2(__fmaf_rn(sc[v][e], p.scale_log2, -shift));
-        const h8 ones = {(half_t)1.0f, (half_t)1.0f, (half_t)1.0f, (half_t)1.0f,
-                         (half_t)1.0f, (half_t)1.0f, (half_t)1.0f, (half_t)1.0f};
-        sum[v] = dot8(w[v][0], ones, dot8(w[v][1], ones, sum[v]));
-      }
-      typedef __fp16 v4fp16 __attribute__((__vector_size__(8)));
-      typedef __attribute__((address_space(3))) v4fp16 lds_v4;
-      const char __attribute__((address_space(3)))* sv =
-          (const char __attribute__((address_space(3)))*)(buf + SPAN * D);
+      for (int s = 0; s < KS; ++s)
+        k[s] = *reinterpret_cast<const h8*>(
+            sk + 8 * ((2 * s + half) ^ (D == 128 ? col & 15 : (col >> 1) & 7)));
+    };
+    auto read_values = [&](const half_t* buf, int R0) {
+      lds_char* sv = (lds_char*)(buf + SPAN * D);
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -847,145 +792,160 @@ __global__ __launch_bounds__(kChunkWaves * kWave) void window_chunk_kernel(Windo
                 h4, __builtin_amdgcn_ds_read_tr16_b64_v4f16(
                         (lds_v4*)(sv + R * D * 2 + 32 * unit + 8 * (lane & 3))));
           }
-          const h8 a = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-          for (int v = 0; v < VT; ++v)
-            o[v][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, w[v][c], o[v][t], 0, 0, 0);
+          va[c][t] = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
         }
+    };
+    // Position of place u of the tile.
+    auto position = [&](int u) { return u < sinks ? u : u + gap; };
+    // Whether any of the wave's vectors sees some of a step.
+    auto seen = [&](int u0) {
+      const int p0 = position(u0);
+      return p0 < max_len && (position(u0 + 31) >= min_from || p0 < p.sinks);
+    };
+    f16v sc;
+    auto scores = [&]() {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[e] = 0.0f;
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[s], qb[s], sc, 0, 0, 0);
+    };
+    h8 w[2];
+    // out of sight: positions from the length on and [p.sinks, from)
+    const unsigned hidden = (unsigned)max(0, min(from, 0x7ffffffe) - p.sinks);
+    auto weigh = [&](int u0) {
+      const int p0 = position(u0), p1 = position(u0 + 31);
+      if (p1 >= min_len || (p0 < max_from && p1 >= sinks)) {  // not all of it in sight
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int pos = position(u0 + 8 * (e >> 2) + 4 * half + (e & 3));
+          const int away = (pos >= len) | ((unsigned)(pos - p.sinks) < hidden);
+          sc[e] = away ? -INFINITY : sc[e];
+        }
+      }
+      float top = sc[0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) top = fmaxf(top, sc[e]);
+      const unsigned x = __builtin_bit_cast(unsigned, top);
+      const auto sw = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+      const unsigned s0 = sw[0], s1 = sw[1];
+      top = fmaxf(__builtin_bit_cast(float, s0), __builtin_bit_cast(float, s1)) * p.scale_log2;
+      if (__builtin_amdgcn_ballot_w64(top > m + kLag) != 0) {
+        const float next_m = top > m + kLag ? top : m;
+        const float alpha = next_m == m ? 1.0f : fast_exp2(m - next_m);
+        m = next_m;
+        sum *= alpha;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) o[t] *= alpha;
+      }
+      const float shift = m == -INFINITY ? 0.0f : m - kChunkRaise;
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        w[e >> 3][e & 7] = (half_t)fast_exp2(__fmaf_rn(sc[e], p.scale_log2, -shift));
+      const h8 ones = {(half_t)1.0f, (half_t)1.0f, (half_t)1.0f, (half_t)1.0f,
+                       (half_t)1.0f, (half_t)1.0f, (half_t)1.0f, (half_t)1.0f};
+      sum = dot8(w[0], ones, dot8(w[1], ones, sum));
+    };
+    auto add_values = [&]() {
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+          o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[c][t], w[c], o[t], 0, 0, 0);
     };
 
     // ---- the stages
-    const int stages = (count + SPAN - 1) / SPAN;
-    int slot_row, next_row;
-    int page = locate(0, slot_row);
-    int next = locate(1, next_row);
-    load(place(0, page, slot_row));
-    if constexpr (SPLIT) {
-      for (int i = 0; i < stages; ++i) {
-        store(s_kv);  // this wave's part alone: its own LDS order is enough
-        __builtin_amdgcn_wave_barrier();
-        if (i + 1 < stages) {
-          const unsigned unit = place(i + 1, next, next_row);
-          next = locate(i + 2, next_row);
-          load(unit);
-        }
-        step(s_kv, 32 * wave, i * SPAN + 32 * wave);
-        __builtin_amdgcn_wave_barrier();
-      }
-    } else {
-      store(s_kv);
-      if (stages > 1) {
-        const unsigned unit = place(1, next, next_row);
-        next = locate(2, next_row);
-        load(unit);
-      }
-      for (int i = 0; i < stages; ++i) {
-        lds_barrier();  // stage i is in LDS, stage i - 1 has been read
-        if (i + 1 < stages) store(s_kv + ((i + 1) & 1) * STAGE);
-        if (i + 2 < stages) {
-          const unsigned unit = place(i + 2, next, next_row);
-          next = locate(i + 3, next_row);
-          load(unit);
-        }
-        const half_t* buf = s_kv + (i & 1) * STAGE;
+    store(s_kv);
+    load_stage(1);
+    for (int i = 0; i < stages; ++i) {
+      const half_t* buf = s_kv + (i & 1) * STAGE;
+      // stage i is in LDS, stage i - 1 has been read
+      lds_barrier();
+      if (i + 1 < stages) store(s_kv + ((i + 1) & 1) * STAGE);
+      load_stage(i + 2);
 #pragma unroll
-        for (int s = 0; s < SUBS; ++s) step(buf, 32 * s, i * SPAN + 32 * s);
+      for (int s = 0; s < (PG > 1 ? 1 : 2); ++s) {
+        const int R0 = PG > 1 ? 32 * pg : 32 * s, u0 = i * SPAN + R0;
+        if (!seen(u0)) continue;
+        read_keys(buf, R0);
+        scores();
+        __builtin_amdgcn_sched_barrier(0);
+        read_values(buf, R0);
+        __builtin_amdgcn_sched_barrier(0);
+        weigh(u0);
+        add_values();
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
 
     // ---- join and store
     bad = __syncthreads_or(bad);
-    bool ok[VT];
-#pragma unroll
-    for (int v = 0; v < VT; ++v) {
-      ok[v] = len[v] > 0;
-      sum[v] += __shfl_xor(sum[v], 32, kWave);
-      if (bad && ok[v]) {  // some position of the tile has no page: one of this vector's?
-        const int sink_pages = from[v] > 0 && p.sinks > 0
-                                   ? window_page(p, min(p.sinks, from[v]) - 1) + 1 : 0;
-        for (int i = 0; i < sink_pages; ++i) ok[v] &= window_page_ok(p, table[i]);
-        for (int i = window_page(p, from[v]); i <= window_page(p, len[v] - 1); ++i)
-          ok[v] &= window_page_ok(p, table[i]);
-      }
+    sum += __shfl_xor(sum, 32, kWave);
+    if (bad && len > 0) {  // some position of the tile has no page: one of this vector's?
+      const int sink_end = min(p.sinks, from);
+      bool whole = true;
+      for (int i = 0; i * (long)p.page_size < sink_end; ++i) whole &= window_page_ok(p, table[i]);
+      for (int i = window_page(p, from); i <= window_page(p, len - 1); ++i)
+        whole &= window_page_ok(p, table[i]);
+      if (!whole) len = 0;
     }
-    auto put = [&](int v, int t, const f16v& value, float inv) {
-      half_t* out = p.out + ((size_t)row[v] * p.q_heads + head[v]) * D + 32 * t + 4 * half;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        *reinterpret_cast<h4*>(out + 8 * e) =
-            h4{(half_t)(value[4 * e] * inv), (half_t)(value[4 * e + 1] * inv),
-               (half_t)(value[4 * e + 2] * inv), (half_t)(value[4 * e + 3] * inv)};
-    };
-    if constexpr (!SPLIT) {
-#pragma unroll
-      for (int v = 0; v < VT; ++v)
-        if (ok[v])
-#pragma unroll
-          for (int t = 0; t < DT; ++t) put(v, t, o[v][t], 1.0f / sum[v]);
-    } else {
-      // pair (v, t) is finished by wave (v DT + t) % 4; the others hand it over
-      constexpr int PAIRS = VT * DT;
-      __shared__ float s_max[kChunkWaves][VT][32], s_sum[kChunkWaves][VT][32];
-      constexpr int kPair = 16 * kWave;  // floats of a pair
-      float* hand = reinterpret_cast<float*>(s_kv);
-      static_assert(sizeof(float) * 2 * kChunkWaves * kPair <= sizeof(s_kv),
-                    "two pairs of every wave fit the stage");
-      if (half == 0)
-#pragma unroll
-        for (int v = 0; v < VT; ++v) {
-          s_max[wave][v][col] = m[v];
-          s_sum[wave][v][col] = sum[v];
-        }
-      __syncthreads();
-      float scale[VT], inv[VT];
-#pragma unroll
-      for (int v = 0; v < VT; ++v) {
-        float top = -INFINITY, total = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kChunkWaves; ++w) top = fmaxf(top, s_max[w][v][col]);
-#pragma unroll
-        for (int w = 0; w < kChunkWaves; ++w) {
-          const float high = s_max[w][v][col];
-          total += high == -INFINITY ? 0.0f : fast_exp2(high - top) * s_sum[w][v][col];
-        }
-        scale[v] = m[v] == -INFINITY ? 0.0f : fast_exp2(m[v] - top);
-        inv[v] = 1.0f / total;
+    float scale = 1.0f / sum;
+    if constexpr (PG > 1) {
+      if (half == 0) {
+        s_max[wave][col] = m;
+        s_sum[wave][col] = sum;
       }
-      // two pairs a pass
+      __syncthreads();
+      float top = -INFINITY, total = 0.0f;
 #pragma unroll
-      for (int pass = 0; pass < PAIRS; pass += 2) {
-        if (pass) __syncthreads();
+      for (int g = 0; g < PG; ++g) top = fmaxf(top, s_max[g * VG + vg][col]);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int v = (pass + k) / DT, t = (pass + k) % DT;
-          float* to = hand + (k * kChunkWaves + wave) * kPair + lane;
+      for (int g = 0; g < PG; ++g) {
+        const float other = s_max[g * VG + vg][col];
+        total += other == -INFINITY ? 0.0f : fast_exp2(other - top) * s_sum[g * VG + vg][col];
+      }
+      scale = m == -INFINITY ? 0.0f : fast_exp2(m - top) / total;
+      // the other groups' sums in fp32, a 32-dim tile a pass: group pg finishes
+      // the elements 4 pg ... 4 pg + 3 (dims 8 pg + 4 half ...) of it
+      float* hand = reinterpret_cast<float*>(s_kv);
+      constexpr int kTile = 16 * kWave;
+      static_assert(PG == 4 && sizeof(float) * WAVES * kTile <= sizeof(s_kv), "a pass fits");
 #pragma unroll
-          for (int e = 0; e < 16; ++e) to[e * kWave] = o[v][t][e] * scale[v];
-        }
+      for (int t = 0; t < DT; ++t) {
+        if (t) __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) hand[wave * kTile + e * kWave + lane] = o[t][e] * scale;
         __syncthreads();
-        // wave w: pair pass + w / 2, elements 8 (w % 2) ... of it
+        float val[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          if (wave / 2 != k) continue;
-          const int v = (pass + k) / DT, t = (pass + k) % DT, e0 = 8 * (wave % 2);
-          float val[8];
+        for (int g = 0; g < PG; ++g)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            val[e] = 0.0f;
+          for (int e = 0; e < 4; ++e)
+            val[e] += hand[(g * VG + vg) * kTile + (4 * pg + e) * kWave + lane];
+        if (len > 0)
+          *reinterpret_cast<h4*>(p.out + ((size_t)row * p.q_heads + head) * D + 32 * t + 8 * pg +
+                                 4 * half) =
+              h4{(half_t)val[0], (half_t)val[1], (half_t)val[2], (half_t)val[3]};
+      }
+    } else {
+      // rows through LDS (16-byte chunks swizzled by the row), so that whole
+      // rows are stored: lane l then holds chunk l % CH of row l / CH
+      half_t* rows = s_kv + wave * 32 * D;
 #pragma unroll
-            for (int w = 0; w < kChunkWaves; ++w)
-              val[e] += hand[(k * kChunkWaves + w) * kPair + (e0 + e) * kWave + lane];
-            val[e] *= inv[v];
-          }
-          if (ok[v]) {
-            half_t* out = p.out + ((size_t)row[v] * p.q_heads + head[v]) * D + 32 * t + 4 * half +
-                          8 * (e0 / 4);
-            *reinterpret_cast<h4*>(out) = h4{(half_t)val[0], (half_t)val[1], (half_t)val[2],
-                                             (half_t)val[3]};
-            *reinterpret_cast<h4*>(out + 8) = h4{(half_t)val[4], (half_t)val[5], (half_t)val[6],
-                                                 (half_t)val[7]};
-          }
-        }
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<h4*>(rows + col * D + (((4 * t + e) ^ (col & (CH - 1))) << 3) + 4 * half) =
+              h4{(half_t)(o[t][4 * e] * scale), (half_t)(o[t][4 * e + 1] * scale),
+                 (half_t)(o[t][4 * e + 2] * scale), (half_t)(o[t][4 * e + 3] * scale)};
+      __builtin_amdgcn_wave_barrier();
+      const int put = len > 0 ? row * p.q_heads + head : -1;
+#pragma unroll
+      for (int i = 0; i < 32 / RPL; ++i) {
+        const int R = RPL * i + lane / CH, chunk = lane % CH;
+        const int to = __shfl(put, R, kWave);
+        const h8 val = *reinterpret_cast<const h8*>(rows + R * D + ((chunk ^ (R & (CH - 1))) << 3));
+        if (to >= 0) *reinterpret_cast<h8*>(p.out + (size_t)to * D + 8 * chunk) = val;
       }
     }
     __syncthreads();  // the next run clears s_run and loads the stages again
@@ -1153,18 +1113,17 @@ extern "C" int tmc_window_prefill_attention_f16(
       (uint64_t)pool_pages * (uint64_t)page_stride / 8 >= 0xFFFFFFFFull)
     return launch_plain(p, as_stream(stream));
   const int wide = 256 / p.group, narrow = 64 / p.group;  // tokens a tile
-  const int64_t blocks = (rows + wide - 1) / wide * kv_heads;
-  const bool split = blocks < 192;
+  const bool split = (rows + wide - 1) / wide * kv_heads < 192;
   const int tokens = split ? narrow : wide;
   const int tiles = (int)((rows + tokens - 1) / tokens);
   const dim3 grid((unsigned)(tiles * kv_heads)), block(kChunkWaves * kWave);
-#define TMC_CHUNK(DIM, SPLIT)                                                                     \
-  hipLaunchKernelGGL((window_chunk_kernel<DIM, 2, SPLIT>), grid, block, 0, as_stream(stream), p, \
-                     tiles, tokens)
+#define TMC_CHUNK(DIM, PG)                                                                        \
+  hipLaunchKernelGGL((window_chunk_kernel<DIM, PG>), grid, block, 0, as_stream(stream), p, tiles, \
+                     tokens)
   if (head_dim == 128) {
-    if (split) TMC_CHUNK(128, true); else TMC_CHUNK(128, false);
+    if (split) TMC_CHUNK(128, 4); else TMC_CHUNK(128, 1);
   } else {
-    if (split) TMC_CHUNK(64, true); else TMC_CHUNK(64, false);
+    if (split) TMC_CHUNK(64, 4); else TMC_CHUNK(64, 1);
   }
 #undef TMC_CHUNK
   return check_launch("window_chunk_kernel");

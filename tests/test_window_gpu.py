@@ -302,6 +302,11 @@ CHUNK = [
     (512, 1024, 4, 1, 128, 16, 512, 16),
     (129, 64, 4, 4, 128, 64, 10 ** 12, 3),
     (515, 0, 2, 2, 128, 16, 200, 70),
+    # many kv heads: the wide tiles
+    (70, 100, 192, 192, 128, 16, 50, 4),
+    (300, 40, 192, 96, 64, 12, 77, 9),
+    (515, 300, 128, 64, 128, 16, 200, 70),
+    (130, 0, 600, 200, 64, 16, 60, 0),
 ]
 
 
@@ -327,7 +332,8 @@ def test_chunk_matches_the_formula(tmc, torch, rows, start, qh, kvh, d, page, wi
     check_rows(torch, out[index], cache, q[index], expect, qh, d, window, sinks, 7.5)
 
 
-@pytest.mark.parametrize("qh,kvh,d,page", [(4, 4, 128, 16), (8, 2, 64, 12), (8, 1, 128, 16), (4, 2, 32, 16)])
+@pytest.mark.parametrize("qh,kvh,d,page", [(4, 4, 128, 16), (8, 2, 64, 12), (8, 1, 128, 16),
+                                           (4, 2, 32, 16), (200, 200, 64, 16), (200, 200, 128, 12)])
 def test_chunk_of_several_requests(tmc, torch, qh, kvh, d, page):
     """Rows of several requests in any packing, with invalid lengths, table rows
     outside the tables, and a request whose window reaches a missing page."""
