@@ -7,10 +7,11 @@
 // order of tmc_argmax_f32 (the greater first, equals by the lower index, NaN
 // never).
 //
-// Bound by reading the logits once.  A row is cut into parts, one block each;
-// a wave holds its elements of the part in registers, so the maximum, the sums
-// and the alternatives are three passes over registers, not over memory.  The
-// last block of a row to arrive joins the parts in their order.
+// Bound by reading the logits once.  A block holds a part of a row in
+// registers at a time, so the maximum, the sums and the alternatives are three
+// passes over registers, not over memory, while the next part is on its way.
+// Where several blocks share a row, the last to arrive joins them in their
+// order.
 #include "tmc_abi.hpp"
 #include "tmc_device.hpp"
 
@@ -40,7 +41,8 @@ struct LogprobParams {
   int* arrivals;  // [rows]
   long stride;
   int rows, vocab, top;
-  int count;      // parts a row
+  int count;      // blocks a row
+  int walk;       // parts a block
 };
 
 // A logit and its index as one number, greater in the greedy order first: the
@@ -66,26 +68,16 @@ __device__ __forceinline__ float wave_max(float v) {
   return fmaxf(fmaxf(readlane(v, 0), readlane(v, 16)), fmaxf(readlane(v, 32), readlane(v, 48)));
 }
 
-// (m, S, T) of two sets of logits together.  S and T are relative to m.
-struct Mass {
-  float m;
-  double s, t;
-  __device__ __forceinline__ void add(float om, double os, double ot) {
-    const float next = fmaxf(m, om);
-    if (next == -INFINITY) {  // two empty sets (their NaNs stay)
-      s += os;
-      t += ot;
-      return;
-    }
-    const double da = (double)m - next, db = (double)om - next;
-    // an empty set weighs nothing; 0 * inf must not arise
-    const double ea = m == -INFINITY ? 0.0 : (double)expf((float)da);
-    const double eb = om == -INFINITY ? 0.0 : (double)expf((float)db);
-    t = (m == -INFINITY ? t : ea * (t + s * da)) + (om == -INFINITY ? ot : eb * (ot + os * db));
-    s = (m == -INFINITY ? s : ea * s) + (om == -INFINITY ? os : eb * os);
-    m = next;
-  }
-};
+// What a set of logits with maximum m and sums s, t (relative to m) adds to the
+// sums relative to `high` >= m: nothing when it is empty (m = -inf), but for
+// the NaNs that an empty maximum hides.
+__device__ __forceinline__ void add_mass(float m, double s, double t, float high, double& sum_s,
+                                         double& sum_t) {
+  const float d = m == -INFINITY ? 0.0f : m - high;
+  const double e = (double)fast_exp2(d * 1.44269504f);
+  sum_s += e * s;
+  sum_t += e == 0.0 ? 0.0 : e * (t + s * (double)d);
+}
 
 // The best `top` of `count` distinct keys (at most kCandidates) to the places their rank
 // gives them, the rest of the places empty.  Ends with a barrier.
@@ -106,11 +98,13 @@ __device__ __forceinline__ void rank_keys(const long long* keys, int count, int 
   __syncthreads();
 }
 
-// EACH: elements a lane holds; a part is kLpThreads * EACH elements.
+// EACH: elements a lane holds; a part is kLpThreads * EACH elements.  A block
+// walks `walk` parts of its row, the next one's loads in flight.
 template <typename T, int EACH>
 __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
   constexpr int VEC = 16 / (int)sizeof(T);  // elements a load
   constexpr int LOADS = EACH / VEC;
+  constexpr int PART = kLpThreads * EACH;
   typedef T vec __attribute__((ext_vector_type(VEC)));
   // rows start anywhere on an element boundary
   typedef vec unaligned __attribute__((aligned(sizeof(T))));
@@ -120,146 +114,183 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
   __shared__ float s_m[kLpWaves], s_bound[kLpWaves];
   __shared__ double s_s[kLpWaves], s_t[kLpWaves];
   __shared__ int s_reach[kLpWaves], s_found, s_last;
-  const int part = blockIdx.x % p.count, row = blockIdx.x / p.count;
+  const int split = blockIdx.x % p.count, row = blockIdx.x / p.count;
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const T* x = static_cast<const T*>(p.logits) + (size_t)row * p.stride;
-  // the wave's elements: loads of 64 lanes x VEC, load after load
-  const int base = part * (kLpThreads * EACH) + wave * (kWave * EACH) + lane * VEC;
-  float v[EACH];
-#pragma unroll
-  for (int i = 0; i < LOADS; ++i) {
-    const int at = base + i * kWave * VEC;
-    if (at + VEC <= p.vocab) {
-      const vec in = *reinterpret_cast<const unaligned*>(x + at);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[i * VEC + e] = (float)in[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        v[i * VEC + e] = at + e < p.vocab ? (float)x[at + e] : -INFINITY;
-    }
-  }
-  float mine = -INFINITY;  // the lane's greatest (NaN left out)
-#pragma unroll
-  for (int i = 0; i < EACH; ++i) mine = fmaxf(mine, v[i]);
-  const float m = wave_max(mine);
-  // A wave of -inf or nothing adds nothing; its NaNs spoil the sums all the same.
-  const float shift = m == -INFINITY ? 0.0f : m;
-  float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f}, t4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-  for (int i = 0; i < EACH; ++i) {
-    const float d = v[i] - shift, e = fast_exp2(d * 1.44269504f);
-    s4[i & 3] += e;
-    t4[i & 3] += e == 0.0f ? 0.0f : e * d;
-  }
-  // 32 bits over at most 8 + 2 + 4 additions, 64 above
-  const float s16 = group_sum<16>((s4[0] + s4[1]) + (s4[2] + s4[3]));
-  const float t16 = group_sum<16>((t4[0] + t4[1]) + (t4[2] + t4[3]));
-  double s = 0.0, t = 0.0;
-#pragma unroll
-  for (int r = 0; r < kWave; r += 16) {
-    s += readlane(s16, r);
-    t += readlane(t16, r);
-  }
-  // ---- a bound that at least `top` of the block's elements reach, from the
-  // lanes' greatest: each wave finds what its share of them reach
+  const int begin = split * p.walk * PART, end = min(p.vocab, begin + p.walk * PART);
   const int top = p.top;
-  const int part_at = part * (kLpThreads * EACH);
-  if (top > 0) {
-    // waves whose lanes all hold elements
-    const int full = min(kLpWaves, (p.vocab - part_at + kWave * (EACH - VEC)) / (kWave * EACH));
-    const int need = full > 0 ? (top + full - 1) / full : top;
-    float rest = mine, bound = -INFINITY;
-    int reach = 0;
-    while (reach < need) {
-      const float most = wave_max(rest);
-      if (most == -INFINITY) {
-        bound = -INFINITY;
-        break;
+  // the wave's elements of a part: loads of 64 lanes x VEC, load after load
+  const int own = wave * (kWave * EACH) + lane * VEC;
+  auto fetch = [&](int part_at, vec (&in)[LOADS]) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int at = part_at + own + i * kWave * VEC;
+      if (at + VEC <= end) {
+        in[i] = *reinterpret_cast<const unaligned*>(x + at);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) in[i][e] = at + e < end ? x[at + e] : (T)-INFINITY;
       }
-      bound = most;
-      reach += __builtin_popcountll(__builtin_amdgcn_ballot_w64(rest == most));
-      if (rest == most) rest = -INFINITY;
     }
-    if (lane == 0) {
-      s_bound[wave] = bound;
-      s_reach[wave] = reach;
-    }
-  }
-  if (lane == 0) {
-    s_m[wave] = m;
-    s_s[wave] = s;
-    s_t[wave] = t;
-  }
+  };
+  // the lane's own maximum and sums (relative to it)
+  float m = -INFINITY, s = 0.0f, t = 0.0f;
   if (threadIdx.x == 0) s_found = 0;
-  __syncthreads();
-  Mass mass{s_m[0], s_s[0], s_t[0]};
+  int held = 0;             // keys in s_best
+  float floor_v = -INFINITY;  // once `top` are held: the last of them
+  vec next[LOADS];
+  fetch(begin, next);
+  for (int part_at = begin; part_at < end; part_at += PART) {
+    float v[EACH];
 #pragma unroll
-  for (int w = 1; w < kLpWaves; ++w) mass.add(s_m[w], s_s[w], s_t[w]);
-  if (top > 0) {
-    float bound = -INFINITY;
+    for (int i = 0; i < EACH; ++i) v[i] = (float)next[i / VEC][i % VEC];
+    if (part_at + PART < end) fetch(part_at + PART, next);
+    float mine = -INFINITY;  // (NaN left out)
 #pragma unroll
-    for (int w = 0; w < kLpWaves; ++w) {
-      int reach = 0;
-#pragma unroll
-      for (int u = 0; u < kLpWaves; ++u) reach += s_bound[u] >= s_bound[w] ? s_reach[u] : 0;
-      if (reach >= top) bound = fmaxf(bound, s_bound[w]);
-    }
-    // ---- the elements that reach it
-    if (m >= bound) {
+    for (int i = 0; i < EACH; ++i) mine = fmaxf(mine, v[i]);
+    {
+      // A lane of -inf adds nothing; its NaNs spoil the sums all the same.
+      const float high = fmaxf(m, mine), shift = high == -INFINITY ? 0.0f : high;
+      if (m != -INFINITY && m != high) {
+        const float d = m - high, e = fast_exp2(d * 1.44269504f);
+        t = e == 0.0f ? 0.0f : e * (t + s * d);
+        s *= e;
+      }
+      m = high;
+      float s4[4] = {s, 0.0f, 0.0f, 0.0f}, t4[4] = {t, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int i = 0; i < EACH; ++i) {
-        const int at = base + i / VEC * kWave * VEC + i % VEC;
-        const bool in = v[i] >= bound && at < p.vocab;  // a NaN never
+        const float d = v[i] - shift, e = fast_exp2(d * 1.44269504f);
+        s4[i & 3] += e;
+        t4[i & 3] += e == 0.0f ? 0.0f : e * d;
+      }
+      s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+      t = (t4[0] + t4[1]) + (t4[2] + t4[3]);
+    }
+    if (top == 0) continue;
+
+    // ---- a bound that at least `top` of the block's elements reach: what is
+    // held, or from the lanes' greatest, of which each wave finds what its
+    // share reaches
+    float bound = floor_v;
+    if (held < top) {
+      // waves whose lanes all hold elements
+      const int full = min(kLpWaves, (end - part_at + kWave * (EACH - VEC)) / (kWave * EACH));
+      const int need = full > 0 ? (top + full - 1) / full : top;
+      float rest = mine, most = -INFINITY;
+      int reach = 0;
+      while (reach < need) {
+        const float now = wave_max(rest);
+        most = now;
+        if (now == -INFINITY) break;
+        reach += __builtin_popcountll(__builtin_amdgcn_ballot_w64(rest == now));
+        if (rest == now) rest = -INFINITY;
+      }
+      if (lane == 0) {
+        s_bound[wave] = most;
+        s_reach[wave] = reach;
+      }
+      __syncthreads();
+      bound = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kLpWaves; ++w) {
+        int total = 0;
+#pragma unroll
+        for (int u = 0; u < kLpWaves; ++u) total += s_bound[u] >= s_bound[w] ? s_reach[u] : 0;
+        if (total >= top) bound = fmaxf(bound, s_bound[w]);
+      }
+    }
+    // ---- the elements that reach it, beside the ones held
+    if (__builtin_amdgcn_ballot_w64(mine >= bound) != 0) {
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        const int at = part_at + own + i / VEC * kWave * VEC + i % VEC;
+        const bool in = v[i] >= bound && at < end;  // a NaN never
         if (__builtin_amdgcn_ballot_w64(in) != 0 && in) {
-          const int place = atomicAdd(&s_found, 1);
+          const int place = held + atomicAdd(&s_found, 1);
           if (place < kCandidates) s_keys[place] = key_of(v[i], at);
         }
       }
     }
     __syncthreads();
     const int found = s_found;
-    if (found <= kCandidates) {
-      rank_keys(s_keys, found, top, s_best);
-    } else {
-      // too many: one a round, the best behind the one before
-      long long last = 0x7FFFFFFFFFFFFFFFll;
-      for (int k = 0; k < top; ++k) {
-        long long best = kNoKey;
+    if (found > 0) {  // the same in every thread
+      if ((int)threadIdx.x < held) s_keys[threadIdx.x] = s_best[threadIdx.x];
+      if (held + found <= kCandidates) {
+        __syncthreads();
+        rank_keys(s_keys, held + found, top, s_best);
+      } else {
+        // too many: one a round, the best behind the one before
+        long long last = 0x7FFFFFFFFFFFFFFFll;
+        const long long mine_held = (int)threadIdx.x < held ? s_best[threadIdx.x] : kNoKey;
+        for (int k = 0; k < top; ++k) {
+          long long best = mine_held < last ? mine_held : kNoKey;
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-          const int at = base + i / VEC * kWave * VEC + i % VEC;
-          const long long key = key_of(v[i], at);
-          if (at < p.vocab && v[i] == v[i] && key < last && key > best) best = key;
-        }
+          for (int i = 0; i < EACH; ++i) {
+            const int at = part_at + own + i / VEC * kWave * VEC + i % VEC;
+            const long long key = key_of(v[i], at);
+            if (at < end && v[i] == v[i] && key < last && key > best) best = key;
+          }
 #pragma unroll
-        for (int off = 1; off < kWave; off <<= 1) {
-          const long long other = __shfl_xor(best, off, kWave);
-          best = other > best ? other : best;
+          for (int off = 1; off < kWave; off <<= 1) {
+            const long long other = __shfl_xor(best, off, kWave);
+            best = other > best ? other : best;
+          }
+          __syncthreads();
+          if (lane == 0) s_keys[wave] = best;
+          __syncthreads();
+#pragma unroll
+          for (int w = 0; w < kLpWaves; ++w) best = s_keys[w] > best ? s_keys[w] : best;
+          if (threadIdx.x == 0) s_best[k] = best;
+          last = best;
         }
         __syncthreads();
-        if (lane == 0) s_keys[wave] = best;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kLpWaves; ++w) best = s_keys[w] > best ? s_keys[w] : best;
-        if (threadIdx.x == 0) s_best[k] = best;
-        last = best;
       }
+      held = min(top, held + found);
+      if (held == top) floor_v = key_value(s_best[top - 1]);
+      if (threadIdx.x == 0) s_found = 0;
       __syncthreads();
     }
   }
+  if (top > 0 && (int)threadIdx.x >= held && (int)threadIdx.x < top) s_best[threadIdx.x] = kNoKey;
+  {
+    // the lanes of a row of 16 in 32 bits, rows and waves in 64
+    const float high = wave_max(m);
+    const float e = m == -INFINITY ? 1.0f : fast_exp2((m - high) * 1.44269504f);
+    const float d = m == -INFINITY ? 0.0f : m - high;
+    const float s16 = group_sum<16>(e * s);
+    const float t16 = group_sum<16>(e == 0.0f ? 0.0f : e * (t + s * d));
+    double sw = 0.0, tw = 0.0;
+#pragma unroll
+    for (int r = 0; r < kWave; r += 16) {
+      sw += readlane(s16, r);
+      tw += readlane(t16, r);
+    }
+    if (lane == 0) {
+      s_m[wave] = high;
+      s_s[wave] = sw;
+      s_t[wave] = tw;
+    }
+  }
+  __syncthreads();
+  float row_m = s_m[0];
+#pragma unroll
+  for (int w = 1; w < kLpWaves; ++w) row_m = fmaxf(row_m, s_m[w]);
+  double row_s = 0.0, row_t = 0.0;
+#pragma unroll
+  for (int w = 0; w < kLpWaves; ++w) add_mass(s_m[w], s_s[w], s_t[w], row_m, row_s, row_t);
 
   // ---- the row's blocks together
   if (p.count > 1) {
-    const size_t slots = (size_t)p.rows * p.count, slot = (size_t)row * p.count + part;
+    const size_t slots = (size_t)p.rows * p.count, slot = (size_t)row * p.count + split;
     double* sums = reinterpret_cast<double*>(p.parts);            // [slots][2]
     long long* keys = reinterpret_cast<long long*>(sums + 2 * slots);  // [slots][top]
     float* maxima = reinterpret_cast<float*>(keys + slots * top);
     // every word at agent scope, completed before the arrival is counted
     if (threadIdx.x == 0) {
-      __hip_atomic_store(sums + 2 * slot, mass.s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      __hip_atomic_store(sums + 2 * slot + 1, mass.t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      __hip_atomic_store(maxima + slot, mass.m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(sums + 2 * slot, row_s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(sums + 2 * slot + 1, row_t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(maxima + slot, row_m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     if ((int)threadIdx.x < top)
       __hip_atomic_store(keys + slot * top + threadIdx.x, s_best[threadIdx.x], __ATOMIC_RELAXED,
@@ -276,38 +307,59 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
     if (threadIdx.x == 0)
       __hip_atomic_store(p.arrivals + row, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     const size_t first = (size_t)row * p.count;
-    // lane by lane over the parts, then over the lanes: the same order each time
-    Mass all{-INFINITY, 0.0, 0.0};
-    long long bound = kNoKey;  // the greatest of the parts' last keys: `top` keys reach it
-    for (int i = lane; i < p.count; i += kWave) {
-      all.add(__hip_atomic_load(maxima + first + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
-              __hip_atomic_load(sums + 2 * (first + i), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
-              __hip_atomic_load(sums + 2 * (first + i) + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-      if (top > 0) {
-        const long long key = __hip_atomic_load(keys + (first + i) * top + top - 1,
-                                                __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        bound = key > bound ? key : bound;
-      }
-    }
+    // each wave by itself: the maximum, then the sums relative to it, lane by
+    // lane over the parts and then over the lanes: the same order each time
+    row_m = -INFINITY;
+    for (int i = lane; i < p.count; i += kWave)
+      row_m = fmaxf(row_m, __hip_atomic_load(maxima + first + i, __ATOMIC_RELAXED,
+                                             __HIP_MEMORY_SCOPE_AGENT));
+    // A bound that at least `top` keys reach: where `deep` parts are needed to
+    // give `top` keys with their best `each` ones, the deep-th greatest of the
+    // parts' each-th keys.
+    const int some = min(p.count, kCandidates), each = (top + some - 1) / some;
+    if (top > 0 && (int)threadIdx.x < some)
+      s_keys[threadIdx.x] = __hip_atomic_load(keys + (first + threadIdx.x) * top + each - 1,
+                                              __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    row_m = wave_max(row_m);
+    row_s = row_t = 0.0;
+    for (int i = lane; i < p.count; i += kWave)
+      add_mass(__hip_atomic_load(maxima + first + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
+               __hip_atomic_load(sums + 2 * (first + i), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
+               __hip_atomic_load(sums + 2 * (first + i) + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
+               row_m, row_s, row_t);
 #pragma unroll
     for (int off = 1; off < kWave; off <<= 1) {
-      const float om = __shfl_xor(all.m, off, kWave);
-      const double os = __shfl_xor(all.s, off, kWave), ot = __shfl_xor(all.t, off, kWave);
-      all.add(om, os, ot);
-      const long long other = __shfl_xor(bound, off, kWave);
-      bound = other > bound ? other : bound;
+      row_s += __shfl_xor(row_s, off, kWave);
+      row_t += __shfl_xor(row_t, off, kWave);
     }
-    mass = all;
     if (top > 0) {
+      const int deep = (top + each - 1) / each;  // at most `some`
+      if (threadIdx.x == 0) s_best[0] = kNoKey;
+      __syncthreads();
+      if ((int)threadIdx.x < some) {
+        const long long mine = s_keys[threadIdx.x];
+        int rank = 0;
+        for (int o = 0; o < some; ++o) rank += s_keys[o] > mine ? 1 : 0;
+        if (rank == deep - 1 && mine != kNoKey) s_best[0] = mine;  // keys are distinct
+      }
+      __syncthreads();
+      const long long bound = s_best[0];
+      __syncthreads();
       const int total = p.count * top;
       const long long* from = keys + first * top;
-      for (int i = threadIdx.x; i < total; i += kLpThreads) {
-        const long long key =
-            __hip_atomic_load(from + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (key != kNoKey && key >= bound) {
-          const int place = atomicAdd(&s_found, 1);
-          if (place < kCandidates) s_keys[place] = key;
-        }
+      constexpr int kAhead = 4;  // keys a thread loads at once
+      for (int i = threadIdx.x; i < total; i += kAhead * kLpThreads) {
+        long long key[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+          key[u] = __hip_atomic_load(from + min(i + u * kLpThreads, total - 1), __ATOMIC_RELAXED,
+                                     __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+          if (i + u * kLpThreads < total && key[u] != kNoKey && key[u] >= bound) {
+            const int place = atomicAdd(&s_found, 1);
+            if (place < kCandidates) s_keys[place] = key[u];
+          }
       }
       __syncthreads();
       if (s_found <= kCandidates) {
@@ -332,33 +384,46 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
 
   // ---- the row
   // -inf alone: 0 / 0, a NaN as the other rows without a distribution
-  const float log_s = mass.m == -INFINITY ? __builtin_nanf("") : logf((float)mass.s);
+  const float log_s = row_m == -INFINITY ? __builtin_nanf("") : logf((float)row_s);
   if (threadIdx.x == 0) {
-    if (p.entropy) p.entropy[row] = log_s - (float)(mass.t / mass.s);
+    if (p.entropy) p.entropy[row] = log_s - (float)row_t / (float)row_s;
     if (p.tokens) {
       const int token = p.tokens[row];
-      if (token >= 0 && token < p.vocab) p.logprob[row] = (float)x[token] - mass.m - log_s;
+      if (token >= 0 && token < p.vocab) p.logprob[row] = (float)x[token] - row_m - log_s;
     }
   }
   if ((int)threadIdx.x < top) {
     const long long key = s_best[threadIdx.x];
     const size_t to = (size_t)row * top + threadIdx.x;
     p.top_tokens[to] = key == kNoKey ? -1 : key_index(key);
-    p.top_logprobs[to] = key == kNoKey ? -INFINITY : key_value(key) - mass.m - log_s;
+    p.top_logprobs[to] = key == kNoKey ? -INFINITY : key_value(key) - row_m - log_s;
   }
 }
 
-// Elements a lane holds: 8 where the rows are too few to fill the chip, else 32.
-int each_of(int64_t rows, int64_t vocabulary) {
-  return rows * ((vocabulary + 32 * kLpThreads - 1) / (32 * kLpThreads)) < 512 ? 8 : 32;
-}
-int64_t parts_of(int64_t rows, int64_t vocabulary) {
-  const int64_t span = (int64_t)kLpThreads * each_of(rows, vocabulary);
-  return (vocabulary + span - 1) / span;
+// How a row is shared out: elements a lane holds, parts a block, blocks a row.
+// Rows in the hundreds take a block each; fewer are cut until there are kFill
+// blocks or parts run out, the fewest rows into small parts.  MI355X, fp32:
+// 2048 rows of 32003, 5 alternatives 64 us with 16 elements a lane, 92 with 32
+// (two waves a SIMD), 71 with 8; without alternatives 51.5 (5.1 TB/s).  16 rows
+// of 32000, 20 alternatives 12.6 us from 16 blocks of 8 elements a row; 64 rows
+// of 32003 11.9 us from 8 blocks a row, 16.8 from 2.  The few rows are bound by
+// the latency of the steps: logits, bound, ranks, arrival, join.
+constexpr int64_t kFill = 512;
+struct LogprobPlan {
+  int each, walk, count;
+};
+LogprobPlan logprob_plan(int64_t rows, int64_t vocabulary) {
+  LogprobPlan plan{16, 1, 1};
+  if (rows * ((vocabulary + 16 * kLpThreads - 1) / (16 * kLpThreads)) < kFill) plan.each = 8;
+  const int64_t span = (int64_t)kLpThreads * plan.each, parts = (vocabulary + span - 1) / span;
+  const int64_t blocks = std::min(parts, std::max<int64_t>(1, (kFill + rows - 1) / rows));
+  plan.walk = (int)((parts + blocks - 1) / blocks);
+  plan.count = (int)((parts + plan.walk - 1) / plan.walk);
+  return plan;
 }
 bool logprob_shape(int64_t rows, int64_t vocabulary, int64_t top) {
   return rows > 0 && rows < (1LL << 24) && vocabulary > 0 && vocabulary < (1LL << 28) && top >= 0 &&
-         top <= kTopMax && top <= vocabulary && rows * parts_of(rows, vocabulary) < (1LL << 31);
+         top <= kTopMax && top <= vocabulary;
 }
 size_t logprob_counter_bytes(int64_t rows) {
   return std::max(kLpCounterBytes, (size_t)(rows * 4 + 255) / 256 * 256);
@@ -371,7 +436,7 @@ using namespace tmc;
 
 extern "C" size_t tmc_logprobs_workspace_bytes(int64_t rows, int64_t vocabulary, int64_t top) {
   if (!logprob_shape(rows, vocabulary, top)) return 0;
-  const int64_t parts = parts_of(rows, vocabulary);
+  const int64_t parts = logprob_plan(rows, vocabulary).count;
   return parts == 1 ? 0 : logprob_counter_bytes(rows) + (size_t)(rows * parts) * (20 + 8 * top);
 }
 
@@ -388,7 +453,6 @@ extern "C" int tmc_logprobs(const void* logits, int dtype, int64_t row_stride,
               "Log probabilities: invalid shape.");
   TMC_REQUIRE(top >= 0 && top <= kTopMax && top <= vocabulary,
               "Log probabilities: top must be in [0, 64] and within the vocabulary.");
-  TMC_REQUIRE(logprob_shape(rows, vocabulary, top), "Log probabilities: invalid shape.");
   TMC_REQUIRE(!tokens == !logprob, "Log probabilities: tokens and logprob go together.");
   TMC_REQUIRE(!top || (top_tokens && top_logprobs),
               "Log probabilities: null pointer for the alternatives.");
@@ -409,7 +473,9 @@ extern "C" int tmc_logprobs(const void* logits, int dtype, int64_t row_stride,
   p.rows = (int)rows;
   p.vocab = (int)vocabulary;
   p.top = (int)top;
-  p.count = (int)parts_of(rows, vocabulary);
+  const LogprobPlan plan = logprob_plan(rows, vocabulary);
+  p.walk = plan.walk;
+  p.count = plan.count;
   if (need) {
     p.arrivals = static_cast<int*>(workspace);
     p.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + logprob_counter_bytes(rows));
@@ -418,11 +484,11 @@ extern "C" int tmc_logprobs(const void* logits, int dtype, int64_t row_stride,
   const hipStream_t s = as_stream(stream);
 #define TMC_LP(TYPE, EACH) \
   hipLaunchKernelGGL((logprobs_kernel<TYPE, EACH>), grid, dim3(kLpThreads), 0, s, p)
-  const bool few = each_of(rows, vocabulary) == 8;
+  const bool few = plan.each == 8;
   if (dtype == TMC_F32) {
-    if (few) TMC_LP(float, 8); else TMC_LP(float, 32);
+    if (few) TMC_LP(float, 8); else TMC_LP(float, 16);
   } else {
-    if (few) TMC_LP(half_t, 8); else TMC_LP(half_t, 32);
+    if (few) TMC_LP(half_t, 8); else TMC_LP(half_t, 16);
   }
 #undef TMC_LP
   return check_launch("logprobs_kernel");

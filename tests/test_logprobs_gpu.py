@@ -97,6 +97,16 @@ def test_ties_orders_and_masks(tmc, torch, vocab, kind):
         check(torch, logits, tokens, top, run(tmc, torch, logits, tokens, top))
 
 
+def test_best_tokens_all_in_the_last_parts(tmc, torch):
+    """A long rising row: the parts at its end hold far more good candidates
+    than the join ranks at once."""
+    vocab = 1000003
+    logits = (torch.arange(vocab, device="cuda") * (60.0 / vocab))[None]
+    tokens = torch.tensor([vocab - 1], dtype=torch.int32, device="cuda")
+    for top in (5, 64):
+        check(torch, logits, tokens, top, run(tmc, torch, logits, tokens, top))
+
+
 def test_rows_without_a_distribution(tmc, torch):
     """NaN, +inf and empty rows: NaN log probabilities, the tokens still in the
     greedy order, and their neighbours untouched by it."""
