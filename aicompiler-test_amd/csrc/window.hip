@@ -27,7 +27,9 @@ struct WindowParams {
   const int32_t* active;     // may be null: all rows
   long page_stride, head_stride;
   int pool_pages, rows, table_rows, q_heads, kv_heads, group, dim;
-  int page_size, max_pages, page_shift;
+  int page_size, max_pages;
+  unsigned page_magic;   // pos / page_size = (pos * magic >> 32) >> shift for pos < 2^31;
+  int page_shift;        // magic 0: page_size 1
   int window, sinks;
   int own_table;         // row r reads table row r
   long out_pass;         // > 0: packed activation order, elements per 16-row pass
@@ -35,7 +37,8 @@ struct WindowParams {
 };
 
 __device__ __forceinline__ int window_page(const WindowParams& p, int pos) {
-  return p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
+  const int q = (int)(__umulhi((unsigned)pos, p.page_magic) >> p.page_shift);
+  return p.page_magic ? q : pos;
 }
 __device__ __forceinline__ bool window_page_ok(const WindowParams& p, int page) {
   return page >= 0 && page < p.pool_pages;
@@ -62,27 +65,29 @@ __device__ __forceinline__ size_t window_out(const WindowParams& p, int row, int
 // dims for P V.  Online softmax in fp32.
 constexpr int kPlainMaxDim = 256;
 
-__global__ __launch_bounds__(kWave) void window_plain_kernel(WindowParams p) {
-  __shared__ __align__(16) half_t s_q[kPlainMaxDim];
-  __shared__ float s_p[kWave];
-  __shared__ long s_at[kWave];
-  const int lane = threadIdx.x, row = blockIdx.x, head = blockIdx.y;
-  if (row >= (p.active ? min(p.active[0], p.rows) : p.rows)) return;
-  const int valid = p.valid[row], table_row = window_table(p, row);
-  if (valid < 1 || valid > p.page_size * p.max_pages || table_row < 0) return;
-  const int32_t* table = p.tables + (size_t)table_row * p.max_pages;
+struct PlainScratch {  // of one wave
+  __align__(16) half_t q[kPlainMaxDim];
+  float weight[kWave];
+  long at[kWave];
+};
+
+// One (row, query head), whose length and table row are valid.
+__device__ __noinline__ void plain_row(WindowParams p, int row, int head, PlainScratch& scratch) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const int valid = p.valid[row];
+  const int32_t* table = p.tables + (size_t)window_table(p, row) * p.max_pages;
   const int kvh = head / p.group, d = p.dim;
   const half_t* q = p.q + ((size_t)row * p.q_heads + head) * d;
-  for (int i = lane; i < d; i += kWave) s_q[i] = q[i];
+  for (int i = lane; i < d; i += kWave) scratch.q[i] = q[i];
   const int begin = window_begin(p, valid), first = min(p.sinks, begin);
   const int count = first + valid - begin;
   float m = -INFINITY, sum = 0.0f, o[kPlainMaxDim / kWave] = {};
   bool bad = false;
-  __syncthreads();
   for (int u0 = 0; u0 < count; u0 += kWave) {
     const int u = u0 + lane, pos = u < first ? u : begin + u - first;
     float score = -INFINITY;
     long at = -1;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     if (u < count) {
       const int slot = window_page(p, pos), page = table[slot];
       if (window_page_ok(p, page)) {
@@ -90,7 +95,7 @@ __global__ __launch_bounds__(kWave) void window_plain_kernel(WindowParams p) {
              (long)(pos - slot * p.page_size) * d;
         float dot = 0.0f;
         for (int c = 0; c < d; c += 8)
-          dot = dot8(load_h8(s_q + c), load_h8(p.k + at + c), dot);
+          dot = dot8(load_h8(scratch.q + c), load_h8(p.k + at + c), dot);
         score = dot * p.scale_log2;
       } else {
         bad = true;
@@ -101,21 +106,20 @@ __global__ __launch_bounds__(kWave) void window_plain_kernel(WindowParams p) {
     const float w = score == -INFINITY ? 0.0f : fast_exp2(score - next);
     m = next;
     sum = sum * alpha + w;
-    s_p[lane] = w;
-    s_at[lane] = at;
-    __syncthreads();
+    scratch.weight[lane] = w;
+    scratch.at[lane] = at;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
     for (int t = 0; t < kPlainMaxDim / kWave; ++t) o[t] *= alpha;
     const int live = min(kWave, count - u0);
     for (int i = 0; i < live; ++i) {
-      const long from = s_at[i];
-      const float wi = s_p[i];
+      const long from = scratch.at[i];
+      const float wi = scratch.weight[i];
       if (from < 0) continue;
 #pragma unroll
       for (int t = 0; t < kPlainMaxDim / kWave; ++t)
         if (lane + t * kWave < d) o[t] += wi * (float)p.v[from + lane + t * kWave];
     }
-    __syncthreads();
   }
   if (__any(bad)) return;
   sum = cross_sum<1>(sum);
@@ -123,6 +127,15 @@ __global__ __launch_bounds__(kWave) void window_plain_kernel(WindowParams p) {
   for (int t = 0; t < kPlainMaxDim / kWave; ++t)
     if (lane + t * kWave < d)
       p.out[window_out(p, row, head * d + lane + t * kWave)] = (half_t)(o[t] / sum);
+}
+
+__global__ __launch_bounds__(kWave) void window_plain_kernel(WindowParams p) {
+  __shared__ PlainScratch scratch;
+  const int row = blockIdx.x, head = blockIdx.y;
+  if (row >= (p.active ? min(p.active[0], p.rows) : p.rows)) return;
+  const int valid = p.valid[row];
+  if (valid < 1 || valid > p.page_size * p.max_pages || window_table(p, row) < 0) return;
+  plain_row(p, row, head, scratch);
 }
 
 // ------------------------------------------------------------ one token a request
@@ -605,6 +618,11 @@ constexpr int kChunkWaves = 8;
 // 2^(kChunkRaise + kLag) in fp16 and keep 11 bits down to 2^-24 of that scale.
 constexpr float kLag = 5.0f, kChunkRaise = 10.0f;
 
+__device__ __forceinline__ unsigned opaque(unsigned v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
 template <int D, int PG>
 __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(WindowParams p,
                                                                               int tiles,
@@ -616,7 +634,7 @@ __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(Wi
   constexpr int RPL = kWave / CH, LOADS = OWN / RPL;  // rows a load, loads of K (of V)
   constexpr int STAGE = 2 * SPAN * D;                 // halves: K rows, V rows
   static_assert(LOADS >= 1 && 2 * STAGE >= WAVES * 32 * D, "results fit the stages");
-  __shared__ __align__(16) half_t s_kv[2 * STAGE];
+  __shared__ __align__(256) half_t s_kv[2 * STAGE];
   __shared__ int s_run, s_low, s_high;
   __shared__ float s_max[WAVES][32], s_sum[WAVES][32];
 
@@ -765,33 +783,40 @@ __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(Wi
 
     // ---- one step of 32 positions: rows R0 ... of a stage, u0 ... of the tile.
     // V's operands are read before the weights are computed (the fences keep
-    // the reads there), into the registers that K's have left.
+    // the reads there), into the registers that K's have left.  Rows start at
+    // multiples of 128 bytes, so the swizzled chunk is an exclusive or on the
+    // address; the addresses are rebuilt in every step (opaque()), not kept in
+    // registers that the step has no room for.
     typedef __fp16 v4fp16 __attribute__((__vector_size__(8)));
     typedef __attribute__((address_space(3))) v4fp16 lds_v4;
-    typedef const __attribute__((address_space(3))) char lds_char;
+    typedef const __attribute__((address_space(3))) h8 lds_h8;
     h8 k[KS], va[2][DT];
-    auto read_keys = [&](const half_t* buf, int R0) {
-      const half_t* sk = buf + (R0 + col) * D;
+    const unsigned key_at =
+        lds_address(s_kv) +
+        (unsigned)(col * D * 2 + ((half ^ (D == 128 ? col & 15 : (col >> 1) & 7)) << 4));
+    const int value_row = 4 * half + ((lane & 15) >> 2);
+    const unsigned value_at =
+        lds_address(s_kv) +
+        (unsigned)((SPAN + value_row) * D * 2 +
+                   ((((lane >> 4) & 1) ^ (D == 128 ? value_row & 7 : (value_row >> 1) & 3)) << 5) +
+                   ((lane & 3) << 3));
+    auto read_keys = [&](unsigned buf, int R0) {
+      const unsigned at = opaque(key_at) + buf + (unsigned)(R0 * D * 2);
 #pragma unroll
-      for (int s = 0; s < KS; ++s)
-        k[s] = *reinterpret_cast<const h8*>(
-            sk + 8 * ((2 * s + half) ^ (D == 128 ? col & 15 : (col >> 1) & 7)));
+      for (int s = 0; s < KS; ++s) k[s] = *(lds_h8*)(uintptr_t)(at ^ (unsigned)(s << 5));
     };
-    auto read_values = [&](const half_t* buf, int R0) {
-      lds_char* sv = (lds_char*)(buf + SPAN * D);
+    auto read_values = [&](unsigned buf, int R0) {
+      const unsigned at = opaque(value_at) + buf + (unsigned)(R0 * D * 2);
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
           h4 part[2];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int R = R0 + 16 * c + 8 * h + 4 * half + ((lane & 15) >> 2);
-            const int unit = (2 * t + ((lane >> 4) & 1)) ^ (D == 128 ? R & 7 : (R >> 1) & 3);
+          for (int h = 0; h < 2; ++h)
             part[h] = __builtin_bit_cast(
-                h4, __builtin_amdgcn_ds_read_tr16_b64_v4f16(
-                        (lds_v4*)(sv + R * D * 2 + 32 * unit + 8 * (lane & 3))));
-          }
+                h4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_v4*)(uintptr_t)(
+                        (at ^ (unsigned)(t << 6)) + (unsigned)((16 * c + 8 * h) * D * 2))));
           va[c][t] = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
         }
     };
@@ -816,9 +841,10 @@ __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(Wi
     auto weigh = [&](int u0) {
       const int p0 = position(u0), p1 = position(u0 + 31);
       if (p1 >= min_len || (p0 < max_from && p1 >= sinks)) {  // not all of it in sight
+        const int first = u0 + 4 * (int)opaque(half);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int pos = position(u0 + 8 * (e >> 2) + 4 * half + (e & 3));
+          const int pos = position(first + 8 * (e >> 2) + (e & 3));
           const int away = (pos >= len) | ((unsigned)(pos - p.sinks) < hidden);
           sc[e] = away ? -INFINITY : sc[e];
         }
@@ -858,7 +884,7 @@ __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(Wi
     store(s_kv);
     load_stage(1);
     for (int i = 0; i < stages; ++i) {
-      const half_t* buf = s_kv + (i & 1) * STAGE;
+      const unsigned buf = (unsigned)((i & 1) * STAGE * 2);
       // stage i is in LDS, stage i - 1 has been read
       lds_barrier();
       if (i + 1 < stages) store(s_kv + ((i + 1) & 1) * STAGE);
@@ -890,6 +916,7 @@ __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(Wi
       if (!whole) len = 0;
     }
     float scale = 1.0f / sum;
+    bool nan = false;  // in what this lane stored of its vector
     if constexpr (PG > 1) {
       if (half == 0) {
         s_max[wave][col] = m;
@@ -926,11 +953,17 @@ __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(Wi
           *reinterpret_cast<h4*>(p.out + ((size_t)row * p.q_heads + head) * D + 32 * t + 8 * pg +
                                  4 * half) =
               h4{(half_t)val[0], (half_t)val[1], (half_t)val[2], (half_t)val[3]};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) nan |= !(val[e] == val[e]);
       }
     } else {
       // rows through LDS (16-byte chunks swizzled by the row), so that whole
       // rows are stored: lane l then holds chunk l % CH of row l / CH
       half_t* rows = s_kv + wave * 32 * D;
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) nan |= !(o[t][e] == o[t][e]);
 #pragma unroll
       for (int t = 0; t < DT; ++t)
 #pragma unroll
@@ -948,7 +981,21 @@ __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(Wi
         if (to >= 0) *reinterpret_cast<h8*>(p.out + (size_t)to * D + 8 * chunk) = val;
       }
     }
-    __syncthreads();  // the next run clears s_run and loads the stages again
+    // A weight of 0 times an infinity or NaN of V that the vector does not see
+    // (another one of the tile does) is a NaN: such vectors are done again, one
+    // at a time and over their own positions alone.
+    if (__syncthreads_or(nan && len > 0)) {
+      unsigned long long again = __builtin_amdgcn_ballot_w64(nan && len > 0);
+      again = (again | again >> 32) & 0xFFFFFFFFull;
+      PlainScratch& scratch = reinterpret_cast<PlainScratch*>(s_kv)[wave];
+      static_assert(sizeof(PlainScratch) * WAVES <= sizeof(s_kv), "a scratch for every wave");
+      while (again) {
+        const int from_lane = __builtin_ctzll(again);
+        again &= again - 1;
+        plain_row(p, __shfl(row, from_lane, kWave), __shfl(head, from_lane, kWave), scratch);
+      }
+      __syncthreads();
+    }
   }
 }
 
@@ -994,9 +1041,14 @@ int window_params(WindowParams& p, const char* what, const void* q, const void* 
   p.dim = (int)head_dim;
   p.page_size = (int)page_size;
   p.max_pages = (int)max_pages;
-  p.page_shift = -1;
-  for (int b = 0; b < 30; ++b)
-    if (page_size == (int64_t)1 << b) p.page_shift = b;
+  if (page_size > 1) {
+    // magic = floor(2^(31 + s) / d) + 1 with d <= 2^s: magic d - 2^(31 + s) is
+    // in (0, 2^s], so the quotient is exact below 2^31
+    int s = 1;
+    while (((int64_t)1 << s) < page_size) ++s;
+    p.page_magic = (unsigned)(((uint64_t)1 << (31 + s)) / (uint64_t)page_size + 1);
+    p.page_shift = s - 1;
+  }
   const int64_t capacity = page_size * max_pages;
   p.window = (int)std::min(window, capacity);
   p.sinks = (int)std::min(sinks, capacity);

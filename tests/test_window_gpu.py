@@ -230,6 +230,27 @@ def test_pools_past_4_gib(tmc, torch, d, page):
         assert ((got.double().reshape(qh, d) - o).abs() <= tolerance).all()
 
 
+@pytest.mark.parametrize("d,batch,kvh", [(64, 300, 8), (128, 300, 8), (128, 2100, 1)])
+def test_decode_batches_of_many_rows(tmc, torch, d, batch, kvh):
+    """More (request, kv head) rows than the shared list takes."""
+    page, window, sinks, cap_pages = 16, 40, 4, 8
+    lengths = [1 + (37 * i) % 128 for i in range(batch)]
+    cache = Cache(torch, batch, [set(visible(n, window, sinks)) for n in lengths], kvh, d, page, cap_pages)
+    qh = 2 * kvh
+    q = torch.randn(batch, qh * d, device="cuda").to(torch.float16)
+    out = torch.full((batch, qh * d), 7.5, dtype=torch.float16, device="cuda")
+    assert tmc.window_attention_workspace_bytes(batch, qh, kvh, d, 128, window, sinks) == 0
+    valid = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    active = torch.tensor([batch - 1], dtype=torch.int32, device="cuda")
+    tmc.window_decode_attention(q, cache.k, cache.v, valid, cache.tables_dev, active, out, batch, qh,
+                                kvh, d, page, cap_pages, cache.page_stride, cache.head_stride,
+                                window, sinks)
+    picked = sorted({*range(0, batch, 13), batch - 2, batch - 1})
+    check_rows(torch, out[torch.tensor(picked, device="cuda")], cache,
+               q[torch.tensor(picked, device="cuda")],
+               [(r, lengths[r]) if r < batch - 1 else None for r in picked], qh, d, window, sinks, 7.5)
+
+
 def test_decode_packed_layout(tmc, torch):
     lengths, kvh, qh, d, page, window, sinks = [5, 100, 400, 77] * 5, 2, 8, 128, 16, 90, 4
     cache = Cache(torch, 13, [set(visible(n, window, sinks)) for n in lengths], kvh, d, page, 25)
@@ -274,6 +295,47 @@ def test_decode_infinite_values_stay(tmc, torch):
     assert ((got - o).abs() <= tolerance)[:, keep].all()
     for head in (0, 1, 3):
         assert got[head, 5] == math.inf
+
+
+@pytest.mark.parametrize("qh,kvh,d", [(4, 1, 128), (4, 1, 64), (200, 200, 64), (200, 200, 128)])
+def test_chunk_special_values_stay_with_those_that_see_them(tmc, torch, qh, kvh, d):
+    """An infinity in V and a NaN in K change the rows that see their positions
+    and no other row of the tile."""
+    rows, start, page, window, sinks = 70, 100, 16, 40, 4
+    valid = list(range(start + 1, start + rows + 1))
+    max_pages = -(-(start + rows) // page)
+    cache = Cache(torch, 19, [set().union(*(visible(n, window, sinks) for n in valid))], kvh, d,
+                  page, max_pages)
+    ids = cache.tables[0].tolist()
+    odd_v, odd_k = start + 20, start + 45
+    head = kvh - 1
+    cache.v.view(-1, kvh, page, d)[ids[odd_v // page], head, odd_v % page, 7] = math.inf
+    cache.k.view(-1, kvh, page, d)[ids[odd_k // page], head, odd_k % page, 9] = math.nan
+    q = torch.randn(rows, qh * d, device="cuda").to(torch.float16)
+    out = torch.full((rows, qh * d), 7.5, dtype=torch.float16, device="cuda")
+    tmc.window_prefill_attention(q, cache.k, cache.v,
+                                 torch.tensor(valid, dtype=torch.int32, device="cuda"),
+                                 cache.tables_dev, None,
+                                 torch.tensor([rows], dtype=torch.int32, device="cuda"), out, rows,
+                                 qh, kvh, d, page, max_pages, cache.page_stride, cache.head_stride,
+                                 window, sinks)
+    seen, kk, vv = cache.kv[0]
+    at = {p: i for i, p in enumerate(seen)}
+    group = qh // kvh
+    for r, n in enumerate(valid):
+        see = visible(n, window, sinks)
+        index = torch.tensor([at[p] for p in see], device="cuda")
+        o, tolerance = attend64(torch, q[r].reshape(qh, d), kk[index], vv[index])
+        got = out[r].double().reshape(qh, d)
+        near = (got - o).abs() <= tolerance
+        mine = torch.zeros_like(near)
+        if odd_k in see:
+            assert torch.isnan(got[head * group:]).all(), r
+            mine[head * group:] = True
+        elif odd_v in see:
+            assert (got[head * group:, 7] == math.inf).all(), r
+            mine[head * group:, 7] = True
+        assert (near | mine).all(), r
 
 
 CHUNK = [
