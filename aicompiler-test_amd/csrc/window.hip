@@ -247,12 +247,22 @@ __device__ __forceinline__ void read_values(const unsigned* at, h8* v) {
 constexpr float kRaiseLog = 15.0f;
 constexpr unsigned kNoUnit = 0xFFFFFFFFu;
 
-// Visible positions of a row, in steps.
-__device__ __forceinline__ int row_steps(const WindowParams& p, int row, int active) {
-  const int valid = p.valid[row];
-  if (row >= active || valid < 1 || valid > p.page_size * p.max_pages) return 0;
+// Visible positions of a row of length `valid`, in steps.
+__device__ __forceinline__ int steps_of(const WindowParams& p, int valid, bool active) {
+  if (!active || valid < 1 || valid > p.page_size * p.max_pages) return 0;
   const int begin = window_begin(p, valid);
   return (min(p.sinks, begin) + valid - begin + kStep - 1) / kStep;
+}
+
+// Inclusive sums over the lanes, inside registers.
+__device__ __forceinline__ int scan_lanes(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast 15 to rows 1, 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast 31 to rows 2, 3
+  return v;
 }
 
 template <int D, int STAGES>
@@ -264,7 +274,7 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void window_decode_kernel(Win
   constexpr int THREADS = kDecodeWaves * kWave;
   __shared__ __align__(16) half_t s_ring[kDecodeWaves * STAGES * STAGE];
   __shared__ int s_pages[kDecodeWaves * STAGES * kWave];
-  __shared__ int s_start[kDecodeMaxRows + 1];
+  __shared__ int s_start[kDecodeMaxRows];
   __shared__ int s_wave[kDecodeWaves];
   __shared__ int s_last;
   typedef __attribute__((address_space(3))) void lds_void;
@@ -278,50 +288,63 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void window_decode_kernel(Win
   const int active = p.active ? min(p.active[0], p.rows) : p.rows;
 
   // ---- this block's part [at, stop) of the list
+  // Where each row's steps start: up to 64 rows in the lanes of every wave (no
+  // LDS, no barrier), more of them in s_start.
+  const bool in_lanes = p.rows <= kWave;
   int row = 0, at = 0, stop = 0, per = 0, kvh = 0;
+  int lane_start = 0, lane_valid = 0, total = 0;
+  auto start_of = [&](int r) {
+    return r >= p.rows ? total : in_lanes ? __builtin_amdgcn_readlane(lane_start, r) : s_start[r];
+  };
   if (plan.blocks == 0) {
     row = blockIdx.x / p.kv_heads;
     kvh = blockIdx.x % p.kv_heads;
-    stop = row_steps(p, row, active);
+    stop = steps_of(p, p.valid[row], row < active);
   } else {
-    // exclusive sums of the rows' steps
-    const int each = (p.rows + THREADS - 1) / THREADS;
-    const int from = threadIdx.x * each, to = min(p.rows, from + each);
-    int sum = 0;
-    for (int r = from; r < to; ++r) sum += row_steps(p, r, active);
-    int scan = sum;
+    if (in_lanes) {
+      lane_valid = p.valid[min(lane, p.rows - 1)];
+      const int mine = steps_of(p, lane_valid, lane < p.rows && lane < active);
+      const int upto = scan_lanes(mine);
+      lane_start = upto - mine;
+      total = __builtin_amdgcn_readlane(upto, kWave - 1);
+    } else {
+      const int each = (p.rows + THREADS - 1) / THREADS;
+      const int from = threadIdx.x * each, to = min(p.rows, from + each);
+      int sum = 0;
+      for (int r = from; r < to; ++r) sum += steps_of(p, p.valid[r], r < active);
+      const int scan = scan_lanes(sum);
+      if (lane == kWave - 1) s_wave[wave] = scan;
+      __syncthreads();
+      int before = 0;
 #pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) {
-      const int below = __shfl_up(scan, off, kWave);
-      if (lane >= off) scan += below;
+      for (int w = 0; w < kDecodeWaves; ++w) {
+        if (w < wave) before += s_wave[w];
+        total += s_wave[w];
+      }
+      before += scan - sum;
+      for (int r = from; r < to; ++r) {
+        s_start[r] = before;
+        if (r + 1 < to) before += steps_of(p, p.valid[r], r < active);
+      }
+      __syncthreads();
     }
-    if (lane == kWave - 1) s_wave[wave] = scan;
-    __syncthreads();
-    int total = 0, before = 0;
-#pragma unroll
-    for (int w = 0; w < kDecodeWaves; ++w) {
-      if (w < wave) before += s_wave[w];
-      total += s_wave[w];
-    }
-    before += scan - sum;
-    for (int r = from; r < to; ++r) {
-      s_start[r] = before;
-      if (r + 1 < to) before += row_steps(p, r, active);
-    }
-    if (threadIdx.x == 0) s_start[p.rows] = total;
-    __syncthreads();
     const int steps = total * p.kv_heads;
     per = max(plan.least, (steps + plan.blocks - 1) / plan.blocks);
     at = min(steps, (int)blockIdx.x * per);
     stop = min(steps, at + per);
     if (at >= stop) return;
     // the row of the first step: the last one that starts at or before it
-    int low = 0, high = p.rows;
-    while (high - low > 1) {
-      const int mid = (low + high) / 2;
-      if (s_start[mid] * p.kv_heads <= at) low = mid; else high = mid;
+    if (in_lanes) {
+      row = __builtin_popcountll(
+                __builtin_amdgcn_ballot_w64(lane < p.rows && lane_start * p.kv_heads <= at)) - 1;
+    } else {
+      int low = 0, high = p.rows;
+      while (high - low > 1) {
+        const int mid = (low + high) / 2;
+        if (s_start[mid] * p.kv_heads <= at) low = mid; else high = mid;
+      }
+      row = low;
     }
-    row = low;
   }
   const int block_at = at;
 
@@ -348,13 +371,16 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void window_decode_kernel(Win
       steps = stop;
       unit_at = 0;
     } else {
-      while (s_start[row + 1] * p.kv_heads <= at) ++row;
-      steps = s_start[row + 1] - s_start[row];
-      kvh = (at - s_start[row] * p.kv_heads) / steps;
-      unit_at = s_start[row] * p.kv_heads + kvh * steps;
+      while (start_of(row + 1) * p.kv_heads <= at) ++row;
+      const int start = start_of(row);
+      steps = start_of(row + 1) - start;
+      kvh = (at - start * p.kv_heads) / steps;
+      unit_at = start * p.kv_heads + kvh * steps;
     }
     const int first_step = at - unit_at, last_step = min(stop - unit_at, steps);
-    const int valid = p.valid[row], begin = window_begin(p, valid), sinks = min(p.sinks, begin);
+    const int valid = plan.blocks != 0 && in_lanes ? __builtin_amdgcn_readlane(lane_valid, row)
+                                                   : p.valid[row];
+    const int begin = window_begin(p, valid), sinks = min(p.sinks, begin);
     const int count = sinks + valid - begin;
     const int32_t* table = p.tables + (size_t)row * p.max_pages;
     const unsigned head_unit = (unsigned)((size_t)kvh * p.head_stride / 8);
@@ -568,18 +594,35 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void window_decode_kernel(Win
           const int head = i / D, d = i % D;
           float top = -INFINITY, sum = 0.0f, val = 0.0f;
           bool spoiled = false;
-          for (int b = from; b <= to; ++b) {
-            const int which = 2 * b + (b == from && unit_at != b * per ? 1 : 0);
-            const float* in = plan.slots + ((size_t)which * p.group + head) * (D + 2);
-            const float x = __hip_atomic_load(in + d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            const float hi = __hip_atomic_load(in + D, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            const float s = __hip_atomic_load(in + D + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            spoiled |= s < 0.0f;
-            const float next = fmaxf(top, hi);
+          constexpr int kAhead = 8;  // partials loaded at once
+          for (int b = from; b <= to; b += kAhead) {
+            float x[kAhead], hi[kAhead], s[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+              const int which = min(b + u, to);
+              const int place = 2 * which + (which == from && unit_at != which * per ? 1 : 0);
+              const float* in = plan.slots + ((size_t)place * p.group + head) * (D + 2);
+              x[u] = __hip_atomic_load(in + d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+              hi[u] = __hip_atomic_load(in + D, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+              s[u] = __hip_atomic_load(in + D + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            float next = top;
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+              if (b + u <= to) {
+                spoiled |= s[u] < 0.0f;
+                next = fmaxf(next, hi[u]);
+              }
             const float a = top == -INFINITY ? 0.0f : fast_exp2(top - next);
-            const float c = hi == -INFINITY ? 0.0f : fast_exp2(hi - next);
-            sum = sum * a + s * c;
-            val = val * a + x * c;
+            sum *= a;
+            val *= a;
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+              if (b + u <= to) {
+                const float c = hi[u] == -INFINITY ? 0.0f : fast_exp2(hi[u] - next);
+                sum += s[u] * c;
+                val += x[u] * c;
+              }
             top = next;
           }
           if (!spoiled)
