@@ -139,12 +139,11 @@ __global__ __launch_bounds__(kWave) void window_plain_kernel(WindowParams p) {
 }
 
 // ------------------------------------------------------------ one token a request
-// D = 64 and 128, groups up to 16.  A step is 32 visible positions of one
-// (request, kv head) row.  The steps of all rows form one list, row after row,
-// that the blocks share out evenly whatever the lengths are (each block finds
-// its part from the lengths alone); a row cut by a block border is joined from
-// partials (max, sum, weighted) in the workspace by the last of its blocks to
-// arrive, in block order.
+// D = 64 and 128.  A step is 32 (D = 64) or 16 visible positions
+// of one (request, kv head) row.  A row is a block's, or, where rows are few,
+// shared by up to `parts` blocks in even shares of at least kDecodeLeast steps;
+// each writes a partial (max, sum, weighted) to the workspace and the last one
+// to arrive joins them, in block order.
 //
 // Inside a block the waves take the steps of a part in turn.  Each wave has a
 // ring of kStages steps in LDS that only it touches, filled by 16-byte loads
@@ -155,20 +154,26 @@ __global__ __launch_bounds__(kWave) void window_plain_kernel(WindowParams p) {
 // does not exist reads a zero row.  Scores S^T = K Q^T (16 positions x 16
 // heads) leave lane (head j, group g) with positions 4g .. 4g+3, the order in
 // which O^T = V^T P^T wants its weights; V^T comes from transposing LDS reads.
-constexpr int kStep = 32;
 constexpr int kDecodeWaves = 4;
-constexpr int kDecodeBlocks = 256;  // one a CU
-constexpr int kDecodeMaxRows = 2048;  // rows whose lengths a block scans
-constexpr size_t kWindowCounterBytes = 64u << 10;
+constexpr int kDecodeBlocks = 512;  // two a CU
+constexpr int kDecodeLeast = 8;
+constexpr size_t kDecodeCounterBytes = kDecodeBlocks * sizeof(int);  // shared rows are fewer
 
 struct DecodePlan {
-  float* slots;    // [blocks][2][group][D + 2]
-  int* arrivals;   // [rows][kv_heads]
-  int blocks;      // blocks of the shared list; 0: one block per (row, kv head)
-  int least;       // steps a block takes at least
+  float* slots;   // [rows][kv_heads][splits][parts][heads][D + 2]
+  int* arrivals;  // [rows][kv_heads][splits]
+  int parts, splits, heads;
 };
 
 static __device__ __align__(16) unsigned s_zero_row[4];  // what absent positions read
+
+// A matrix product's result may be read by vector instructions only some wait
+// states later.  The compiler puts them in within a block of code, but hipcc
+// 7.2 left them out where a branch follows the product: the scores' maximum
+// was then taken of old registers.
+template <typename T> __device__ __forceinline__ void settle(T& result) {
+  asm volatile("s_nop 15" : "+v"(result));
+}
 
 template <int N> __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
@@ -192,21 +197,19 @@ __device__ __forceinline__ float max_of_groups(float v) {
 
 // The operands of one step out of LDS, waits included: the compiler would let
 // such reads wait for every load to LDS in flight.
-template <int D, int OFFSET, int PAGE_OFFSET>
+template <int D, int STEP, int OFFSET, int PAGE_OFFSET>
 __device__ __forceinline__ void read_keys(const unsigned (&at)[D / 32], unsigned page_at,
-                                          h8 (&k)[2][D / 32], int& page) {
+                                          h8 (&k)[STEP / 16][D / 32], int& page) {
+  static_assert((D == 128 && STEP == 16) || (D == 64 && STEP == 32), "four operands a step");
   if constexpr (D == 128) {
     asm volatile(
-        "ds_read_b32 %8, %13 offset:%16\n\t"
-        "ds_read_b128 %0, %9 offset:%14\n\tds_read_b128 %1, %10 offset:%14\n\t"
-        "ds_read_b128 %2, %11 offset:%14\n\tds_read_b128 %3, %12 offset:%14\n\t"
-        "ds_read_b128 %4, %9 offset:%15\n\tds_read_b128 %5, %10 offset:%15\n\t"
-        "ds_read_b128 %6, %11 offset:%15\n\tds_read_b128 %7, %12 offset:%15\n\t"
+        "ds_read_b32 %4, %9 offset:%11\n\t"
+        "ds_read_b128 %0, %5 offset:%10\n\tds_read_b128 %1, %6 offset:%10\n\t"
+        "ds_read_b128 %2, %7 offset:%10\n\tds_read_b128 %3, %8 offset:%10\n\t"
         "s_waitcnt lgkmcnt(0)"
-        : "=&v"(k[0][0]), "=&v"(k[0][1]), "=&v"(k[0][2]), "=&v"(k[0][3]), "=&v"(k[1][0]),
-          "=&v"(k[1][1]), "=&v"(k[1][2]), "=&v"(k[1][3]), "=&v"(page)
+        : "=&v"(k[0][0]), "=&v"(k[0][1]), "=&v"(k[0][2]), "=&v"(k[0][3]), "=&v"(page)
         : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "v"(page_at), "n"(OFFSET),
-          "n"(OFFSET + 32 * D), "n"(PAGE_OFFSET)
+          "n"(PAGE_OFFSET)
         : "memory");
   } else {
     asm volatile(
@@ -221,24 +224,34 @@ __device__ __forceinline__ void read_keys(const unsigned (&at)[D / 32], unsigned
   }
 }
 
-// V^T of dims 16 t + j, t = T .. T + 3: slots 0 .. 3 hold positions 4g .. 4g+3,
-// slots 4 .. 7 positions 16 + 4g ...
-template <int D, int OFFSET>
-__device__ __forceinline__ void read_values(const unsigned* at, h8* v) {
-  h4 a0, a1, a2, a3, b0, b1, b2, b3;
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %9 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %2, %10 offset:%12\n\tds_read_b64_tr_b16 %3, %11 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %4, %8 offset:%13\n\tds_read_b64_tr_b16 %5, %9 offset:%13\n\t"
-      "ds_read_b64_tr_b16 %6, %10 offset:%13\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(a0), "=&v"(a1), "=&v"(a2), "=&v"(a3), "=&v"(b0), "=&v"(b1), "=&v"(b2), "=&v"(b3)
-      : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(OFFSET), "n"(OFFSET + 32 * D)
-      : "memory");
-  v[0] = __builtin_shufflevector(a0, b0, 0, 1, 2, 3, 4, 5, 6, 7);
-  v[1] = __builtin_shufflevector(a1, b1, 0, 1, 2, 3, 4, 5, 6, 7);
-  v[2] = __builtin_shufflevector(a2, b2, 0, 1, 2, 3, 4, 5, 6, 7);
-  v[3] = __builtin_shufflevector(a3, b3, 0, 1, 2, 3, 4, 5, 6, 7);
+// V^T, lane (j, g): dims 16 t + j, positions 4g .. 4g+3 of the step's first 16
+// (v[0]) and, D = 64, of its last 16 (v[1]).
+template <int D, int STEP, int OFFSET>
+__device__ __forceinline__ void read_values(const unsigned (&at)[D / 16], h4 (&v)[STEP / 16][D / 16]) {
+  if constexpr (D == 128) {
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8 offset:%16\n\tds_read_b64_tr_b16 %1, %9 offset:%16\n\t"
+        "ds_read_b64_tr_b16 %2, %10 offset:%16\n\tds_read_b64_tr_b16 %3, %11 offset:%16\n\t"
+        "ds_read_b64_tr_b16 %4, %12 offset:%16\n\tds_read_b64_tr_b16 %5, %13 offset:%16\n\t"
+        "ds_read_b64_tr_b16 %6, %14 offset:%16\n\tds_read_b64_tr_b16 %7, %15 offset:%16\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[0][2]), "=&v"(v[0][3]), "=&v"(v[0][4]),
+          "=&v"(v[0][5]), "=&v"(v[0][6]), "=&v"(v[0][7])
+        : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "v"(at[4]), "v"(at[5]), "v"(at[6]),
+          "v"(at[7]), "n"(OFFSET)
+        : "memory");
+  } else {
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %9 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %2, %10 offset:%12\n\tds_read_b64_tr_b16 %3, %11 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %4, %8 offset:%13\n\tds_read_b64_tr_b16 %5, %9 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %6, %10 offset:%13\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[0][2]), "=&v"(v[0][3]), "=&v"(v[1][0]),
+          "=&v"(v[1][1]), "=&v"(v[1][2]), "=&v"(v[1][3])
+        : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(OFFSET), "n"(OFFSET + 32 * D)
+        : "memory");
+  }
 }
 
 // Weights are stored 2^kRaiseLog times their value in fp16 (the greatest is
@@ -247,35 +260,39 @@ __device__ __forceinline__ void read_values(const unsigned* at, h8* v) {
 constexpr float kRaiseLog = 15.0f;
 constexpr unsigned kNoUnit = 0xFFFFFFFFu;
 
+// Two floats that other blocks read, and two of theirs: at agent scope.
+__device__ __forceinline__ void store_pair(float* to, float a, float b) {
+  const float2 v = {a, b};
+  __hip_atomic_store(reinterpret_cast<unsigned long long*>(to),
+                     __builtin_bit_cast(unsigned long long, v), __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 load_pair(const float* from) {
+  return __builtin_bit_cast(
+      float2, __hip_atomic_load(reinterpret_cast<const unsigned long long*>(from),
+                                __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+__device__ __forceinline__ void put_pair(const WindowParams& p, int row, int col, float a, float b) {
+  *reinterpret_cast<h2*>(p.out + window_out(p, row, col)) = h2{(half_t)a, (half_t)b};
+}
+
 // Visible positions of a row of length `valid`, in steps.
+template <int STEP>
 __device__ __forceinline__ int steps_of(const WindowParams& p, int valid, bool active) {
   if (!active || valid < 1 || valid > p.page_size * p.max_pages) return 0;
   const int begin = window_begin(p, valid);
-  return (min(p.sinks, begin) + valid - begin + kStep - 1) / kStep;
+  return (min(p.sinks, begin) + valid - begin + STEP - 1) / STEP;
 }
 
-// Inclusive sums over the lanes, inside registers.
-__device__ __forceinline__ int scan_lanes(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast 15 to rows 1, 3
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast 31 to rows 2, 3
-  return v;
-}
-
-template <int D, int STAGES>
-__global__ __launch_bounds__(kDecodeWaves * kWave) void window_decode_kernel(WindowParams p,
+template <int D, int STEP, int STAGES>
+__global__ __launch_bounds__(kDecodeWaves * kWave, 2) void window_decode_kernel(WindowParams p,
                                                                              DecodePlan plan) {
-  constexpr int KS = D / 32, DT = D / 16, CH = D / 8;
-  constexpr int RPL = kWave / CH, LOADS = kStep / RPL;  // rows a load, loads of K (of V) a step
-  constexpr int STAGE = 2 * kStep * D;                  // halves
+  constexpr int KS = D / 32, DT = D / 16, CH = D / 8, TILES = STEP / 16;
+  constexpr int RPL = kWave / CH, LOADS = STEP / RPL;  // rows a load, loads of K (of V) a step
+  constexpr int STAGE = 2 * STEP * D;                  // halves
   constexpr int THREADS = kDecodeWaves * kWave;
   __shared__ __align__(16) half_t s_ring[kDecodeWaves * STAGES * STAGE];
   __shared__ int s_pages[kDecodeWaves * STAGES * kWave];
-  __shared__ int s_start[kDecodeMaxRows];
-  __shared__ int s_wave[kDecodeWaves];
   __shared__ int s_last;
   typedef __attribute__((address_space(3))) void lds_void;
   typedef __attribute__((address_space(1))) const void global_void;
@@ -287,66 +304,19 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void window_decode_kernel(Win
   const int j = lane & 15, g = lane >> 4;
   const int active = p.active ? min(p.active[0], p.rows) : p.rows;
 
-  // ---- this block's part [at, stop) of the list
-  // Where each row's steps start: up to 64 rows in the lanes of every wave (no
-  // LDS, no barrier), more of them in s_start.
-  const bool in_lanes = p.rows <= kWave;
-  int row = 0, at = 0, stop = 0, per = 0, kvh = 0;
-  int lane_start = 0, lane_valid = 0, total = 0;
-  auto start_of = [&](int r) {
-    return r >= p.rows ? total : in_lanes ? __builtin_amdgcn_readlane(lane_start, r) : s_start[r];
-  };
-  if (plan.blocks == 0) {
-    row = blockIdx.x / p.kv_heads;
-    kvh = blockIdx.x % p.kv_heads;
-    stop = steps_of(p, p.valid[row], row < active);
-  } else {
-    if (in_lanes) {
-      lane_valid = p.valid[min(lane, p.rows - 1)];
-      const int mine = steps_of(p, lane_valid, lane < p.rows && lane < active);
-      const int upto = scan_lanes(mine);
-      lane_start = upto - mine;
-      total = __builtin_amdgcn_readlane(upto, kWave - 1);
-    } else {
-      const int each = (p.rows + THREADS - 1) / THREADS;
-      const int from = threadIdx.x * each, to = min(p.rows, from + each);
-      int sum = 0;
-      for (int r = from; r < to; ++r) sum += steps_of(p, p.valid[r], r < active);
-      const int scan = scan_lanes(sum);
-      if (lane == kWave - 1) s_wave[wave] = scan;
-      __syncthreads();
-      int before = 0;
-#pragma unroll
-      for (int w = 0; w < kDecodeWaves; ++w) {
-        if (w < wave) before += s_wave[w];
-        total += s_wave[w];
-      }
-      before += scan - sum;
-      for (int r = from; r < to; ++r) {
-        s_start[r] = before;
-        if (r + 1 < to) before += steps_of(p, p.valid[r], r < active);
-      }
-      __syncthreads();
-    }
-    const int steps = total * p.kv_heads;
-    per = max(plan.least, (steps + plan.blocks - 1) / plan.blocks);
-    at = min(steps, (int)blockIdx.x * per);
-    stop = min(steps, at + per);
-    if (at >= stop) return;
-    // the row of the first step: the last one that starts at or before it
-    if (in_lanes) {
-      row = __builtin_popcountll(
-                __builtin_amdgcn_ballot_w64(lane < p.rows && lane_start * p.kv_heads <= at)) - 1;
-    } else {
-      int low = 0, high = p.rows;
-      while (high - low > 1) {
-        const int mid = (low + high) / 2;
-        if (s_start[mid] * p.kv_heads <= at) low = mid; else high = mid;
-      }
-      row = low;
-    }
-  }
-  const int block_at = at;
+  // ---- this block's steps [first_step, last_step) of its row
+  const int unit = blockIdx.x / plan.parts, part = blockIdx.x - unit * plan.parts;
+  const int pair = unit / plan.splits, split = unit - pair * plan.splits;
+  const int row = pair / p.kv_heads, kvh = pair - row * p.kv_heads;
+  const int first_head = kvh * p.group + split * plan.heads;
+  const int heads = min(plan.heads, p.group - split * plan.heads);
+  const int valid = p.valid[row];
+  const int steps = steps_of<STEP>(p, valid, row < active);
+  const int shares = min(plan.parts, (steps + kDecodeLeast - 1) / kDecodeLeast);
+  if (part >= shares) return;
+  const int even = steps / shares, over = steps - even * shares;
+  const int first_step = part * even + min(part, over);
+  const int last_step = first_step + even + (part < over);
 
   // ---- LDS places: loads are linear (lane l: row l / CH, slot l % CH)
   half_t* ring = s_ring + wave * STAGES * STAGE;
@@ -358,280 +328,267 @@ __global__ __launch_bounds__(kDecodeWaves * kWave) void window_decode_kernel(Win
 #pragma unroll
   for (int t = 0; t < DT; ++t) {
     const int R = 4 * g + (j >> 2), unit = t ^ (D == 128 ? R & 7 : (R >> 1) & 3);
-    value_at[t] = lds_address(ring) + (unsigned)(kStep * D * 2 + R * D * 2 + (unit << 5) + ((j & 3) << 3));
+    value_at[t] = lds_address(ring) + (unsigned)(STEP * D * 2 + R * D * 2 + (unit << 5) + ((j & 3) << 3));
   }
   int* pages = s_pages + wave * STAGES * kWave;
   const unsigned page_at = lds_address(pages + lane);
   const char* zero = reinterpret_cast<const char*>(s_zero_row);
 
-  while (at < stop) {
-    // ---- a part of one row
-    int steps, unit_at;
-    if (plan.blocks == 0) {
-      steps = stop;
-      unit_at = 0;
-    } else {
-      while (start_of(row + 1) * p.kv_heads <= at) ++row;
-      const int start = start_of(row);
-      steps = start_of(row + 1) - start;
-      kvh = (at - start * p.kv_heads) / steps;
-      unit_at = start * p.kv_heads + kvh * steps;
-    }
-    const int first_step = at - unit_at, last_step = min(stop - unit_at, steps);
-    const int valid = plan.blocks != 0 && in_lanes ? __builtin_amdgcn_readlane(lane_valid, row)
-                                                   : p.valid[row];
-    const int begin = window_begin(p, valid), sinks = min(p.sinks, begin);
-    const int count = sinks + valid - begin;
-    const int32_t* table = p.tables + (size_t)row * p.max_pages;
-    const unsigned head_unit = (unsigned)((size_t)kvh * p.head_stride / 8);
-    h8 qb[KS];
-    {
-      const half_t* q = p.q + ((size_t)row * p.q_heads + kvh * p.group + min(j, p.group - 1)) * D;
+  const int begin = window_begin(p, valid), sinks = min(p.sinks, begin);
+  const int count = sinks + valid - begin;
+  const int32_t* table = p.tables + (size_t)row * p.max_pages;
+  const unsigned head_unit = (unsigned)((size_t)kvh * p.head_stride / 8);
+  h8 qb[KS];
+  {
+    const half_t* q = p.q + ((size_t)row * p.q_heads + first_head + min(j, heads - 1)) * D;
 #pragma unroll
-      for (int s = 0; s < KS; ++s) qb[s] = load_h8(q + 32 * s + 8 * g);
-    }
-    f4 o[DT];
+    for (int s = 0; s < KS; ++s) qb[s] = load_h8(q + 32 * s + 8 * g);
+  }
+  f4 o[DT];
 #pragma unroll
-    for (int t = 0; t < DT; ++t) o[t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    float m = -INFINITY, lsum = 0.0f;
-    int bad = 0;
+  for (int t = 0; t < DT; ++t) o[t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+  float m = -INFINITY, lsum = 0.0f;
+  int bad = 0;
 
-    // Table slot of the position that lane (l & 31) stands for in a step (past
-    // the end: of the last one) and its row in that page.
-    auto locate = [&](int step, int& slot_row) -> const int32_t* {
-      const int u = min(step * kStep + (lane & (kStep - 1)), count - 1);
-      const int pos = u < sinks ? u : begin + u - sinks;
-      const int slot = window_page(p, pos);
-      slot_row = pos - slot * p.page_size;
-      return table + slot;
-    };
-    // 16-byte unit where that position's row starts, kNoUnit when it has none
-    auto place = [&](int step, int page, int slot_row) -> unsigned {
-      const bool ok = window_page_ok(p, page);
-      bad |= !ok;
-      return ok && step * kStep + (lane & (kStep - 1)) < count
-                 ? (unsigned)page * (unsigned)(p.page_stride / 8) + head_unit +
-                       (unsigned)(slot_row * CH)
-                 : kNoUnit;
-    };
-    // K and V rows of a step, and the pages of the step that follows it in the
-    // stage: those too by loads to LDS, so that no load the compiler could wait
-    // for mixes with the ones in flight.
-    auto issue = [&](unsigned unit, const int32_t* next, int stage) {
-      half_t* to = ring + stage * STAGE;
-      __builtin_amdgcn_global_load_lds((global_void*)next, (lds_void*)(pages + stage * kWave), 4, 0, 0);
+  // Table slot of the position that lane (l & 31) stands for in a step (past
+  // the end: of the last one) and its row in that page.
+  auto locate = [&](int step, int& slot_row) -> const int32_t* {
+    const int u = min(step * STEP + (lane & (STEP - 1)), count - 1);
+    const int pos = u < sinks ? u : begin + u - sinks;
+    const int slot = window_page(p, pos);
+    slot_row = pos - slot * p.page_size;
+    return table + slot;
+  };
+  // 16-byte unit where that position's row starts, kNoUnit when it has none
+  auto place = [&](int step, int page, int slot_row) -> unsigned {
+    const bool ok = window_page_ok(p, page);
+    bad |= !ok;
+    return ok && step * STEP + (lane & (STEP - 1)) < count
+               ? (unsigned)page * (unsigned)(p.page_stride / 8) + head_unit +
+                     (unsigned)(slot_row * CH)
+               : kNoUnit;
+  };
+  // K and V rows of a step, and the pages of the step that follows it in the
+  // stage: those too by loads to LDS, so that no load the compiler could wait
+  // for mixes with the ones in flight.
+  auto issue = [&](unsigned unit, const int32_t* next, int stage) {
+    half_t* to = ring + stage * STAGE;
+    __builtin_amdgcn_global_load_lds((global_void*)next, (lds_void*)(pages + stage * kWave), 4, 0, 0);
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const int R = RPL * i + lane / CH, slot = lane % CH;
-        const unsigned row_unit = (unsigned)__shfl((int)unit, R, kWave);
-        const unsigned kc = slot ^ (D == 128 ? R & 15 : (R >> 1) & 7);
-        const unsigned vc = (((slot >> 1) ^ (D == 128 ? R & 7 : (R >> 1) & 3)) << 1) | (slot & 1);
-        const bool here = row_unit != kNoUnit;
-        const char* ka = here ? reinterpret_cast<const char*>(p.k) + (size_t)(row_unit + kc) * 16 : zero;
-        const char* va = here ? reinterpret_cast<const char*>(p.v) + (size_t)(row_unit + vc) * 16 : zero;
-        __builtin_amdgcn_global_load_lds((global_void*)ka, (lds_void*)(to + RPL * i * D), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((global_void*)va, (lds_void*)(to + (kStep + RPL * i) * D),
-                                         16, 0, 0);
-      }
-    };
-    auto consume = [&](int step, const h8 (&k)[2][KS], const h8 (&v)[DT]) {
-      f4 sc[2];
+    for (int i = 0; i < LOADS; ++i) {
+      const int R = RPL * i + lane / CH, slot = lane % CH;
+      const unsigned row_unit = (unsigned)__shfl((int)unit, R, kWave);
+      const unsigned kc = slot ^ (D == 128 ? R & 15 : (R >> 1) & 7);
+      const unsigned vc = (((slot >> 1) ^ (D == 128 ? R & 7 : (R >> 1) & 3)) << 1) | (slot & 1);
+      const bool here = row_unit != kNoUnit;
+      const char* ka = here ? reinterpret_cast<const char*>(p.k) + (size_t)(row_unit + kc) * 16 : zero;
+      const char* va = here ? reinterpret_cast<const char*>(p.v) + (size_t)(row_unit + vc) * 16 : zero;
+      __builtin_amdgcn_global_load_lds((global_void*)ka, (lds_void*)(to + RPL * i * D), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((global_void*)va, (lds_void*)(to + (STEP + RPL * i) * D),
+                                       16, 0, 0);
+    }
+  };
+  auto consume = [&](int step, const h8 (&k)[TILES][KS], const h4 (&v)[TILES][DT]) {
+    f4 sc[TILES];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        sc[t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int t = 0; t < TILES; ++t) {
+      sc[t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
-          sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][s], qb[s], sc[t], 0, 0, 0);
-      }
-      const int left = count - step * kStep;  // positions of the step that exist
-      if (left < kStep)
+      for (int s = 0; s < KS; ++s)
+        sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][s], qb[s], sc[t], 0, 0, 0);
+    }
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < TILES; ++t) settle(sc[t]);
+    const int left = count - step * STEP;  // positions of the step that exist
+    if (left < STEP)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (16 * t + 4 * g + r >= left) sc[t][r] = -INFINITY;
-      float top = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
-                        fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
-      top = max_of_groups(top) * p.scale_log2;
-      if (__builtin_amdgcn_ballot_w64(top > m) != 0) {
-        const float next = fmaxf(m, top);
-        const float alpha = next == m ? 1.0f : fast_exp2(m - next);
-        m = next;
-        lsum *= alpha;
-#pragma unroll
-        for (int t = 0; t < DT; ++t) o[t] *= alpha;
-      }
-      const float shift = m == -INFINITY ? 0.0f : m - kRaiseLog;
-      h8 w;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < TILES; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          w[4 * t + r] = (half_t)fast_exp2(__fmaf_rn(sc[t][r], p.scale_log2, -shift));
-      const h8 ones = {(half_t)1.0f, (half_t)1.0f, (half_t)1.0f, (half_t)1.0f,
-                       (half_t)1.0f, (half_t)1.0f, (half_t)1.0f, (half_t)1.0f};
-      lsum = dot8(w, ones, lsum);
+          if (16 * t + 4 * g + r >= left) sc[t][r] = -INFINITY;
+    float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
+    if constexpr (TILES == 2)
+      top = fmaxf(top, fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+    top = max_of_groups(top) * p.scale_log2;
+    if (__builtin_amdgcn_ballot_w64(top > m) != 0) {
+      const float next = fmaxf(m, top);
+      const float alpha = next == m ? 1.0f : fast_exp2(m - next);
+      m = next;
+      lsum *= alpha;
 #pragma unroll
-      for (int t = 0; t < DT; ++t)
-        o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[t], w, o[t], 0, 0, 0);
-    };
-
-    // ---- the wave's steps: every kDecodeWaves-th of the part
-    const int mine = first_step + wave;
-    int slot_row[STAGES];  // of the step that a stage takes next
-    {
-      int first_page[STAGES], first_row[STAGES];
-#pragma unroll
-      for (int st = 0; st < STAGES; ++st)
-        first_page[st] = *locate(mine + st * kDecodeWaves, first_row[st]);
-#pragma unroll
-      for (int st = 0; st < STAGES; ++st) {
-        const int32_t* next = locate(mine + (STAGES + st) * kDecodeWaves, slot_row[st]);
-        if (mine + st * kDecodeWaves < last_step)
-          issue(place(mine + st * kDecodeWaves, first_page[st], first_row[st]), next, st);
-      }
+      for (int t = 0; t < DT; ++t) o[t] *= alpha;
     }
-    // One step out of its stage, and the stage loaded again.  BODY: every step
-    // that is waited for or loaded exists.
-    auto turn = [&](auto stage, auto body, int step) {
-      constexpr int ST = decltype(stage)::value;
-      constexpr bool BODY = decltype(body)::value;
-      const int again = step + STAGES * kDecodeWaves;
-      if (BODY || step + (STAGES - 1) * kDecodeWaves < last_step)
-        wait_loads<(2 * LOADS + 1) * (STAGES - 1)>();
+    const float shift = m == -INFINITY ? 0.0f : m - kRaiseLog;
+    h4 w[TILES];
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        w[t][r] = (half_t)fast_exp2(__fmaf_rn(sc[t][r], p.scale_log2, -shift));
+      const h2 ones = {(half_t)1.0f, (half_t)1.0f};
+      lsum = __builtin_amdgcn_fdot2(__builtin_shufflevector(w[t], w[t], 0, 1), ones, lsum, false);
+      lsum = __builtin_amdgcn_fdot2(__builtin_shufflevector(w[t], w[t], 2, 3), ones, lsum, false);
+    }
+#pragma unroll
+    for (int t = 0; t < DT; ++t) {
+      if constexpr (TILES == 2)
+        o[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+            __builtin_shufflevector(v[0][t], v[1][t], 0, 1, 2, 3, 4, 5, 6, 7),
+            __builtin_shufflevector(w[0], w[1], 0, 1, 2, 3, 4, 5, 6, 7), o[t], 0, 0, 0);
       else
-        wait_loads<0>();
-      h8 k[2][KS], v[DT];
-      int page;
-      read_keys<D, ST * STAGE * 2, ST * kWave * 4>(key_at, page_at, k, page);
-#pragma unroll
-      for (int t = 0; t < DT; t += 4) read_values<D, ST * STAGE * 2>(value_at + t, v + t);
-      if (BODY || again < last_step) {
-        const unsigned unit = place(again, page, slot_row[ST]);
-        issue(unit, locate(again + STAGES * kDecodeWaves, slot_row[ST]), ST);
-      }
-      consume(step, k, v);
-    };
-    auto round = [&](auto body, int step) {
-      constexpr bool BODY = decltype(body)::value;
-      turn(std::integral_constant<int, 0>{}, body, step);
-      if constexpr (STAGES > 1)
-        if (BODY || step + kDecodeWaves < last_step)
-          turn(std::integral_constant<int, 1>{}, body, step + kDecodeWaves);
-      if constexpr (STAGES > 2)
-        if (BODY || step + 2 * kDecodeWaves < last_step)
-          turn(std::integral_constant<int, 2>{}, body, step + 2 * kDecodeWaves);
-      if constexpr (STAGES > 3)
-        if (BODY || step + 3 * kDecodeWaves < last_step)
-          turn(std::integral_constant<int, 3>{}, body, step + 3 * kDecodeWaves);
-    };
-    int step = mine;
-    for (; step + (2 * STAGES - 1) * kDecodeWaves < last_step; step += STAGES * kDecodeWaves)
-      round(std::true_type{}, step);
-    for (; step < last_step; step += STAGES * kDecodeWaves) round(std::false_type{}, step);
+        o[t] = __builtin_amdgcn_mfma_f32_16x16x16f16(v[0][t], w[0], o[t], 0, 0, 0);
+    }
+  };
 
-    // ---- the waves meet in LDS (the ring: every load into it has landed)
-    lsum = cross_sum<16>(lsum);
-    bad = __syncthreads_or(bad);
-    float* s_max = reinterpret_cast<float*>(s_ring);  // [waves][16]
-    float* s_sum = s_max + kDecodeWaves * 16;
-    float* s_out = s_sum + kDecodeWaves * 16;         // [waves][group][D]
-    if (j < p.group) {
-      if (g == 0) {
-        s_max[wave * 16 + j] = m;
-        s_sum[wave * 16 + j] = lsum;
-      }
+  // ---- the wave's steps: every kDecodeWaves-th of the part
+  const int mine = first_step + wave;
+  int slot_row[STAGES];  // of the step that a stage takes next
+  {
+    int first_page[STAGES], first_row[STAGES];
 #pragma unroll
-      for (int t = 0; t < DT; ++t)
-        *reinterpret_cast<f4*>(s_out + (size_t)(wave * p.group + j) * D + 16 * t + 4 * g) = o[t];
+    for (int st = 0; st < STAGES; ++st)
+      first_page[st] = *locate(mine + st * kDecodeWaves, first_row[st]);
+#pragma unroll
+    for (int st = 0; st < STAGES; ++st) {
+      const int32_t* next = locate(mine + (STAGES + st) * kDecodeWaves, slot_row[st]);
+      if (mine + st * kDecodeWaves < last_step)
+        issue(place(mine + st * kDecodeWaves, first_page[st], first_row[st]), next, st);
     }
+  }
+  // One step out of its stage, and the stage loaded again.  BODY: every step
+  // that is waited for or loaded exists.
+  auto turn = [&](auto stage, auto body, int step) {
+    constexpr int ST = decltype(stage)::value;
+    constexpr bool BODY = decltype(body)::value;
+    const int again = step + STAGES * kDecodeWaves;
+    if (BODY || step + (STAGES - 1) * kDecodeWaves < last_step)
+      wait_loads<(2 * LOADS + 1) * (STAGES - 1)>();
+    else
+      wait_loads<0>();
+    h8 k[TILES][KS];
+    h4 v[TILES][DT];
+    int page;
+    read_keys<D, STEP, ST * STAGE * 2, ST * kWave * 4>(key_at, page_at, k, page);
+    read_values<D, STEP, ST * STAGE * 2>(value_at, v);
+    if (BODY || again < last_step) {
+      const unsigned unit = place(again, page, slot_row[ST]);
+      issue(unit, locate(again + STAGES * kDecodeWaves, slot_row[ST]), ST);
+    }
+    consume(step, k, v);
+  };
+  auto round = [&](auto body, int step) {
+    constexpr bool BODY = decltype(body)::value;
+    turn(std::integral_constant<int, 0>{}, body, step);
+    if constexpr (STAGES > 1)
+      if (BODY || step + kDecodeWaves < last_step)
+        turn(std::integral_constant<int, 1>{}, body, step + kDecodeWaves);
+    if constexpr (STAGES > 2)
+      if (BODY || step + 2 * kDecodeWaves < last_step)
+        turn(std::integral_constant<int, 2>{}, body, step + 2 * kDecodeWaves);
+    if constexpr (STAGES > 3)
+      if (BODY || step + 3 * kDecodeWaves < last_step)
+        turn(std::integral_constant<int, 3>{}, body, step + 3 * kDecodeWaves);
+  };
+  int step = mine;
+  for (; step + (2 * STAGES - 1) * kDecodeWaves < last_step; step += STAGES * kDecodeWaves)
+    round(std::true_type{}, step);
+  for (; step < last_step; step += STAGES * kDecodeWaves) round(std::false_type{}, step);
+
+  // ---- the waves meet in LDS (the ring: every load into it has landed)
+  lsum = cross_sum<16>(lsum);
+  bad = __syncthreads_or(bad);
+  float* s_max = reinterpret_cast<float*>(s_ring);  // [waves][16]
+  float* s_sum = s_max + kDecodeWaves * 16;
+  float* s_out = s_sum + kDecodeWaves * 16;         // [waves][heads][D]
+  if (j < heads) {
+    if (g == 0) {
+      s_max[wave * 16 + j] = m;
+      s_sum[wave * 16 + j] = lsum;
+    }
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+      *reinterpret_cast<f4*>(s_out + (size_t)(wave * heads + j) * D + 16 * t + 4 * g) = o[t];
+  }
+  __syncthreads();
+  const bool whole = shares == 1;
+  const size_t slot_floats = (size_t)plan.heads * (D + 2);
+  float* slots = plan.slots + (size_t)unit * plan.parts * slot_floats;
+  // two dims a thread
+  for (int i = threadIdx.x; i < heads * (D / 2); i += THREADS) {
+    const int head = i / (D / 2), d = i % (D / 2) * 2;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kDecodeWaves; ++w) top = fmaxf(top, s_max[w * 16 + head]);
+    float sum = 0.0f, val0 = 0.0f, val1 = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kDecodeWaves; ++w) {
+      const float high = s_max[w * 16 + head];
+      const float scale = high == -INFINITY ? 0.0f : fast_exp2(high - top);
+      sum += scale * s_sum[w * 16 + head];
+      const float2 part = *reinterpret_cast<const float2*>(
+          s_out + (size_t)(w * heads + head) * D + d);
+      val0 += scale * part.x;
+      val1 += scale * part.y;
+    }
+    if (whole) {
+      if (!bad) put_pair(p, row, (first_head + head) * D + d, val0 / sum, val1 / sum);
+    } else {
+      float* out = slots + part * slot_floats + (size_t)head * (D + 2);
+      store_pair(out + d, val0, val1);
+      if (d == 0) store_pair(out + D, top, bad ? -1.0f : sum);
+    }
+  }
+  if (!whole) {
+    // the last of the row's blocks joins the partials, in block order (every
+    // word is written and read at agent scope; the stores have completed
+    // before the arrival is counted)
+    int* counter = plan.arrivals + unit;
+    __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    const bool whole = first_step == 0 && last_step == steps;
-    const int slot = whole ? 0 : 2 * blockIdx.x + (at == block_at ? 0 : 1);
-    float* part = plan.slots + (size_t)slot * p.group * (D + 2);
-    for (int i = threadIdx.x; i < p.group * D; i += THREADS) {
-      const int head = i / D, d = i % D;
-      float top = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kDecodeWaves; ++w) top = fmaxf(top, s_max[w * 16 + head]);
-      float sum = 0.0f, val = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kDecodeWaves; ++w) {
-        const float high = s_max[w * 16 + head];
-        const float scale = high == -INFINITY ? 0.0f : fast_exp2(high - top);
-        sum += scale * s_sum[w * 16 + head];
-        val += scale * s_out[(size_t)(w * p.group + head) * D + d];
-      }
-      if (whole) {
-        if (!bad)
-          p.out[window_out(p, row, (kvh * p.group + head) * D + d)] = (half_t)(val / sum);
-      } else {
-        float* to = part + (size_t)head * (D + 2);
-        __hip_atomic_store(to + d, val, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (d == 0) {
-          __hip_atomic_store(to + D, top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-          __hip_atomic_store(to + D + 1, bad ? -1.0f : sum, __ATOMIC_RELAXED,
-                             __HIP_MEMORY_SCOPE_AGENT);
-        }
-      }
-    }
-    if (!whole) {
-      // the last of the row's blocks joins the partials, in block order (every
-      // word is written and read at agent scope; the stores have completed
-      // before the arrival is counted)
-      const int from = unit_at / per, to = (unit_at + steps - 1) / per;
-      int* counter = plan.arrivals + (size_t)row * p.kv_heads + kvh;
-      __builtin_amdgcn_s_waitcnt(0);
-      __syncthreads();
+    if (threadIdx.x == 0)
+      s_last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+               shares - 1;
+    __syncthreads();
+    if (s_last) {
       if (threadIdx.x == 0)
-        s_last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-                 to - from;
-      __syncthreads();
-      if (s_last) {
-        if (threadIdx.x == 0)
-          __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        for (int i = threadIdx.x; i < p.group * D; i += THREADS) {
-          const int head = i / D, d = i % D;
-          float top = -INFINITY, sum = 0.0f, val = 0.0f;
-          bool spoiled = false;
-          constexpr int kAhead = 8;  // partials loaded at once
-          for (int b = from; b <= to; b += kAhead) {
-            float x[kAhead], hi[kAhead], s[kAhead];
+        __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      for (int i = threadIdx.x; i < heads * (D / 2); i += THREADS) {
+        const int head = i / (D / 2), d = i % (D / 2) * 2;
+        float top = -INFINITY, sum = 0.0f, val0 = 0.0f, val1 = 0.0f;
+        bool spoiled = false;
+        constexpr int kAhead = 16;  // partials loaded at once
+        for (int b = 0; b < shares; b += kAhead) {
+          float2 x[kAhead], y[kAhead];
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-              const int which = min(b + u, to);
-              const int place = 2 * which + (which == from && unit_at != which * per ? 1 : 0);
-              const float* in = plan.slots + ((size_t)place * p.group + head) * (D + 2);
-              x[u] = __hip_atomic_load(in + d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-              hi[u] = __hip_atomic_load(in + D, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-              s[u] = __hip_atomic_load(in + D + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
-            float next = top;
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u)
-              if (b + u <= to) {
-                spoiled |= s[u] < 0.0f;
-                next = fmaxf(next, hi[u]);
-              }
-            const float a = top == -INFINITY ? 0.0f : fast_exp2(top - next);
-            sum *= a;
-            val *= a;
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u)
-              if (b + u <= to) {
-                const float c = hi[u] == -INFINITY ? 0.0f : fast_exp2(hi[u] - next);
-                sum += s[u] * c;
-                val += x[u] * c;
-              }
-            top = next;
+          for (int u = 0; u < kAhead; ++u) {
+            const float* in = slots + min(b + u, shares - 1) * slot_floats + (size_t)head * (D + 2);
+            x[u] = load_pair(in + d);
+            y[u] = load_pair(in + D);
           }
-          if (!spoiled)
-            p.out[window_out(p, row, (kvh * p.group + head) * D + d)] = (half_t)(val / sum);
+          float next = top;
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u)
+            if (b + u < shares) {
+              spoiled |= y[u].y < 0.0f;
+              next = fmaxf(next, y[u].x);
+            }
+          const float a = top == -INFINITY ? 0.0f : fast_exp2(top - next);
+          sum *= a;
+          val0 *= a;
+          val1 *= a;
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u)
+            if (b + u < shares) {
+              const float c = y[u].x == -INFINITY ? 0.0f : fast_exp2(y[u].x - next);
+              sum += y[u].y * c;
+              val0 += x[u].x * c;
+              val1 += x[u].y * c;
+            }
+          top = next;
         }
+        if (!spoiled) put_pair(p, row, (first_head + head) * D + d, val0 / sum, val1 / sum);
       }
     }
-    at = unit_at + last_step;
-    if (at < stop) __syncthreads();  // the ring is loaded again
   }
 }
 
@@ -882,6 +839,7 @@ __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(Wi
     // out of sight: positions from the length on and [p.sinks, from)
     const unsigned hidden = (unsigned)max(0, min(from, 0x7ffffffe) - p.sinks);
     auto weigh = [&](int u0) {
+      settle(sc);
       const int p0 = position(u0), p1 = position(u0 + 31);
       if (p1 >= min_len || (p0 < max_from && p1 >= sinks)) {  // not all of it in sight
         const int first = u0 + 4 * (int)opaque(half);
@@ -1113,15 +1071,29 @@ using namespace tmc;
 namespace tmc {
 namespace {
 // The shapes window_decode_kernel takes; the others run window_plain_kernel.
-bool decode_shape(int64_t q_heads, int64_t kv_heads, int64_t head_dim) {
-  return (head_dim == 64 || head_dim == 128) && q_heads / kv_heads <= 16;
+bool decode_shape(int64_t head_dim) {
+  return head_dim == 64 || head_dim == 128;
 }
-// One list of steps over all blocks, unless the rows alone are many per CU.
-bool shared_list(int64_t batch, int64_t kv_heads) {
-  return batch <= kDecodeMaxRows && batch * kv_heads < 8 * kDecodeBlocks;
+// Query heads of one kv head beyond 16 are done 16 or fewer at a time, as if
+// they had a kv head each.
+int64_t decode_splits(int64_t q_heads, int64_t kv_heads) {
+  return (q_heads / kv_heads + 15) / 16;
 }
-size_t window_counter_bytes(int64_t batch, int64_t kv_heads) {
-  return std::max(kWindowCounterBytes, (size_t)(batch * kv_heads * 4 + 255) / 256 * 256);
+// Blocks a row of `units`: as many as fill the card's resident blocks, while a
+// full row leaves each kDecodeLeast steps, and not more than the square root of
+// the steps: a step takes about as long as one more partial at the join (0.16
+// and 0.22 us at 4 query heads of 128 dims).  The join takes 16 partials at a
+// time.  Both sides, 8 kv heads of 128 dims, one request of 8192 positions: 13.7
+// us at 16 parts, 15.0 at 32, 23 at 64, 42 alone.
+int decode_parts(int64_t units, int64_t head_dim, int64_t capacity, int64_t window,
+                 int64_t sinks) {
+  const int64_t step = head_dim == 128 ? 16 : 32;
+  const int64_t seen = std::min(capacity, std::min(window, capacity) + std::min(sinks, capacity));
+  const int64_t steps = (seen + step - 1) / step;
+  const int64_t parts = std::min<int64_t>({(steps + kDecodeLeast - 1) / kDecodeLeast,
+                                           (kDecodeBlocks + units - 1) / units,
+                                           (int64_t)std::ceil(std::sqrt((double)steps))});
+  return (int)(parts > 16 ? parts / 16 * 16 : parts);
 }
 }  // namespace
 }  // namespace tmc
@@ -1131,11 +1103,14 @@ extern "C" size_t tmc_window_attention_workspace_bytes(int64_t batch, int64_t q_
                                                        int64_t capacity, int64_t window,
                                                        int64_t sinks) {
   if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || capacity <= 0 || q_heads % kv_heads ||
-      window < 1 || sinks < 0 || !decode_shape(q_heads, kv_heads, head_dim) ||
-      !shared_list(batch, kv_heads))
+      window < 1 || sinks < 0 || !decode_shape(head_dim))
     return 0;
-  return window_counter_bytes(batch, kv_heads) +
-         (size_t)kDecodeBlocks * 2 * (q_heads / kv_heads) * (head_dim + 2) * sizeof(float);
+  const int64_t splits = decode_splits(q_heads, kv_heads), units = batch * kv_heads * splits;
+  const int parts = decode_parts(units, head_dim, capacity, window, sinks);
+  const int64_t heads = (q_heads / kv_heads + splits - 1) / splits;
+  return parts < 2 ? 0
+                   : kDecodeCounterBytes +
+                         (size_t)units * parts * heads * (head_dim + 2) * sizeof(float);
 }
 
 extern "C" int tmc_window_decode_attention(
@@ -1156,32 +1131,33 @@ extern "C" int tmc_window_decode_attention(
               "Window attention: layout must be 0 or TMC_LAYOUT_Y_PACKED.");
   const size_t need = tmc_window_attention_workspace_bytes(
       max_batch, q_heads, kv_heads, head_dim, page_size * max_pages, window, sinks);
-  TMC_REQUIRE(workspace_bytes >= need && (need == 0 || workspace),
+  TMC_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned16(workspace))),
               "Window attention: workspace is smaller than "
-              "tmc_window_attention_workspace_bytes().");
+              "tmc_window_attention_workspace_bytes() or not 16-byte aligned.");
   p.active = active_count;
   p.table_rows = p.rows;
   p.own_table = 1;
   if (layout) p.out_pass = (long)((q_heads * head_dim + 31) / 32) * 512;
   // 16-byte units of the pools are counted in 32 bits: below 64 GiB each
-  if (!decode_shape(q_heads, kv_heads, head_dim) ||
+  if (!decode_shape(head_dim) ||
       (uint64_t)pool_pages * (uint64_t)page_stride / 8 >= 0xFFFFFFFFull)
     return launch_plain(p, as_stream(stream));
   DecodePlan plan{};
-  unsigned blocks = (unsigned)(max_batch * kv_heads);
-  if (shared_list(max_batch, kv_heads)) {
+  plan.splits = (int)decode_splits(q_heads, kv_heads);
+  const int64_t units = max_batch * kv_heads * plan.splits;
+  plan.heads = (p.group + plan.splits - 1) / plan.splits;
+  plan.parts = decode_parts(units, head_dim, page_size * max_pages, window, sinks);
+  const unsigned blocks = (unsigned)(units * plan.parts);
+  if (need) {
     plan.arrivals = static_cast<int*>(workspace);
     plan.slots = reinterpret_cast<float*>(static_cast<char*>(workspace) +
-                                          window_counter_bytes(max_batch, kv_heads));
-    plan.blocks = kDecodeBlocks;
-    plan.least = kDecodeWaves;
-    blocks = kDecodeBlocks;
+                                          kDecodeCounterBytes);
   }
   if (head_dim == 128)
-    hipLaunchKernelGGL((window_decode_kernel<128, 2>), dim3(blocks), dim3(kDecodeWaves * kWave), 0,
+    hipLaunchKernelGGL((window_decode_kernel<128, 16, 2>), dim3(blocks), dim3(kDecodeWaves * kWave), 0,
                        as_stream(stream), p, plan);
   else
-    hipLaunchKernelGGL((window_decode_kernel<64, 4>), dim3(blocks), dim3(kDecodeWaves * kWave), 0,
+    hipLaunchKernelGGL((window_decode_kernel<64, 32, 2>), dim3(blocks), dim3(kDecodeWaves * kWave), 0,
                        as_stream(stream), p, plan);
   return check_launch("window_decode_kernel");
 }

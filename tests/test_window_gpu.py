@@ -104,6 +104,9 @@ DECODE = [
     (6, 2, 128, 16, 50, 3, [20, 200]),              # 3 query heads a kv head
     (10, 2, 64, 16, 50, 3, [20, 200]),
     (34, 2, 64, 16, 50, 3, [20, 200]),              # 17 of them
+    (71, 1, 64, 16, 400, 3, [1, 20, 2000]),         # 71: 15, 15, 15, 15 and 11 at a time
+    (48, 2, 128, 16, 1500, 30, [1400, 3000, 129]),  # 24: 12 and 12
+    (128, 1, 128, 64, 5000, 4, [6000, 128]),
     (8, 2, 64, 16, 1, 0, [1, 2, 16, 17, 100]),      # a window of one
     (8, 2, 64, 16, 1, 5, [1, 3, 5, 6, 100]),
     (4, 4, 64, 12, 40, 7, [1, 11, 12, 13, 47, 48, 49, 500]),
@@ -230,21 +233,23 @@ def test_pools_past_4_gib(tmc, torch, d, page):
         assert ((got.double().reshape(qh, d) - o).abs() <= tolerance).all()
 
 
-@pytest.mark.parametrize("d,batch,kvh", [(64, 300, 8), (128, 300, 8), (128, 2100, 1)])
+@pytest.mark.parametrize("d,batch,kvh", [(64, 300, 8), (128, 300, 8), (128, 2100, 1), (128, 70, 8),
+                                         (64, 100, 8), (128, 1000, 1), (64, 40, 32), (128, 64, 8)])
 def test_decode_batches_of_many_rows(tmc, torch, d, batch, kvh):
-    """More (request, kv head) rows than the shared list takes."""
+    """Many (request, kv head) rows: one list of steps, and a block a row."""
     page, window, sinks, cap_pages = 16, 40, 4, 8
     lengths = [1 + (37 * i) % 128 for i in range(batch)]
     cache = Cache(torch, batch, [set(visible(n, window, sinks)) for n in lengths], kvh, d, page, cap_pages)
     qh = 2 * kvh
     q = torch.randn(batch, qh * d, device="cuda").to(torch.float16)
     out = torch.full((batch, qh * d), 7.5, dtype=torch.float16, device="cuda")
-    assert tmc.window_attention_workspace_bytes(batch, qh, kvh, d, 128, window, sinks) == 0
+    ws = torch.zeros(max(1, tmc.window_attention_workspace_bytes(batch, qh, kvh, d, 128, window,
+                                                                 sinks) // 4), device="cuda")
     valid = torch.tensor(lengths, dtype=torch.int32, device="cuda")
     active = torch.tensor([batch - 1], dtype=torch.int32, device="cuda")
     tmc.window_decode_attention(q, cache.k, cache.v, valid, cache.tables_dev, active, out, batch, qh,
                                 kvh, d, page, cap_pages, cache.page_stride, cache.head_stride,
-                                window, sinks)
+                                window, sinks, ws)
     picked = sorted({*range(0, batch, 13), batch - 2, batch - 1})
     check_rows(torch, out[torch.tensor(picked, device="cuda")], cache,
                q[torch.tensor(picked, device="cuda")],
