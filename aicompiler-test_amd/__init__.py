@@ -767,54 +767,60 @@ def lm_head_argmax_packed_norm(x, packed_scaled, workspace, tokens, batch, in_fe
 
 
 # ---------------------------------------------------------------- streaming generation
-def _on_gpu(what, stream, *tensors):
-    """Refuse what a kernel on the current GPU could not read: host tensors,
-    tensors of another GPU, a stream of another GPU, gaps between elements."""
-    import torch
-    device = torch.cuda.current_device()
-    for t in tensors:
+def _refuse(what, device, dtype, name, t, count):
+    if not t.is_cuda or t.get_device() != device:
+        raise TmcError(f"{what}: tensors must be on the current GPU (cuda:{device}), "
+                       f"not on {t.device}")
+    if not t.is_contiguous():
+        raise TmcError(f"{what}: {name} must be contiguous")
+    if t.dtype is not dtype:
+        raise TmcError(f"{what}: {name} must be {dtype}, not {t.dtype}")
+    raise TmcError(f"{what}: {name} holds {t.numel()} elements, {count} are needed")
+
+
+def _addresses(what, device, dtype, *operands):
+    """Device addresses of (name, tensor or None, elements needed), after a
+    refusal of what a kernel on the current GPU could not read: host tensors,
+    tensors of another GPU or type, gaps between elements, too few of them."""
+    found = []
+    for name, t, count in operands:
         if t is None:
+            found.append(None)
             continue
-        if not t.is_cuda or t.device.index != device:
-            raise TmcError(f"{what}: tensors must be on the current GPU (cuda:{device}), "
-                           f"not on {t.device}")
-        if not t.is_contiguous():
-            raise TmcError(f"{what}: tensors must be contiguous")
-    if stream is not None and stream.device.index != device:
-        raise TmcError(f"{what}: the stream belongs to another GPU than the current one")
+        if t.get_device() != device or t.dtype is not dtype or not t.is_contiguous() or \
+                t.numel() < count:
+            _refuse(what, device, dtype, name, t, count)
+        found.append(t.data_ptr())
+    return found
 
 
-def _typed(what, dtype, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.dtype != dtype:
-            raise TmcError(f"{what}: {name} must be {dtype}, not {t.dtype}")
+def _workspace(what, device, t):
+    """(address, bytes) of a workspace tensor of any type."""
+    if t is None:
+        return None, 0
+    if t.get_device() != device or not t.is_contiguous():
+        _refuse(what, device, t.dtype, "workspace", t, 0)
+    return t.data_ptr(), t.numel() * t.element_size()
 
 
-def _room(what, t, count, name):
-    if t.numel() < count:
-        raise TmcError(f"{what}: {name} holds {t.numel()} elements, {count} are needed")
-
-
-def _window_checks(what, q, k_pool, v_pool, valid_lengths, tables, row_table, active, out, rows,
-                   q_heads, kv_heads, head_dim, max_pages, page_stride, stream, pool_pages):
+def _launch_stream(what, device, stream):
     import torch
-    _on_gpu(what, stream, q, k_pool, v_pool, valid_lengths, tables, row_table, active, out)
-    _typed(what, torch.float16, q=q, k_pool=k_pool, v_pool=v_pool, out=out)
-    _typed(what, torch.int32, valid_lengths=valid_lengths, tables=tables, row_table=row_table,
-           active=active)
+    if stream is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    if stream.device.index != device:
+        raise TmcError(f"{what}: the stream belongs to another GPU than the current one")
+    return stream.cuda_stream
+
+
+def _window_pages(what, k_pool, v_pool, rows, q_heads, kv_heads, head_dim, max_pages, page_stride,
+                  pool_pages):
     if min(rows, q_heads, kv_heads, head_dim, max_pages, page_stride) < 1:
         raise TmcError(f"{what}: rows, heads, head_dim, pages and strides must be positive")
     held = min(k_pool.numel(), v_pool.numel()) // page_stride
     if pool_pages is None:
-        pool_pages = held
-    elif pool_pages > held:
+        return held
+    if pool_pages > held:
         raise TmcError(f"{what}: the pools hold {held} pages, not {pool_pages}")
-    _room(what, q, rows * q_heads * head_dim, "q")
-    _room(what, valid_lengths, rows, "valid_lengths")
-    if row_table is not None:
-        _room(what, row_table, rows, "row_table")
-    if active is not None:
-        _room(what, active, 1, "active")
     return pool_pages
 
 
@@ -831,21 +837,25 @@ def window_decode_attention(q, k_pool, v_pool, valid_lengths, tables, active, ou
     """Paged decode attention over the last `window` positions and the first
     `sinks` ones (tmc_window_decode_attention); active may be None.  The
     workspace must be zero before its first use."""
+    import torch
     what = "tmc_window_decode_attention"
-    pool_pages = _window_checks(what, q, k_pool, v_pool, valid_lengths, tables, None, active, out,
-                                max_batch, q_heads, kv_heads, head_dim, max_pages, page_stride,
-                                stream, pool_pages)
-    _room(what, tables, max_batch * max_pages, "tables")
+    device = torch.cuda.current_device()
+    pool_pages = _window_pages(what, k_pool, v_pool, max_batch, q_heads, kv_heads, head_dim,
+                               max_pages, page_stride, pool_pages)
     width = q_heads * head_dim
-    _room(what, out, packed_activation_elements(max_batch, width) if layout == Y_PACKED
-          else max_batch * width, "out")
-    _on_gpu(what, None, workspace)
-    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    queries, keys, values, output = _addresses(
+        what, device, torch.float16, ("q", q, max_batch * width), ("k_pool", k_pool, 0),
+        ("v_pool", v_pool, 0),
+        ("out", out, packed_activation_elements(max_batch, width) if layout == Y_PACKED
+         else max_batch * width))
+    lengths, table, rows = _addresses(
+        what, device, torch.int32, ("valid_lengths", valid_lengths, max_batch),
+        ("tables", tables, max_batch * max_pages), ("active", active, 1))
+    space, space_bytes = _workspace(what, device, workspace)
     check(lib().tmc_window_decode_attention(
-        _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(valid_lengths), _ptr(tables), _ptr(active),
-        _ptr(out), _dtype_code(q), max_batch, q_heads, kv_heads, head_dim, page_size, max_pages,
-        pool_pages, page_stride, head_stride, window, sinks, _ptr(workspace), ws_bytes, layout,
-        _stream(stream)), what)
+        queries, keys, values, lengths, table, rows, output, F16, max_batch, q_heads, kv_heads,
+        head_dim, page_size, max_pages, pool_pages, page_stride, head_stride, window, sinks, space,
+        space_bytes, layout, _launch_stream(what, device, stream)), what)
 
 
 def window_prefill_attention(q, k_pool, v_pool, valid_lengths, tables, row_table, active, out,
@@ -853,17 +863,23 @@ def window_prefill_attention(q, k_pool, v_pool, valid_lengths, tables, row_table
                              head_stride, window, sinks, stream=None, pool_pages=None):
     """The chunk form of window_decode_attention: rows of one request
     (row_table None, one table row) or of several."""
+    import torch
     what = "tmc_window_prefill_attention_f16"
-    pool_pages = _window_checks(what, q, k_pool, v_pool, valid_lengths, tables, row_table, active,
-                                out, rows, q_heads, kv_heads, head_dim, max_pages, page_stride,
-                                stream, pool_pages)
+    device = torch.cuda.current_device()
+    pool_pages = _window_pages(what, k_pool, v_pool, rows, q_heads, kv_heads, head_dim, max_pages,
+                               page_stride, pool_pages)
+    width = q_heads * head_dim
+    queries, keys, values, output = _addresses(
+        what, device, torch.float16, ("q", q, rows * width), ("k_pool", k_pool, 0),
+        ("v_pool", v_pool, 0), ("out", out, rows * width))
+    lengths, table, of_row, count = _addresses(
+        what, device, torch.int32, ("valid_lengths", valid_lengths, rows),
+        ("tables", tables, max_pages), ("row_table", row_table, rows), ("active", active, 1))
     table_rows = 1 if row_table is None else tables.numel() // max_pages
-    _room(what, tables, max_pages, "tables")
-    _room(what, out, rows * q_heads * head_dim, "out")
     check(lib().tmc_window_prefill_attention_f16(
-        _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(valid_lengths), _ptr(tables), _ptr(row_table),
-        table_rows, _ptr(active), _ptr(out), rows, q_heads, kv_heads, head_dim, page_size,
-        max_pages, pool_pages, page_stride, head_stride, window, sinks, _stream(stream)), what)
+        queries, keys, values, lengths, table, of_row, table_rows, count, output, rows, q_heads,
+        kv_heads, head_dim, page_size, max_pages, pool_pages, page_stride, head_stride, window,
+        sinks, _launch_stream(what, device, stream)), what)
 
 
 def page_moves(moves, pools, pool_pages, page_size):
@@ -884,26 +900,29 @@ def move_pages(k_pools, v_pools, moves, heads, page_size, head_dim, page_stride=
     page_moves)."""
     import torch
     what = "tmc_move_pages"
-    if not k_pools or len(k_pools) != len(v_pools):
+    count = len(k_pools)
+    if not count or count != len(v_pools):
         raise TmcError(f"{what}: as many K pools as V pools, and at least one")
-    _on_gpu(what, stream, *k_pools, *v_pools, moves)
-    _typed(what, torch.int32, moves=moves)
-    _typed(what, k_pools[0].dtype, **{f"pool {i}": t for i, t in enumerate([*k_pools, *v_pools])})
-    if moves.dim() != 2 or moves.shape[1] != 4:
-        raise TmcError(f"{what}: moves must be [count, 4]")
     head_stride = page_size * head_dim if head_stride is None else head_stride
     page_stride = heads * head_stride if page_stride is None else page_stride
     if min(heads, page_size, head_dim, page_stride) < 1:
         raise TmcError(f"{what}: heads, page_size, head_dim and strides must be positive")
+    if moves.dim() != 2 or moves.shape[1] != 4:
+        raise TmcError(f"{what}: moves must be [count, 4]")
+    device, dtype = torch.cuda.current_device(), k_pools[0].dtype
+    move_list, = _addresses(what, device, torch.int32, ("moves", moves, 0))
+    pools = [*k_pools, *v_pools]
+    for i, t in enumerate(pools):
+        if t.get_device() != device or t.dtype is not dtype or not t.is_contiguous():
+            _refuse(what, device, dtype, f"pool {i}", t, 0)
     if moves.shape[0] == 0:
         return
-    pool_pages = min(t.numel() for t in [*k_pools, *v_pools]) // page_stride
-    count = len(k_pools)
-    keys = (C.c_void_p * count)(*[t.data_ptr() for t in k_pools])
-    values = (C.c_void_p * count)(*[t.data_ptr() for t in v_pools])
-    check(lib().tmc_move_pages(keys, values, count, _ptr(moves), moves.shape[0],
-                               _dtype_code(k_pools[0]), pool_pages, heads, page_size, head_dim,
-                               page_stride, head_stride, _stream(stream)), what)
+    pool_pages = min([t.numel() for t in pools]) // page_stride
+    addresses = (C.c_void_p * (2 * count))(*[t.data_ptr() for t in pools])
+    check(lib().tmc_move_pages(addresses, C.byref(addresses, count * C.sizeof(C.c_void_p)), count,
+                               move_list, moves.shape[0], _dtype_code(k_pools[0]), pool_pages,
+                               heads, page_size, head_dim, page_stride, head_stride,
+                               _launch_stream(what, device, stream)), what)
 
 
 def rebuild_tables(tables, out, pool_pages, parents=None, remap=None, tail_slots=None, tails=None,
@@ -912,21 +931,19 @@ def rebuild_tables(tables, out, pool_pages, parents=None, remap=None, tail_slots
     and tails [layers, rows]) or a compaction (remap [layers, pool_pages])."""
     import torch
     what = "tmc_rebuild_tables"
-    _on_gpu(what, stream, tables, out, parents, remap, tail_slots, tails)
-    _typed(what, torch.int32, tables=tables, out=out, parents=parents, remap=remap,
-           tail_slots=tail_slots, tails=tails)
     if tables.dim() != 3 or out.dim() != 3 or tables.shape[0] != out.shape[0] or \
             tables.shape[2] != out.shape[2]:
         raise TmcError(f"{what}: tables and out must be [layers, rows, max_pages] of the same "
                        "layers and pages")
+    device = torch.cuda.current_device()
     layers, rows, max_pages = out.shape
-    for name, t, count in (("parents", parents, rows), ("remap", remap, layers * pool_pages),
-                           ("tail_slots", tail_slots, rows), ("tails", tails, layers * rows)):
-        if t is not None:
-            _room(what, t, count, name)
-    check(lib().tmc_rebuild_tables(_ptr(tables), _ptr(parents), _ptr(remap), _ptr(tail_slots),
-                                   _ptr(tails), _ptr(out), layers, tables.shape[1], rows,
-                                   max_pages, pool_pages, _stream(stream)), what)
+    old, new, parent, renamed, slots, tail = _addresses(
+        what, device, torch.int32, ("tables", tables, 0), ("out", out, 0),
+        ("parents", parents, rows), ("remap", remap, layers * pool_pages),
+        ("tail_slots", tail_slots, rows), ("tails", tails, layers * rows))
+    check(lib().tmc_rebuild_tables(old, parent, renamed, slots, tail, new, layers, tables.shape[1],
+                                   rows, max_pages, pool_pages,
+                                   _launch_stream(what, device, stream)), what)
 
 
 def logprobs_workspace_bytes(rows, vocabulary, top) -> int:
@@ -943,11 +960,10 @@ def logprobs(logits, tokens, logprob, entropy=None, top_tokens=None, top_logprob
     what = "tmc_logprobs"
     if logits.dim() != 2 or logits.stride(1) != 1:
         raise TmcError(f"{what}: logits must be [rows, vocabulary] with adjacent elements")
-    if not logits.is_cuda or logits.device.index != torch.cuda.current_device():
-        raise TmcError(f"{what}: tensors must be on the current GPU, not on {logits.device}")
-    _on_gpu(what, stream, tokens, logprob, entropy, top_tokens, top_logprobs, workspace)
-    _typed(what, torch.int32, tokens=tokens, top_tokens=top_tokens)
-    _typed(what, torch.float32, logprob=logprob, entropy=entropy, top_logprobs=top_logprobs)
+    device = torch.cuda.current_device()
+    if logits.get_device() != device:
+        _refuse(what, device, logits.dtype, "logits", logits, 0)
+    code = F32 if logits.dtype is torch.float32 else _dtype_code(logits)
     rows, vocabulary = logits.shape
     top = 0
     if top_tokens is not None:
@@ -955,15 +971,16 @@ def logprobs(logits, tokens, logprob, entropy=None, top_tokens=None, top_logprob
                 top_logprobs.shape != top_tokens.shape:
             raise TmcError(f"{what}: top_tokens and top_logprobs must be [rows, top]")
         top = top_tokens.shape[1]
-    for name, t in (("tokens", tokens), ("logprob", logprob), ("entropy", entropy)):
-        if t is not None:
-            _room(what, t, rows, name)
-    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    given, greatest = _addresses(what, device, torch.int32, ("tokens", tokens, rows),
+                                 ("top_tokens", top_tokens, 0))
+    chosen, spread, best = _addresses(what, device, torch.float32, ("logprob", logprob, rows),
+                                      ("entropy", entropy, rows),
+                                      ("top_logprobs", top_logprobs, 0))
+    space, space_bytes = _workspace(what, device, workspace)
     check(lib().tmc_logprobs(
-        _ptr(logits), _dtype_code(logits), logits.stride(0) if rows > 1 else vocabulary,
-        _ptr(tokens), _ptr(logprob), _ptr(entropy), _ptr(top_tokens) if top else None,
-        _ptr(top_logprobs) if top else None, rows, vocabulary, top, _ptr(workspace), ws_bytes,
-        _stream(stream)), what)
+        logits.data_ptr(), code, logits.stride(0) if rows > 1 else vocabulary, given, chosen,
+        spread, greatest if top else None, best if top else None, rows, vocabulary, top, space,
+        space_bytes, _launch_stream(what, device, stream)), what)
 
 
 def fill_normal(t, seed, mean=0.0, std=1.0, stream=None):
