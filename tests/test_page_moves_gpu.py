@@ -30,7 +30,9 @@ def same(torch, a, b):
 @pytest.mark.parametrize("dtype,layers,heads,page,d", [
     ("float16", 3, 8, 16, 128), ("float16", 33, 2, 12, 64), ("float16", 70, 1, 1, 8),
     ("float32", 2, 4, 16, 32), ("bfloat16", 1, 3, 5, 10), ("float16", 2, 3, 7, 5),
-    ("float32", 1, 1, 3, 1), ("float16", 1, 32, 256, 128), ("float32", 1, 5, 9, 6)])
+    ("float32", 1, 1, 3, 1), ("float16", 1, 32, 256, 128), ("float32", 1, 5, 9, 6),
+    ("float16", 130, 2, 3, 8), ("float16", 2, 3, 1100, 8), ("float16", 1, 1, 4096, 256),
+    ("bfloat16", 2, 5, 700, 3)])
 def test_moves_copy_the_positions(tmc, torch, dtype, layers, heads, page, d):
     dtype = getattr(torch, dtype)
     pages = 23
