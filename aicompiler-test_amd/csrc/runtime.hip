@@ -1006,6 +1006,157 @@ bool make_spec(const std::string& name, const Params& p, KernelSpec& s) {
     };
     return true;
   }
+  if (name == "window_attention") {
+    const int64_t b = param_int(p, "max_batch"), qh = param_int(p, "q_heads"),
+                  kvh = param_int(p, "kv_heads", param_int(p, "q_heads")),
+                  d = param_int(p, "head_dim"), ps = param_int(p, "page_size"),
+                  mp = param_int(p, "max_pages"), window = param_int(p, "window"),
+                  sinks = param_int(p, "sinks", 0);
+    NEED(b > 0 && qh > 0 && kvh > 0 && d > 0 && ps > 0 && mp > 0 && window > 0 && sinks >= 0 &&
+             dt == TMC_F16,
+         "window_attention needs max_batch, q_heads, head_dim, page_size, max_pages, window and "
+         "dtype=f16.");
+    const int64_t head_stride = param_int(p, "head_stride", ps * d);
+    const int64_t page_stride = param_int(p, "page_stride", kvh * ps * d);
+    const auto lit = p.find("out_layout");
+    const bool packed_out = lit != p.end() && lit->second == "packed";
+    NEED(lit == p.end() || packed_out || lit->second == "row_major",
+         "window_attention out_layout must be row_major or packed.");
+    s.inputs = {dt, dt, dt, TMC_I32, TMC_I32, TMC_I32};
+    s.outputs = {dt};
+    s.counts = {(size_t)(b * qh * d), 0, 0, (size_t)b, (size_t)(b * mp), 1,
+                packed_out ? (size_t)tmc_packed_activation_elements(b, qh * d)
+                           : (size_t)(b * qh * d)};
+    s.workspace_bytes = tmc_window_attention_workspace_bytes(b, qh, kvh, d, ps * mp, window, sinks);
+    s.launch = [=](const LaunchContext& c) {
+      const int64_t pool_pages =
+          (int64_t)(std::min(c.counts[1], c.counts[2]) / (size_t)page_stride);
+      return tmc_window_decode_attention(
+          c.ptrs[0], c.ptrs[1], c.ptrs[2], static_cast<const int32_t*>(c.ptrs[3]),
+          static_cast<const int32_t*>(c.ptrs[4]), static_cast<const int32_t*>(c.ptrs[5]),
+          c.ptrs[6], dt, b, qh, kvh, d, ps, mp, pool_pages, page_stride, head_stride, window,
+          sinks, c.workspace, c.workspace_bytes, packed_out ? TMC_LAYOUT_Y_PACKED : 0, c.stream);
+    };
+    return true;
+  }
+  if (name == "window_prefill_attention") {
+    const int64_t rows = param_int(p, "rows"), qh = param_int(p, "q_heads"),
+                  kvh = param_int(p, "kv_heads", param_int(p, "q_heads")),
+                  d = param_int(p, "head_dim"), ps = param_int(p, "page_size"),
+                  mp = param_int(p, "max_pages"), window = param_int(p, "window"),
+                  sinks = param_int(p, "sinks", 0);
+    NEED(rows > 0 && qh > 0 && kvh > 0 && d > 0 && ps > 0 && mp > 0 && window > 0 && sinks >= 0 &&
+             dt == TMC_F16,
+         "window_prefill_attention needs rows, q_heads, head_dim, page_size, max_pages, window "
+         "and dtype=f16.");
+    const int64_t head_stride = param_int(p, "head_stride", ps * d);
+    const int64_t page_stride = param_int(p, "page_stride", kvh * ps * d);
+    const int64_t tr = param_int(p, "tables", 0);  // > 0: table rows + a row table
+    NEED(tr >= 0 && tr < (1 << 20), "window_prefill_attention: tables must be >= 0.");
+    // bindings as prefill_attention's
+    s.inputs = {dt, dt, dt, TMC_I32, TMC_I32};
+    s.counts = {(size_t)(rows * qh * d), 0, 0, (size_t)rows, (size_t)(mp * (tr ? tr : 1))};
+    if (tr) {
+      s.inputs.push_back(TMC_I32);
+      s.counts.push_back((size_t)rows);
+    }
+    s.inputs.push_back(TMC_I32);
+    s.counts.push_back(1);
+    s.outputs = {dt};
+    s.counts.push_back((size_t)(rows * qh * d));
+    const int a = tr ? 6 : 5;  // index of the active count
+    s.launch = [=](const LaunchContext& c) {
+      const int64_t pool_pages =
+          (int64_t)(std::min(c.counts[1], c.counts[2]) / (size_t)page_stride);
+      const auto i32 = [&](int i) { return static_cast<const int32_t*>(c.ptrs[i]); };
+      return tmc_window_prefill_attention_f16(
+          c.ptrs[0], c.ptrs[1], c.ptrs[2], i32(3), i32(4), tr ? i32(5) : nullptr, tr ? tr : 1,
+          i32(a), c.ptrs[a + 1], rows, qh, kvh, d, ps, mp, pool_pages, page_stride, head_stride,
+          window, sinks, c.stream);
+    };
+    return true;
+  }
+  if (name == "move_pages") {
+    // Input the moves (int32 [moves, 4]); outputs the K pools, then the V pools.
+    const int64_t n = param_int(p, "moves"), pools = param_int(p, "pools", 1),
+                  h = param_int(p, "heads"), d = param_int(p, "head_dim"),
+                  ps = param_int(p, "page_size");
+    NEED(n > 0 && h > 0 && d > 0 && ps > 0, "move_pages needs moves, heads, head_dim, page_size.");
+    NEED(pools > 0 && pools <= 15, "move_pages: 1 to 15 pools (32 bindings).");
+    const int64_t head_stride = param_int(p, "head_stride", ps * d);
+    const int64_t page_stride = param_int(p, "page_stride", h * ps * d);
+    NEED(page_stride > 0, "move_pages: page_stride must be positive.");
+    s.inputs = {TMC_I32};
+    s.outputs.assign((size_t)(2 * pools), dt);
+    s.counts.assign((size_t)(1 + 2 * pools), 0);
+    s.counts[0] = (size_t)(4 * n);
+    s.launch = [=](const LaunchContext& c) {
+      size_t least = c.counts[1];
+      for (int64_t i = 2; i <= 2 * pools; ++i) least = std::min(least, c.counts[i]);
+      return tmc_move_pages(c.ptrs.data() + 1, c.ptrs.data() + 1 + pools, pools,
+                            static_cast<const int32_t*>(c.ptrs[0]), n, dt,
+                            (int64_t)(least / (size_t)page_stride), h, ps, d, page_stride,
+                            head_stride, c.stream);
+    };
+    return true;
+  }
+  if (name == "rebuild_tables") {
+    // Inputs the tables (, parents with parents=1) (, remap with remap=1)
+    // (, tail slots and tails with tails=1); output the new tables.
+    const int64_t layers = param_int(p, "layers", 1), rows = param_int(p, "rows"),
+                  tr = param_int(p, "table_rows", param_int(p, "rows")),
+                  mp = param_int(p, "max_pages"), pages = param_int(p, "pool_pages");
+    const bool parents = param_int(p, "parents", 0) != 0, remap = param_int(p, "remap", 0) != 0,
+               tails = param_int(p, "tails", 0) != 0;
+    NEED(layers > 0 && rows > 0 && tr > 0 && mp > 0 && pages > 0,
+         "rebuild_tables needs rows, max_pages, pool_pages.");
+    NEED(parents || tr == rows, "rebuild_tables: table_rows other than rows needs parents=1.");
+    s.counts = {(size_t)(layers * tr * mp)};
+    if (parents) s.counts.push_back((size_t)rows);
+    if (remap) s.counts.push_back((size_t)(layers * pages));
+    if (tails) s.counts.insert(s.counts.end(), {(size_t)rows, (size_t)(layers * rows)});
+    s.inputs.assign(s.counts.size(), TMC_I32);
+    s.outputs = {TMC_I32};
+    s.counts.push_back((size_t)(layers * rows * mp));
+    s.launch = [=](const LaunchContext& c) {
+      int next = 0;
+      const auto take = [&](bool here) {
+        return here ? static_cast<int32_t*>(c.ptrs[next++]) : nullptr;
+      };
+      const int32_t *old = take(true), *parent = take(parents), *to = take(remap),
+                    *slots = take(tails), *tail = take(tails);
+      return tmc_rebuild_tables(old, parent, to, slots, tail, take(true), layers, tr, rows, mp,
+                                pages, c.stream);
+    };
+    return true;
+  }
+  if (name == "logprobs") {
+    // Inputs logits and tokens; outputs log probability, entropy (, the top
+    // tokens and their log probabilities).
+    const int64_t rows = param_int(p, "rows"), v = param_int(p, "vocab"),
+                  top = param_int(p, "top", 0);
+    const int type = param_dtype(p, "dtype", TMC_F32);
+    NEED(rows > 0 && v > 0 && (type == TMC_F32 || type == TMC_F16),
+         "logprobs needs rows, vocab and dtype f32|f16.");
+    NEED(top >= 0 && top <= 64 && top <= v, "logprobs: top must be at most 64 and the vocabulary.");
+    s.inputs = {type, TMC_I32};
+    s.outputs = {TMC_F32, TMC_F32};
+    s.counts = {(size_t)(rows * v), (size_t)rows, (size_t)rows, (size_t)rows};
+    if (top) {
+      s.outputs.insert(s.outputs.end(), {TMC_I32, TMC_F32});
+      s.counts.insert(s.counts.end(), 2, (size_t)(rows * top));
+    }
+    s.workspace_bytes = tmc_logprobs_workspace_bytes(rows, v, top);
+    s.groups = (size_t)rows;
+    s.launch = [=](const LaunchContext& c) {
+      return tmc_logprobs(c.ptrs[0], type, v, static_cast<const int32_t*>(c.ptrs[1]),
+                          static_cast<float*>(c.ptrs[2]), static_cast<float*>(c.ptrs[3]),
+                          top ? static_cast<int32_t*>(c.ptrs[4]) : nullptr,
+                          top ? static_cast<float*>(c.ptrs[5]) : nullptr, rows, v, top,
+                          c.workspace, c.workspace_bytes, c.stream);
+    };
+    return true;
+  }
   if (name == "argmax") {
     const int64_t rows = param_int(p, "rows"), v = param_int(p, "vocab");
     NEED(rows > 0 && v > 0, "argmax needs rows and vocab.");
