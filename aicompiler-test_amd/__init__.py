@@ -9,6 +9,7 @@ every call raises.
 """
 from __future__ import annotations
 
+import array
 import ctypes as C
 import os
 
@@ -806,7 +807,7 @@ def _workspace(what, device, t):
 def _launch_stream(what, device, stream):
     import torch
     if stream is None:
-        return torch.cuda.current_stream(device).cuda_stream
+        return torch._C._cuda_getCurrentRawStream(device)
     if stream.device.index != device:
         raise TmcError(f"{what}: the stream belongs to another GPU than the current one")
     return stream.cuda_stream
@@ -912,14 +913,18 @@ def move_pages(k_pools, v_pools, moves, heads, page_size, head_dim, page_stride=
     device, dtype = torch.cuda.current_device(), k_pools[0].dtype
     move_list, = _addresses(what, device, torch.int32, ("moves", moves, 0))
     pools = [*k_pools, *v_pools]
-    for i, t in enumerate(pools):
-        if t.get_device() != device or t.dtype is not dtype or not t.is_contiguous():
-            _refuse(what, device, dtype, f"pool {i}", t, 0)
+    tensor = torch.Tensor
+    if set(map(tensor.get_device, pools)) != {device} or \
+            not all(map(tensor.is_contiguous, pools)) or {t.dtype for t in pools} != {dtype}:
+        for i, t in enumerate(pools):
+            if t.get_device() != device or t.dtype is not dtype or not t.is_contiguous():
+                _refuse(what, device, dtype, f"pool {i}", t, 0)
     if moves.shape[0] == 0:
         return
-    pool_pages = min([t.numel() for t in pools]) // page_stride
-    addresses = (C.c_void_p * (2 * count))(*[t.data_ptr() for t in pools])
-    check(lib().tmc_move_pages(addresses, C.byref(addresses, count * C.sizeof(C.c_void_p)), count,
+    pool_pages = min(map(tensor.numel, pools)) // page_stride
+    addresses = array.array("Q", map(tensor.data_ptr, pools))
+    first, size = addresses.buffer_info()[0], addresses.itemsize
+    check(lib().tmc_move_pages(first, first + count * size, count,
                                move_list, moves.shape[0], _dtype_code(k_pools[0]), pool_pages,
                                heads, page_size, head_dim, page_stride, head_stride,
                                _launch_stream(what, device, stream)), what)
