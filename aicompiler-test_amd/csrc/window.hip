@@ -634,7 +634,9 @@ __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(Wi
   constexpr int RPL = kWave / CH, LOADS = OWN / RPL;  // rows a load, loads of K (of V)
   constexpr int STAGE = 2 * SPAN * D;                 // halves: K rows, V rows
   static_assert(LOADS >= 1 && 2 * STAGE >= WAVES * 32 * D, "results fit the stages");
+  constexpr int PER = SPAN / kWave, TURNS = WAVES / PER;  // waves that find a stage's rows
   __shared__ __align__(256) half_t s_kv[2 * STAGE];
+  __shared__ unsigned s_units[4][SPAN];  // 16-byte units where the rows of four stages start
   __shared__ int s_run, s_low, s_high;
   __shared__ float s_max[WAVES][32], s_sum[WAVES][32];
 
@@ -654,7 +656,6 @@ __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(Wi
   }
   const int active = p.active ? min(p.active[0], p.rows) : p.rows;
   const int t0 = tile * tokens_per_tile, tokens = min(tokens_per_tile, active - t0);
-  const char* zero = reinterpret_cast<const char*>(s_zero_row);
   const unsigned head_unit = (unsigned)((size_t)kvh * p.head_stride / 8);
   const int capacity = p.page_size * p.max_pages;
   // this lane's vector
@@ -713,36 +714,42 @@ __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(Wi
     const int sinks = min(p.sinks, low), gap = low - sinks;
     const int count = high - gap;  // positions of the tile: u < sinks, then u + gap
 
-    // ---- loads: lane l stands for row l % OWN of the wave's part of a stage
-    int bad = 0;
-    auto locate = [&](int stage, int& slot_row) -> int {
-      const int u = min(stage * SPAN + wave * OWN + (lane & (OWN - 1)), count - 1);
+    // ---- loads.  The waves take turns to find a stage's rows: their table entries
+    // four stages ahead, their units three ahead.  Places past the end take the
+    // last position's row and positions without a page page 0's: such scores are
+    // masked, or their vectors not stored.
+    int bad = 0, page = 0, slot_row = 0;
+    auto my_turn = [&](int stage) { return stage % TURNS == wave / PER; };
+    const int turn_row = wave % PER * kWave + lane;
+    auto look_up = [&](int stage) {
+      const int u = min(stage * SPAN + turn_row, count - 1);
       const int pos = u < sinks ? u : u + gap;
-      const int slot = window_page(p, pos);
-      slot_row = pos - slot * p.page_size;
-      return table[slot];
+      const int at = window_page(p, pos);
+      slot_row = pos - at * p.page_size;
+      page = table[at];
     };
-    auto place = [&](int stage, int page, int slot_row) -> unsigned {
+    auto put_units = [&](int stage) {
       const bool ok = window_page_ok(p, page);
       bad |= !ok;
-      return ok && stage * SPAN + wave * OWN + (lane & (OWN - 1)) < count
-                 ? (unsigned)page * (unsigned)(p.page_stride / 8) + head_unit +
-                       (unsigned)(slot_row * CH)
-                 : kNoUnit;
+      s_units[stage % 4][turn_row] = (unsigned)(ok ? page : 0) * (unsigned)(p.page_stride / 8) +
+                                     head_unit + (unsigned)(slot_row * CH);
     };
+    const int own_row = OWN * wave + lane / CH, slot = lane % CH;
+    // 16-byte chunk of its row that a lane loads; RPL i changes other bits of the row
+    const unsigned key_chunk = slot ^ (D == 128 ? own_row & 15 : (own_row >> 1) & 7);
+    const unsigned value_chunk =
+        (((slot >> 1) ^ (D == 128 ? own_row & 7 : (own_row >> 1) & 3)) << 1) | (slot & 1);
     h8 kr[LOADS], vr[LOADS];
-    auto load = [&](unsigned unit) {
+    auto load = [&](int stage) {
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        const int R = OWN * wave + RPL * i + lane / CH, slot = lane % CH;
-        const unsigned row_unit = (unsigned)__shfl((int)unit, RPL * i + lane / CH, kWave);
-        const unsigned kc = slot ^ (D == 128 ? R & 15 : (R >> 1) & 7);
-        const unsigned vc = (((slot >> 1) ^ (D == 128 ? R & 7 : (R >> 1) & 3)) << 1) | (slot & 1);
-        const bool here = row_unit != kNoUnit;
-        const char* ka = here ? reinterpret_cast<const char*>(p.k) + (size_t)(row_unit + kc) * 16 : zero;
-        const char* va = here ? reinterpret_cast<const char*>(p.v) + (size_t)(row_unit + vc) * 16 : zero;
-        kr[i] = *reinterpret_cast<const h8*>(ka);
-        vr[i] = *reinterpret_cast<const h8*>(va);
+        const unsigned unit = s_units[stage % 4][own_row + RPL * i];
+        const unsigned kx = D == 128 ? RPL * i & 15 : (RPL * i >> 1) & 7;
+        const unsigned vx = (D == 128 ? RPL * i & 7 : (RPL * i >> 1) & 3) << 1;
+        kr[i] = *reinterpret_cast<const h8*>(reinterpret_cast<const char*>(p.k) +
+                                             (size_t)(unit + (key_chunk ^ kx)) * 16);
+        vr[i] = *reinterpret_cast<const h8*>(reinterpret_cast<const char*>(p.v) +
+                                             (size_t)(unit + (value_chunk ^ vx)) * 16);
       }
     };
     auto store = [&](half_t* buf) {
@@ -754,18 +761,14 @@ __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(Wi
       }
     };
     const int stages = (count + SPAN - 1) / SPAN;
-    int slot_row, next_row;
-    const int page = locate(0, slot_row);
-    int next = locate(1, next_row);
-    load(place(0, page, slot_row));
-    // stage `at` into registers, if there is one
-    auto load_stage = [&](int at) {
-      if (at < stages) {
-        const unsigned unit = place(at, next, next_row);
-        next = locate(at + 1, next_row);
-        load(unit);
+#pragma unroll
+    for (int stage = 0; stage < 4; ++stage)
+      if (my_turn(stage)) {
+        look_up(stage);
+        if (stage < 3) put_units(stage);
       }
-    };
+    __syncthreads();
+    load(0);
 
     const h8 nothing = {0, 0, 0, 0, 0, 0, 0, 0};
     h8 qb[KS];
@@ -822,10 +825,13 @@ __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(Wi
     };
     // Position of place u of the tile.
     auto position = [&](int u) { return u < sinks ? u : u + gap; };
-    // Whether any of the wave's vectors sees some of a step.
-    auto seen = [&](int u0) {
-      const int p0 = position(u0);
-      return p0 < max_len && (position(u0 + 31) >= min_from || p0 < p.sinks);
+    // Steps that some of the wave's vectors see, and those of which all of them
+    // see all.
+    const int sink_steps = (int)((min((long)p.sinks, (long)count) + 31) / 32);
+    const int live_from = (min_from - gap) / 32, live_to = (max_len - gap + 31) / 32;
+    const int clear_from = (max_from - gap + 31) / 32, clear_to = (min_len - gap) / 32;
+    auto seen = [&](int step) {
+      return (step < sink_steps || step >= live_from) && step < live_to && max_len > 0;
     };
     f16v sc;
     auto scores = [&]() {
@@ -838,11 +844,10 @@ __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(Wi
     h8 w[2];
     // out of sight: positions from the length on and [p.sinks, from)
     const unsigned hidden = (unsigned)max(0, min(from, 0x7ffffffe) - p.sinks);
-    auto weigh = [&](int u0) {
+    auto weigh = [&](int step) {
       settle(sc);
-      const int p0 = position(u0), p1 = position(u0 + 31);
-      if (p1 >= min_len || (p0 < max_from && p1 >= sinks)) {  // not all of it in sight
-        const int first = u0 + 4 * (int)opaque(half);
+      if (step < clear_from || step >= clear_to) {
+        const int first = 32 * step + 4 * (int)opaque(half);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int pos = position(first + 8 * (e >> 2) + (e & 3));
@@ -883,23 +888,26 @@ __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(Wi
 
     // ---- the stages
     store(s_kv);
-    load_stage(1);
+    load(1);
     for (int i = 0; i < stages; ++i) {
       const unsigned buf = (unsigned)((i & 1) * STAGE * 2);
-      // stage i is in LDS, stage i - 1 has been read
+      // stage i and the units of stage i + 2 are in LDS, stage i - 1 has been read
       lds_barrier();
-      if (i + 1 < stages) store(s_kv + ((i + 1) & 1) * STAGE);
-      load_stage(i + 2);
+      store(s_kv + ((i + 1) & 1) * STAGE);
+      load(i + 2);
+      if (my_turn(i + 3)) put_units(i + 3);
+      if (my_turn(i + 4)) look_up(i + 4);
 #pragma unroll
       for (int s = 0; s < (PG > 1 ? 1 : 2); ++s) {
-        const int R0 = PG > 1 ? 32 * pg : 32 * s, u0 = i * SPAN + R0;
-        if (!seen(u0)) continue;
+        const int R0 = PG > 1 ? 32 * pg : 32 * s, step = i * (SPAN / 32) + R0 / 32;
+        if (!seen(step)) continue;
         read_keys(buf, R0);
+        __builtin_amdgcn_sched_barrier(0);
         scores();
         __builtin_amdgcn_sched_barrier(0);
         read_values(buf, R0);
         __builtin_amdgcn_sched_barrier(0);
-        weigh(u0);
+        weigh(step);
         add_values();
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -976,10 +984,10 @@ __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(Wi
       const int put = len > 0 ? row * p.q_heads + head : -1;
 #pragma unroll
       for (int i = 0; i < 32 / RPL; ++i) {
-        const int R = RPL * i + lane / CH, chunk = lane % CH;
+        const int R = RPL * i + lane / CH;
         const int to = __shfl(put, R, kWave);
-        const h8 val = *reinterpret_cast<const h8*>(rows + R * D + ((chunk ^ (R & (CH - 1))) << 3));
-        if (to >= 0) *reinterpret_cast<h8*>(p.out + (size_t)to * D + 8 * chunk) = val;
+        const h8 val = *reinterpret_cast<const h8*>(rows + R * D + ((slot ^ (R & (CH - 1))) << 3));
+        if (to >= 0) *reinterpret_cast<h8*>(p.out + (size_t)to * D + 8 * slot) = val;
       }
     }
     // A weight of 0 times an infinity or NaN of V that the vector does not see
