@@ -623,6 +623,15 @@ __device__ __forceinline__ unsigned opaque(unsigned v) {
   return v;
 }
 
+// The least of lanes 0 ... 31 (32 ... 63 hold the same), in all lanes.
+__device__ __forceinline__ int least_of_half(int v) {
+  v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x121, 0xF, 0xF, false));  // row_ror 1, 2, 4, 8
+  v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x122, 0xF, 0xF, false));
+  v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x124, 0xF, 0xF, false));
+  v = min(v, __builtin_amdgcn_update_dpp(v, v, 0x128, 0xF, 0xF, false));
+  return min(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16));
+}
+
 template <int D, int PG>
 __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(WindowParams p,
                                                                               int tiles,
@@ -661,6 +670,14 @@ __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(Wi
   // this lane's vector
   const int token = (32 * vg + col) / p.group, row = t0 + token;
   const int head = kvh * p.group + 32 * vg + col - token * p.group;
+  const int any_row = min(row, p.rows - 1);  // one that exists
+  const int row_len = p.valid[any_row];
+  h8 qb[KS];
+  {
+    const half_t* q = p.q + ((size_t)any_row * p.q_heads + head) * D;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qb[s] = load_h8(q + 16 * s + 8 * half);
+  }
 
   for (int run = 0; run < tokens;) {
     // ---- the run of tokens [run, run_end) of one request
@@ -682,24 +699,16 @@ __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(Wi
     run = run_end;
     int len = 0;
     if (table_row >= 0 && token >= run_at && token < run_end) {
-      len = p.valid[row];
-      if (len < 1 || len > capacity) len = 0;
+      len = row_len < 1 || row_len > capacity ? 0 : row_len;
     }
     const int from = len > 0 ? window_begin(p, len) : 0x7fffffff;
     // the wave's extremes, then the tile's
     int min_len = len > 0 ? len : 0x7fffffff, max_len = len, min_from = from,
         max_from = len > 0 ? from : 0;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      min_len = min(min_len, __shfl_xor(min_len, off, kWave));
-      max_len = max(max_len, __shfl_xor(max_len, off, kWave));
-      min_from = min(min_from, __shfl_xor(min_from, off, kWave));
-      max_from = max(max_from, __shfl_xor(max_from, off, kWave));
-    }
-    min_len = __builtin_amdgcn_readfirstlane(min_len);
-    max_len = __builtin_amdgcn_readfirstlane(max_len);
-    min_from = __builtin_amdgcn_readfirstlane(min_from);
-    max_from = __builtin_amdgcn_readfirstlane(max_from);
+    min_len = least_of_half(min_len);
+    max_len = -least_of_half(-max_len);
+    min_from = least_of_half(min_from);
+    max_from = -least_of_half(-max_from);
     if (lane == 0 && max_len > 0) {
       atomicMin(&s_low, min_from);
       atomicMax(&s_high, max_len);
@@ -770,13 +779,6 @@ __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(Wi
     __syncthreads();
     load(0);
 
-    const h8 nothing = {0, 0, 0, 0, 0, 0, 0, 0};
-    h8 qb[KS];
-    {
-      const half_t* q = p.q + ((size_t)row * p.q_heads + head) * D;
-#pragma unroll
-      for (int s = 0; s < KS; ++s) qb[s] = len > 0 ? load_h8(q + 16 * s + 8 * half) : nothing;
-    }
     f16v o[DT];
     float m = -INFINITY, sum = 0.0f;
 #pragma unroll
@@ -941,23 +943,25 @@ __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(Wi
         total += other == -INFINITY ? 0.0f : fast_exp2(other - top) * s_sum[g * VG + vg][col];
       }
       scale = m == -INFINITY ? 0.0f : fast_exp2(m - top) / total;
-      // the other groups' sums in fp32, a 32-dim tile a pass: group pg finishes
-      // the elements 4 pg ... 4 pg + 3 (dims 8 pg + 4 half ...) of it
+      // the groups' sums in fp32: group pg finishes the elements 4 pg ... 4 pg + 3
+      // (dims 8 pg + 4 half ...) of every 32-dim tile
       float* hand = reinterpret_cast<float*>(s_kv);
       constexpr int kTile = 16 * kWave;
-      static_assert(PG == 4 && sizeof(float) * WAVES * kTile <= sizeof(s_kv), "a pass fits");
+      static_assert(PG == 4 && sizeof(float) * WAVES * DT * kTile <= sizeof(s_kv), "the sums fit");
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          hand[(wave * DT + t) * kTile + e * kWave + lane] = o[t][e] * scale;
+      __syncthreads();
 #pragma unroll
       for (int t = 0; t < DT; ++t) {
-        if (t) __syncthreads();
-#pragma unroll
-        for (int e = 0; e < 16; ++e) hand[wave * kTile + e * kWave + lane] = o[t][e] * scale;
-        __syncthreads();
         float val[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int g = 0; g < PG; ++g)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            val[e] += hand[(g * VG + vg) * kTile + (4 * pg + e) * kWave + lane];
+            val[e] += hand[((g * VG + vg) * DT + t) * kTile + (4 * pg + e) * kWave + lane];
         if (len > 0)
           *reinterpret_cast<h4*>(p.out + ((size_t)row * p.q_heads + head) * D + 32 * t + 8 * pg +
                                  4 * half) =
