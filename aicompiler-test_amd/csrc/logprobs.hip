@@ -24,7 +24,6 @@ namespace {
 constexpr int kTopMax = 64;
 constexpr int kLpThreads = 256;
 constexpr int kLpWaves = kLpThreads / kWave;
-constexpr size_t kLpCounterBytes = 64u << 10;
 // Candidates a block ranks; one with more (many equal logits) picks its best
 // one by one.
 constexpr int kCandidates = 256;
@@ -409,6 +408,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
 // of 32003 11.9 us from 8 blocks a row, 16.8 from 2.  The few rows are bound by
 // the latency of the steps: logits, bound, ranks, arrival, join.
 constexpr int64_t kFill = 512;
+static_assert(kFill <= kSharedRows, "every shared row has its counter");
 struct LogprobPlan {
   int each, walk, count;
 };
@@ -425,9 +425,6 @@ bool logprob_shape(int64_t rows, int64_t vocabulary, int64_t top) {
   return rows > 0 && rows < (1LL << 24) && vocabulary > 0 && vocabulary < (1LL << 28) && top >= 0 &&
          top <= kTopMax && top <= vocabulary;
 }
-size_t logprob_counter_bytes(int64_t rows) {
-  return std::max(kLpCounterBytes, (size_t)(rows * 4 + 255) / 256 * 256);
-}
 
 }  // namespace
 }  // namespace tmc
@@ -437,7 +434,7 @@ using namespace tmc;
 extern "C" size_t tmc_logprobs_workspace_bytes(int64_t rows, int64_t vocabulary, int64_t top) {
   if (!logprob_shape(rows, vocabulary, top)) return 0;
   const int64_t parts = logprob_plan(rows, vocabulary).count;
-  return parts == 1 ? 0 : logprob_counter_bytes(rows) + (size_t)(rows * parts) * (20 + 8 * top);
+  return parts == 1 ? 0 : kCounterBytes + (size_t)(rows * parts) * (20 + 8 * top);
 }
 
 extern "C" int tmc_logprobs(const void* logits, int dtype, int64_t row_stride,
@@ -478,7 +475,7 @@ extern "C" int tmc_logprobs(const void* logits, int dtype, int64_t row_stride,
   p.count = plan.count;
   if (need) {
     p.arrivals = static_cast<int*>(workspace);
-    p.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + logprob_counter_bytes(rows));
+    p.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
   }
   const dim3 grid((unsigned)(rows * p.count));
   const hipStream_t s = as_stream(stream);

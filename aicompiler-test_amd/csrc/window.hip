@@ -157,7 +157,7 @@ __global__ __launch_bounds__(kWave) void window_plain_kernel(WindowParams p) {
 constexpr int kDecodeWaves = 4;
 constexpr int kDecodeBlocks = 512;  // two a CU
 constexpr int kDecodeLeast = 8;
-constexpr size_t kDecodeCounterBytes = kDecodeBlocks * sizeof(int);  // shared rows are fewer
+static_assert(kDecodeBlocks <= kSharedRows, "every shared row has its counter");
 
 struct DecodePlan {
   float* slots;   // [rows][kv_heads][splits][parts][heads][D + 2]
@@ -1121,7 +1121,7 @@ extern "C" size_t tmc_window_attention_workspace_bytes(int64_t batch, int64_t q_
   const int parts = decode_parts(units, head_dim, capacity, window, sinks);
   const int64_t heads = (q_heads / kv_heads + splits - 1) / splits;
   return parts < 2 ? 0
-                   : kDecodeCounterBytes +
+                   : kCounterBytes +
                          (size_t)units * parts * heads * (head_dim + 2) * sizeof(float);
 }
 
@@ -1163,7 +1163,7 @@ extern "C" int tmc_window_decode_attention(
   if (need) {
     plan.arrivals = static_cast<int*>(workspace);
     plan.slots = reinterpret_cast<float*>(static_cast<char*>(workspace) +
-                                          kDecodeCounterBytes);
+                                          kCounterBytes);
   }
   if (head_dim == 128)
     hipLaunchKernelGGL((window_decode_kernel<128, 16, 2>), dim3(blocks), dim3(kDecodeWaves * kWave), 0,
@@ -1196,7 +1196,11 @@ extern "C" int tmc_window_prefill_attention_f16(
       (uint64_t)pool_pages * (uint64_t)page_stride / 8 >= 0xFFFFFFFFull)
     return launch_plain(p, as_stream(stream));
   const int wide = 256 / p.group, narrow = 64 / p.group;  // tokens a tile
-  const bool split = (rows + wide - 1) / wide * kv_heads < 192;
+  // A block a CU: four narrow tiles, whose waves share the positions, while that
+  // is at most two rounds of blocks.  us, split and wide, 32 heads of 128 dims,
+  // window 2048: 64 wide tiles 38 and 79, 128 70 and 85, 160 103 and 87, 256 151
+  // and 101.
+  const bool split = (rows + wide - 1) / wide * kv_heads <= 128;
   const int tokens = split ? narrow : wide;
   const int tiles = (int)((rows + tokens - 1) / tokens);
   const dim3 grid((unsigned)(tiles * kv_heads)), block(kChunkWaves * kWave);

@@ -801,10 +801,11 @@ int tmc_copy_pages(const void *src, void *dst, const int32_t *pages, int64_t cou
  * whose pages belong to one request each and whose sampling is greedy. */
 
 /* Bytes of device workspace tmc_window_decode_attention needs for these
- * limits (capacity = page_size * max_pages; 0 when none is needed).  The
- * workspace must be zero before its first use; every launch leaves its
- * counters at zero, so it serves launches of any shapes, in any order, whose
- * needs it covers.  Launches that share one workspace must not overlap. */
+ * limits (capacity = page_size * max_pages; 0 when none is needed; a larger
+ * batch can need less).  The workspace is 16-byte aligned and must be zero
+ * before its first use; every launch leaves its counters at zero, so it serves
+ * launches of any shapes, in any order, whose needs it covers.  Launches that
+ * share one workspace must not overlap. */
 size_t tmc_window_attention_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads,
                                             int64_t head_dim, int64_t capacity, int64_t window,
                                             int64_t sinks);
@@ -880,8 +881,9 @@ int tmc_rebuild_tables(const int32_t *tables, const int32_t *parents, const int3
                        int64_t layers, int64_t table_rows, int64_t rows, int64_t max_pages,
                        int64_t pool_pages, void *stream);
 
-/* Bytes of device workspace tmc_logprobs needs (0 when none is needed; zeroed
- * and shared by the rules of tmc_window_attention_workspace_bytes). */
+/* Bytes of device workspace tmc_logprobs needs (0 when none is needed; by the
+ * rules of tmc_window_attention_workspace_bytes, and launches of both may use
+ * one workspace in turn). */
 size_t tmc_logprobs_workspace_bytes(int64_t rows, int64_t vocabulary, int64_t top);
 
 /* Log probabilities from logits [rows, vocabulary] (f32 or f16, rows

@@ -504,6 +504,80 @@ def test_graph_replays_and_streams(tmc, torch):
         assert torch.equal(away.view(torch.int16), eager.view(torch.int16)), step
 
 
+def test_one_workspace_for_attention_and_scores(tmc, torch):
+    """Launches of several shapes and of tmc_logprobs use one workspace in turn,
+    eagerly and in two captured graphs that share it."""
+    shapes = [(1, 8, 2, 128, 900), (6, 40, 1, 64, 700), (3, 4, 4, 128, 2000), (40, 8, 8, 64, 300)]
+    page, window, sinks = 16, 600, 4
+    vocab, top = 20000, 5
+    need = [tmc.logprobs_workspace_bytes(2, vocab, top)]
+    calls = []
+    for i, (b, qh, kvh, d, length) in enumerate(shapes):
+        pages = -(-length // page)
+        cache = Cache(torch, 31 + i, [set(range(length))] * b, kvh, d, page, pages)
+        need.append(tmc.window_attention_workspace_bytes(b, qh, kvh, d, pages * page, window, sinks))
+        q = torch.randn(b, qh * d, device="cuda").to(torch.float16)
+        valid = torch.full((b,), length, dtype=torch.int32, device="cuda")
+
+        def attend(out, ws, q=q, cache=cache, valid=valid, pages=pages, shape=shapes[i]):
+            b, qh, kvh, d, _ = shape
+            tmc.window_decode_attention(q, cache.k, cache.v, valid, cache.tables_dev, None, out, b,
+                                        qh, kvh, d, page, pages, cache.page_stride,
+                                        cache.head_stride, window, sinks, ws)
+        calls.append((attend, q.shape))
+    assert all(need)
+    logits = torch.randn(2, vocab, device="cuda")
+    tokens = torch.tensor([5, vocab - 1], dtype=torch.int32, device="cuda")
+
+    best = torch.empty(2, top, dtype=torch.int32, device="cuda")
+    best_lp = torch.empty(2, top, device="cuda")
+
+    def score(out, ws):
+        tmc.logprobs(logits, tokens, out[0], out[1], best, best_lp, ws)
+
+    def all_of_them(outs, lp, ws):
+        for (attend, _), out in zip(calls, outs):
+            attend(out, ws)
+            score(lp, ws)
+
+    def outputs():
+        return ([torch.zeros(shape, dtype=torch.float16, device="cuda") for _, shape in calls],
+                torch.zeros(2, 2, device="cuda"))
+
+    want, want_lp = outputs()
+    for (attend, _), out, n in zip(calls, want, need[1:]):
+        attend(out, torch.zeros(n // 4 + 1, device="cuda"))  # each on a workspace of its own
+    score(want_lp, torch.zeros(need[0] // 4 + 1, device="cuda"))
+    ws = torch.zeros(max(need) // 4 + 1, device="cuda")
+    graphs, results = [], []
+    for _ in range(2):
+        outs, lp = outputs()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            all_of_them(outs, lp, ws)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            all_of_them(outs, lp, ws)
+        graphs.append(graph)
+        results.append((outs, lp))
+    for _ in range(3):
+        for graph, (outs, lp) in zip(graphs, results):
+            for t in (*outs, lp):
+                t.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            for a, b in zip((*outs, lp), (*want, want_lp)):
+                assert torch.equal(a, b)
+        outs, lp = outputs()
+        all_of_them(outs, lp, ws)
+        torch.cuda.synchronize()
+        for a, b in zip((*outs, lp), (*want, want_lp)):
+            assert torch.equal(a, b)
+
+
 def test_wrappers_refuse(tmc, torch):
     kvh, qh, d, page, max_pages = 2, 8, 128, 16, 4
     k = torch.zeros(8, kvh, page, d, dtype=torch.float16, device="cuda")
