@@ -62,7 +62,10 @@ __device__ __forceinline__ size_t window_out(const WindowParams& p, int row, int
 // ------------------------------------------------------------ any geometry
 // One wave per (row, query head): 64 visible positions at a time, one per
 // lane for the scores (whole K rows in 16-byte chunks), then lanes over the
-// dims for P V.  Online softmax in fp32.
+// dims for P V.  Online softmax in fp32.  For the head dims that the matrix
+// core kernels do not take and pools of 64 GiB; at 128 dims it takes 94 us where
+// they take 7 (one request of 300 positions, 32 heads) and 10.3 ms where they
+// take 91 us (2048 tokens, window 2048).
 constexpr int kPlainMaxDim = 256;
 
 struct PlainScratch {  // of one wave
@@ -139,14 +142,15 @@ __global__ __launch_bounds__(kWave) void window_plain_kernel(WindowParams p) {
 }
 
 // ------------------------------------------------------------ one token a request
-// D = 64 and 128.  A step is 32 (D = 64) or 16 visible positions
-// of one (request, kv head) row.  A row is a block's, or, where rows are few,
-// shared by up to `parts` blocks in even shares of at least kDecodeLeast steps;
-// each writes a partial (max, sum, weighted) to the workspace and the last one
-// to arrive joins them, in block order.
+// D = 64 and 128.  A step is 32 (D = 64) or 16 visible positions of one
+// (request, kv head) row; kv heads of more than 16 query heads make a row for
+// every 16 or fewer of them.  A row is a block's, or, where rows are few, shared
+// by up to `parts` blocks in even shares of about kDecodeLeast steps or more; each
+// writes a partial (max, sum, weighted) to the workspace and the last one to
+// arrive joins them, in block order.
 //
-// Inside a block the waves take the steps of a part in turn.  Each wave has a
-// ring of kStages steps in LDS that only it touches, filled by 16-byte loads
+// Inside a block the waves take the steps of a share in turn.  Each wave has a
+// ring of STAGES steps in LDS that only it touches, filled by 16-byte loads
 // straight to LDS: no barrier, no register holds a load in flight, and a
 // stage is reloaded as soon as its operands are in registers.  K and V rows lie
 // in LDS as in their pages, 16-byte chunks (K) and 32-byte units (V) swizzled
@@ -154,11 +158,21 @@ __global__ __launch_bounds__(kWave) void window_plain_kernel(WindowParams p) {
 // does not exist reads a zero row.  Scores S^T = K Q^T (16 positions x 16
 // heads) leave lane (head j, group g) with positions 4g .. 4g+3, the order in
 // which O^T = V^T P^T wants its weights; V^T comes from transposing LDS reads.
+//
+// Bound by reading K and V: 64 requests, 8 kv heads of 128 dims, window 2048, 516
+// MB: 89 us, 5.8 TB/s (a large copy moves 5.2).  Two blocks of 64 KiB rings a CU
+// rather than one of 128 KiB (103 us).  Few rows are bound by latency: lengths,
+// pages, K and V, and at the join stores, arrival and loads, 3 to 4 us of it.
 constexpr int kDecodeWaves = 4;
 constexpr int kDecodeBlocks = 512;  // two a CU
-constexpr int kDecodeLeast = 8;
+constexpr int kDecodeLeast = 8, kDecodeAlone = 20;
 static_assert(kDecodeBlocks <= kSharedRows, "every shared row has its counter");
 
+// Blocks that share a row of `steps`, of at most `parts`.
+__host__ __device__ inline int decode_shares(int64_t steps, int64_t parts) {
+  const int64_t shares = steps <= kDecodeAlone ? (steps > 0) : (steps + kDecodeLeast - 1) / kDecodeLeast;
+  return (int)(shares < parts ? shares : parts);
+}
 struct DecodePlan {
   float* slots;   // [rows][kv_heads][splits][parts][heads][D + 2]
   int* arrivals;  // [rows][kv_heads][splits]
@@ -312,7 +326,7 @@ __global__ __launch_bounds__(kDecodeWaves * kWave, 2) void window_decode_kernel(
   const int heads = min(plan.heads, p.group - split * plan.heads);
   const int valid = p.valid[row];
   const int steps = steps_of<STEP>(p, valid, row < active);
-  const int shares = min(plan.parts, (steps + kDecodeLeast - 1) / kDecodeLeast);
+  const int shares = decode_shares(steps, plan.parts);
   if (part >= shares) return;
   const int even = steps / shares, over = steps - even * shares;
   const int first_step = part * even + min(part, over);
@@ -605,6 +619,13 @@ __global__ __launch_bounds__(kDecodeWaves * kWave, 2) void window_decode_kernel(
 // positions of a stage each; the four partials join at the end.  K and V go
 // through registers, loaded one stage ahead of the LDS one; one barrier a
 // stage.
+//
+// Bound by the products, the softmax and the LDS together: 2048 tokens, 32 heads
+// of 128 dims, window 2048: 91 us, 760 TFLOP/s; matrix cores, vector ALUs and LDS
+// are busy 36, 41 and 44% of the time, the products with loads alone take 78 us.
+// Measured and no faster: 4 waves of 64 vectors with the products of one tile
+// beside the softmax of the other (130), opposite phases or priorities for the
+// two waves of a SIMD, loads placed among the products, K read a step ahead.
 //
 // A tile's positions are those that any of its tokens sees, sinks first.
 // Positions that a vector does not see are masked in the steps where that can
@@ -1091,21 +1112,22 @@ bool decode_shape(int64_t head_dim) {
 int64_t decode_splits(int64_t q_heads, int64_t kv_heads) {
   return (q_heads / kv_heads + 15) / 16;
 }
-// Blocks a row of `units`: as many as fill the card's resident blocks, while a
-// full row leaves each kDecodeLeast steps, and not more than the square root of
-// the steps: a step takes about as long as one more partial at the join (0.16
-// and 0.22 us at 4 query heads of 128 dims).  The join takes 16 partials at a
-// time.  Both sides, 8 kv heads of 128 dims, one request of 8192 positions: 13.7
-// us at 16 parts, 15.0 at 32, 23 at 64, 42 alone.
+// Blocks a row, one of `units`: as many as fill the card's resident blocks, while
+// a full row leaves each kDecodeLeast steps, and not more than the square root
+// of the steps: a step takes about as long as one more partial at the join (0.16
+// and 0.22 us at 4 query heads of 128 dims), which takes 16 at a time.  Rows of
+// up to kDecodeAlone steps are a block's.  us, shared and alone, one request, 8
+// kv heads of 128 dims: 512 positions 7.6 and 9.8, 1024 8.1 and 14.5, 4096 11.2
+// and 43, 8192 13.8 (15.0 in 32 parts, 23 in 64) and 80; 300 positions, 32 kv
+// heads, 7.2 and 7.1; 24 requests of 500 positions, 8 kv heads of 64, 10.0 and 8.2.
 int decode_parts(int64_t units, int64_t head_dim, int64_t capacity, int64_t window,
                  int64_t sinks) {
   const int64_t step = head_dim == 128 ? 16 : 32;
   const int64_t seen = std::min(capacity, std::min(window, capacity) + std::min(sinks, capacity));
   const int64_t steps = (seen + step - 1) / step;
-  const int64_t parts = std::min<int64_t>({(steps + kDecodeLeast - 1) / kDecodeLeast,
-                                           (kDecodeBlocks + units - 1) / units,
-                                           (int64_t)std::ceil(std::sqrt((double)steps))});
-  return (int)(parts > 16 ? parts / 16 * 16 : parts);
+  const int parts = decode_shares(steps, std::min((kDecodeBlocks + units - 1) / units,
+                                                  (int64_t)std::ceil(std::sqrt((double)steps))));
+  return parts > 16 ? parts / 16 * 16 : parts;
 }
 }  // namespace
 }  // namespace tmc

@@ -507,12 +507,14 @@ def test_graph_replays_and_streams(tmc, torch):
 def test_one_workspace_for_attention_and_scores(tmc, torch):
     """Launches of several shapes and of tmc_logprobs use one workspace in turn,
     eagerly and in two captured graphs that share it."""
-    shapes = [(1, 8, 2, 128, 900), (6, 40, 1, 64, 700), (3, 4, 4, 128, 2000), (40, 8, 8, 64, 300)]
-    page, window, sinks = 16, 600, 4
+    # batch, heads, kv heads, dim, length, window; the last two share no row
+    shapes = [(1, 8, 2, 128, 900, 600), (3, 4, 4, 128, 2000, 600), (6, 40, 1, 64, 3000, 2500),
+              (40, 8, 8, 64, 1500, 1400), (6, 40, 1, 64, 700, 600), (40, 8, 8, 64, 300, 600)]
+    page, sinks = 16, 4
     vocab, top = 20000, 5
     need = [tmc.logprobs_workspace_bytes(2, vocab, top)]
     calls = []
-    for i, (b, qh, kvh, d, length) in enumerate(shapes):
+    for i, (b, qh, kvh, d, length, window) in enumerate(shapes):
         pages = -(-length // page)
         cache = Cache(torch, 31 + i, [set(range(length))] * b, kvh, d, page, pages)
         need.append(tmc.window_attention_workspace_bytes(b, qh, kvh, d, pages * page, window, sinks))
@@ -520,12 +522,12 @@ def test_one_workspace_for_attention_and_scores(tmc, torch):
         valid = torch.full((b,), length, dtype=torch.int32, device="cuda")
 
         def attend(out, ws, q=q, cache=cache, valid=valid, pages=pages, shape=shapes[i]):
-            b, qh, kvh, d, _ = shape
+            b, qh, kvh, d, _, window = shape
             tmc.window_decode_attention(q, cache.k, cache.v, valid, cache.tables_dev, None, out, b,
                                         qh, kvh, d, page, pages, cache.page_stride,
                                         cache.head_stride, window, sinks, ws)
         calls.append((attend, q.shape))
-    assert all(need)
+    assert all(need[:5])
     logits = torch.randn(2, vocab, device="cuda")
     tokens = torch.tensor([5, vocab - 1], dtype=torch.int32, device="cuda")
 
