@@ -888,7 +888,7 @@ def page_moves(moves, pools, pool_pages, page_size):
     positions) for move_pages, checked (tmc_check_page_moves): existing pages,
     none written twice, none both read and written."""
     import torch
-    host_moves = torch.tensor(moves, dtype=torch.int32).reshape(-1, 4).contiguous()
+    host_moves = torch.tensor(moves, dtype=torch.int32).reshape(len(moves), 4).contiguous()
     check(lib().tmc_check_page_moves(_ptr(host_moves), host_moves.shape[0], pools, pool_pages,
                                      page_size), "tmc_check_page_moves")
     return host_moves.cuda()
@@ -911,6 +911,8 @@ def move_pages(k_pools, v_pools, moves, heads, page_size, head_dim, page_stride=
     if moves.dim() != 2 or moves.shape[1] != 4:
         raise TmcError(f"{what}: moves must be [count, 4]")
     device, dtype = torch.cuda.current_device(), k_pools[0].dtype
+    if dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        raise TmcError(f"{what}: pools must be float16, bfloat16 or float32, not {dtype}")
     move_list, = _addresses(what, device, torch.int32, ("moves", moves, 0))
     pools = [*k_pools, *v_pools]
     tensor = torch.Tensor
@@ -968,7 +970,9 @@ def logprobs(logits, tokens, logprob, entropy=None, top_tokens=None, top_logprob
     device = torch.cuda.current_device()
     if logits.get_device() != device:
         _refuse(what, device, logits.dtype, "logits", logits, 0)
-    code = F32 if logits.dtype is torch.float32 else _dtype_code(logits)
+    if logits.dtype not in (torch.float32, torch.float16):
+        raise TmcError(f"{what}: logits must be f32 or f16, not {logits.dtype}")
+    code = F32 if logits.dtype is torch.float32 else F16
     rows, vocabulary = logits.shape
     top = 0
     if top_tokens is not None:

@@ -5,9 +5,9 @@
 #include "tmc_device.hpp"
 
 #include <algorithm>
-#include <map>
+#include <exception>
 #include <set>
-#include <vector>
+#include <utility>
 
 namespace tmc {
 namespace {
@@ -93,21 +93,25 @@ extern "C" int tmc_check_page_moves(const int32_t* moves, int64_t count, int64_t
   TMC_REQUIRE(moves || count == 0, "Page moves: null pointer.");
   TMC_REQUIRE(count >= 0 && pools > 0 && pool_pages > 0 && page_size > 0,
               "Page moves: invalid shape.");
-  std::set<std::pair<int32_t, int32_t>> sources, targets;
-  for (int64_t i = 0; i < count; ++i) {
-    const int32_t *m = moves + 4 * i, pool = m[0], from = m[1], to = m[2], positions = m[3];
-    const std::string which = "Page moves: move " + std::to_string(i);
-    TMC_REQUIRE(pool >= 0 && pool < pools && from >= 0 && from < pool_pages && to >= 0 &&
-                    to < pool_pages,
-                which + " names a pool or page that does not exist.");
-    TMC_REQUIRE(positions >= 1 && positions <= page_size,
-                which + " must copy 1 to page_size positions.");
-    TMC_REQUIRE(targets.insert({pool, to}).second, which + " writes a page that another move writes.");
-    sources.insert({pool, from});
+  try {
+    std::set<std::pair<int32_t, int32_t>> sources, targets;
+    for (int64_t i = 0; i < count; ++i) {
+      const int32_t *m = moves + 4 * i, pool = m[0], from = m[1], to = m[2], positions = m[3];
+      const std::string which = "Page moves: move " + std::to_string(i);
+      TMC_REQUIRE(pool >= 0 && pool < pools && from >= 0 && from < pool_pages && to >= 0 &&
+                      to < pool_pages,
+                  which + " names a pool or page that does not exist.");
+      TMC_REQUIRE(positions >= 1 && positions <= page_size,
+                  which + " must copy 1 to page_size positions.");
+      TMC_REQUIRE(targets.insert({pool, to}).second, which + " writes a page that another move writes.");
+      sources.insert({pool, from});
+    }
+    for (const auto& t : targets)
+      TMC_REQUIRE(!sources.count(t), "Page moves: page " + std::to_string(t.second) + " of pool " +
+                                         std::to_string(t.first) + " is both read and written.");
+  } catch (const std::exception& e) {  // out of memory
+    TMC_REQUIRE(false, std::string("Page moves: ") + e.what());
   }
-  for (const auto& t : targets)
-    TMC_REQUIRE(!sources.count(t), "Page moves: page " + std::to_string(t.second) + " of pool " +
-                                       std::to_string(t.first) + " is both read and written.");
   return 0;
 }
 

@@ -203,6 +203,7 @@ def test_wrappers_refuse(tmc, torch):
                        ((logits, tokens[:1], out), "tokens holds"), ((logits, tokens, None), "go together"),
                        ((logits, tokens, out, None, tt, None), "top_logprobs"),
                        ((logits, tokens, out, None, tt, tl[:, :2].contiguous()), "rows, top"),
-                       ((logits.bfloat16(), tokens, out), "f32 or f16")):
+                       ((logits.bfloat16(), tokens, out), "f32 or f16"),
+                       ((logits.double(), tokens, out), "f32 or f16")):
         with pytest.raises(RuntimeError, match=text):
             tmc.logprobs(*args)

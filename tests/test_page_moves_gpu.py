@@ -97,6 +97,7 @@ def test_bad_moves_copy_nothing(tmc, torch):
     tmc.move_pages([k], [v], moves, heads, page, d)
     assert same(torch, k, kw) and same(torch, v, vw)
     tmc.move_pages([k], [v], moves[:0], heads, page, d)
+    tmc.move_pages([k], [v], tmc.page_moves([], 1, pages, page), heads, page, d)
     assert same(torch, k, kw)
 
 
@@ -169,7 +170,8 @@ def test_wrappers_refuse(tmc, torch):
     for args, text in ((([k], [k, k], moves), "as many"), (([], [], moves), "as many"),
                        (([k.cpu()], [k], moves), "current GPU"), (([k], [k], moves.cpu()), "current GPU"),
                        (([k], [k.float()], moves), "must be"), (([k], [k], moves.long()), "moves must"),
-                       (([k], [k], moves[0]), "count, 4")):
+                       (([k], [k], moves[0]), "count, 4"),
+                       (([k.double()], [k.double()], moves), "float16, bfloat16")):
         with pytest.raises(RuntimeError, match=text):
             tmc.move_pages(*args, 2, 4, 8)
     tables = torch.zeros(1, 3, 4, dtype=torch.int32, device="cuda")
