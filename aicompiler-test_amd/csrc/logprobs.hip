@@ -139,6 +139,10 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
   float floor_v = -INFINITY;  // once `top` are held: the last of them
   vec next[LOADS];
   fetch(begin, next);
+  // the given token's logit comes beside the row's, not at the end
+  const int token = p.tokens ? p.tokens[row] : -1;
+  const bool known = token >= 0 && token < p.vocab;
+  const float given = known ? (float)x[token] : 0.0f;
   for (int part_at = begin; part_at < end; part_at += PART) {
     float v[EACH];
 #pragma unroll
@@ -306,10 +310,27 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
     if (threadIdx.x == 0)
       __hip_atomic_store(p.arrivals + row, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     const size_t first = (size_t)row * p.count;
+    // What the first round of each of the steps below needs, in flight at once.
+    const size_t here = first + min(lane, p.count - 1);
+    const float part_m = __hip_atomic_load(maxima + here, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const double part_s = __hip_atomic_load(sums + 2 * here, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const double part_t =
+        __hip_atomic_load(sums + 2 * here + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const int total = p.count * top;
+    const long long* from = keys + first * top;
+    constexpr int kAhead = 4;  // keys a thread loads at once
+    long long key[kAhead];
+    auto load_keys = [&](int i) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        key[u] = __hip_atomic_load(from + min(i + u * kLpThreads, total - 1), __ATOMIC_RELAXED,
+                                   __HIP_MEMORY_SCOPE_AGENT);
+    };
+    if (top > 0) load_keys(threadIdx.x);
     // each wave by itself: the maximum, then the sums relative to it, lane by
     // lane over the parts and then over the lanes: the same order each time
-    row_m = -INFINITY;
-    for (int i = lane; i < p.count; i += kWave)
+    row_m = lane < p.count ? part_m : -INFINITY;
+    for (int i = lane + kWave; i < p.count; i += kWave)
       row_m = fmaxf(row_m, __hip_atomic_load(maxima + first + i, __ATOMIC_RELAXED,
                                              __HIP_MEMORY_SCOPE_AGENT));
     // A bound that at least `top` keys reach: where `deep` parts are needed to
@@ -321,7 +342,8 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
                                               __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     row_m = wave_max(row_m);
     row_s = row_t = 0.0;
-    for (int i = lane; i < p.count; i += kWave)
+    if (lane < p.count) add_mass(part_m, part_s, part_t, row_m, row_s, row_t);
+    for (int i = lane + kWave; i < p.count; i += kWave)
       add_mass(__hip_atomic_load(maxima + first + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
                __hip_atomic_load(sums + 2 * (first + i), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
                __hip_atomic_load(sums + 2 * (first + i) + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
@@ -344,15 +366,8 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
       __syncthreads();
       const long long bound = s_best[0];
       __syncthreads();
-      const int total = p.count * top;
-      const long long* from = keys + first * top;
-      constexpr int kAhead = 4;  // keys a thread loads at once
       for (int i = threadIdx.x; i < total; i += kAhead * kLpThreads) {
-        long long key[kAhead];
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u)
-          key[u] = __hip_atomic_load(from + min(i + u * kLpThreads, total - 1), __ATOMIC_RELAXED,
-                                     __HIP_MEMORY_SCOPE_AGENT);
+        if (i != (int)threadIdx.x) load_keys(i);
 #pragma unroll
         for (int u = 0; u < kAhead; ++u)
           if (i + u * kLpThreads < total && key[u] != kNoKey && key[u] >= bound) {
@@ -386,10 +401,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
   const float log_s = row_m == -INFINITY ? __builtin_nanf("") : logf((float)row_s);
   if (threadIdx.x == 0) {
     if (p.entropy) p.entropy[row] = log_s - (float)row_t / (float)row_s;
-    if (p.tokens) {
-      const int token = p.tokens[row];
-      if (token >= 0 && token < p.vocab) p.logprob[row] = (float)x[token] - row_m - log_s;
-    }
+    if (known) p.logprob[row] = given - row_m - log_s;
   }
   if ((int)threadIdx.x < top) {
     const long long key = s_best[threadIdx.x];
