@@ -10,6 +10,8 @@
 // Bound by reading the logits once.  A block holds a part of a row in
 // registers at a time, so the maximum, the sums and the alternatives are three
 // passes over registers, not over memory, while the next part is on its way.
+// Each wave keeps the candidates for the alternatives that it meets, without
+// waiting for the others; they are ranked together at the row's end.
 // Where several blocks share a row, the last to arrive joins them in their
 // order.
 #include "tmc_abi.hpp"
@@ -24,9 +26,10 @@ namespace {
 constexpr int kTopMax = 64;
 constexpr int kLpThreads = 256;
 constexpr int kLpWaves = kLpThreads / kWave;
-// Candidates a block ranks; one with more (many equal logits) picks its best
-// one by one.
-constexpr int kCandidates = 256;
+constexpr int kCandidates = kLpThreads;  // that a block ranks at once
+constexpr int kWaveKeys = 128;           // candidates a wave holds
+static_assert(kLpWaves * kTopMax <= kCandidates && kTopMax + kWave <= kWaveKeys,
+              "the waves' best fit a ranking, a wave's best and a round of new ones its list");
 constexpr long long kNoKey = (long long)0x8000000000000000ull;
 
 struct LogprobParams {
@@ -79,23 +82,68 @@ __device__ __forceinline__ void add_mass(float m, double s, double t, float high
 }
 
 // The best `top` of `count` distinct keys (at most kCandidates) to the places their rank
-// gives them, the rest of the places empty.  Ends with a barrier.
+// gives them, the rest of the places empty.  Up to 64 keys: four threads a key.
+// Ends with a barrier.
 __device__ __forceinline__ void rank_keys(const long long* keys, int count, int top,
                                           long long* out) {
-  const int me = threadIdx.x;
-  if (me < top) out[me] = kNoKey;
+  const bool few = count * 4 <= kLpThreads;
+  const int me = few ? threadIdx.x >> 2 : threadIdx.x, step = few ? 4 : 1;
+  if ((int)threadIdx.x < top) out[threadIdx.x] = kNoKey;
   __syncthreads();
   const long long mine = me < count ? keys[me] : kNoKey;
-  if (mine != kNoKey) {
-    int rank = 0, o = 0;
-    for (; o + 8 <= count; o += 8)
+  int rank = 0, o = few ? threadIdx.x & 3 : 0;
+  for (; o + 7 * step < count; o += 8 * step)
 #pragma unroll
-      for (int u = 0; u < 8; ++u) rank += keys[o + u] > mine ? 1 : 0;
-    for (; o < count; ++o) rank += keys[o] > mine ? 1 : 0;
-    if (rank < top) out[rank] = mine;
+    for (int u = 0; u < 8; ++u) rank += keys[o + u * step] > mine ? 1 : 0;
+  for (; o < count; o += step) rank += keys[o] > mine ? 1 : 0;
+  if (few) {
+    rank += __shfl_xor(rank, 1, kWave);
+    rank += __shfl_xor(rank, 2, kWave);
   }
+  if (mine != kNoKey && rank < top) out[rank] = mine;
   __syncthreads();
 }
+
+// The candidates of one wave, in LDS that only it touches: every key above
+// `floor`, behind which at least `top` keys of the block's row are known to lie.
+struct WaveKeys {
+  long long* list;
+  int held;
+  float floor_v;
+  long long floor;
+
+  // A key a lane, where `in` and above the floor; there is room for them.
+  __device__ __forceinline__ void add(float v, int index, bool in) {
+    const long long key = key_of(v, index);
+    in = in && key > floor;
+    const unsigned long long mask = __builtin_amdgcn_ballot_w64(in);
+    const int lane = threadIdx.x & (kWave - 1);
+    if (in) list[held + __builtin_popcountll(mask & ((1ull << lane) - 1))] = key;
+    held += __builtin_popcountll(mask);
+  }
+  // The best `top`, in order; the last of them is then the floor.
+  __device__ __forceinline__ void keep_best(int top) {
+    const int lane = threadIdx.x & (kWave - 1);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const long long a = lane < held ? list[lane] : kNoKey;
+    const long long b = lane + kWave < held ? list[lane + kWave] : kNoKey;
+    int rank_a = 0, rank_b = 0;
+    for (int o = 0; o < held; ++o) {
+      const long long other = list[o];
+      rank_a += other > a ? 1 : 0;
+      rank_b += other > b ? 1 : 0;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (a != kNoKey && rank_a < top) list[rank_a] = a;
+    if (b != kNoKey && rank_b < top) list[rank_b] = b;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    held = min(held, top);
+    if (held == top) {
+      floor = list[top - 1];
+      floor_v = key_value(floor);
+    }
+  }
+};
 
 // EACH: elements a lane holds; a part is kLpThreads * EACH elements.  A block
 // walks `walk` parts of its row, the next one's loads in flight.
@@ -107,12 +155,12 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
   typedef T vec __attribute__((ext_vector_type(VEC)));
   // rows start anywhere on an element boundary
   typedef vec unaligned __attribute__((aligned(sizeof(T))));
-  static_assert(kCandidates == kLpThreads, "a thread a candidate");
+  __shared__ __align__(16) long long s_lists[kLpWaves][kWaveKeys];
   __shared__ __align__(16) long long s_keys[kCandidates];
   __shared__ __align__(16) long long s_best[kTopMax];
   __shared__ float s_m[kLpWaves], s_bound[kLpWaves];
   __shared__ double s_s[kLpWaves], s_t[kLpWaves];
-  __shared__ int s_reach[kLpWaves], s_found, s_last;
+  __shared__ int s_reach[kLpWaves], s_held[kLpWaves], s_found, s_last;
   const int split = blockIdx.x % p.count, row = blockIdx.x / p.count;
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const T* x = static_cast<const T*>(p.logits) + (size_t)row * p.stride;
@@ -134,9 +182,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
   };
   // the lane's own maximum and sums (relative to it)
   float m = -INFINITY, s = 0.0f, t = 0.0f;
-  if (threadIdx.x == 0) s_found = 0;
-  int held = 0;             // keys in s_best
-  float floor_v = -INFINITY;  // once `top` are held: the last of them
+  WaveKeys best{s_lists[wave], 0, -INFINITY, kNoKey};
   vec next[LOADS];
   fetch(begin, next);
   // the given token's logit comes beside the row's, not at the end
@@ -172,11 +218,9 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
     }
     if (top == 0) continue;
 
-    // ---- a bound that at least `top` of the block's elements reach: what is
-    // held, or from the lanes' greatest, of which each wave finds what its
-    // share reaches
-    float bound = floor_v;
-    if (held < top) {
+    // ---- a bound that at least `top` of the first part's elements reach, from the
+    // lanes' greatest: each wave finds what its share of them reaches
+    if (part_at == begin) {
       // waves whose lanes all hold elements
       const int full = min(kLpWaves, (end - part_at + kWave * (EACH - VEC)) / (kWave * EACH));
       const int need = full > 0 ? (top + full - 1) / full : top;
@@ -194,68 +238,65 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
         s_reach[wave] = reach;
       }
       __syncthreads();
-      bound = -INFINITY;
 #pragma unroll
       for (int w = 0; w < kLpWaves; ++w) {
         int total = 0;
 #pragma unroll
         for (int u = 0; u < kLpWaves; ++u) total += s_bound[u] >= s_bound[w] ? s_reach[u] : 0;
-        if (total >= top) bound = fmaxf(bound, s_bound[w]);
+        if (total >= top) best.floor_v = fmaxf(best.floor_v, s_bound[w]);
       }
     }
-    // ---- the elements that reach it, beside the ones held
-    if (__builtin_amdgcn_ballot_w64(mine >= bound) != 0) {
+    // ---- the elements that reach it: no other wave is waited for
+    const int lanes = __builtin_popcountll(__builtin_amdgcn_ballot_w64(mine >= best.floor_v));
+    if (lanes != 0) {
+      auto place = [&](int i) { return part_at + own + i / VEC * kWave * VEC + i % VEC; };
+      int more = lanes * EACH;  // at most
+      if (best.held + more > kWaveKeys) {
+        more = 0;
 #pragma unroll
-      for (int i = 0; i < EACH; ++i) {
-        const int at = part_at + own + i / VEC * kWave * VEC + i % VEC;
-        const bool in = v[i] >= bound && at < end;  // a NaN never
-        if (__builtin_amdgcn_ballot_w64(in) != 0 && in) {
-          const int place = held + atomicAdd(&s_found, 1);
-          if (place < kCandidates) s_keys[place] = key_of(v[i], at);
+        for (int i = 0; i < EACH; ++i)
+          more += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v[i] >= best.floor_v));
+      }
+      if (best.held + more <= kWaveKeys) {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+          const bool in = v[i] >= best.floor_v;  // (a NaN never)
+          if (__builtin_amdgcn_ballot_w64(in) != 0) best.add(v[i], place(i), in && place(i) < end);
+        }
+      } else {  // many (equal logits, say): the best of them now and then
+#pragma clang loop unroll(disable)
+        for (int i = 0; i < EACH; ++i) {
+          if (best.held > kWaveKeys - kWave) best.keep_best(top);
+          best.add(v[0], place(i), v[0] >= best.floor_v && place(i) < end);
+#pragma unroll
+          for (int e = 0; e + 1 < EACH; ++e) v[e] = v[e + 1];
         }
       }
-    }
-    __syncthreads();
-    const int found = s_found;
-    if (found > 0) {  // the same in every thread
-      if ((int)threadIdx.x < held) s_keys[threadIdx.x] = s_best[threadIdx.x];
-      if (held + found <= kCandidates) {
-        __syncthreads();
-        rank_keys(s_keys, held + found, top, s_best);
-      } else {
-        // too many: one a round, the best behind the one before
-        long long last = 0x7FFFFFFFFFFFFFFFll;
-        const long long mine_held = (int)threadIdx.x < held ? s_best[threadIdx.x] : kNoKey;
-        for (int k = 0; k < top; ++k) {
-          long long best = mine_held < last ? mine_held : kNoKey;
-#pragma unroll
-          for (int i = 0; i < EACH; ++i) {
-            const int at = part_at + own + i / VEC * kWave * VEC + i % VEC;
-            const long long key = key_of(v[i], at);
-            if (at < end && v[i] == v[i] && key < last && key > best) best = key;
-          }
-#pragma unroll
-          for (int off = 1; off < kWave; off <<= 1) {
-            const long long other = __shfl_xor(best, off, kWave);
-            best = other > best ? other : best;
-          }
-          __syncthreads();
-          if (lane == 0) s_keys[wave] = best;
-          __syncthreads();
-#pragma unroll
-          for (int w = 0; w < kLpWaves; ++w) best = s_keys[w] > best ? s_keys[w] : best;
-          if (threadIdx.x == 0) s_best[k] = best;
-          last = best;
-        }
-        __syncthreads();
-      }
-      held = min(top, held + found);
-      if (held == top) floor_v = key_value(s_best[top - 1]);
-      if (threadIdx.x == 0) s_found = 0;
-      __syncthreads();
     }
   }
-  if (top > 0 && (int)threadIdx.x >= held && (int)threadIdx.x < top) s_best[threadIdx.x] = kNoKey;
+  if (top > 0) {
+    // ---- the waves' candidates together
+    if (lane == 0) s_held[wave] = best.held;
+    __syncthreads();
+    int total = 0, before = 0;
+#pragma unroll
+    for (int w = 0; w < kLpWaves; ++w) total += s_held[w];
+    if (total > kCandidates) {  // the same in every thread
+      best.keep_best(top);      // (of fewer than that, nothing changes but their order)
+      __syncthreads();
+      if (lane == 0) s_held[wave] = best.held;
+      __syncthreads();
+      total = 0;
+#pragma unroll
+      for (int w = 0; w < kLpWaves; ++w) total += s_held[w];
+    }
+#pragma unroll
+    for (int w = 0; w < kLpWaves; ++w) before += w < wave ? s_held[w] : 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    for (int i = lane; i < best.held; i += kWave) s_keys[before + i] = best.list[i];
+    __syncthreads();
+    rank_keys(s_keys, total, top, s_best);
+  }
   {
     // the lanes of a row of 16 in 32 bits, rows and waves in 64
     const float high = wave_max(m);
@@ -414,11 +455,11 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
 // How a row is shared out: elements a lane holds, parts a block, blocks a row.
 // Rows in the hundreds take a block each; fewer are cut until there are kFill
 // blocks or parts run out, the fewest rows into small parts.  MI355X, fp32:
-// 2048 rows of 32003, 5 alternatives 64 us with 16 elements a lane, 92 with 32
-// (two waves a SIMD), 71 with 8; without alternatives 51.5 (5.1 TB/s).  16 rows
-// of 32000, 20 alternatives 12.6 us from 16 blocks of 8 elements a row; 64 rows
-// of 32003 11.9 us from 8 blocks a row, 16.8 from 2.  The few rows are bound by
-// the latency of the steps: logits, bound, ranks, arrival, join.
+// 2048 rows of 32003, 5 alternatives 58 us with 16 elements a lane, 62 with 8;
+// without alternatives 48.5 (5.4 TB/s; a large copy moves 5.2).  16 rows of 32000,
+// 20 alternatives 11.7 us from 16 blocks a row; 64 rows 12.8 us from 8 blocks a
+// row, 13.3 from 4, 18.2 from 2; 200 rows 19.4 from 3, 27.5 from one.  The few
+// rows are bound by the latency of the steps: logits, bound, ranks, arrival, join.
 constexpr int64_t kFill = 512;
 static_assert(kFill <= kSharedRows, "every shared row has its counter");
 struct LogprobPlan {

@@ -107,6 +107,20 @@ def test_best_tokens_all_in_the_last_parts(tmc, torch):
         check(torch, logits, tokens, top, run(tmc, torch, logits, tokens, top))
 
 
+@pytest.mark.parametrize("rows,vocab", [(600, 32003), (3, 32003), (600, 5000)])
+@pytest.mark.parametrize("top", [1, 20, 64])
+@pytest.mark.parametrize("order", ["rising", "falling", "equal", "steps"])
+def test_rows_that_fill_the_candidates(tmc, torch, rows, vocab, top, order):
+    """Rows in whose every part all elements, none, or hundreds of equal ones reach
+    the best so far."""
+    at = torch.arange(vocab, device="cuda", dtype=torch.float32)
+    row = {"rising": at / vocab, "falling": -at / vocab, "equal": torch.zeros_like(at) + 0.5,
+           "steps": torch.floor(at / 300)}[order]
+    logits = (row[None] + torch.arange(rows, device="cuda")[:, None] / 7).contiguous()
+    tokens = torch.arange(rows, dtype=torch.int32, device="cuda") % vocab
+    check(torch, logits, tokens, top, run(tmc, torch, logits, tokens, top))
+
+
 def test_rows_without_a_distribution(tmc, torch):
     """NaN, +inf and empty rows: NaN log probabilities, the tokens still in the
     greedy order, and their neighbours untouched by it."""
