@@ -52,7 +52,7 @@ struct LogprobParams {
 // index.
 __device__ __forceinline__ long long key_of(float v, int index) {
   const int b = __builtin_bit_cast(int, v + 0.0f);
-  const int order = b >= 0 ? b : b ^ 0x7FFFFFFF;
+  const int order = b ^ (b >> 31 & 0x7FFFFFFF);
   return ((long long)order << 32) | (unsigned)~index;
 }
 __device__ __forceinline__ float key_value(long long key) {
@@ -112,13 +112,12 @@ struct WaveKeys {
   float floor_v;
   long long floor;
 
-  // A key a lane, where `in` and above the floor; there is room for them.
-  __device__ __forceinline__ void add(float v, int index, bool in) {
-    const long long key = key_of(v, index);
-    in = in && key > floor;
+  // A key a lane, where `in`; there is room for them.
+  __device__ __forceinline__ void add(long long key, bool in) {
     const unsigned long long mask = __builtin_amdgcn_ballot_w64(in);
-    const int lane = threadIdx.x & (kWave - 1);
-    if (in) list[held + __builtin_popcountll(mask & ((1ull << lane) - 1))] = key;
+    const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32),
+                                                 __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0));
+    if (in) list[held + before] = key;
     held += __builtin_popcountll(mask);
   }
   // The best `top`, in order; the last of them is then the floor.
@@ -211,7 +210,8 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
       for (int i = 0; i < EACH; ++i) {
         const float d = v[i] - shift, e = fast_exp2(d * 1.44269504f);
         s4[i & 3] += e;
-        t4[i & 3] += e == 0.0f ? 0.0f : e * d;
+        // (finite: 0 times it is 0; a NaN is in e)
+        t4[i & 3] = __fmaf_rn(e, fmaxf(d, -1e30f), t4[i & 3]);
       }
       s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
       t = (t4[0] + t4[1]) + (t4[2] + t4[3]);
@@ -257,17 +257,19 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
         for (int i = 0; i < EACH; ++i)
           more += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v[i] >= best.floor_v));
       }
-      if (best.held + more <= kWaveKeys) {
+      if (best.held + more <= kWaveKeys && best.floor == kNoKey && best.floor_v != -INFINITY) {
+        // (what lies past the end is -inf)
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
           const bool in = v[i] >= best.floor_v;  // (a NaN never)
-          if (__builtin_amdgcn_ballot_w64(in) != 0) best.add(v[i], place(i), in && place(i) < end);
+          if (__builtin_amdgcn_ballot_w64(in) != 0) best.add(key_of(v[i], place(i)), in);
         }
-      } else {  // many (equal logits, say): the best of them now and then
+      } else {  // no bound, or many (equal logits, say): the best of them now and then
 #pragma clang loop unroll(disable)
         for (int i = 0; i < EACH; ++i) {
           if (best.held > kWaveKeys - kWave) best.keep_best(top);
-          best.add(v[0], place(i), v[0] >= best.floor_v && place(i) < end);
+          const long long key = key_of(v[0], place(i));
+          best.add(key, v[0] >= best.floor_v && place(i) < end && key > best.floor);
 #pragma unroll
           for (int e = 0; e + 1 < EACH; ++e) v[e] = v[e + 1];
         }
@@ -455,11 +457,12 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
 // How a row is shared out: elements a lane holds, parts a block, blocks a row.
 // Rows in the hundreds take a block each; fewer are cut until there are kFill
 // blocks or parts run out, the fewest rows into small parts.  MI355X, fp32:
-// 2048 rows of 32003, 5 alternatives 58 us with 16 elements a lane, 62 with 8;
-// without alternatives 48.5 (5.4 TB/s; a large copy moves 5.2).  16 rows of 32000,
-// 20 alternatives 11.7 us from 16 blocks a row; 64 rows 12.8 us from 8 blocks a
-// row, 13.3 from 4, 18.2 from 2; 200 rows 19.4 from 3, 27.5 from one.  The few
-// rows are bound by the latency of the steps: logits, bound, ranks, arrival, join.
+// 2048 rows of 32003, 5 alternatives 55 us with 16 elements a lane, 60 with 8;
+// without alternatives 47.7 (5.5 TB/s; a large copy moves 5.2).  16 rows of 32000,
+// 20 alternatives 11.6 us from 16 blocks a row; 64 rows 12.4 us from 8 blocks a
+// row, 12.7 from 4, 17.4 from 2; 200 rows 18.5 from 3, 27.9 from one.  Many rows
+// are bound by the vector ALUs and the memory alike, few by the latency of the
+// steps: logits, bound, ranks, arrival, join.
 constexpr int64_t kFill = 512;
 static_assert(kFill <= kSharedRows, "every shared row has its counter");
 struct LogprobPlan {
