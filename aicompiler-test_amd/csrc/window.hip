@@ -164,9 +164,9 @@ __global__ __launch_bounds__(kWave) void window_plain_kernel(WindowParams p) {
 // rather than one of 128 KiB (103 us).  Few rows are bound by latency: lengths,
 // pages, K and V, and at the join stores, arrival and loads, 3 to 4 us of it.
 constexpr int kDecodeWaves = 4;
-constexpr int kDecodeBlocks = 512;  // two a CU
+constexpr int kDecodeCus = 256;  // of an MI355X
 constexpr int kDecodeLeast = 8, kDecodeAlone = 20;
-static_assert(kDecodeBlocks <= kSharedRows, "every shared row has its counter");
+static_assert(kDecodeCus <= kSharedRows, "every shared row has its counter");
 
 // Blocks that share a row of `steps`, of at most `parts`.
 __host__ __device__ inline int decode_shares(int64_t steps, int64_t parts) {
@@ -1112,21 +1112,25 @@ bool decode_shape(int64_t head_dim) {
 int64_t decode_splits(int64_t q_heads, int64_t kv_heads) {
   return (q_heads / kv_heads + 15) / 16;
 }
-// Blocks a row, one of `units`: as many as fill the card's resident blocks, while
-// a full row leaves each kDecodeLeast steps, and not more than the square root
-// of the steps: a step takes about as long as one more partial at the join (0.16
-// and 0.22 us at 4 query heads of 128 dims), which takes 16 at a time.  Rows of
-// up to kDecodeAlone steps are a block's.  us, shared and alone, one request, 8
-// kv heads of 128 dims: 512 positions 7.6 and 9.8, 1024 8.1 and 14.5, 4096 11.2
-// and 43, 8192 13.8 (15.0 in 32 parts, 23 in 64) and 80; 300 positions, 32 kv
-// heads, 7.2 and 7.1; 24 requests of 500 positions, 8 kv heads of 64, 10.0 and 8.2.
+// Blocks a row, one of `units`: as many as give every CU one, twice that where
+// shares are then long (rows of unlike lengths), while a full row leaves each
+// kDecodeLeast steps, and not more than the square root of the steps: a step
+// takes about as long as one more partial at the join (0.16 and 0.22 us at 4
+// query heads of 128 dims), which takes 16 at a time.  Rows of up to
+// kDecodeAlone steps are a block's.  us, 8 kv heads of 128 dims.  One request,
+// shared and alone: 512 positions 7.6 and 9.8, 1024 8.1 and 14.5, 4096 11.2 and
+// 43, 8192 13.8 (15.0 in 32 parts, 23 in 64) and 80; 300 positions, 32 kv heads,
+// 7.2 and 7.1.  16 requests, window 1024: 15.4 in 2 parts, 16.4 in 4 or 1; window
+// 4096 35.9 in 2, 33.5 in 4; 32 requests 26.4 in 2, 23.6 in 1.
 int decode_parts(int64_t units, int64_t head_dim, int64_t capacity, int64_t window,
                  int64_t sinks) {
   const int64_t step = head_dim == 128 ? 16 : 32;
   const int64_t seen = std::min(capacity, std::min(window, capacity) + std::min(sinks, capacity));
   const int64_t steps = (seen + step - 1) / step;
-  const int parts = decode_shares(steps, std::min((kDecodeBlocks + units - 1) / units,
-                                                  (int64_t)std::ceil(std::sqrt((double)steps))));
+  int64_t most = (kDecodeCus + units - 1) / units;
+  if (most > 1 && steps / most > 96) most *= 2;
+  const int parts =
+      decode_shares(steps, std::min(most, (int64_t)std::ceil(std::sqrt((double)steps))));
   return parts > 16 ? parts / 16 * 16 : parts;
 }
 }  // namespace

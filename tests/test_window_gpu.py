@@ -507,9 +507,10 @@ def test_graph_replays_and_streams(tmc, torch):
 def test_one_workspace_for_attention_and_scores(tmc, torch):
     """Launches of several shapes and of tmc_logprobs use one workspace in turn,
     eagerly and in two captured graphs that share it."""
-    # batch, heads, kv heads, dim, length, window; the last two share no row
+    # batch, heads, kv heads, dim, length, window; the last three share no row
     shapes = [(1, 8, 2, 128, 900, 600), (3, 4, 4, 128, 2000, 600), (6, 40, 1, 64, 3000, 2500),
-              (40, 8, 8, 64, 1500, 1400), (6, 40, 1, 64, 700, 600), (40, 8, 8, 64, 300, 600)]
+              (16, 8, 8, 64, 1500, 1400), (40, 8, 8, 64, 1500, 1400), (6, 40, 1, 64, 700, 600),
+              (40, 8, 8, 64, 300, 600)]
     page, sinks = 16, 4
     vocab, top = 20000, 5
     need = [tmc.logprobs_workspace_bytes(2, vocab, top)]
