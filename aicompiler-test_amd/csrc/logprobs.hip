@@ -40,7 +40,7 @@ struct LogprobParams {
   int32_t* top_tokens;
   float* top_logprobs;
   float* parts;   // [rows][count](m, S, T), then [rows][count][top] values, then indices
-  int* arrivals;  // [rows]
+  int* arrivals;  // [rows], kCounterStride apart
   long stride;
   int rows, vocab, top;
   int count;      // blocks a row
@@ -344,14 +344,14 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     if (threadIdx.x == 0) {
-      s_last = __hip_atomic_fetch_add(p.arrivals + row, 1, __ATOMIC_RELAXED,
+      s_last = __hip_atomic_fetch_add(p.arrivals + row * kCounterStride, 1, __ATOMIC_RELAXED,
                                       __HIP_MEMORY_SCOPE_AGENT) == p.count - 1;
       s_found = 0;
     }
     __syncthreads();
     if (!s_last) return;
     if (threadIdx.x == 0)
-      __hip_atomic_store(p.arrivals + row, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(p.arrivals + row * kCounterStride, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     const size_t first = (size_t)row * p.count;
     // What the first round of each of the steps below needs, in flight at once.
     const size_t here = first + min(lane, p.count - 1);

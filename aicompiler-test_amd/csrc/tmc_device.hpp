@@ -23,9 +23,10 @@ constexpr int kWave = 64;
 // Arrival counters at the front of the workspaces of windowed attention and log
 // probabilities: in one place and left at zero, so that the launches of both
 // can share a workspace.  Neither shares a row among blocks where there are
-// 512 rows or more.
-constexpr int kSharedRows = 512;
-constexpr size_t kCounterBytes = kSharedRows * sizeof(int);
+// 512 rows or more.  Each counter has 128 bytes to itself: arrivals at one line
+// wait for each other.
+constexpr int kSharedRows = 512, kCounterStride = 32;
+constexpr size_t kCounterBytes = kSharedRows * kCounterStride * sizeof(int);
 
 // ------------------------------------------------------------------ loads
 __device__ __forceinline__ h8 load_h8(const half_t* p) {

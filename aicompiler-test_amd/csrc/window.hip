@@ -175,7 +175,7 @@ __host__ __device__ inline int decode_shares(int64_t steps, int64_t parts) {
 }
 struct DecodePlan {
   float* slots;   // [rows][kv_heads][splits][parts][heads][D + 2]
-  int* arrivals;  // [rows][kv_heads][splits]
+  int* arrivals;  // [rows][kv_heads][splits], kCounterStride apart
   int parts, splits, heads;
 };
 
@@ -556,7 +556,7 @@ __global__ __launch_bounds__(kDecodeWaves * kWave, 2) void window_decode_kernel(
     // the last of the row's blocks joins the partials, in block order (every
     // word is written and read at agent scope; the stores have completed
     // before the arrival is counted)
-    int* counter = plan.arrivals + unit;
+    int* counter = plan.arrivals + unit * kCounterStride;
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     if (threadIdx.x == 0)
