@@ -21,31 +21,33 @@ struct MoveParams {
   int first_pool, pools, pool_pages, heads, page_size;
   long page_bytes, head_bytes;  // strides
   int row_bytes;                // one head's position
-  int parts;                    // of a head's positions
+  int parts, head_blocks;       // blocks a head, or blocks the heads share
 };
 
-// One block per (move, K or V, kMoveUnits of the move's positions of every
-// kMoveHeads-th head), in units of UNIT bytes: pure copying, bound by memory,
-// so a thread copies unit by unit (eight loads ahead of their stores took 1.5
-// times as long over a large pool).  Four copies each of 8 requests' last pages in
-// 32 layers, 20 MB: 12 us, against 8 at a large copy's rate; a quarter of 1 GiB
-// of pools compacted: 104 us, 5.2 TB/s, that rate.  Pages of 256 positions, 8 heads of
-// 128: 13 us where a block a page took 40.
-constexpr int kMoveHeads = 2, kMoveUnits = 1024;
+// One block per (move, K or V, about kMoveUnits of the page: a part of one head's
+// positions, or every head_blocks-th head), in units of UNIT bytes: pure copying,
+// bound by memory, so a thread copies unit by unit (eight loads ahead of their
+// stores took 1.5 times as long over a large pool).  Four copies each of 8
+// requests' last pages in 32 layers, 20 MB: 12 us, against 8 at a large copy's
+// rate; a quarter of 1 GiB of pools compacted: 104 us, 5.2 TB/s, that rate.  Pages
+// of 256 positions, 8 heads of 128: 13 us where a block a page took 40; pages of
+// 32 positions, 32 heads, compacted: 10 us where two blocks a page took 17.
+constexpr int kMoveUnits = 1024;
 template <typename UNIT>
 __global__ __launch_bounds__(256) void move_pages_kernel(MoveParams p) {
   const int4 m = p.moves[blockIdx.x];
   const int from = m.y, to = m.z, count = m.w;
-  if (m.x < p.first_pool || m.x - p.first_pool >= p.pools || from < 0 || from >= p.pool_pages || to < 0 ||
-      to >= p.pool_pages || from == to || count < 1 || count > p.page_size)
+  if (m.x < p.first_pool || m.x - p.first_pool >= p.pools || from < 0 ||
+      from >= p.pool_pages || to < 0 || to >= p.pool_pages || from == to || count < 1 ||
+      count > p.page_size)
     return;
   const int pool = m.x - p.first_pool;
   char* base = static_cast<char*>(blockIdx.y ? p.value[pool] : p.key[pool]);
   const char* src = base + (size_t)from * p.page_bytes;
   char* dst = base + (size_t)to * p.page_bytes;
   const unsigned run = (unsigned)((long)count * p.row_bytes / (int)sizeof(UNIT));  // units a head
-  const int head_blocks = min(p.heads, kMoveHeads), part = blockIdx.z / head_blocks;
-  for (int h = blockIdx.z - part * head_blocks; h < p.heads; h += head_blocks) {
+  const int part = blockIdx.z / p.head_blocks;
+  for (int h = blockIdx.z - part * p.head_blocks; h < p.heads; h += p.head_blocks) {
     const UNIT* s = reinterpret_cast<const UNIT*>(src + (size_t)h * p.head_bytes);
     UNIT* d = reinterpret_cast<UNIT*>(dst + (size_t)h * p.head_bytes);
     for (unsigned first = part * kMoveUnits; first < run; first += p.parts * kMoveUnits)
@@ -160,8 +162,11 @@ extern "C" int tmc_move_pages(void* const* key_pools, void* const* value_pools, 
     p.head_bytes = (long)head_stride * size;
     p.row_bytes = (int)head_dim * size;
     const int unit = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 2;
-    p.parts = (int)std::min<int64_t>((page_size * p.row_bytes / unit + kMoveUnits - 1) / kMoveUnits, 64);
-    const dim3 grid((unsigned)count, 2, (unsigned)(p.parts * std::min<int64_t>(heads, kMoveHeads)));
+    const int64_t units = page_size * p.row_bytes / unit;  // a head's
+    p.parts = (int)std::min<int64_t>((units + kMoveUnits - 1) / kMoveUnits, 64);
+    const int64_t together = std::max<int64_t>(kMoveUnits / units, 1);  // heads a block
+    p.head_blocks = (int)std::min<int64_t>((heads + together - 1) / together, 512);
+    const dim3 grid((unsigned)count, 2, (unsigned)(p.parts * p.head_blocks));
     if (bits % 16 == 0)
       hipLaunchKernelGGL((move_pages_kernel<uint4>), grid, dim3(256), 0, s, p);
     else if (bits % 4 == 0)
