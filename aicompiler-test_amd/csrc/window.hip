@@ -163,7 +163,6 @@ __global__ __launch_bounds__(kWave) void window_plain_kernel(WindowParams p) {
 // MB: 89 us, 5.8 TB/s (a large copy moves 5.2).  Two blocks of 64 KiB rings a CU
 // rather than one of 128 KiB (103 us).  Few rows are bound by latency: lengths,
 // pages, K and V, and at the join stores, arrival and loads, 3 to 4 us of it.
-constexpr int kDecodeWaves = 4;
 constexpr int kDecodeCus = 256;  // of an MI355X
 constexpr int kDecodeLeast = 8, kDecodeAlone = 20;
 static_assert(kDecodeCus <= kSharedRows, "every shared row has its counter");
@@ -298,19 +297,19 @@ __device__ __forceinline__ int steps_of(const WindowParams& p, int valid, bool a
   return (min(p.sinks, begin) + valid - begin + STEP - 1) / STEP;
 }
 
-template <int D, int STEP, int STAGES>
-__global__ __launch_bounds__(kDecodeWaves * kWave, 2) void window_decode_kernel(WindowParams p,
-                                                                             DecodePlan plan) {
+template <int D, int STEP, int STAGES, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave, 2) void window_decode_kernel(WindowParams p,
+                                                                         DecodePlan plan) {
   constexpr int KS = D / 32, DT = D / 16, CH = D / 8, TILES = STEP / 16;
   constexpr int RPL = kWave / CH, LOADS = STEP / RPL;  // rows a load, loads of K (of V) a step
   constexpr int STAGE = 2 * STEP * D;                  // halves
-  constexpr int THREADS = kDecodeWaves * kWave;
-  __shared__ __align__(16) half_t s_ring[kDecodeWaves * STAGES * STAGE];
-  __shared__ int s_pages[kDecodeWaves * STAGES * kWave];
+  constexpr int THREADS = WAVES * kWave;
+  __shared__ __align__(16) half_t s_ring[WAVES * STAGES * STAGE];
+  __shared__ int s_pages[WAVES * STAGES * kWave];
   __shared__ int s_last;
   typedef __attribute__((address_space(3))) void lds_void;
   typedef __attribute__((address_space(1))) const void global_void;
-  static_assert(sizeof(s_ring) >= kDecodeWaves * 16 * (D + 2) * sizeof(float),
+  static_assert(sizeof(s_ring) >= WAVES * 16 * (D + 2) * sizeof(float),
                 "the waves' results fit the ring");
 
   const int lane = threadIdx.x & (kWave - 1);
@@ -454,19 +453,19 @@ __global__ __launch_bounds__(kDecodeWaves * kWave, 2) void window_decode_kernel(
     }
   };
 
-  // ---- the wave's steps: every kDecodeWaves-th of the part
+  // ---- the wave's steps: every WAVES-th of the part
   const int mine = first_step + wave;
   int slot_row[STAGES];  // of the step that a stage takes next
   {
     int first_page[STAGES], first_row[STAGES];
 #pragma unroll
     for (int st = 0; st < STAGES; ++st)
-      first_page[st] = *locate(mine + st * kDecodeWaves, first_row[st]);
+      first_page[st] = *locate(mine + st * WAVES, first_row[st]);
 #pragma unroll
     for (int st = 0; st < STAGES; ++st) {
-      const int32_t* next = locate(mine + (STAGES + st) * kDecodeWaves, slot_row[st]);
-      if (mine + st * kDecodeWaves < last_step)
-        issue(place(mine + st * kDecodeWaves, first_page[st], first_row[st]), next, st);
+      const int32_t* next = locate(mine + (STAGES + st) * WAVES, slot_row[st]);
+      if (mine + st * WAVES < last_step)
+        issue(place(mine + st * WAVES, first_page[st], first_row[st]), next, st);
     }
   }
   // One step out of its stage, and the stage loaded again.  BODY: every step
@@ -474,8 +473,8 @@ __global__ __launch_bounds__(kDecodeWaves * kWave, 2) void window_decode_kernel(
   auto turn = [&](auto stage, auto body, int step) {
     constexpr int ST = decltype(stage)::value;
     constexpr bool BODY = decltype(body)::value;
-    const int again = step + STAGES * kDecodeWaves;
-    if (BODY || step + (STAGES - 1) * kDecodeWaves < last_step)
+    const int again = step + STAGES * WAVES;
+    if (BODY || step + (STAGES - 1) * WAVES < last_step)
       wait_loads<(2 * LOADS + 1) * (STAGES - 1)>();
     else
       wait_loads<0>();
@@ -486,7 +485,7 @@ __global__ __launch_bounds__(kDecodeWaves * kWave, 2) void window_decode_kernel(
     read_values<D, STEP, ST * STAGE * 2>(value_at, v);
     if (BODY || again < last_step) {
       const unsigned unit = place(again, page, slot_row[ST]);
-      issue(unit, locate(again + STAGES * kDecodeWaves, slot_row[ST]), ST);
+      issue(unit, locate(again + STAGES * WAVES, slot_row[ST]), ST);
     }
     consume(step, k, v);
   };
@@ -494,26 +493,26 @@ __global__ __launch_bounds__(kDecodeWaves * kWave, 2) void window_decode_kernel(
     constexpr bool BODY = decltype(body)::value;
     turn(std::integral_constant<int, 0>{}, body, step);
     if constexpr (STAGES > 1)
-      if (BODY || step + kDecodeWaves < last_step)
-        turn(std::integral_constant<int, 1>{}, body, step + kDecodeWaves);
+      if (BODY || step + WAVES < last_step)
+        turn(std::integral_constant<int, 1>{}, body, step + WAVES);
     if constexpr (STAGES > 2)
-      if (BODY || step + 2 * kDecodeWaves < last_step)
-        turn(std::integral_constant<int, 2>{}, body, step + 2 * kDecodeWaves);
+      if (BODY || step + 2 * WAVES < last_step)
+        turn(std::integral_constant<int, 2>{}, body, step + 2 * WAVES);
     if constexpr (STAGES > 3)
-      if (BODY || step + 3 * kDecodeWaves < last_step)
-        turn(std::integral_constant<int, 3>{}, body, step + 3 * kDecodeWaves);
+      if (BODY || step + 3 * WAVES < last_step)
+        turn(std::integral_constant<int, 3>{}, body, step + 3 * WAVES);
   };
   int step = mine;
-  for (; step + (2 * STAGES - 1) * kDecodeWaves < last_step; step += STAGES * kDecodeWaves)
+  for (; step + (2 * STAGES - 1) * WAVES < last_step; step += STAGES * WAVES)
     round(std::true_type{}, step);
-  for (; step < last_step; step += STAGES * kDecodeWaves) round(std::false_type{}, step);
+  for (; step < last_step; step += STAGES * WAVES) round(std::false_type{}, step);
 
   // ---- the waves meet in LDS (the ring: every load into it has landed)
   lsum = cross_sum<16>(lsum);
   bad = __syncthreads_or(bad);
   float* s_max = reinterpret_cast<float*>(s_ring);  // [waves][16]
-  float* s_sum = s_max + kDecodeWaves * 16;
-  float* s_out = s_sum + kDecodeWaves * 16;         // [waves][heads][D]
+  float* s_sum = s_max + WAVES * 16;
+  float* s_out = s_sum + WAVES * 16;         // [waves][heads][D]
   if (j < heads) {
     if (g == 0) {
       s_max[wave * 16 + j] = m;
@@ -532,10 +531,10 @@ __global__ __launch_bounds__(kDecodeWaves * kWave, 2) void window_decode_kernel(
     const int head = i / (D / 2), d = i % (D / 2) * 2;
     float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kDecodeWaves; ++w) top = fmaxf(top, s_max[w * 16 + head]);
+    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, s_max[w * 16 + head]);
     float sum = 0.0f, val0 = 0.0f, val1 = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kDecodeWaves; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       const float high = s_max[w * 16 + head];
       const float scale = high == -INFINITY ? 0.0f : fast_exp2(high - top);
       sum += scale * s_sum[w * 16 + head];
@@ -1191,12 +1190,18 @@ extern "C" int tmc_window_decode_attention(
     plan.slots = reinterpret_cast<float*>(static_cast<char*>(workspace) +
                                           kCounterBytes);
   }
-  if (head_dim == 128)
-    hipLaunchKernelGGL((window_decode_kernel<128, 16, 2>), dim3(blocks), dim3(kDecodeWaves * kWave), 0,
-                       as_stream(stream), p, plan);
-  else
-    hipLaunchKernelGGL((window_decode_kernel<64, 32, 2>), dim3(blocks), dim3(kDecodeWaves * kWave), 0,
-                       as_stream(stream), p, plan);
+  // Two waves a SIMD: of two blocks, or of one where there is one a CU.  us, 4 waves
+  // and 8, one request: 8192 positions 13.7 and 13.0, 300 positions of 32 kv heads
+  // 7.1 and 6.5 (four stages a ring instead: 14.6 and 7.4).
+#define TMC_DECODE(DIM, STEP, WAVES)                                                             \
+  hipLaunchKernelGGL((window_decode_kernel<DIM, STEP, 2, WAVES>), dim3(blocks), dim3(WAVES * kWave), \
+                     0, as_stream(stream), p, plan)
+  if (head_dim == 128) {
+    if (blocks <= kDecodeCus) TMC_DECODE(128, 16, 8); else TMC_DECODE(128, 16, 4);
+  } else {
+    if (blocks <= kDecodeCus) TMC_DECODE(64, 32, 8); else TMC_DECODE(64, 32, 4);
+  }
+#undef TMC_DECODE
   return check_launch("window_decode_kernel");
 }
 
