@@ -779,20 +779,16 @@ def _refuse(what, device, dtype, name, t, count):
     raise TmcError(f"{what}: {name} holds {t.numel()} elements, {count} are needed")
 
 
-def _addresses(what, device, dtype, *operands):
-    """Device addresses of (name, tensor or None, elements needed), after a
-    refusal of what a kernel on the current GPU could not read: host tensors,
-    tensors of another GPU or type, gaps between elements, too few of them."""
-    found = []
-    for name, t, count in operands:
-        if t is None:
-            found.append(None)
-            continue
-        if t.get_device() != device or t.dtype is not dtype or not t.is_contiguous() or \
-                t.numel() < count:
-            _refuse(what, device, dtype, name, t, count)
-        found.append(t.data_ptr())
-    return found
+def _address(what, device, dtype, name, t, count):
+    """Device address of a tensor (None: NULL), after a refusal of what a kernel
+    on the current GPU could not read: host tensors, tensors of another GPU or
+    type, gaps between elements, fewer than `count` of them."""
+    if t is None:
+        return None
+    if t.get_device() != device or t.dtype is not dtype or not t.is_contiguous() or \
+            t.numel() < count:
+        _refuse(what, device, dtype, name, t, count)
+    return t.data_ptr()
 
 
 def _workspace(what, device, t):
@@ -801,11 +797,10 @@ def _workspace(what, device, t):
         return None, 0
     if t.get_device() != device or not t.is_contiguous():
         _refuse(what, device, t.dtype, "workspace", t, 0)
-    return t.data_ptr(), t.numel() * t.element_size()
+    return t.data_ptr(), t.nbytes
 
 
-def _launch_stream(what, device, stream):
-    import torch
+def _launch_stream(torch, what, device, stream):
     if stream is None:
         return torch._C._cuda_getCurrentRawStream(device)
     if stream.device.index != device:
@@ -815,7 +810,7 @@ def _launch_stream(what, device, stream):
 
 def _window_pages(what, k_pool, v_pool, rows, q_heads, kv_heads, head_dim, max_pages, page_stride,
                   pool_pages):
-    if min(rows, q_heads, kv_heads, head_dim, max_pages, page_stride) < 1:
+    if rows < 1 or q_heads < 1 or kv_heads < 1 or head_dim < 1 or max_pages < 1 or page_stride < 1:
         raise TmcError(f"{what}: rows, heads, head_dim, pages and strides must be positive")
     held = min(k_pool.numel(), v_pool.numel()) // page_stride
     if pool_pages is None:
@@ -843,20 +838,20 @@ def window_decode_attention(q, k_pool, v_pool, valid_lengths, tables, active, ou
     device = torch.cuda.current_device()
     pool_pages = _window_pages(what, k_pool, v_pool, max_batch, q_heads, kv_heads, head_dim,
                                max_pages, page_stride, pool_pages)
-    width = q_heads * head_dim
-    queries, keys, values, output = _addresses(
-        what, device, torch.float16, ("q", q, max_batch * width), ("k_pool", k_pool, 0),
-        ("v_pool", v_pool, 0),
-        ("out", out, packed_activation_elements(max_batch, width) if layout == Y_PACKED
-         else max_batch * width))
-    lengths, table, rows = _addresses(
-        what, device, torch.int32, ("valid_lengths", valid_lengths, max_batch),
-        ("tables", tables, max_batch * max_pages), ("active", active, 1))
+    f16, i32, width = torch.float16, torch.int32, q_heads * head_dim
+    room = packed_activation_elements(max_batch, width) if layout == Y_PACKED else max_batch * width
     space, space_bytes = _workspace(what, device, workspace)
     check(lib().tmc_window_decode_attention(
-        queries, keys, values, lengths, table, rows, output, F16, max_batch, q_heads, kv_heads,
-        head_dim, page_size, max_pages, pool_pages, page_stride, head_stride, window, sinks, space,
-        space_bytes, layout, _launch_stream(what, device, stream)), what)
+        _address(what, device, f16, "q", q, max_batch * width),
+        _address(what, device, f16, "k_pool", k_pool, 0),
+        _address(what, device, f16, "v_pool", v_pool, 0),
+        _address(what, device, i32, "valid_lengths", valid_lengths, max_batch),
+        _address(what, device, i32, "tables", tables, max_batch * max_pages),
+        _address(what, device, i32, "active", active, 1),
+        _address(what, device, f16, "out", out, room),
+        F16, max_batch, q_heads, kv_heads, head_dim, page_size, max_pages, pool_pages, page_stride,
+        head_stride, window, sinks, space, space_bytes, layout,
+        _launch_stream(torch, what, device, stream)), what)
 
 
 def window_prefill_attention(q, k_pool, v_pool, valid_lengths, tables, row_table, active, out,
@@ -869,18 +864,19 @@ def window_prefill_attention(q, k_pool, v_pool, valid_lengths, tables, row_table
     device = torch.cuda.current_device()
     pool_pages = _window_pages(what, k_pool, v_pool, rows, q_heads, kv_heads, head_dim, max_pages,
                                page_stride, pool_pages)
-    width = q_heads * head_dim
-    queries, keys, values, output = _addresses(
-        what, device, torch.float16, ("q", q, rows * width), ("k_pool", k_pool, 0),
-        ("v_pool", v_pool, 0), ("out", out, rows * width))
-    lengths, table, of_row, count = _addresses(
-        what, device, torch.int32, ("valid_lengths", valid_lengths, rows),
-        ("tables", tables, max_pages), ("row_table", row_table, rows), ("active", active, 1))
+    f16, i32, width = torch.float16, torch.int32, q_heads * head_dim
     table_rows = 1 if row_table is None else tables.numel() // max_pages
     check(lib().tmc_window_prefill_attention_f16(
-        queries, keys, values, lengths, table, of_row, table_rows, count, output, rows, q_heads,
-        kv_heads, head_dim, page_size, max_pages, pool_pages, page_stride, head_stride, window,
-        sinks, _launch_stream(what, device, stream)), what)
+        _address(what, device, f16, "q", q, rows * width),
+        _address(what, device, f16, "k_pool", k_pool, 0),
+        _address(what, device, f16, "v_pool", v_pool, 0),
+        _address(what, device, i32, "valid_lengths", valid_lengths, rows),
+        _address(what, device, i32, "tables", tables, max_pages),
+        _address(what, device, i32, "row_table", row_table, rows), table_rows,
+        _address(what, device, i32, "active", active, 1),
+        _address(what, device, f16, "out", out, rows * width),
+        rows, q_heads, kv_heads, head_dim, page_size, max_pages, pool_pages, page_stride,
+        head_stride, window, sinks, _launch_stream(torch, what, device, stream)), what)
 
 
 def page_moves(moves, pools, pool_pages, page_size):
@@ -913,7 +909,7 @@ def move_pages(k_pools, v_pools, moves, heads, page_size, head_dim, page_stride=
     device, dtype = torch.cuda.current_device(), k_pools[0].dtype
     if dtype not in (torch.float16, torch.bfloat16, torch.float32):
         raise TmcError(f"{what}: pools must be float16, bfloat16 or float32, not {dtype}")
-    move_list, = _addresses(what, device, torch.int32, ("moves", moves, 0))
+    move_list = _address(what, device, torch.int32, "moves", moves, 0)
     pools = [*k_pools, *v_pools]
     tensor = torch.Tensor
     if set(map(tensor.get_device, pools)) != {device} or \
@@ -929,7 +925,7 @@ def move_pages(k_pools, v_pools, moves, heads, page_size, head_dim, page_stride=
     check(lib().tmc_move_pages(first, first + count * size, count,
                                move_list, moves.shape[0], _dtype_code(k_pools[0]), pool_pages,
                                heads, page_size, head_dim, page_stride, head_stride,
-                               _launch_stream(what, device, stream)), what)
+                               _launch_stream(torch, what, device, stream)), what)
 
 
 def rebuild_tables(tables, out, pool_pages, parents=None, remap=None, tail_slots=None, tails=None,
@@ -944,13 +940,16 @@ def rebuild_tables(tables, out, pool_pages, parents=None, remap=None, tail_slots
                        "layers and pages")
     device = torch.cuda.current_device()
     layers, rows, max_pages = out.shape
-    old, new, parent, renamed, slots, tail = _addresses(
-        what, device, torch.int32, ("tables", tables, 0), ("out", out, 0),
-        ("parents", parents, rows), ("remap", remap, layers * pool_pages),
-        ("tail_slots", tail_slots, rows), ("tails", tails, layers * rows))
-    check(lib().tmc_rebuild_tables(old, parent, renamed, slots, tail, new, layers, tables.shape[1],
-                                   rows, max_pages, pool_pages,
-                                   _launch_stream(what, device, stream)), what)
+    i32 = torch.int32
+    check(lib().tmc_rebuild_tables(
+        _address(what, device, i32, "tables", tables, 0),
+        _address(what, device, i32, "parents", parents, rows),
+        _address(what, device, i32, "remap", remap, layers * pool_pages),
+        _address(what, device, i32, "tail_slots", tail_slots, rows),
+        _address(what, device, i32, "tails", tails, layers * rows),
+        _address(what, device, i32, "out", out, 0),
+        layers, tables.shape[1], rows, max_pages, pool_pages,
+        _launch_stream(torch, what, device, stream)), what)
 
 
 def logprobs_workspace_bytes(rows, vocabulary, top) -> int:
@@ -965,31 +964,35 @@ def logprobs(logits, tokens, logprob, entropy=None, top_tokens=None, top_logprob
     must be zero before its first use."""
     import torch
     what = "tmc_logprobs"
-    if logits.dim() != 2 or logits.stride(1) != 1:
+    strides = logits.stride()
+    if len(strides) != 2 or strides[1] != 1:
         raise TmcError(f"{what}: logits must be [rows, vocabulary] with adjacent elements")
     device = torch.cuda.current_device()
     if logits.get_device() != device:
         _refuse(what, device, logits.dtype, "logits", logits, 0)
-    if logits.dtype not in (torch.float32, torch.float16):
-        raise TmcError(f"{what}: logits must be f32 or f16, not {logits.dtype}")
-    code = F32 if logits.dtype is torch.float32 else F16
+    dtype = logits.dtype
+    code = F32 if dtype is torch.float32 else F16
+    if code == F16 and dtype is not torch.float16:
+        raise TmcError(f"{what}: logits must be f32 or f16, not {dtype}")
     rows, vocabulary = logits.shape
     top = 0
     if top_tokens is not None:
-        if top_logprobs is None or top_tokens.dim() != 2 or top_tokens.shape[0] != rows or \
-                top_logprobs.shape != top_tokens.shape:
+        shape = top_tokens.shape
+        if top_logprobs is None or len(shape) != 2 or shape[0] != rows or \
+                top_logprobs.shape != shape:
             raise TmcError(f"{what}: top_tokens and top_logprobs must be [rows, top]")
-        top = top_tokens.shape[1]
-    given, greatest = _addresses(what, device, torch.int32, ("tokens", tokens, rows),
-                                 ("top_tokens", top_tokens, 0))
-    chosen, spread, best = _addresses(what, device, torch.float32, ("logprob", logprob, rows),
-                                      ("entropy", entropy, rows),
-                                      ("top_logprobs", top_logprobs, 0))
+        top = shape[1]
+    f32, i32 = torch.float32, torch.int32
+    given = _address(what, device, i32, "tokens", tokens, rows)
+    chosen = _address(what, device, f32, "logprob", logprob, rows)
+    spread = _address(what, device, f32, "entropy", entropy, rows)
+    greatest = _address(what, device, i32, "top_tokens", top_tokens, 0)
+    best = _address(what, device, f32, "top_logprobs", top_logprobs, 0)
     space, space_bytes = _workspace(what, device, workspace)
     check(lib().tmc_logprobs(
-        logits.data_ptr(), code, logits.stride(0) if rows > 1 else vocabulary, given, chosen,
+        logits.data_ptr(), code, strides[0] if rows > 1 else vocabulary, given, chosen,
         spread, greatest if top else None, best if top else None, rows, vocabulary, top, space,
-        space_bytes, _launch_stream(what, device, stream)), what)
+        space_bytes, _launch_stream(torch, what, device, stream)), what)
 
 
 def fill_normal(t, seed, mean=0.0, std=1.0, stream=None):

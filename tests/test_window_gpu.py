@@ -504,6 +504,37 @@ def test_graph_replays_and_streams(tmc, torch):
         assert torch.equal(away.view(torch.int16), eager.view(torch.int16)), step
 
 
+def test_two_streams_at_once(tmc, torch):
+    """Calls that overlap, each with a workspace of its own and both over one cache."""
+    b, qh, kvh, d, page, window, sinks, length = 4, 16, 4, 128, 16, 1500, 4, 2000
+    pages = -(-length // page)
+    cache = Cache(torch, 37, [set(range(length))] * b, kvh, d, page, pages)
+    valid = torch.tensor([length, 1700, 3, 900], dtype=torch.int32, device="cuda")
+    need = tmc.window_attention_workspace_bytes(b, qh, kvh, d, pages * page, window, sinks)
+    assert need
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    queries = [torch.randn(b, qh * d, device="cuda").to(torch.float16) for _ in range(2)]
+    spaces = [torch.zeros(need // 4 + 1, device="cuda") for _ in range(2)]
+
+    def call(i, out, stream=None):
+        tmc.window_decode_attention(queries[i], cache.k, cache.v, valid, cache.tables_dev, None,
+                                    out, b, qh, kvh, d, page, pages, cache.page_stride,
+                                    cache.head_stride, window, sinks, spaces[i], stream=stream)
+
+    want = [torch.zeros(b, qh * d, dtype=torch.float16, device="cuda") for _ in range(2)]
+    for i in range(2):
+        call(i, want[i])
+    outs = [[torch.zeros_like(want[0]) for _ in range(30)] for _ in range(2)]
+    torch.cuda.synchronize()
+    for n in range(30):
+        for i in range(2):
+            call(i, outs[i][n], streams[i])
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in outs[i]:
+            assert torch.equal(out.view(torch.int16), want[i].view(torch.int16))
+
+
 def test_one_workspace_for_attention_and_scores(tmc, torch):
     """Launches of several shapes and of tmc_logprobs use one workspace in turn,
     eagerly and in two captured graphs that share it."""
