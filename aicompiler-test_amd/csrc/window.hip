@@ -149,7 +149,7 @@ __global__ __launch_bounds__(kWave) void window_plain_kernel(WindowParams p) {
 // writes a partial (max, sum, weighted) to the workspace and the last one to
 // arrive joins them, in block order.
 //
-// Inside a block the waves take the steps of a share in turn.  Each wave has a
+// Inside a block its 8, 4 or 1 waves take the steps of a share in turn.  Each wave has a
 // ring of STAGES steps in LDS that only it touches, filled by 16-byte loads
 // straight to LDS: no barrier, no register holds a load in flight, and a
 // stage is reloaded as soon as its operands are in registers.  K and V rows lie
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(kWave) void window_plain_kernel(WindowParams p) {
 //
 // Bound by reading K and V: 64 requests, 8 kv heads of 128 dims, window 2048, 516
 // MB: 89 us, 5.8 TB/s (a large copy moves 5.2).  Two blocks of 64 KiB rings a CU
-// rather than one of 128 KiB (103 us).  Few rows are bound by latency: lengths,
+// rather than one of 128 KiB with steps twice as long (103 us).  Few rows are bound by latency: lengths,
 // pages, K and V, and at the join stores, arrival and loads, 3 to 4 us of it.
 constexpr int kDecodeCus = 256;  // of an MI355X
 constexpr int kDecodeLeast = 8, kDecodeAlone = 20;
@@ -1190,17 +1190,25 @@ extern "C" int tmc_window_decode_attention(
     plan.slots = reinterpret_cast<float*>(static_cast<char*>(workspace) +
                                           kCounterBytes);
   }
-  // Two waves a SIMD: of two blocks, or of one where there is one a CU.  us, 4 waves
-  // and 8, one request: 8192 positions 13.7 and 13.0, 300 positions of 32 kv heads
-  // 7.1 and 6.5 (four stages a ring instead: 14.6 and 7.4).
+  // Eight waves (two a SIMD) where there is a block a CU, four where there are two,
+  // and a wave a block where there are more, which then come and go one by one.
+  // us, one request, 4 waves and 8: 8192 positions 13.7 and 13.0, 300 positions of
+  // 32 kv heads 7.1 and 6.5 (four stages a ring instead: 14.6 and 7.4).  8 kv heads
+  // of 128 dims, 4 waves and 1: 64 requests, window 256 15.1 and 16.0; 96, window 128
+  // 16.3 and 12.6; 250, window 128 38.3 and 28.8; 96, window 2048 144 and 135.
 #define TMC_DECODE(DIM, STEP, WAVES)                                                             \
   hipLaunchKernelGGL((window_decode_kernel<DIM, STEP, 2, WAVES>), dim3(blocks), dim3(WAVES * kWave), \
                      0, as_stream(stream), p, plan)
+#define TMC_DECODE_WAVES(DIM, STEP)                   \
+  if (blocks <= kDecodeCus) TMC_DECODE(DIM, STEP, 8); \
+  else if (blocks <= 2 * kDecodeCus) TMC_DECODE(DIM, STEP, 4); \
+  else TMC_DECODE(DIM, STEP, 1)
   if (head_dim == 128) {
-    if (blocks <= kDecodeCus) TMC_DECODE(128, 16, 8); else TMC_DECODE(128, 16, 4);
+    TMC_DECODE_WAVES(128, 16);
   } else {
-    if (blocks <= kDecodeCus) TMC_DECODE(64, 32, 8); else TMC_DECODE(64, 32, 4);
+    TMC_DECODE_WAVES(64, 32);
   }
+#undef TMC_DECODE_WAVES
 #undef TMC_DECODE
   return check_launch("window_decode_kernel");
 }

@@ -234,9 +234,10 @@ def test_pools_past_4_gib(tmc, torch, d, page):
 
 
 @pytest.mark.parametrize("d,batch,kvh", [(64, 300, 8), (128, 300, 8), (128, 2100, 1), (128, 70, 8),
-                                         (64, 100, 8), (128, 1000, 1), (64, 40, 32), (128, 64, 8)])
+                                         (64, 100, 8), (128, 1000, 1), (64, 40, 32), (128, 64, 8),
+                                         (64, 40, 8)])
 def test_decode_batches_of_many_rows(tmc, torch, d, batch, kvh):
-    """Many (request, kv head) rows: one list of steps, and a block a row."""
+    """Many (request, kv head) rows: blocks of four waves and of one."""
     page, window, sinks, cap_pages = 16, 40, 4, 8
     lengths = [1 + (37 * i) % 128 for i in range(batch)]
     cache = Cache(torch, batch, [set(visible(n, window, sinks)) for n in lengths], kvh, d, page, cap_pages)
@@ -254,6 +255,41 @@ def test_decode_batches_of_many_rows(tmc, torch, d, batch, kvh):
     check_rows(torch, out[torch.tensor(picked, device="cuda")], cache,
                q[torch.tensor(picked, device="cuda")],
                [(r, lengths[r]) if r < batch - 1 else None for r in picked], qh, d, window, sinks, 7.5)
+
+
+@pytest.mark.parametrize("d,batch,kvh,group", [(128, 90, 8, 4), (64, 90, 8, 2), (128, 40, 8, 3),
+                                               (64, 60, 8, 1), (128, 45, 6, 20)])
+def test_decode_rows_that_keep_their_output(tmc, torch, d, batch, kvh, group):
+    """Batches in which blocks hold one wave or four, with rows of no length, of
+    one past the capacity, of a missing page, and padding."""
+    page, window, sinks, cap_pages = 16, 150, 4, 20
+    rng = torch.Generator()
+    rng.manual_seed(batch + d)
+    valid = torch.randint(1, cap_pages * page + 1, (batch,), generator=rng).tolist()
+    for i, r in enumerate(range(0, batch, 7)):
+        valid[r] = [0, -3, cap_pages * page + 1, 2 ** 31 - 1][i % 4]
+    sees = [set(visible(n, window, sinks)) if 1 <= n <= cap_pages * page else set() for n in valid]
+    cache = Cache(torch, 43, sees, kvh, d, page, cap_pages)
+    tables, missing = cache.tables.clone(), set()
+    for r in range(3, batch, 11):
+        if sees[r]:
+            tables[r, (valid[r] - 1) // page] = cache.pages  # a page past the pool
+            missing.add(r)
+    q = torch.randn(batch, kvh * group * d, device="cuda").to(torch.float16)
+    out = torch.full((batch, kvh * group * d), 7.5, dtype=torch.float16, device="cuda")
+    ws = torch.zeros(tmc.window_attention_workspace_bytes(batch, kvh * group, kvh, d,
+                                                          cap_pages * page, window, sinks) // 4 + 1,
+                     device="cuda")
+    active = batch - 2
+    tmc.window_decode_attention(q, cache.k, cache.v,
+                                torch.tensor(valid, dtype=torch.int32, device="cuda"), tables.cuda(),
+                                torch.tensor([active], dtype=torch.int32, device="cuda"), out, batch,
+                                kvh * group, kvh, d, page, cap_pages, cache.page_stride,
+                                cache.head_stride, window, sinks, ws)
+    rows = [(r, valid[r]) if r < active and sees[r] and r not in missing else None
+            for r in range(batch)]
+    assert missing and sum(item is None for item in rows) > batch // 7
+    check_rows(torch, out, cache, q, rows, kvh * group, d, window, sinks, 7.5)
 
 
 def test_decode_packed_layout(tmc, torch):
