@@ -25,11 +25,8 @@ namespace {
 
 constexpr int kTopMax = 64;
 constexpr int kLpThreads = 256;
-constexpr int kLpWaves = kLpThreads / kWave;
-constexpr int kCandidates = kLpThreads;  // that a block ranks at once
 constexpr int kWaveKeys = 128;           // candidates a wave holds
-static_assert(kLpWaves * kTopMax <= kCandidates && kTopMax + kWave <= kWaveKeys,
-              "the waves' best fit a ranking, a wave's best and a round of new ones its list");
+static_assert(kTopMax + kWave <= kWaveKeys, "a wave's best and a round of new ones fit its list");
 constexpr long long kNoKey = (long long)0x8000000000000000ull;
 
 struct LogprobParams {
@@ -81,12 +78,13 @@ __device__ __forceinline__ void add_mass(float m, double s, double t, float high
   sum_t += e == 0.0 ? 0.0 : e * (t + s * (double)d);
 }
 
-// The best `top` of `count` distinct keys (at most kCandidates) to the places their rank
+// The best `top` of `count` distinct keys (at most THREADS) to the places their rank
 // gives them, the rest of the places empty.  Up to 64 keys: four threads a key.
 // Ends with a barrier.
+template <int THREADS>
 __device__ __forceinline__ void rank_keys(const long long* keys, int count, int top,
                                           long long* out) {
-  const bool few = count * 4 <= kLpThreads;
+  const bool few = count * 4 <= THREADS;
   const int me = few ? threadIdx.x >> 2 : threadIdx.x, step = few ? 4 : 1;
   if ((int)threadIdx.x < top) out[threadIdx.x] = kNoKey;
   __syncthreads();
@@ -144,22 +142,24 @@ struct WaveKeys {
   }
 };
 
-// EACH: elements a lane holds; a part is kLpThreads * EACH elements.  A block
+// EACH: elements a lane holds; a part is THREADS * EACH elements.  A block
 // walks `walk` parts of its row, the next one's loads in flight.
-template <typename T, int EACH>
-__global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
+template <typename T, int EACH, int THREADS>
+__global__ __launch_bounds__(THREADS) void logprobs_kernel(LogprobParams p) {
+  constexpr int WAVES = THREADS / kWave;
+  static_assert(WAVES * kTopMax <= THREADS, "the waves' best fit a ranking");
   constexpr int VEC = 16 / (int)sizeof(T);  // elements a load
   constexpr int LOADS = EACH / VEC;
-  constexpr int PART = kLpThreads * EACH;
+  constexpr int PART = THREADS * EACH;
   typedef T vec __attribute__((ext_vector_type(VEC)));
   // rows start anywhere on an element boundary
   typedef vec unaligned __attribute__((aligned(sizeof(T))));
-  __shared__ __align__(16) long long s_lists[kLpWaves][kWaveKeys];
-  __shared__ __align__(16) long long s_keys[kCandidates];
+  __shared__ __align__(16) long long s_lists[WAVES][kWaveKeys];
+  __shared__ __align__(16) long long s_keys[THREADS];
   __shared__ __align__(16) long long s_best[kTopMax];
-  __shared__ float s_m[kLpWaves], s_bound[kLpWaves];
-  __shared__ double s_s[kLpWaves], s_t[kLpWaves];
-  __shared__ int s_reach[kLpWaves], s_held[kLpWaves], s_found, s_last;
+  __shared__ float s_m[WAVES], s_bound[WAVES];
+  __shared__ double s_s[WAVES], s_t[WAVES];
+  __shared__ int s_reach[WAVES], s_held[WAVES], s_found, s_last;
   const int split = blockIdx.x % p.count, row = blockIdx.x / p.count;
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const T* x = static_cast<const T*>(p.logits) + (size_t)row * p.stride;
@@ -222,7 +222,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
     // lanes' greatest: each wave finds what its share of them reaches
     if (part_at == begin) {
       // waves whose lanes all hold elements
-      const int full = min(kLpWaves, (end - part_at + kWave * (EACH - VEC)) / (kWave * EACH));
+      const int full = min(WAVES, (end - part_at + kWave * (EACH - VEC)) / (kWave * EACH));
       const int need = full > 0 ? (top + full - 1) / full : top;
       float rest = mine, most = -INFINITY;
       int reach = 0;
@@ -239,10 +239,10 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
       }
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < kLpWaves; ++w) {
+      for (int w = 0; w < WAVES; ++w) {
         int total = 0;
 #pragma unroll
-        for (int u = 0; u < kLpWaves; ++u) total += s_bound[u] >= s_bound[w] ? s_reach[u] : 0;
+        for (int u = 0; u < WAVES; ++u) total += s_bound[u] >= s_bound[w] ? s_reach[u] : 0;
         if (total >= top) best.floor_v = fmaxf(best.floor_v, s_bound[w]);
       }
     }
@@ -282,22 +282,22 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
     __syncthreads();
     int total = 0, before = 0;
 #pragma unroll
-    for (int w = 0; w < kLpWaves; ++w) total += s_held[w];
-    if (total > kCandidates) {  // the same in every thread
+    for (int w = 0; w < WAVES; ++w) total += s_held[w];
+    if (total > THREADS) {  // the same in every thread
       best.keep_best(top);      // (of fewer than that, nothing changes but their order)
       __syncthreads();
       if (lane == 0) s_held[wave] = best.held;
       __syncthreads();
       total = 0;
 #pragma unroll
-      for (int w = 0; w < kLpWaves; ++w) total += s_held[w];
+      for (int w = 0; w < WAVES; ++w) total += s_held[w];
     }
 #pragma unroll
-    for (int w = 0; w < kLpWaves; ++w) before += w < wave ? s_held[w] : 0;
+    for (int w = 0; w < WAVES; ++w) before += w < wave ? s_held[w] : 0;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     for (int i = lane; i < best.held; i += kWave) s_keys[before + i] = best.list[i];
     __syncthreads();
-    rank_keys(s_keys, total, top, s_best);
+    rank_keys<THREADS>(s_keys, total, top, s_best);
   }
   {
     // the lanes of a row of 16 in 32 bits, rows and waves in 64
@@ -321,13 +321,13 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
   __syncthreads();
   float row_m = s_m[0];
 #pragma unroll
-  for (int w = 1; w < kLpWaves; ++w) row_m = fmaxf(row_m, s_m[w]);
+  for (int w = 1; w < WAVES; ++w) row_m = fmaxf(row_m, s_m[w]);
   double row_s = 0.0, row_t = 0.0;
 #pragma unroll
-  for (int w = 0; w < kLpWaves; ++w) add_mass(s_m[w], s_s[w], s_t[w], row_m, row_s, row_t);
+  for (int w = 0; w < WAVES; ++w) add_mass(s_m[w], s_s[w], s_t[w], row_m, row_s, row_t);
 
   // ---- the row's blocks together
-  if (p.count > 1) {
+  if (THREADS == kLpThreads && p.count > 1) {
     const size_t slots = (size_t)p.rows * p.count, slot = (size_t)row * p.count + split;
     double* sums = reinterpret_cast<double*>(p.parts);            // [slots][2]
     long long* keys = reinterpret_cast<long long*>(sums + 2 * slots);  // [slots][top]
@@ -366,7 +366,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
     auto load_keys = [&](int i) {
 #pragma unroll
       for (int u = 0; u < kAhead; ++u)
-        key[u] = __hip_atomic_load(from + min(i + u * kLpThreads, total - 1), __ATOMIC_RELAXED,
+        key[u] = __hip_atomic_load(from + min(i + u * THREADS, total - 1), __ATOMIC_RELAXED,
                                    __HIP_MEMORY_SCOPE_AGENT);
     };
     if (top > 0) load_keys(threadIdx.x);
@@ -379,7 +379,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
     // A bound that at least `top` keys reach: where `deep` parts are needed to
     // give `top` keys with their best `each` ones, the deep-th greatest of the
     // parts' each-th keys.
-    const int some = min(p.count, kCandidates), each = (top + some - 1) / some;
+    const int some = min(p.count, THREADS), each = (top + some - 1) / some;
     if (top > 0 && (int)threadIdx.x < some)
       s_keys[threadIdx.x] = __hip_atomic_load(keys + (first + threadIdx.x) * top + each - 1,
                                               __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -409,21 +409,21 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
       __syncthreads();
       const long long bound = s_best[0];
       __syncthreads();
-      for (int i = threadIdx.x; i < total; i += kAhead * kLpThreads) {
+      for (int i = threadIdx.x; i < total; i += kAhead * THREADS) {
         if (i != (int)threadIdx.x) load_keys(i);
 #pragma unroll
         for (int u = 0; u < kAhead; ++u)
-          if (i + u * kLpThreads < total && key[u] != kNoKey && key[u] >= bound) {
+          if (i + u * THREADS < total && key[u] != kNoKey && key[u] >= bound) {
             const int place = atomicAdd(&s_found, 1);
-            if (place < kCandidates) s_keys[place] = key[u];
+            if (place < THREADS) s_keys[place] = key[u];
           }
       }
       __syncthreads();
-      if (s_found <= kCandidates) {
-        rank_keys(s_keys, s_found, top, s_best);
+      if (s_found <= THREADS) {
+        rank_keys<THREADS>(s_keys, s_found, top, s_best);
       } else {
         // the best so far and the next keys, as many as fit
-        constexpr int kNext = kCandidates - kTopMax;
+        constexpr int kNext = THREADS > kTopMax ? THREADS - kTopMax : 1;
         if ((int)threadIdx.x < top) s_best[threadIdx.x] = kNoKey;
         __syncthreads();
         for (int at = 0; at < total; at += kNext) {
@@ -433,7 +433,7 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
             s_keys[top + i] =
                 __hip_atomic_load(from + at + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
           __syncthreads();
-          rank_keys(s_keys, top + n, top, s_best);
+          rank_keys<THREADS>(s_keys, top + n, top, s_best);
         }
       }
     }
@@ -454,22 +454,31 @@ __global__ __launch_bounds__(kLpThreads) void logprobs_kernel(LogprobParams p) {
   }
 }
 
-// How a row is shared out: elements a lane holds, parts a block, blocks a row.
+// How a row is shared out: threads a block, elements a lane holds, parts a block,
+// blocks a row.  Short rows take a wave each, which waits for no other: 3578 rows,
+// 10 alternatives, of 130 21.4 us in blocks of four waves, 9.1 in one, of 1000 21.8 and
+// 10.3, of 2000 20.8 and 14.9, of 4000 21.5 and 20.4; 600 rows of 1000 8.0 and 6.1, of
+// 4000 7.4 and 12.8.
 // Rows in the hundreds take a block each; fewer are cut until there are kFill
 // blocks or parts run out, the fewest rows into small parts.  MI355X, fp32:
 // 2048 rows of 32003, 5 alternatives 55 us with 16 elements a lane, 60 with 8;
 // without alternatives 47.7 (5.5 TB/s; a large copy moves 5.2).  16 rows of 32000,
-// 20 alternatives 11.6 us from 16 blocks a row; 64 rows 12.4 us from 8 blocks a
-// row, 12.7 from 4, 17.4 from 2; 200 rows 18.5 from 3, 27.9 from one.  Many rows
+// 20 alternatives 9.6 us from 16 blocks a row; 64 rows 12.3 us from 8 blocks a
+// row, 12.7 from 4, 17.4 from 2; 200 rows 18.4 from 3, 27.9 from one.  Many rows
 // are bound by the vector ALUs and the memory alike, few by the latency of the
 // steps: logits, bound, ranks, arrival, join.
-constexpr int64_t kFill = 512;
+constexpr int64_t kFill = 512, kNarrow = 1024;
 static_assert(kFill <= kSharedRows, "every shared row has its counter");
 struct LogprobPlan {
-  int each, walk, count;
+  int threads, each, walk, count;
 };
 LogprobPlan logprob_plan(int64_t rows, int64_t vocabulary) {
-  LogprobPlan plan{16, 1, 1};
+  LogprobPlan plan{kLpThreads, 16, 1, 1};
+  if (vocabulary <= (rows < 2048 ? kNarrow : 2 * kNarrow)) {
+    plan.threads = kWave;
+    plan.walk = (int)((vocabulary + 16 * kWave - 1) / (16 * kWave));
+    return plan;
+  }
   if (rows * ((vocabulary + 16 * kLpThreads - 1) / (16 * kLpThreads)) < kFill) plan.each = 8;
   const int64_t span = (int64_t)kLpThreads * plan.each, parts = (vocabulary + span - 1) / span;
   const int64_t blocks = std::min(parts, std::max<int64_t>(1, (kFill + rows - 1) / rows));
@@ -535,14 +544,18 @@ extern "C" int tmc_logprobs(const void* logits, int dtype, int64_t row_stride,
   }
   const dim3 grid((unsigned)(rows * p.count));
   const hipStream_t s = as_stream(stream);
-#define TMC_LP(TYPE, EACH) \
-  hipLaunchKernelGGL((logprobs_kernel<TYPE, EACH>), grid, dim3(kLpThreads), 0, s, p)
-  const bool few = plan.each == 8;
+#define TMC_LP(TYPE, EACH, THREADS) \
+  hipLaunchKernelGGL((logprobs_kernel<TYPE, EACH, THREADS>), grid, dim3(THREADS), 0, s, p)
+#define TMC_LP_PLAN(TYPE)                                \
+  if (plan.threads == kWave) TMC_LP(TYPE, 16, kWave);    \
+  else if (plan.each == 8) TMC_LP(TYPE, 8, kLpThreads);  \
+  else TMC_LP(TYPE, 16, kLpThreads)
   if (dtype == TMC_F32) {
-    if (few) TMC_LP(float, 8); else TMC_LP(float, 16);
+    TMC_LP_PLAN(float);
   } else {
-    if (few) TMC_LP(half_t, 8); else TMC_LP(half_t, 16);
+    TMC_LP_PLAN(half_t);
   }
+#undef TMC_LP_PLAN
 #undef TMC_LP
   return check_launch("logprobs_kernel");
 }
