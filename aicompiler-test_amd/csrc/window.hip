@@ -614,8 +614,8 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void window_decode_kernel(WindowP
 // beside the other's products.
 //
 // PG = 1: the waves hold 8 x 32 vectors and all take the 64 positions of a
-// stage.  PG = 4: they hold 2 x 32 vectors and take a quarter of the 128
-// positions of a stage each; the four partials join at the end.  K and V go
+// stage.  PG = 2 (4): they hold 4 (2) x 32 vectors and take a half (quarter) of
+// the 64 (128) positions of a stage each; the partials join at the end.  K and V go
 // through registers, loaded one stage ahead of the LDS one; one barrier a
 // stage.
 //
@@ -963,31 +963,40 @@ __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(Wi
         total += other == -INFINITY ? 0.0f : fast_exp2(other - top) * s_sum[g * VG + vg][col];
       }
       scale = m == -INFINITY ? 0.0f : fast_exp2(m - top) / total;
-      // the groups' sums in fp32: group pg finishes the elements 4 pg ... 4 pg + 3
-      // (dims 8 pg + 4 half ...) of every 32-dim tile
+      // the groups' sums in fp32, as many 32-dim tiles a pass as fit: group pg
+      // finishes EPG of a tile's elements (element e: dim 8 (e / 4) + 4 half + e % 4)
       float* hand = reinterpret_cast<float*>(s_kv);
-      constexpr int kTile = 16 * kWave;
-      static_assert(PG == 4 && sizeof(float) * WAVES * DT * kTile <= sizeof(s_kv), "the sums fit");
+      constexpr int kTile = 16 * kWave, EPG = 16 / PG;
+      constexpr int FIT = (int)(sizeof(s_kv) / (sizeof(float) * WAVES * kTile));
+      constexpr int TILES = FIT < DT ? FIT : DT;
+      static_assert(TILES > 0 && DT % TILES == 0, "a pass fits");
 #pragma unroll
-      for (int t = 0; t < DT; ++t)
+      for (int first = 0; first < DT; first += TILES) {
+        if (first) __syncthreads();
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          hand[(wave * DT + t) * kTile + e * kWave + lane] = o[t][e] * scale;
-      __syncthreads();
+        for (int t = 0; t < TILES; ++t)
 #pragma unroll
-      for (int t = 0; t < DT; ++t) {
-        float val[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          for (int e = 0; e < 16; ++e)
+            hand[(wave * TILES + t) * kTile + e * kWave + lane] = o[first + t][e] * scale;
+        __syncthreads();
 #pragma unroll
-        for (int g = 0; g < PG; ++g)
+        for (int t = 0; t < TILES; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            val[e] += hand[((g * VG + vg) * DT + t) * kTile + (4 * pg + e) * kWave + lane];
-        if (len > 0)
-          *reinterpret_cast<h4*>(p.out + ((size_t)row * p.q_heads + head) * D + 32 * t + 8 * pg +
-                                 4 * half) =
-              h4{(half_t)val[0], (half_t)val[1], (half_t)val[2], (half_t)val[3]};
+          for (int part = 0; part < EPG / 4; ++part) {
+            const int quad = pg * (EPG / 4) + part;
+            float val[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) nan |= !(val[e] == val[e]);
+            for (int g = 0; g < PG; ++g)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                val[e] += hand[((g * VG + vg) * TILES + t) * kTile + (4 * quad + e) * kWave + lane];
+            if (len > 0)
+              *reinterpret_cast<h4*>(p.out + ((size_t)row * p.q_heads + head) * D +
+                                     32 * (first + t) + 8 * quad + 4 * half) =
+                  h4{(half_t)val[0], (half_t)val[1], (half_t)val[2], (half_t)val[3]};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) nan |= !(val[e] == val[e]);
+          }
       }
     } else {
       // rows through LDS (16-byte chunks swizzled by the row), so that whole
@@ -1234,23 +1243,28 @@ extern "C" int tmc_window_prefill_attention_f16(
   if ((head_dim != 64 && head_dim != 128) || p.group > 64 ||
       (uint64_t)pool_pages * (uint64_t)page_stride / 8 >= 0xFFFFFFFFull)
     return launch_plain(p, as_stream(stream));
-  const int wide = 256 / p.group, narrow = 64 / p.group;  // tokens a tile
-  // A block a CU: four narrow tiles, whose waves share the positions, while that
-  // is at most two rounds of blocks.  us, split and wide, 32 heads of 128 dims,
-  // window 2048: 64 wide tiles 38 and 79, 128 70 and 85, 160 103 and 87, 256 151
-  // and 101.
-  const bool split = (rows + wide - 1) / wide * kv_heads <= 128;
-  const int tokens = split ? narrow : wide;
+  // A block a CU: tiles of 256 vectors, or of 128 or 64, whose waves share the
+  // positions, while there are few.  us for tiles of 64, 128 and 256, 32 heads of 128
+  // dims, window 2048: 512 tokens 39, 53 and 80, 768 70, 56 and 83, 1024 75, 60 and 84,
+  // 1280 107, 105 and 88.
+  const int64_t wide = (rows + 256 / p.group - 1) / (256 / p.group) * kv_heads;
+  const int vectors = wide <= 64 ? 64 : wide <= 128 ? 128 : 256;
+  const int tokens = vectors / p.group;
   const int tiles = (int)((rows + tokens - 1) / tokens);
   const dim3 grid((unsigned)(tiles * kv_heads)), block(kChunkWaves * kWave);
 #define TMC_CHUNK(DIM, PG)                                                                        \
   hipLaunchKernelGGL((window_chunk_kernel<DIM, PG>), grid, block, 0, as_stream(stream), p, tiles, \
                      tokens)
+#define TMC_CHUNK_VECTORS(DIM)                  \
+  if (vectors == 64) TMC_CHUNK(DIM, 4);         \
+  else if (vectors == 128) TMC_CHUNK(DIM, 2);   \
+  else TMC_CHUNK(DIM, 1)
   if (head_dim == 128) {
-    if (split) TMC_CHUNK(128, 4); else TMC_CHUNK(128, 1);
+    TMC_CHUNK_VECTORS(128);
   } else {
-    if (split) TMC_CHUNK(64, 4); else TMC_CHUNK(64, 1);
+    TMC_CHUNK_VECTORS(64);
   }
+#undef TMC_CHUNK_VECTORS
 #undef TMC_CHUNK
   return check_launch("window_chunk_kernel");
 }

@@ -338,7 +338,8 @@ def test_decode_infinite_values_stay(tmc, torch):
         assert got[head, 5] == math.inf
 
 
-@pytest.mark.parametrize("qh,kvh,d", [(4, 1, 128), (4, 1, 64), (200, 200, 64), (200, 200, 128)])
+@pytest.mark.parametrize("qh,kvh,d", [(4, 1, 128), (4, 1, 64), (200, 200, 64), (200, 200, 128),
+                                     (100, 100, 64), (100, 100, 128)])
 def test_chunk_special_values_stay_with_those_that_see_them(tmc, torch, qh, kvh, d):
     """An infinity in V and a NaN in K change the rows that see their positions
     and no other row of the tile."""
@@ -410,6 +411,13 @@ CHUNK = [
     (300, 40, 192, 96, 64, 12, 77, 9),
     (515, 300, 128, 64, 128, 16, 200, 70),
     (130, 0, 600, 200, 64, 16, 60, 0),
+    # between them: tiles of 128
+    (70, 100, 100, 100, 128, 16, 50, 4),
+    (300, 40, 64, 32, 64, 12, 77, 9),
+    (200, 300, 80, 80, 128, 16, 200, 70),
+    (130, 0, 150, 50, 64, 16, 60, 0),
+    (515, 1000, 36, 36, 128, 64, 700, 20),
+    (100, 64, 500, 100, 128, 16, 10 ** 12, 3),
 ]
 
 
@@ -436,7 +444,8 @@ def test_chunk_matches_the_formula(tmc, torch, rows, start, qh, kvh, d, page, wi
 
 
 @pytest.mark.parametrize("qh,kvh,d,page", [(4, 4, 128, 16), (8, 2, 64, 12), (8, 1, 128, 16),
-                                           (4, 2, 32, 16), (200, 200, 64, 16), (200, 200, 128, 12)])
+                                           (4, 2, 32, 16), (200, 200, 64, 16), (200, 200, 128, 12),
+                                           (90, 90, 64, 12), (90, 90, 128, 16)])
 def test_chunk_of_several_requests(tmc, torch, qh, kvh, d, page):
     """Rows of several requests in any packing, with invalid lengths, table rows
     outside the tables, and a request whose window reaches a missing page."""
