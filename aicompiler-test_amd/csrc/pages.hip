@@ -32,6 +32,7 @@ struct MoveParams {
 // rate; a quarter of 1 GiB of pools compacted: 104 us, 5.2 TB/s, that rate.  Pages
 // of 256 positions, 8 heads of 128: 13 us where a block a page took 40; pages of
 // 32 positions, 32 heads, compacted: 10 us where two blocks a page took 17.
+// Pages of one position, 32 heads, forked: 13 us where a head at a time took 30.
 constexpr int kMoveUnits = 1024;
 template <typename UNIT>
 __global__ __launch_bounds__(256) void move_pages_kernel(MoveParams p) {
@@ -47,11 +48,16 @@ __global__ __launch_bounds__(256) void move_pages_kernel(MoveParams p) {
   char* dst = base + (size_t)to * p.page_bytes;
   const unsigned run = (unsigned)((long)count * p.row_bytes / (int)sizeof(UNIT));  // units a head
   const int part = blockIdx.z / p.head_blocks;
-  for (int h = blockIdx.z - part * p.head_blocks; h < p.heads; h += p.head_blocks) {
+  // threads a head: short runs of several heads are copied side by side
+  const unsigned wide = min(run, 256u), at_once = 256u / wide;
+  const unsigned mine = threadIdx.x / wide, lane = threadIdx.x - mine * wide;
+  if (mine >= at_once) return;
+  for (unsigned h = blockIdx.z - part * p.head_blocks + mine * p.head_blocks; h < (unsigned)p.heads;
+       h += at_once * p.head_blocks) {
     const UNIT* s = reinterpret_cast<const UNIT*>(src + (size_t)h * p.head_bytes);
     UNIT* d = reinterpret_cast<UNIT*>(dst + (size_t)h * p.head_bytes);
     for (unsigned first = part * kMoveUnits; first < run; first += p.parts * kMoveUnits)
-      for (unsigned u = first + threadIdx.x; u < min(first + kMoveUnits, run); u += 256) d[u] = s[u];
+      for (unsigned u = first + lane; u < min(first + kMoveUnits, run); u += wide) d[u] = s[u];
   }
 }
 
