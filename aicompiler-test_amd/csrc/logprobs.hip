@@ -464,7 +464,9 @@ __global__ __launch_bounds__(THREADS) void logprobs_kernel(LogprobParams p) {
 // 2048 rows of 32003, 5 alternatives 55 us with 16 elements a lane, 60 with 8;
 // without alternatives 47.7 (5.5 TB/s; a large copy moves 5.2).  16 rows of 32000,
 // 20 alternatives 9.6 us from 16 blocks a row; 64 rows 12.3 us from 8 blocks a
-// row, 12.7 from 4, 17.4 from 2; 200 rows 18.4 from 3, 27.9 from one.  Many rows
+// row, 12.7 from 4, 17.4 from 2; 200 rows 18.4 from 3, 27.9 from one.  Twice the
+// blocks where each would walk more than 4 parts: 186 rows of 121000 36 us in 3
+// blocks a row, 30 in 6 (400 rows of 32000 in 2 and 3 blocks 18.7 and 19.4).  Many rows
 // are bound by the vector ALUs and the memory alike, few by the latency of the
 // steps: logits, bound, ranks, arrival, join.
 constexpr int64_t kFill = 512, kNarrow = 1024;
@@ -481,7 +483,8 @@ LogprobPlan logprob_plan(int64_t rows, int64_t vocabulary) {
   }
   if (rows * ((vocabulary + 16 * kLpThreads - 1) / (16 * kLpThreads)) < kFill) plan.each = 8;
   const int64_t span = (int64_t)kLpThreads * plan.each, parts = (vocabulary + span - 1) / span;
-  const int64_t blocks = std::min(parts, std::max<int64_t>(1, (kFill + rows - 1) / rows));
+  int64_t blocks = std::min(parts, std::max<int64_t>(1, (kFill + rows - 1) / rows));
+  if (rows < kFill && parts > 4 * blocks) blocks *= 2;
   plan.walk = (int)((parts + blocks - 1) / blocks);
   plan.count = (int)((parts + plan.walk - 1) / plan.walk);
   return plan;

@@ -60,7 +60,8 @@ def check(torch, logits, tokens, top, out):
 SHAPES = [(1, 1, 1), (1, 2, 2), (3, 7, 7), (2, 63, 5), (2, 64, 64), (2, 65, 64), (5, 100, 20),
           (1, 32000, 5), (16, 32000, 20), (7, 32003, 1), (300, 2049, 3), (2, 8192, 64),
           (2, 8193, 64), (3, 160001, 20), (1, 1000000, 64), (64, 4097, 0), (2000, 515, 4),
-          (2100, 1900, 20), (2048, 2048, 64), (2047, 1025, 5), (3, 1024, 64)]
+          (2100, 1900, 20), (2048, 2048, 64), (2047, 1025, 5), (3, 1024, 64),
+          (300, 60000, 20), (511, 25000, 3)]
 
 
 @pytest.mark.parametrize("rows,vocab,top", SHAPES)
