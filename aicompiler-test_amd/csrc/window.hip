@@ -324,7 +324,8 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void window_decode_kernel(WindowP
   const int first_head = kvh * p.group + split * plan.heads;
   const int heads = min(plan.heads, p.group - split * plan.heads);
   const int valid = p.valid[row];
-  const int steps = steps_of<STEP>(p, valid, row < active);
+  const int table_row = window_table(p, row);
+  const int steps = steps_of<STEP>(p, valid, row < active && table_row >= 0);
   const int shares = decode_shares(steps, plan.parts);
   if (part >= shares) return;
   const int even = steps / shares, over = steps - even * shares;
@@ -349,7 +350,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void window_decode_kernel(WindowP
 
   const int begin = window_begin(p, valid), sinks = min(p.sinks, begin);
   const int count = sinks + valid - begin;
-  const int32_t* table = p.tables + (size_t)row * p.max_pages;
+  const int32_t* table = p.tables + (size_t)table_row * p.max_pages;
   const unsigned head_unit = (unsigned)((size_t)kvh * p.head_stride / 8);
   h8 qb[KS];
   {
@@ -1141,6 +1142,30 @@ int decode_parts(int64_t units, int64_t head_dim, int64_t capacity, int64_t wind
       decode_shares(steps, std::min(most, (int64_t)std::ceil(std::sqrt((double)steps))));
   return parts > 16 ? parts / 16 * 16 : parts;
 }
+int launch_decode(const WindowParams& p, const DecodePlan& plan, unsigned blocks,
+                  hipStream_t stream) {
+  // Eight waves (two a SIMD) where there is a block a CU, four where there are two,
+  // and a wave a block where there are more, which then come and go one by one.
+  // us, one request, 4 waves and 8: 8192 positions 13.7 and 13.0, 300 positions of
+  // 32 kv heads 7.1 and 6.5 (four stages a ring instead: 14.6 and 7.4).  8 kv heads
+  // of 128 dims, 4 waves and 1: 64 requests, window 256 15.1 and 16.0; 96, window 128
+  // 16.3 and 12.6; 250, window 128 38.3 and 28.8; 96, window 2048 144 and 135.
+#define TMC_DECODE(DIM, STEP, WAVES)                                                             \
+  hipLaunchKernelGGL((window_decode_kernel<DIM, STEP, 2, WAVES>), dim3(blocks), dim3(WAVES * kWave), \
+                     0, stream, p, plan)
+#define TMC_DECODE_WAVES(DIM, STEP)                   \
+  if (blocks <= kDecodeCus) TMC_DECODE(DIM, STEP, 8); \
+  else if (blocks <= 2 * kDecodeCus) TMC_DECODE(DIM, STEP, 4); \
+  else TMC_DECODE(DIM, STEP, 1)
+  if (p.dim == 128) {
+    TMC_DECODE_WAVES(128, 16);
+  } else {
+    TMC_DECODE_WAVES(64, 32);
+  }
+#undef TMC_DECODE_WAVES
+#undef TMC_DECODE
+  return check_launch("window_decode_kernel");
+}
 }  // namespace
 }  // namespace tmc
 
@@ -1199,27 +1224,7 @@ extern "C" int tmc_window_decode_attention(
     plan.slots = reinterpret_cast<float*>(static_cast<char*>(workspace) +
                                           kCounterBytes);
   }
-  // Eight waves (two a SIMD) where there is a block a CU, four where there are two,
-  // and a wave a block where there are more, which then come and go one by one.
-  // us, one request, 4 waves and 8: 8192 positions 13.7 and 13.0, 300 positions of
-  // 32 kv heads 7.1 and 6.5 (four stages a ring instead: 14.6 and 7.4).  8 kv heads
-  // of 128 dims, 4 waves and 1: 64 requests, window 256 15.1 and 16.0; 96, window 128
-  // 16.3 and 12.6; 250, window 128 38.3 and 28.8; 96, window 2048 144 and 135.
-#define TMC_DECODE(DIM, STEP, WAVES)                                                             \
-  hipLaunchKernelGGL((window_decode_kernel<DIM, STEP, 2, WAVES>), dim3(blocks), dim3(WAVES * kWave), \
-                     0, as_stream(stream), p, plan)
-#define TMC_DECODE_WAVES(DIM, STEP)                   \
-  if (blocks <= kDecodeCus) TMC_DECODE(DIM, STEP, 8); \
-  else if (blocks <= 2 * kDecodeCus) TMC_DECODE(DIM, STEP, 4); \
-  else TMC_DECODE(DIM, STEP, 1)
-  if (head_dim == 128) {
-    TMC_DECODE_WAVES(128, 16);
-  } else {
-    TMC_DECODE_WAVES(64, 32);
-  }
-#undef TMC_DECODE_WAVES
-#undef TMC_DECODE
-  return check_launch("window_decode_kernel");
+  return launch_decode(p, plan, blocks, as_stream(stream));
 }
 
 extern "C" int tmc_window_prefill_attention_f16(
@@ -1240,9 +1245,20 @@ extern "C" int tmc_window_prefill_attention_f16(
   p.active = active_count;
   p.row_table = row_table;
   p.table_rows = (int)table_rows;
-  if ((head_dim != 64 && head_dim != 128) || p.group > 64 ||
-      (uint64_t)pool_pages * (uint64_t)page_stride / 8 >= 0xFFFFFFFFull)
+  if (!decode_shape(head_dim) || (uint64_t)pool_pages * (uint64_t)page_stride / 8 >= 0xFFFFFFFFull)
     return launch_plain(p, as_stream(stream));
+  // A few tokens: each as if it were a request of its own.  us, in tiles and here,
+  // 8 kv heads of 128 dims: one token over 673 positions 16.0 and 9.3, 8 over 1024
+  // 19.9 and 11.8, 32 over 8000 94 and 67, 32 over 30 9.3 and 5.1.
+  const int64_t splits = decode_splits(q_heads, kv_heads);
+  if (rows * kv_heads * splits <= kDecodeCus) {
+    DecodePlan plan{};
+    plan.parts = 1;
+    plan.splits = (int)splits;
+    plan.heads = (int)((p.group + splits - 1) / splits);
+    return launch_decode(p, plan, (unsigned)(rows * kv_heads * splits), as_stream(stream));
+  }
+  if (p.group > 64) return launch_plain(p, as_stream(stream));
   // A block a CU: tiles of 256 vectors, or of 128 or 64, whose waves share the
   // positions, while there are few.  us for tiles of 64, 128 and 256, 32 heads of 128
   // dims, window 2048: 512 tokens 39, 53 and 80, 768 70, 56 and 83, 1024 75, 60 and 84,
