@@ -1121,6 +1121,12 @@ bool decode_shape(int64_t head_dim) {
 int64_t decode_splits(int64_t q_heads, int64_t kv_heads) {
   return (q_heads / kv_heads + 15) / 16;
 }
+// Steps of a row that sees as much as it can.
+int64_t decode_steps(int64_t head_dim, int64_t capacity, int64_t window, int64_t sinks) {
+  const int64_t step = head_dim == 128 ? 16 : 32;
+  const int64_t seen = std::min(capacity, std::min(window, capacity) + std::min(sinks, capacity));
+  return (seen + step - 1) / step;
+}
 // Blocks a row, one of `units`: as many as give every CU one, twice that where
 // shares are then long (rows of unlike lengths), while a full row leaves each
 // kDecodeLeast steps, and not more than the square root of the steps: a step
@@ -1133,9 +1139,7 @@ int64_t decode_splits(int64_t q_heads, int64_t kv_heads) {
 // 4096 35.9 in 2, 33.5 in 4; 32 requests 26.4 in 2, 23.6 in 1.
 int decode_parts(int64_t units, int64_t head_dim, int64_t capacity, int64_t window,
                  int64_t sinks) {
-  const int64_t step = head_dim == 128 ? 16 : 32;
-  const int64_t seen = std::min(capacity, std::min(window, capacity) + std::min(sinks, capacity));
-  const int64_t steps = (seen + step - 1) / step;
+  const int64_t steps = decode_steps(head_dim, capacity, window, sinks);
   int64_t most = (kDecodeCus + units - 1) / units;
   if (most > 1 && steps / most > 96) most *= 2;
   const int parts =
@@ -1247,16 +1251,19 @@ extern "C" int tmc_window_prefill_attention_f16(
   p.table_rows = (int)table_rows;
   if (!decode_shape(head_dim) || (uint64_t)pool_pages * (uint64_t)page_stride / 8 >= 0xFFFFFFFFull)
     return launch_plain(p, as_stream(stream));
-  // A few tokens: each as if it were a request of its own.  us, in tiles and here,
-  // 8 kv heads of 128 dims: one token over 673 positions 16.0 and 9.3, 8 over 1024
-  // 19.9 and 11.8, 32 over 8000 94 and 67, 32 over 30 9.3 and 5.1.
-  const int64_t splits = decode_splits(q_heads, kv_heads);
-  if (rows * kv_heads * splits <= kDecodeCus) {
+  // Few tokens, or short windows: each token as if it were a request of its own.  us,
+  // in tiles and here, 8 kv heads of 128 dims: one token over 673 positions 16.0 and
+  // 9.3, 8 over 1024 19.9 and 11.8, 32 over 8000 94 and 67, 32 over 30 9.3 and 5.1; 64
+  // over 100 9.8 and 6.6, over 1024 20.7 and 20.5, over 3000 42 and 51; 256 over 20 9.7
+  // and 7.2, over 100 10.2 and 12.1.
+  const int64_t splits = decode_splits(q_heads, kv_heads), units = rows * kv_heads * splits;
+  const int64_t steps = decode_steps(head_dim, page_size * max_pages, window, sinks);
+  if (units <= kDecodeCus || (units <= 2 * kDecodeCus && steps <= 64) || units * steps <= 4096) {
     DecodePlan plan{};
     plan.parts = 1;
     plan.splits = (int)splits;
     plan.heads = (int)((p.group + splits - 1) / splits);
-    return launch_decode(p, plan, (unsigned)(rows * kv_heads * splits), as_stream(stream));
+    return launch_decode(p, plan, (unsigned)units, as_stream(stream));
   }
   if (p.group > 64) return launch_plain(p, as_stream(stream));
   // A block a CU: tiles of 256 vectors, or of 128 or 64, whose waves share the

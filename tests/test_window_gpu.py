@@ -339,7 +339,7 @@ def test_decode_infinite_values_stay(tmc, torch):
 
 
 @pytest.mark.parametrize("qh,kvh,d", [(4, 1, 128), (4, 1, 64), (200, 200, 64), (200, 200, 128),
-                                     (100, 100, 64), (100, 100, 128)])
+                                     (100, 100, 64), (100, 100, 128), (60, 60, 64), (60, 60, 128)])
 def test_chunk_special_values_stay_with_those_that_see_them(tmc, torch, qh, kvh, d):
     """An infinity in V and a NaN in K change the rows that see their positions
     and no other row of the tile."""
@@ -443,9 +443,49 @@ def test_chunk_matches_the_formula(tmc, torch, rows, start, qh, kvh, d, page, wi
     check_rows(torch, out[index], cache, q[index], expect, qh, d, window, sinks, 7.5)
 
 
+@pytest.mark.parametrize("rows,start,qh,kvh,d,page,window,sinks", [
+    (300, 400, 6, 2, 128, 16, 900, 9),        # 3 query heads a kv head
+    (600, 400, 10, 2, 64, 32, 90, 9),         # 5
+    (350, 200, 34, 2, 64, 16, 290, 9),        # 17
+    (300, 1000, 32, 2, 128, 16, 100, 4),      # 16
+    (600, 1000, 64, 1, 128, 16, 257, 33),     # 64
+    (300, 500, 65, 1, 64, 16, 200, 3),        # 65: past the tiles
+    (600, 90, 4, 2, 128, 12, 77, 20),
+    (700, 100, 8, 2, 64, 1, 130, 4),          # pages of one position
+    (2100, 100, 8, 2, 128, 5, 1, 0),          # a window of one
+    (600, 2000, 4, 2, 128, 256, 500, 300),
+    (700, 0, 4, 4, 128, 16, 1000, 4),
+    (1100, 0, 4, 4, 128, 16, 16, 0),
+    (513, 3000, 4, 1, 128, 16, 10 ** 12, 0),
+])
+def test_chunk_tiles_match_the_formula(tmc, torch, rows, start, qh, kvh, d, page, window, sinks):
+    """Chunks long enough for the tiles; some of their rows are checked."""
+    n = start + rows
+    max_pages = -(-n // page)
+    seen = set()
+    for valid in range(start + 1, n + 1):
+        seen |= set(range(max(0, valid - min(window, n)), valid)) if valid in (start + 1, n) else {valid - 1}
+    seen |= set(range(min(sinks, n)))
+    cache = Cache(torch, rows + d, [seen], kvh, d, page, max_pages)
+    q = torch.randn(rows, qh * d, device="cuda").to(torch.float16)
+    out = torch.full((rows, qh * d), 7.5, dtype=torch.float16, device="cuda")
+    tmc.window_prefill_attention(q, cache.k, cache.v,
+                                 torch.arange(start + 1, n + 1, dtype=torch.int32, device="cuda"),
+                                 cache.tables_dev, None,
+                                 torch.tensor([rows - 1], dtype=torch.int32, device="cuda"), out,
+                                 rows, qh, kvh, d, page, max_pages, cache.page_stride,
+                                 cache.head_stride, window, sinks)
+    picked = sorted({*range(0, rows, 29), 1, 63, 64, 127, 128, 255, 256, rows - 2, rows - 1})
+    index = torch.tensor(picked, device="cuda")
+    check_rows(torch, out[index], cache, q[index],
+               [(0, start + 1 + r) if r < rows - 1 else None for r in picked], qh, d, window, sinks,
+               7.5)
+
+
 @pytest.mark.parametrize("qh,kvh,d,page", [(4, 4, 128, 16), (8, 2, 64, 12), (8, 1, 128, 16),
                                            (4, 2, 32, 16), (200, 200, 64, 16), (200, 200, 128, 12),
-                                           (90, 90, 64, 12), (90, 90, 128, 16)])
+                                           (90, 90, 64, 12), (90, 90, 128, 16),
+                                           (16, 16, 128, 16), (48, 16, 64, 12)])
 def test_chunk_of_several_requests(tmc, torch, qh, kvh, d, page):
     """Rows of several requests in any packing, with invalid lengths, table rows
     outside the tables, and a request whose window reaches a missing page."""
