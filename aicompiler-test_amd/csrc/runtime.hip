@@ -849,6 +849,7 @@ bool make_spec(const std::string& name, const Params& p, KernelSpec& s) {
          "paged_attention needs max_batch, q_heads, head_dim, page_size, max_pages.");
     const int64_t head_stride = param_int(p, "head_stride", ps * d);
     const int64_t page_stride = param_int(p, "page_stride", kvh * ps * d);
+    NEED(page_stride > 0, name + ": page_stride must be positive.");
     const auto lit = p.find("out_layout");
     const bool packed_out = lit != p.end() && lit->second == "packed";
     NEED(lit == p.end() || packed_out || lit->second == "row_major",
@@ -885,6 +886,7 @@ bool make_spec(const std::string& name, const Params& p, KernelSpec& s) {
          "dtype=f16.");
     const int64_t head_stride = param_int(p, "head_stride", ps * d);
     const int64_t page_stride = param_int(p, "page_stride", kvh * ps * d);
+    NEED(page_stride > 0, name + ": page_stride must be positive.");
     s.inputs = {dt, dt, dt, TMC_I32, TMC_I32, TMC_I32, dt};
     s.counts = {(size_t)(qh * d), 0, 0, 1, (size_t)mp, 1, (size_t)(n * qh * d)};
     if (res) {
@@ -980,6 +982,7 @@ bool make_spec(const std::string& name, const Params& p, KernelSpec& s) {
          "prefill_attention needs rows, q_heads, head_dim, page_size, max_pages and dtype=f16.");
     const int64_t head_stride = param_int(p, "head_stride", ps * d);
     const int64_t page_stride = param_int(p, "page_stride", kvh * ps * d);
+    NEED(page_stride > 0, name + ": page_stride must be positive.");
     const int64_t tr = param_int(p, "tables", 0);  // > 0: table rows + a row table
     NEED(tr >= 0 && tr < (1 << 20), "prefill_attention: tables must be >= 0.");
     // inputs: q, key pool, value pool, valid_lengths, block table(s)[, row table], active;
@@ -1018,6 +1021,7 @@ bool make_spec(const std::string& name, const Params& p, KernelSpec& s) {
          "dtype=f16.");
     const int64_t head_stride = param_int(p, "head_stride", ps * d);
     const int64_t page_stride = param_int(p, "page_stride", kvh * ps * d);
+    NEED(page_stride > 0, name + ": page_stride must be positive.");
     const auto lit = p.find("out_layout");
     const bool packed_out = lit != p.end() && lit->second == "packed";
     NEED(lit == p.end() || packed_out || lit->second == "row_major",
@@ -1051,6 +1055,7 @@ bool make_spec(const std::string& name, const Params& p, KernelSpec& s) {
          "and dtype=f16.");
     const int64_t head_stride = param_int(p, "head_stride", ps * d);
     const int64_t page_stride = param_int(p, "page_stride", kvh * ps * d);
+    NEED(page_stride > 0, name + ": page_stride must be positive.");
     const int64_t tr = param_int(p, "tables", 0);  // > 0: table rows + a row table
     NEED(tr >= 0 && tr < (1 << 20), "window_prefill_attention: tables must be >= 0.");
     // bindings as prefill_attention's
