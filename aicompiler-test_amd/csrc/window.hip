@@ -75,7 +75,8 @@ struct PlainScratch {  // of one wave
 };
 
 // One (row, query head), whose length and table row are valid.
-__device__ __noinline__ void plain_row(WindowParams p, int row, int head, PlainScratch& scratch) {
+__device__ __forceinline__ void plain_row_inline(const WindowParams& p, int row, int head,
+                                                 PlainScratch& scratch) {
   const int lane = threadIdx.x & (kWave - 1);
   const int valid = p.valid[row];
   const int32_t* table = p.tables + (size_t)window_table(p, row) * p.max_pages;
@@ -130,6 +131,9 @@ __device__ __noinline__ void plain_row(WindowParams p, int row, int head, PlainS
   for (int t = 0; t < kPlainMaxDim / kWave; ++t)
     if (lane + t * kWave < d)
       p.out[window_out(p, row, head * d + lane + t * kWave)] = (half_t)(o[t] / sum);
+}
+__device__ __noinline__ void plain_row(WindowParams p, int row, int head, PlainScratch& scratch) {
+  plain_row_inline(p, row, head, scratch);
 }
 
 __global__ __launch_bounds__(kWave) void window_plain_kernel(WindowParams p) {
@@ -285,8 +289,10 @@ __device__ __forceinline__ float2 load_pair(const float* from) {
       float2, __hip_atomic_load(reinterpret_cast<const unsigned long long*>(from),
                                 __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
-__device__ __forceinline__ void put_pair(const WindowParams& p, int row, int col, float a, float b) {
+// Two dims of an output; whether one of them is a NaN.
+__device__ __forceinline__ bool put_pair(const WindowParams& p, int row, int col, float a, float b) {
   *reinterpret_cast<h2*>(p.out + window_out(p, row, col)) = h2{(half_t)a, (half_t)b};
+  return !(a == a) | !(b == b);
 }
 
 // Visible positions of a row of length `valid`, in steps.
@@ -528,6 +534,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void window_decode_kernel(WindowP
   const size_t slot_floats = (size_t)plan.heads * (D + 2);
   float* slots = plan.slots + (size_t)unit * plan.parts * slot_floats;
   // two dims a thread
+  unsigned again = 0;  // heads with a NaN among the dims that this thread put
   for (int i = threadIdx.x; i < heads * (D / 2); i += THREADS) {
     const int head = i / (D / 2), d = i % (D / 2) * 2;
     float top = -INFINITY;
@@ -545,7 +552,8 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void window_decode_kernel(WindowP
       val1 += scale * part.y;
     }
     if (whole) {
-      if (!bad) put_pair(p, row, (first_head + head) * D + d, val0 / sum, val1 / sum);
+      if (!bad && put_pair(p, row, (first_head + head) * D + d, val0 / sum, val1 / sum))
+        again |= 1u << head;
     } else {
       float* out = slots + part * slot_floats + (size_t)head * (D + 2);
       store_pair(out + d, val0, val1);
@@ -600,9 +608,28 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void window_decode_kernel(WindowP
             }
           top = next;
         }
-        if (!spoiled) put_pair(p, row, (first_head + head) * D + d, val0 / sum, val1 / sum);
+        if (!spoiled && put_pair(p, row, (first_head + head) * D + d, val0 / sum, val1 / sum))
+          again |= 1u << head;
       }
     }
+  }
+  // A weight that fp16 rounds to 0 times an infinity of V, or one past its range
+  // (scores of 2^24 and more, whose fp32 maximum is several powers of two off),
+  // is a NaN that weights of fp32 do not give: such heads are done again with
+  // those, by the wave that put them, in LDS behind what the waves met in.
+  unsigned long long waiting = __builtin_amdgcn_ballot_w64(again != 0);
+  if (waiting) {
+    unsigned todo = 0;
+    for (; waiting; waiting &= waiting - 1)
+      todo |= (unsigned)__shfl((int)again, __builtin_ctzll(waiting), kWave);
+    constexpr int kMet = WAVES * 16 * (D + 2) * (int)sizeof(float);
+    static_assert(kMet % 16 == 0 && kMet + sizeof(PlainScratch) * WAVES <= sizeof(s_ring),
+                  "a scratch for every wave");
+    PlainScratch& scratch =
+        reinterpret_cast<PlainScratch*>(reinterpret_cast<char*>(s_ring) + kMet)[wave];
+    __builtin_amdgcn_s_waitcnt(0);  // the NaNs are stored
+    for (; todo; todo &= todo - 1)
+      plain_row_inline(p, row, first_head + __builtin_ctz(todo), scratch);
   }
 }
 

@@ -820,7 +820,9 @@ size_t tmc_window_attention_workspace_bytes(int64_t batch, int64_t q_heads, int6
  * active_count[0] (NULL: all are active), lengths outside [1, page_size * max_pages] and
  * requests that would see a page outside [0, pool_pages) leave their output
  * untouched.  A NaN or infinity in the cache outside the visible positions
- * changes nothing.  Requests may share pages. */
+ * changes nothing; an infinity of V at a visible one makes its dim infinite, or
+ * NaN where another of the other sign is seen or its weight is below 2^-126 of
+ * the greatest.  Requests may share pages. */
 int tmc_window_decode_attention(const void *q, const void *key_pool, const void *value_pool,
                                 const int32_t *valid_lengths, const int32_t *block_tables,
                                 const int32_t *active_count, void *out, int dtype,
