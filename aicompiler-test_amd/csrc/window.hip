@@ -1033,14 +1033,17 @@ __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(Wi
 #pragma unroll
       for (int t = 0; t < DT; ++t)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) nan |= !(o[t][e] == o[t][e]);
+        for (int e = 0; e < 16; ++e) {
+          o[t][e] *= scale;
+          nan |= !(o[t][e] == o[t][e]);
+        }
 #pragma unroll
       for (int t = 0; t < DT; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           *reinterpret_cast<h4*>(rows + col * D + (((4 * t + e) ^ (col & (CH - 1))) << 3) + 4 * half) =
-              h4{(half_t)(o[t][4 * e] * scale), (half_t)(o[t][4 * e + 1] * scale),
-                 (half_t)(o[t][4 * e + 2] * scale), (half_t)(o[t][4 * e + 3] * scale)};
+              h4{(half_t)o[t][4 * e], (half_t)o[t][4 * e + 1], (half_t)o[t][4 * e + 2],
+                 (half_t)o[t][4 * e + 3]};
       __builtin_amdgcn_wave_barrier();
       const int put = len > 0 ? row * p.q_heads + head : -1;
 #pragma unroll
@@ -1052,8 +1055,10 @@ __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(Wi
       }
     }
     // A weight of 0 times an infinity or NaN of V that the vector does not see
-    // (another one of the tile does) is a NaN: such vectors are done again, one
-    // at a time and over their own positions alone.
+    // (another one of the tile does) is a NaN, and so is what weights past the
+    // range of fp16 leave, or none at all (scores of 2^24 and more, whose fp32
+    // maximum is several powers of two off): such vectors are done again, one at a
+    // time, over their own positions alone and with weights of fp32.
     if (__syncthreads_or(nan && len > 0)) {
       unsigned long long again = __builtin_amdgcn_ballot_w64(nan && len > 0);
       again = (again | again >> 32) & 0xFFFFFFFFull;

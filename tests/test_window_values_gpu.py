@@ -139,9 +139,10 @@ def test_infinite_values_behind_small_weights(tmc, torch, form, rows, qh, kvh, d
             assert near.all(), r
 
 
+@pytest.mark.parametrize("scale", [2000.0, 8000.0])
 @pytest.mark.parametrize("form,rows,qh,kvh,d,page,last,window,sinks", FORMS)
-def test_scores_far_from_zero(tmc, torch, form, rows, qh, kvh, d, page, last, window, sinks):
-    """Scores of 2^25 and more, where a rounding of a score in fp32 is several powers
+def test_scores_far_from_zero(tmc, torch, form, rows, qh, kvh, d, page, last, window, sinks, scale):
+    """Scores of 2^25 to 2^30, where a rounding of a score in fp32 is several powers
     of two of its weight.  Each query is the key of one of its positions, which
     then takes all the weight: the margin to the next score is far above the error
     of fp32 scores (D 2^-24 of the sum of the products' magnitudes), so the output
@@ -149,7 +150,7 @@ def test_scores_far_from_zero(tmc, torch, form, rows, qh, kvh, d, page, last, wi
     s = Stream(tmc, torch, last, kvh, d, page, 5 * rows + d)
     group = qh // kvh
     valid = lengths_of(form, rows, last)
-    s.k.copy_((s.normal(last, kvh, d) * 2000.0).clamp(-60000.0, 60000.0))
+    s.k.copy_((s.normal(last, kvh, d) * scale).clamp(-60000.0, 60000.0))
     s.v.copy_(s.normal(last, kvh, d))
     low, high = max(n - window for n in valid), min(valid)
     at = (low + torch.arange(rows * qh, device="cuda") * 7919 % (high - low)).reshape(rows, qh)
