@@ -880,10 +880,13 @@ def window_prefill_attention(q, k_pool, v_pool, valid_lengths, tables, row_table
 
 
 def page_moves(moves, pools, pool_pages, page_size):
-    """The device array of a list of (pool, source page, destination page,
-    positions) for move_pages, checked (tmc_check_page_moves): existing pages,
-    none written twice, none both read and written."""
+    """The device array of a list (or an array or tensor, wherever it lies) of
+    (pool, source page, destination page, positions) for move_pages, checked
+    (tmc_check_page_moves): existing pages, none written twice, none both read
+    and written."""
     import torch
+    if hasattr(moves, "tolist"):
+        moves = moves.tolist()
     host_moves = torch.tensor(moves, dtype=torch.int32).reshape(len(moves), 4).contiguous()
     check(lib().tmc_check_page_moves(_ptr(host_moves), host_moves.shape[0], pools, pool_pages,
                                      page_size), "tmc_check_page_moves")
