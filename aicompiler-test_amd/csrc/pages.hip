@@ -130,7 +130,7 @@ extern "C" int tmc_move_pages(void* const* key_pools, void* const* value_pools, 
   TMC_REQUIRE(key_pools && value_pools && moves, "Move pages: null pointer.");
   TMC_REQUIRE(dtype == TMC_F16 || dtype == TMC_F32 || dtype == TMC_BF16,
               "Move pages: dtype must be f16, bf16 or f32.");
-  TMC_REQUIRE(pools > 0 && pools < (1LL << 20) && count >= 0 && count < (1LL << 31) &&
+  TMC_REQUIRE(pools > 0 && pools < (1LL << 20) && count >= 0 && count < (1LL << 24) &&
                   pool_pages > 0 && pool_pages < (1LL << 31) && heads > 0 && heads < (1LL << 20) &&
                   page_size > 0 && page_size < (1LL << 24) && head_dim > 0 &&
                   head_dim < (1LL << 16) && page_size * head_dim < (1LL << 29),

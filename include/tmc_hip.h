@@ -853,7 +853,7 @@ int tmc_window_prefill_attention_f16(const void *q, const void *key_pool, const 
  * compaction moves live pages to the front.  key_pools and value_pools are
  * host arrays of `pools` device pointers [pool_pages][heads][page_size]
  * [head_dim] at the strides (elements; dtype f16, bf16 or f32); moves is a
- * 16-byte aligned device array of `count` (pool, source page, destination
+ * 16-byte aligned device array of `count` < 2^24 (pool, source page, destination
  * page, positions): the first `positions` positions of every head are copied,
  * bit for bit.  A move that names a pool or page outside its range, positions
  * outside [1, page_size] or one page twice copies nothing.  All moves take

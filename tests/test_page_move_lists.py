@@ -30,3 +30,13 @@ def test_moves_on_the_device(tmc, dtype):
         tmc.page_moves(moves, 2, 8, 16)
     got = tmc.page_moves(moves[:2], 2, 8, 16)
     assert got.is_cuda and got.dtype is torch.int32 and torch.equal(got, moves[:2].int())
+
+
+def test_more_moves_than_a_launch_takes_are_refused(tmc):
+    """A block of 256 threads a move: 2^24 moves are 2^32 threads, which no launch takes."""
+    import ctypes as C
+    pool = (C.c_void_p * 1)(4096)
+    for count in (1 << 24, (1 << 31) - 1):
+        assert tmc.lib().tmc_move_pages(pool, pool, 1, C.c_void_p(4096), count, 0, 8, 2, 16, 128,
+                                        2 * 16 * 128, 16 * 128, None) != 0
+        assert "shape" in tmc.last_error()
