@@ -36,7 +36,8 @@ struct LogprobParams {
   float* entropy;  // may be null
   int32_t* top_tokens;
   float* top_logprobs;
-  float* parts;   // [rows][count](m, S, T), then [rows][count][top] values, then indices
+  // of shared rows: [rows][count] (S, T) in fp64, [rows][count][top] keys, [rows][count] m
+  float* parts;
   int* arrivals;  // [rows], kCounterStride apart
   long stride;
   int rows, vocab, top;
@@ -458,11 +459,15 @@ __global__ __launch_bounds__(THREADS) void logprobs_kernel(LogprobParams p) {
 // blocks a row.  Short rows take a wave each, which waits for no other: 3578 rows,
 // 10 alternatives, of 130 21.4 us in blocks of four waves, 9.1 in one, of 1000 21.8 and
 // 10.3, of 2000 20.8 and 14.9, of 4000 21.5 and 20.4; 600 rows of 1000 8.0 and 6.1, of
-// 4000 7.4 and 12.8.
+// 4000 7.4 and 12.8; 300 rows of 1000 5.9 and 6.0, of 2000 5.8 and 7.9; 1000 of 2000 8.3
+// and 8.2, of 3000 8.4 and 11.0.  (From 1000 to 2047 rows of 1025 to 2048 the rule takes
+// blocks where waves are as fast or faster: 1500 of 2000 10.2 and 8.9, 2047 of 1500 13.8
+// and 8.9.)
 // Rows in the hundreds take a block each; fewer are cut until there are kFill
 // blocks or parts run out, the fewest rows into small parts.  MI355X, fp32:
 // 2048 rows of 32003, 5 alternatives 55 us with 16 elements a lane, 60 with 8;
-// without alternatives 47.7 (5.5 TB/s; a large copy moves 5.2).  16 rows of 32000,
+// without alternatives 48 to 51 (5.1 to 5.5 TB/s; a large copy moves 5.2); in fp16, half
+// the bytes, 46 and 40.  16 rows of 32000,
 // 20 alternatives 9.6 us from 16 blocks a row; 64 rows 12.3 us from 8 blocks a
 // row, 12.7 from 4, 17.4 from 2; 200 rows 18.4 from 3, 27.9 from one.  Twice the
 // blocks where each would walk more than 4 parts: 186 rows of 121000 36 us in 3

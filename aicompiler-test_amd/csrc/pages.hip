@@ -28,7 +28,7 @@ struct MoveParams {
 // positions, or every head_blocks-th head), in units of UNIT bytes: pure copying,
 // bound by memory, so a thread copies unit by unit (eight loads ahead of their
 // stores took 1.5 times as long over a large pool).  Four copies each of 8
-// requests' last pages in 32 layers, 20 MB: 12 us, against 8 at a large copy's
+// requests' last pages in 32 layers, 8 MB read and 32 written: 12 us, against 8 at a large copy's
 // rate; a quarter of 1 GiB of pools compacted: 104 us, 5.2 TB/s, that rate.  Pages
 // of 256 positions, 8 heads of 128: 13 us where a block a page took 40; pages of
 // 32 positions, 32 heads, compacted: 10 us where two blocks a page took 17.

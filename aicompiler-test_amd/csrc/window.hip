@@ -63,9 +63,12 @@ __device__ __forceinline__ size_t window_out(const WindowParams& p, int row, int
 // One wave per (row, query head): 64 visible positions at a time, one per
 // lane for the scores (whole K rows in 16-byte chunks), then lanes over the
 // dims for P V.  Online softmax in fp32.  For the head dims that the matrix
-// core kernels do not take and pools of 64 GiB; at 128 dims it takes 94 us where
-// they take 7 (one request of 300 positions, 32 heads) and 10.3 ms where they
-// take 91 us (2048 tokens, window 2048).
+// core kernels do not take, pools of 64 GiB, and chunks past the token form of
+// more than 64 query heads a kv head; at 128 dims it takes 94 us where they
+// take 7 (one request of 300 positions, 32 heads) and 10.3 ms where they take
+// 91 us (2048 tokens, window 2048).  512 tokens over 1024 positions, 8 kv heads: 24 us
+// at 128 dims, 2.0 ms at 96, 4.1 at 256; 71 query heads of 64 dims on one kv head
+// 2.8 ms.
 constexpr int kPlainMaxDim = 256;
 
 struct PlainScratch {  // of one wave
@@ -164,7 +167,7 @@ __global__ __launch_bounds__(kWave) void window_plain_kernel(WindowParams p) {
 // which O^T = V^T P^T wants its weights; V^T comes from transposing LDS reads.
 //
 // Bound by reading K and V: 64 requests, 8 kv heads of 128 dims, window 2048, 516
-// MB: 89 us, 5.8 TB/s (a large copy moves 5.2).  Two blocks of 64 KiB rings a CU
+// MB: 90 us, 5.7 TB/s (a large copy moves 5.2).  Two blocks of 64 KiB rings a CU
 // rather than one of 128 KiB with steps twice as long (103 us).  Few rows are bound by latency: lengths,
 // pages, K and V, and at the join stores, arrival and loads, 3 to 4 us of it.
 constexpr int kDecodeCus = 256;  // of an MI355X
@@ -273,7 +276,12 @@ __device__ __forceinline__ void read_values(const unsigned (&at)[D / 16], h4 (&v
 
 // Weights are stored 2^kRaiseLog times their value in fp16 (the greatest is
 // 2^kRaiseLog itself): weights down to 2^-29 of the greatest keep their 11
-// bits, and the sum takes the rounded ones, so the factor cancels.
+// bits, and the sum takes the rounded ones, so the factor cancels.  fp16 is
+// what the matrix cores multiply with V's type; what the rounding left as a
+// second operand (22 bits) would double the products of P V.  An output is off
+// by up to 2^-11 of the mean of |v| for it, beside the 2^-11 of its own fp16: the
+// error against 64 bits is 1.2 to 1.4 times that of fp32 weights (2.5e-4 to
+// 2.9e-4 of the outputs' norm, 2.1e-4 of which is their fp16).
 constexpr float kRaiseLog = 15.0f;
 constexpr unsigned kNoUnit = 0xFFFFFFFFu;
 
@@ -649,7 +657,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void window_decode_kernel(WindowP
 //
 // Bound by the products, the softmax and the LDS together: 2048 tokens, 32 heads
 // of 128 dims, window 2048: 91 us, 760 TFLOP/s; matrix cores, vector ALUs and LDS
-// are busy 36, 41 and 44% of the time, the products with loads alone take 78 us.
+// are busy 37, 42 and 44% of the time, the products with loads alone take 78 us.
 // Measured and no faster: 4 waves of 64 vectors with the products of one tile
 // beside the softmax of the other (130), opposite phases or priorities for the
 // two waves of a SIMD, loads placed among the products, K read a step ahead.
@@ -657,13 +665,15 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void window_decode_kernel(WindowP
 // A tile's positions are those that any of its tokens sees, sinks first.
 // Positions that a vector does not see are masked in the steps where that can
 // be; steps that none of a wave's vectors sees are left out.  Rows of several
-// requests in a tile are done run by run.
+// requests in a tile are done run by run: 256 rows over 1024 positions, 8 kv heads,
+// 22 us as one request, 25 as 16, 339 as 256 (186 as a decode batch).
 typedef float f16v __attribute__((ext_vector_type(16)));
 constexpr int kChunkWaves = 8;
 
 // A new maximum moves the weights' scale only when it is kLag above the one in
 // use, so a wave seldom rescales its sums; weights are then at most
-// 2^(kChunkRaise + kLag) in fp16 and keep 11 bits down to 2^-24 of that scale.
+// 2^(kChunkRaise + kLag) in fp16 and keep 11 bits down to 2^-24 of that scale (fp16
+// for the reason that kRaiseLog states).
 constexpr float kLag = 5.0f, kChunkRaise = 10.0f;
 
 __device__ __forceinline__ unsigned opaque(unsigned v) {
@@ -1165,10 +1175,14 @@ int64_t decode_steps(int64_t head_dim, int64_t capacity, int64_t window, int64_t
 // takes about as long as one more partial at the join (0.16 and 0.22 us at 4
 // query heads of 128 dims), which takes 16 at a time.  Rows of up to
 // kDecodeAlone steps are a block's.  us, 8 kv heads of 128 dims.  One request,
-// shared and alone: 512 positions 7.6 and 9.8, 1024 8.1 and 14.5, 4096 11.2 and
-// 43, 8192 13.8 (15.0 in 32 parts, 23 in 64) and 80; 300 positions, 32 kv heads,
-// 7.2 and 7.1.  16 requests, window 1024: 15.4 in 2 parts, 16.4 in 4 or 1; window
-// 4096 35.9 in 2, 33.5 in 4; 32 requests 26.4 in 2, 23.6 in 1.
+// shared and alone: 320 positions (20 steps) 7.8 and 7.1, 384 8.1 and 7.7, 512 8.1
+// and 8.6, 1024 8.4 and 11.9, 4096 11.5 and 33, 8192 13.9 (15.0 in 32 parts, 23
+// in 64) and 60; of 64 dims 512 (16 steps) 7.2 and 6.4, 768 7.2 and 7.4, 1024 7.3
+// and 8.4.  16 requests up to 4096, window 1024: 16.4 in 2 parts (the rule's), 15.4
+// in 1, 17.3 in 4; window 4096 34.6 in 4 (the rule's), 37 in 2, 50 in 1; 32
+// requests, window 1024, 25.4 in 1 (the rule's), 28.9 in 2.  The lengths are not
+// known here: with 256 rows and more none is shared, and a batch of 32 with one row
+// of 8192 takes 57, active alone 59, where one request takes 12.
 int decode_parts(int64_t units, int64_t head_dim, int64_t capacity, int64_t window,
                  int64_t sinks) {
   const int64_t steps = decode_steps(head_dim, capacity, window, sinks);
@@ -1182,10 +1196,11 @@ int launch_decode(const WindowParams& p, const DecodePlan& plan, unsigned blocks
                   hipStream_t stream) {
   // Eight waves (two a SIMD) where there is a block a CU, four where there are two,
   // and a wave a block where there are more, which then come and go one by one.
-  // us, one request, 4 waves and 8: 8192 positions 13.7 and 13.0, 300 positions of
-  // 32 kv heads 7.1 and 6.5 (four stages a ring instead: 14.6 and 7.4).  8 kv heads
-  // of 128 dims, 4 waves and 1: 64 requests, window 256 15.1 and 16.0; 96, window 128
-  // 16.3 and 12.6; 250, window 128 38.3 and 28.8; 96, window 2048 144 and 135.
+  // us, one request, 4 waves and 8: 8192 positions 14.2 and 13.9, 300 positions of
+  // 32 kv heads 7.7 and 7.1 (four stages a ring instead: 14.6 and 7.4).  8 kv heads
+  // of 128 dims, 8 waves, 4 and 1: 64 requests, window 256 19.6, 15.5 and 15.9; 96,
+  // window 128 20.2, 16.1 and 13.1; 250, window 128 53, 36 and 29; 96, window 2048
+  // 140, 137 and 138.
 #define TMC_DECODE(DIM, STEP, WAVES)                                                             \
   hipLaunchKernelGGL((window_decode_kernel<DIM, STEP, 2, WAVES>), dim3(blocks), dim3(WAVES * kWave), \
                      0, stream, p, plan)
@@ -1284,10 +1299,13 @@ extern "C" int tmc_window_prefill_attention_f16(
   if (!decode_shape(head_dim) || (uint64_t)pool_pages * (uint64_t)page_stride / 8 >= 0xFFFFFFFFull)
     return launch_plain(p, as_stream(stream));
   // Few tokens, or short windows: each token as if it were a request of its own.  us,
-  // in tiles and here, 8 kv heads of 128 dims: one token over 673 positions 16.0 and
-  // 9.3, 8 over 1024 19.9 and 11.8, 32 over 8000 94 and 67, 32 over 30 9.3 and 5.1; 64
-  // over 100 9.8 and 6.6, over 1024 20.7 and 20.5, over 3000 42 and 51; 256 over 20 9.7
-  // and 7.2, over 100 10.2 and 12.1.
+  // in tiles and here, 32 query heads.  8 kv heads of 128 dims: one token over 300
+  // positions 12.0 and 7.1, over 1024 20.5 and 12.1, 32 over 4096 54 and 35, 32 over 20
+  // 9.3 and 5.3; 64 over 100 9.8 and 6.8, over 1024 20.8 and 20.7, over 4096 53 and 67;
+  // 256 over 20 9.9 and 7.5, over 100 10.4 and 12.5.  Of 64 dims: 64 over 300 8.7 and
+  // 7.6, over 1024 13.8 and 13.3; 128 over 300 8.7 and 11.0.  32 kv heads of 128: 16
+  // over 300 11.7 and 9.6, over 4096 54 and 68; 32 over 20 8.7 and 5.2, over 300 12.3
+  // and 16.6, and over 100 10.6 and 8.7, where the rule takes the tiles.
   const int64_t splits = decode_splits(q_heads, kv_heads), units = rows * kv_heads * splits;
   const int64_t steps = decode_steps(head_dim, page_size * max_pages, window, sinks);
   if (units <= kDecodeCus || (units <= 2 * kDecodeCus && steps <= 64) || units * steps <= 4096) {
@@ -1300,8 +1318,9 @@ extern "C" int tmc_window_prefill_attention_f16(
   if (p.group > 64) return launch_plain(p, as_stream(stream));
   // A block a CU: tiles of 256 vectors, or of 128 or 64, whose waves share the
   // positions, while there are few.  us for tiles of 64, 128 and 256, 32 heads of 128
-  // dims, window 2048: 512 tokens 39, 53 and 80, 768 70, 56 and 83, 1024 75, 60 and 84,
-  // 1280 107, 105 and 88.
+  // dims, window 2048: 512 tokens 37, 51 and 79, 768 67, 52 and 79, 1024 67, 55 and 79,
+  // 1280 98, 100 and 80, 2048 132, 107 and 93; over 8 kv heads 512 tokens 35, 46 and 70,
+  // 1024 64, 50 and 71, 1280 95, 91 and 72.
   const int64_t wide = (rows + 256 / p.group - 1) / (256 / p.group) * kv_heads;
   const int vectors = wide <= 64 ? 64 : wide <= 128 ? 128 : 256;
   const int tokens = vectors / p.group;

@@ -822,7 +822,11 @@ size_t tmc_window_attention_workspace_bytes(int64_t batch, int64_t q_heads, int6
  * untouched.  A NaN or infinity in the cache outside the visible positions
  * changes nothing; an infinity of V at a visible one makes its dim infinite, or
  * NaN where another of the other sign is seen or its weight is below 2^-126 of
- * the greatest.  Requests may share pages. */
+ * the greatest.  Requests may share pages.  Softmax weights are rounded to fp16
+ * (11 bits; sums in fp32) at every head_dim, where tmc_paged_decode_attention
+ * keeps 22 bits at head_dim 64.  head_dim 64 and 128 over pools below 64 GiB run
+ * on the matrix cores; the others run a simple kernel that takes 10 to 100 times
+ * as long. */
 int tmc_window_decode_attention(const void *q, const void *key_pool, const void *value_pool,
                                 const int32_t *valid_lengths, const int32_t *block_tables,
                                 const int32_t *active_count, void *out, int dtype,
@@ -837,8 +841,10 @@ int tmc_window_decode_attention(const void *q, const void *key_pool, const void 
  * 0 when row_table is NULL; table_rows must then be 1), attends what
  * tmc_window_decode_attention lets its token attend.  Rows of several requests
  * may follow each other in any order; consecutive rows of one request at
- * consecutive positions are what it is fast for.  Limits and untouched rows as
- * there, and rows whose table row is outside [0, table_rows). */
+ * consecutive positions are what it is fast for (many rows of as many requests
+ * are better a decode batch).  Limits, values and untouched rows as there, and
+ * rows whose table row is outside [0, table_rows).  Long chunks of more than 64
+ * query heads a kv head run the simple kernel, too. */
 int tmc_window_prefill_attention_f16(const void *q, const void *key_pool, const void *value_pool,
                                      const int32_t *valid_lengths, const int32_t *block_tables,
                                      const int32_t *row_table, int64_t table_rows,
