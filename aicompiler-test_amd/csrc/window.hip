@@ -64,11 +64,12 @@ __device__ __forceinline__ size_t window_out(const WindowParams& p, int row, int
 // lane for the scores (whole K rows in 16-byte chunks), then lanes over the
 // dims for P V.  Online softmax in fp32.  For the head dims that the matrix
 // core kernels do not take, pools of 64 GiB, and chunks past the token form of
-// more than 64 query heads a kv head; at 128 dims it takes 94 us where they
-// take 7 (one request of 300 positions, 32 heads) and 10.3 ms where they take
-// 91 us (2048 tokens, window 2048).  512 tokens over 1024 positions, 8 kv heads: 24 us
-// at 128 dims, 2.0 ms at 96, 4.1 at 256; 71 query heads of 64 dims on one kv head
-// 2.8 ms.
+// more than 64 query heads a kv head; at 128 dims it takes 45 us where they
+// take 7 (one request of 300 positions, 32 heads) and 8.3 ms where they take
+// 91 us (2048 tokens, window 2048).  512 tokens over 1024 positions, 8 kv heads: 23 us
+// at 128 dims, 0.85 ms at 96, 1.9 at 256; 71 query heads of 64 dims on one kv head
+// 1.6 ms.  Bound by the latency of its loads: with a branch before each of them it
+// took 2 to 5 times as long.
 constexpr int kPlainMaxDim = 256;
 
 struct PlainScratch {  // of one wave
@@ -77,18 +78,27 @@ struct PlainScratch {  // of one wave
   long at[kWave];
 };
 
-// One (row, query head), whose length and table row are valid.
+// One (row, query head), whose length and table row are valid.  DIM: the head dim
+// where it is known, else 0.  Loads have no branch between them: columns past the
+// head dim and places without a row read the last column and the pool's first
+// row, whatever they hold, and are not used.
+template <int DIM>
 __device__ __forceinline__ void plain_row_inline(const WindowParams& p, int row, int head,
                                                  PlainScratch& scratch) {
+  constexpr int TILES = (DIM ? DIM : kPlainMaxDim) / kWave;
+  constexpr int kAhead = 8;  // chunks of K, rows of V loaded at once
   const int lane = threadIdx.x & (kWave - 1);
   const int valid = p.valid[row];
   const int32_t* table = p.tables + (size_t)window_table(p, row) * p.max_pages;
-  const int kvh = head / p.group, d = p.dim;
+  const int kvh = head / p.group, d = DIM ? DIM : p.dim;
   const half_t* q = p.q + ((size_t)row * p.q_heads + head) * d;
   for (int i = lane; i < d; i += kWave) scratch.q[i] = q[i];
   const int begin = window_begin(p, valid), first = min(p.sinks, begin);
   const int count = first + valid - begin;
-  float m = -INFINITY, sum = 0.0f, o[kPlainMaxDim / kWave] = {};
+  float m = -INFINITY, sum = 0.0f, o[TILES] = {};
+  int column[TILES];
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) column[t] = min(lane + t * kWave, d - 1);
   bool bad = false;
   for (int u0 = 0; u0 < count; u0 += kWave) {
     const int u = u0 + lane, pos = u < first ? u : begin + u - first;
@@ -101,6 +111,7 @@ __device__ __forceinline__ void plain_row_inline(const WindowParams& p, int row,
         at = (long)page * p.page_stride + (long)kvh * p.head_stride +
              (long)(pos - slot * p.page_size) * d;
         float dot = 0.0f;
+#pragma unroll kAhead
         for (int c = 0; c < d; c += 8)
           dot = dot8(load_h8(scratch.q + c), load_h8(p.k + at + c), dot);
         score = dot * p.scale_log2;
@@ -117,26 +128,36 @@ __device__ __forceinline__ void plain_row_inline(const WindowParams& p, int row,
     scratch.at[lane] = at;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-    for (int t = 0; t < kPlainMaxDim / kWave; ++t) o[t] *= alpha;
+    for (int t = 0; t < TILES; ++t) o[t] *= alpha;
     const int live = min(kWave, count - u0);
-    for (int i = 0; i < live; ++i) {
-      const long from = scratch.at[i];
-      const float wi = scratch.weight[i];
-      if (from < 0) continue;
+    for (int i = 0; i < live; i += kAhead) {
+      half_t v[kAhead][TILES];
+      bool here[kAhead];
 #pragma unroll
-      for (int t = 0; t < kPlainMaxDim / kWave; ++t)
-        if (lane + t * kWave < d) o[t] += wi * (float)p.v[from + lane + t * kWave];
+      for (int a = 0; a < kAhead; ++a) {
+        const long from = scratch.at[i + a];
+        here[a] = from >= 0;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) v[a][t] = p.v[max(from, 0L) + column[t]];
+      }
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        const float wa = scratch.weight[i + a];
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) o[t] += here[a] ? wa * (float)v[a][t] : 0.0f;
+      }
     }
   }
   if (__any(bad)) return;
   sum = cross_sum<1>(sum);
 #pragma unroll
-  for (int t = 0; t < kPlainMaxDim / kWave; ++t)
+  for (int t = 0; t < TILES; ++t)
     if (lane + t * kWave < d)
       p.out[window_out(p, row, head * d + lane + t * kWave)] = (half_t)(o[t] / sum);
 }
+template <int DIM>
 __device__ __noinline__ void plain_row(WindowParams p, int row, int head, PlainScratch& scratch) {
-  plain_row_inline(p, row, head, scratch);
+  plain_row_inline<DIM>(p, row, head, scratch);
 }
 
 __global__ __launch_bounds__(kWave) void window_plain_kernel(WindowParams p) {
@@ -145,7 +166,7 @@ __global__ __launch_bounds__(kWave) void window_plain_kernel(WindowParams p) {
   if (row >= (p.active ? min(p.active[0], p.rows) : p.rows)) return;
   const int valid = p.valid[row];
   if (valid < 1 || valid > p.page_size * p.max_pages || window_table(p, row) < 0) return;
-  plain_row(p, row, head, scratch);
+  plain_row_inline<0>(p, row, head, scratch);
 }
 
 // ------------------------------------------------------------ one token a request
@@ -302,6 +323,10 @@ __device__ __forceinline__ bool put_pair(const WindowParams& p, int row, int col
   *reinterpret_cast<h2*>(p.out + window_out(p, row, col)) = h2{(half_t)a, (half_t)b};
   return !(a == a) | !(b == b);
 }
+
+// A greatest score that is infinite, as where all are NaN or -inf, leaves no
+// result but NaN, with weights of any type.
+__device__ __forceinline__ bool finite(float top) { return fabsf(top) < INFINITY; }
 
 // Visible positions of a row of length `valid`, in steps.
 template <int STEP>
@@ -560,7 +585,8 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void window_decode_kernel(WindowP
       val1 += scale * part.y;
     }
     if (whole) {
-      if (!bad && put_pair(p, row, (first_head + head) * D + d, val0 / sum, val1 / sum))
+      if (!bad && put_pair(p, row, (first_head + head) * D + d, val0 / sum, val1 / sum) &&
+          finite(top))
         again |= 1u << head;
     } else {
       float* out = slots + part * slot_floats + (size_t)head * (D + 2);
@@ -616,7 +642,8 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void window_decode_kernel(WindowP
             }
           top = next;
         }
-        if (!spoiled && put_pair(p, row, (first_head + head) * D + d, val0 / sum, val1 / sum))
+        if (!spoiled && put_pair(p, row, (first_head + head) * D + d, val0 / sum, val1 / sum) &&
+            finite(top))
           again |= 1u << head;
       }
     }
@@ -624,7 +651,8 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void window_decode_kernel(WindowP
   // A weight that fp16 rounds to 0 times an infinity of V, or one past its range
   // (scores of 2^24 and more, whose fp32 maximum is several powers of two off),
   // is a NaN that weights of fp32 do not give: such heads are done again with
-  // those, by the wave that put them, in LDS behind what the waves met in.
+  // those, by the wave that put them, in LDS behind what the waves met in.  (0.2 ms
+  // for the heads of 2048 positions; nothing where none is.)
   unsigned long long waiting = __builtin_amdgcn_ballot_w64(again != 0);
   if (waiting) {
     unsigned todo = 0;
@@ -637,7 +665,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void window_decode_kernel(WindowP
         reinterpret_cast<PlainScratch*>(reinterpret_cast<char*>(s_ring) + kMet)[wave];
     __builtin_amdgcn_s_waitcnt(0);  // the NaNs are stored
     for (; todo; todo &= todo - 1)
-      plain_row_inline(p, row, first_head + __builtin_ctz(todo), scratch);
+      plain_row_inline<D>(p, row, first_head + __builtin_ctz(todo), scratch);
   }
 }
 
@@ -984,7 +1012,7 @@ __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(Wi
         whole &= window_page_ok(p, table[i]);
       if (!whole) len = 0;
     }
-    float scale = 1.0f / sum;
+    float scale = 1.0f / sum, top = m;
     bool nan = false;  // in what this lane stored of its vector
     if constexpr (PG > 1) {
       if (half == 0) {
@@ -992,7 +1020,7 @@ __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(Wi
         s_sum[wave][col] = sum;
       }
       __syncthreads();
-      float top = -INFINITY, total = 0.0f;
+      float total = 0.0f;
 #pragma unroll
       for (int g = 0; g < PG; ++g) top = fmaxf(top, s_max[g * VG + vg][col]);
 #pragma unroll
@@ -1069,15 +1097,16 @@ __global__ __launch_bounds__(kChunkWaves * kWave, 2) void window_chunk_kernel(Wi
     // range of fp16 leave, or none at all (scores of 2^24 and more, whose fp32
     // maximum is several powers of two off): such vectors are done again, one at a
     // time, over their own positions alone and with weights of fp32.
-    if (__syncthreads_or(nan && len > 0)) {
-      unsigned long long again = __builtin_amdgcn_ballot_w64(nan && len > 0);
+    nan &= len > 0 && finite(top);
+    if (__syncthreads_or(nan)) {
+      unsigned long long again = __builtin_amdgcn_ballot_w64(nan);
       again = (again | again >> 32) & 0xFFFFFFFFull;
       PlainScratch& scratch = reinterpret_cast<PlainScratch*>(s_kv)[wave];
       static_assert(sizeof(PlainScratch) * WAVES <= sizeof(s_kv), "a scratch for every wave");
       while (again) {
         const int from_lane = __builtin_ctzll(again);
         again &= again - 1;
-        plain_row(p, __shfl(row, from_lane, kWave), __shfl(head, from_lane, kWave), scratch);
+        plain_row<D>(p, __shfl(row, from_lane, kWave), __shfl(head, from_lane, kWave), scratch);
       }
       __syncthreads();
     }

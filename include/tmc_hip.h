@@ -825,7 +825,7 @@ size_t tmc_window_attention_workspace_bytes(int64_t batch, int64_t q_heads, int6
  * the greatest.  Requests may share pages.  Softmax weights are rounded to fp16
  * (11 bits; sums in fp32) at every head_dim, where tmc_paged_decode_attention
  * keeps 22 bits at head_dim 64.  head_dim 64 and 128 over pools below 64 GiB run
- * on the matrix cores; the others run a simple kernel that takes 10 to 100 times
+ * on the matrix cores; the others run a simple kernel that takes 7 to 100 times
  * as long. */
 int tmc_window_decode_attention(const void *q, const void *key_pool, const void *value_pool,
                                 const int32_t *valid_lengths, const int32_t *block_tables,

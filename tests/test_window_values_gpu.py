@@ -193,3 +193,44 @@ def test_long_tails_of_small_weights(tmc, torch, form, rows, qh, kvh, d, positio
     valid = lengths_of(form, rows, positions)
     got = s.attend(form, q.to(torch.float16), valid, window, 4)
     assert ((got.double() - 1.0).abs() <= 2.0 ** -11 + 9400 * 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("form,rows,qh,kvh,d,page,last,window,sinks", FORMS)
+def test_nan_and_infinite_operands_stay_where_they_are(tmc, torch, form, rows, qh, kvh, d, page, last,
+                                                       window, sinks):
+    """A NaN of q makes its head NaN and no other; an infinity of K makes a score
+    +inf, and the head NaN, or -inf, and its position weigh nothing, by the sign
+    of q; a NaN of V makes its dim NaN alone."""
+    s = Stream(tmc, torch, last, kvh, d, page, 7 * rows + d)
+    group = qh // kvh
+    valid = lengths_of(form, rows, last)
+    s.k.copy_(s.normal(last, kvh, d))
+    s.v.copy_(s.normal(last, kvh, d))
+    low = max(n - window for n in valid)
+    odd_k, odd_v = low + 5, low + 9
+    assert sinks <= low and odd_v < min(valid)
+    s.k[odd_k, :, 1] = math.inf
+    s.v[odd_v, :, 7] = math.nan
+    q = s.normal(rows, qh, d).to(torch.float16)
+    q[:, :, 1] = -1.0
+    heads = torch.arange(qh, device="cuda")
+    turn = (heads[None] + torch.arange(rows, device="cuda")[:, None]) % 4
+    q[:, :, 3] = torch.where(turn == 1, math.nan, q[:, :, 3])
+    q[:, :, 1] = torch.where(turn == 2, 1.0, q[:, :, 1])
+    got = s.attend(form, q, valid, window, sinks)
+    lost = (turn == 1) | (turn == 2)
+    assert torch.isnan(got[lost]).all()
+    kept = torch.ones(d, dtype=torch.bool, device="cuda")
+    kept[7] = False
+    assert torch.isnan(got[:, :, 7]).all()
+    assert torch.isfinite(got[~lost][:, kept]).all()
+    clean = s.v.clone()
+    clean[odd_v, :, 7] = 0.0
+    for r in some(rows):
+        see = torch.tensor([p for p in visible(valid[r], window, sinks) if p != odd_k], device="cuda")
+        for kh in {0, kvh - 1}:
+            mine = slice(kh * group, (kh + 1) * group)
+            o, tolerance = attend64(torch, q[r, mine].nan_to_num(0.0), s.k[see, kh:kh + 1],
+                                    clean[see, kh:kh + 1])
+            near = (got[r, mine].double() - o).abs() <= tolerance
+            assert (near | lost[r, mine, None] | ~kept[None]).all(), r
