@@ -125,6 +125,17 @@ def _declare(l):
         "tmc_rebuild_tables": (i32, [vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, vp]),
         "tmc_logprobs_workspace_bytes": (sz, [i64, i64, i64]),
         "tmc_logprobs": (i32, [vp, i32, i64, vp, vp, vp, vp, vp, i64, i64, i64, vp, sz, vp]),
+        "tmc_tree_layout": (i32, [vp, vp, vp, vp, i64, i64, vp]),
+        "tmc_tree_rope_append": (i32, [vp, vp, vp, i64, vp, vp, vp, vp, vp, vp, vp, vp, i32, i64,
+                                       i64, i64, i64, i64, i64, i64, i64, vp]),
+        "tmc_tree_attention_workspace_bytes": (sz, [i64, i64, i64, i64, i64, i64]),
+        "tmc_tree_attention": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, i32, i64, i64, i64, i64,
+                                     i64, i64, i64, i64, i64, i64, vp, sz, vp]),
+        "tmc_sample_workspace_bytes": (sz, [i64, i64]),
+        "tmc_sample": (i32, [vp, i32, i64, vp, vp, vp, vp, vp, vp, vp, i64, i64, vp, sz, vp]),
+        "tmc_tree_accept": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, vp]),
+        "tmc_tree_keep": (i32, [vp, vp, i64, vp, vp, vp, vp, i32, i64, i64, i64, i64, i64, i64,
+                                i64, i64, i64, vp]),
         "tmc_lm_head_argmax_workspace_bytes": (sz, [i64, i64]),
         "tmc_rmsnorm_lm_head_partial_argmax_f16": (i32, [vp, vp, vp, vp, sz, i64, i64, f, vp, vp]),
         "tmc_lm_head_partial_argmax_packed_norm_f16": (i32, [vp, vp, vp, sz, i64, i64, i64, f, i32,
@@ -893,6 +904,20 @@ def page_moves(moves, pools, pool_pages, page_size):
     return host_moves.cuda()
 
 
+def _pool_list(torch, what, device, k_pools, v_pools):
+    """K pools and V pools in one list, and their type, after a refusal of what is
+    not on the current GPU, whole and of one type."""
+    pools, tensor, dtype = [*k_pools, *v_pools], torch.Tensor, k_pools[0].dtype
+    if dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        raise TmcError(f"{what}: pools must be float16, bfloat16 or float32, not {dtype}")
+    if set(map(tensor.get_device, pools)) != {device} or \
+            not all(map(tensor.is_contiguous, pools)) or {t.dtype for t in pools} != {dtype}:
+        for i, t in enumerate(pools):
+            if t.get_device() != device or t.dtype is not dtype or not t.is_contiguous():
+                _refuse(what, device, dtype, f"pool {i}", t, 0)
+    return pools, dtype
+
+
 def move_pages(k_pools, v_pools, moves, heads, page_size, head_dim, page_stride=None,
                head_stride=None, stream=None):
     """Copy pages inside their pools, one K and one V pool per layer, by the
@@ -909,17 +934,10 @@ def move_pages(k_pools, v_pools, moves, heads, page_size, head_dim, page_stride=
         raise TmcError(f"{what}: heads, page_size, head_dim and strides must be positive")
     if moves.dim() != 2 or moves.shape[1] != 4:
         raise TmcError(f"{what}: moves must be [count, 4]")
-    device, dtype = torch.cuda.current_device(), k_pools[0].dtype
-    if dtype not in (torch.float16, torch.bfloat16, torch.float32):
-        raise TmcError(f"{what}: pools must be float16, bfloat16 or float32, not {dtype}")
+    device = torch.cuda.current_device()
     move_list = _address(what, device, torch.int32, "moves", moves, 0)
-    pools = [*k_pools, *v_pools]
+    pools, _ = _pool_list(torch, what, device, k_pools, v_pools)
     tensor = torch.Tensor
-    if set(map(tensor.get_device, pools)) != {device} or \
-            not all(map(tensor.is_contiguous, pools)) or {t.dtype for t in pools} != {dtype}:
-        for i, t in enumerate(pools):
-            if t.get_device() != device or t.dtype is not dtype or not t.is_contiguous():
-                _refuse(what, device, dtype, f"pool {i}", t, 0)
     if moves.shape[0] == 0:
         return
     pool_pages = min(map(tensor.numel, pools)) // page_stride
@@ -996,6 +1014,186 @@ def logprobs(logits, tokens, logprob, entropy=None, top_tokens=None, top_logprob
         logits.data_ptr(), code, strides[0] if rows > 1 else vocabulary, given, chosen,
         spread, greatest if top else None, best if top else None, rows, vocabulary, top, space,
         space_bytes, _launch_stream(torch, what, device, stream)), what)
+
+
+# ---------------------------------------------------------------- speculative decoding
+def _tree_shape(what, parents):
+    if parents.dim() != 2:
+        raise TmcError(f"{what}: trees must be [batch, nodes]")
+    return parents.shape
+
+
+def tree_layout(parents, masks, depths, counts=None, stream=None):
+    """Masks [batch, nodes, ceil(nodes / 32)] and depths [batch, nodes] (int32) of
+    trees given by their nodes' parents [batch, nodes] (tmc_tree_layout)."""
+    import torch
+    what = "tmc_tree_layout"
+    device, i32 = torch.cuda.current_device(), torch.int32
+    batch, nodes = _tree_shape(what, parents)
+    check(lib().tmc_tree_layout(
+        _address(what, device, i32, "parents", parents, 0),
+        _address(what, device, i32, "counts", counts, batch),
+        _address(what, device, i32, "masks", masks, batch * nodes * ((nodes + 31) // 32)),
+        _address(what, device, i32, "depths", depths, batch * nodes), batch, nodes,
+        _launch_stream(torch, what, device, stream)), what)
+
+
+def tree_rope_append(qkv, cosine, sine, cached_lengths, depths, counts, tables, active, q_out,
+                     k_pool, v_pool, batch, nodes, q_heads, kv_heads, head_dim, page_size,
+                     max_pages, stream=None, pool_pages=None):
+    """Rotate the trees' q and k by cached + depth, q to q_out, k and v to slot
+    cached + node of the pools (tmc_tree_rope_append); counts and active may be
+    None."""
+    import torch
+    what = "tmc_tree_rope_append"
+    device, dtype = torch.cuda.current_device(), qkv.dtype
+    pool_pages = _window_pages(what, k_pool, v_pool, batch, q_heads, kv_heads, head_dim, max_pages,
+                               kv_heads * page_size * head_dim, pool_pages)
+    if dtype not in (torch.float16, torch.float32):
+        raise TmcError(f"{what}: qkv must be float16 or float32, not {dtype}")
+    if nodes < 1:
+        raise TmcError(f"{what}: nodes must be positive")
+    pairs = head_dim // 2
+    positions = min(cosine.numel(), sine.numel()) // max(pairs, 1)
+    f32, i32, rows = torch.float32, torch.int32, batch * nodes
+    check(lib().tmc_tree_rope_append(
+        _address(what, device, dtype, "qkv", qkv, rows * (q_heads + 2 * kv_heads) * head_dim),
+        _address(what, device, f32, "cosine", cosine, 0),
+        _address(what, device, f32, "sine", sine, 0), positions,
+        _address(what, device, i32, "cached_lengths", cached_lengths, batch),
+        _address(what, device, i32, "depths", depths, rows),
+        _address(what, device, i32, "counts", counts, batch),
+        _address(what, device, i32, "tables", tables, batch * max_pages),
+        _address(what, device, i32, "active", active, 1),
+        _address(what, device, dtype, "q_out", q_out, rows * q_heads * head_dim),
+        _address(what, device, dtype, "k_pool", k_pool, 0),
+        _address(what, device, dtype, "v_pool", v_pool, 0), _dtype_code(qkv), batch, nodes,
+        q_heads, kv_heads, head_dim, page_size, max_pages, pool_pages,
+        _launch_stream(torch, what, device, stream)), what)
+
+
+def tree_attention_workspace_bytes(batch, nodes, q_heads, kv_heads, head_dim, capacity) -> int:
+    return int(lib().tmc_tree_attention_workspace_bytes(batch, nodes, q_heads, kv_heads, head_dim,
+                                                        capacity))
+
+
+def tree_attention(q, k_pool, v_pool, cached_lengths, masks, counts, tables, active, out, batch,
+                   nodes, q_heads, kv_heads, head_dim, page_size, max_pages, page_stride,
+                   head_stride, workspace=None, stream=None, pool_pages=None):
+    """Attention of the nodes of a tree a request over the cached positions and
+    the tree's slots that their masks name (tmc_tree_attention); counts and active
+    may be None.  The workspace must be zero before its first use."""
+    import torch
+    what = "tmc_tree_attention"
+    device = torch.cuda.current_device()
+    pool_pages = _window_pages(what, k_pool, v_pool, batch, q_heads, kv_heads, head_dim, max_pages,
+                               page_stride, pool_pages)
+    if nodes < 1:
+        raise TmcError(f"{what}: nodes must be positive")
+    f16, i32, rows = torch.float16, torch.int32, batch * nodes
+    space, space_bytes = _workspace(what, device, workspace)
+    check(lib().tmc_tree_attention(
+        _address(what, device, f16, "q", q, rows * q_heads * head_dim),
+        _address(what, device, f16, "k_pool", k_pool, 0),
+        _address(what, device, f16, "v_pool", v_pool, 0),
+        _address(what, device, i32, "cached_lengths", cached_lengths, batch),
+        _address(what, device, i32, "masks", masks, rows * ((nodes + 31) // 32)),
+        _address(what, device, i32, "counts", counts, batch),
+        _address(what, device, i32, "tables", tables, batch * max_pages),
+        _address(what, device, i32, "active", active, 1),
+        _address(what, device, f16, "out", out, rows * q_heads * head_dim),
+        F16, batch, nodes, q_heads, kv_heads, head_dim, page_size, max_pages, pool_pages,
+        page_stride, head_stride, space, space_bytes,
+        _launch_stream(torch, what, device, stream)), what)
+
+
+def sample_workspace_bytes(rows, vocabulary) -> int:
+    return int(lib().tmc_sample_workspace_bytes(rows, vocabulary))
+
+
+def sample(logits, uniforms, tokens, temperature=None, top_k=None, top_p=None, min_p=None,
+           probability=None, workspace=None, stream=None):
+    """A token per row of logits [rows, vocabulary] (f32 or f16; rows may be
+    strided) by the rows' temperature, top_k (int32), top_p and min_p [rows], drawn
+    with uniforms [rows], and its probability among the tokens that stay
+    (tmc_sample).  The workspace must be zero before its first use."""
+    import torch
+    what = "tmc_sample"
+    strides = logits.stride()
+    if len(strides) != 2 or strides[1] != 1:
+        raise TmcError(f"{what}: logits must be [rows, vocabulary] with adjacent elements")
+    device, dtype = torch.cuda.current_device(), logits.dtype
+    if logits.get_device() != device:
+        _refuse(what, device, dtype, "logits", logits, 0)
+    if dtype not in (torch.float32, torch.float16):
+        raise TmcError(f"{what}: logits must be f32 or f16, not {dtype}")
+    rows, vocabulary = logits.shape
+    f32, i32 = torch.float32, torch.int32
+    space, space_bytes = _workspace(what, device, workspace)
+    check(lib().tmc_sample(
+        logits.data_ptr(), F32 if dtype is f32 else F16, strides[0] if rows > 1 else vocabulary,
+        _address(what, device, f32, "temperature", temperature, rows),
+        _address(what, device, i32, "top_k", top_k, rows),
+        _address(what, device, f32, "top_p", top_p, rows),
+        _address(what, device, f32, "min_p", min_p, rows),
+        _address(what, device, f32, "uniforms", uniforms, rows),
+        _address(what, device, i32, "tokens", tokens, rows),
+        _address(what, device, f32, "probability", probability, rows), rows, vocabulary, space,
+        space_bytes, _launch_stream(torch, what, device, stream)), what)
+
+
+def tree_accept(drafted, parents, chosen, path, accepted, emitted, counts=None, active=None,
+                cached_lengths=None, new_lengths=None, stream=None):
+    """The branch of each tree that the tokens chosen at its nodes agree with
+    (tmc_tree_accept); all int32, [batch, nodes] or [batch]."""
+    import torch
+    what = "tmc_tree_accept"
+    device, i32 = torch.cuda.current_device(), torch.int32
+    batch, nodes = _tree_shape(what, parents)
+    rows = batch * nodes
+    check(lib().tmc_tree_accept(
+        _address(what, device, i32, "drafted", drafted, rows),
+        _address(what, device, i32, "parents", parents, rows),
+        _address(what, device, i32, "chosen", chosen, rows),
+        _address(what, device, i32, "counts", counts, batch),
+        _address(what, device, i32, "active", active, 1),
+        _address(what, device, i32, "cached_lengths", cached_lengths, batch),
+        _address(what, device, i32, "path", path, rows),
+        _address(what, device, i32, "accepted", accepted, batch),
+        _address(what, device, i32, "emitted", emitted, rows),
+        _address(what, device, i32, "new_lengths", new_lengths, batch), batch, nodes,
+        _launch_stream(torch, what, device, stream)), what)
+
+
+def tree_keep(k_pools, v_pools, tables, cached_lengths, path, accepted, heads, page_size, head_dim,
+              page_stride=None, head_stride=None, stream=None):
+    """K and V of the path [batch, nodes] moved up to the cached positions, one K
+    and one V pool per layer, tables [layers, batch, max_pages] (tmc_tree_keep)."""
+    import torch
+    what = "tmc_tree_keep"
+    count = len(k_pools)
+    if not count or count != len(v_pools):
+        raise TmcError(f"{what}: as many K pools as V pools, and at least one")
+    head_stride = page_size * head_dim if head_stride is None else head_stride
+    page_stride = heads * head_stride if page_stride is None else page_stride
+    if min(heads, page_size, head_dim, page_stride) < 1:
+        raise TmcError(f"{what}: heads, page_size, head_dim and strides must be positive")
+    batch, nodes = _tree_shape(what, path)
+    if tables.dim() != 3 or tables.shape[0] != count or tables.shape[1] != batch:
+        raise TmcError(f"{what}: tables must be [layers, batch, max_pages]")
+    device, i32 = torch.cuda.current_device(), torch.int32
+    pools, dtype = _pool_list(torch, what, device, k_pools, v_pools)
+    pool_pages = min(map(torch.Tensor.numel, pools)) // page_stride
+    addresses = array.array("Q", map(torch.Tensor.data_ptr, pools))
+    first, size = addresses.buffer_info()[0], addresses.itemsize
+    check(lib().tmc_tree_keep(
+        first, first + count * size, count,
+        _address(what, device, i32, "tables", tables, 0),
+        _address(what, device, i32, "cached_lengths", cached_lengths, batch),
+        _address(what, device, i32, "path", path, 0),
+        _address(what, device, i32, "accepted", accepted, batch), _dtype_code(k_pools[0]), batch,
+        nodes, heads, head_dim, page_size, tables.shape[2], pool_pages, page_stride, head_stride,
+        _launch_stream(torch, what, device, stream)), what)
 
 
 def fill_normal(t, seed, mean=0.0, std=1.0, stream=None):

@@ -41,7 +41,8 @@ CXXFLAGS = ["-std=c++17", "-O2", "-fPIC", "-Wall", "-Wextra", "-Wno-unused-param
             f"-I{INCLUDE}", f"-I{HOST}"]
 
 SOURCES = ["runtime.hip", "gemv.hip", "packed.hip", "elementwise.hip", "attention.hip",
-           "prefill.hip", "gemm.hip", "window.hip", "pages.hip", "logprobs.hip"]
+           "prefill.hip", "gemm.hip", "window.hip", "pages.hip", "logprobs.hip",
+           "tree.hip", "tree_attention.hip", "sample.hip"]
 # The HIP runtime library of the ROCm install (rpath of the built library).
 ROCM_LIB = os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "lib")
 
@@ -62,10 +63,11 @@ FLAGS = [
 ]
 
 
-# Per-source additions.  prefill.hip, window.hip: keep MFMA accumulators in VGPRs (the
+# Per-source additions.  prefill.hip, window.hip, tree_attention.hip: keep MFMA accumulators in VGPRs (the
 # online-softmax rescale multiplies them every block; from AGPRs each one is
 # a read, a multiply and a write back).
-SOURCE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for name in ("prefill.hip", "window.hip")}
+SOURCE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"] 
+                for name in ("prefill.hip", "window.hip", "tree_attention.hip")}
 
 
 def _compile(src: str, variant: str = "", defines: tuple = ()) -> str:

@@ -28,6 +28,27 @@ constexpr int kWave = 64;
 constexpr int kSharedRows = 512, kCounterStride = 32;
 constexpr size_t kCounterBytes = kSharedRows * kCounterStride * sizeof(int);
 
+// Nodes of a tree of drafted tokens, at most, and 32-bit words of a node's mask.
+constexpr int kTreeMost = 256, kTreeWords = kTreeMost / 32;
+
+// Position / page size for positions below 2^31 by a product and a shift:
+// magic = floor(2^(31 + s) / d) + 1 with d <= 2^s: magic d - 2^(31 + s) is in
+// (0, 2^s], so the quotient is exact.
+struct PageDivide {
+  unsigned magic;  // 0: a page size of 1
+  int shift;
+  static PageDivide by(int64_t page_size) {
+    if (page_size == 1) return PageDivide{0, 0};
+    int s = 1;
+    while (((int64_t)1 << s) < page_size) ++s;
+    return PageDivide{(unsigned)(((uint64_t)1 << (31 + s)) / (uint64_t)page_size + 1), s - 1};
+  }
+  __device__ __forceinline__ int operator()(int pos) const {
+    const int q = (int)(__umulhi((unsigned)pos, magic) >> shift);
+    return magic ? q : pos;
+  }
+};
+
 // ------------------------------------------------------------------ loads
 __device__ __forceinline__ h8 load_h8(const half_t* p) {
   return *reinterpret_cast<const h8*>(p);

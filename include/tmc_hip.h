@@ -910,6 +910,122 @@ int tmc_logprobs(const void *logits, int dtype, int64_t row_stride, const int32_
                  int64_t rows, int64_t vocabulary, int64_t top, void *workspace,
                  size_t workspace_bytes, void *stream);
 
+/* -------------------------------------------------- speculative decoding
+ * A request's next tokens drafted as a tree and verified in one step: the
+ * tree's K and V enter the paged cache, every node attends the cache and its
+ * own branch, a token is sampled at every node, and the branch that the samples
+ * agree with is kept.  No counterparts in the reference, which decodes one
+ * greedy token a step.
+ *
+ * A tree has up to 256 nodes: node 0 is the request's last token, whose K and V
+ * are not cached yet.  parents [batch, nodes] names an earlier node for each; a
+ * parent outside [0, i) makes node i a root that sees only itself.  counts
+ * [batch] (NULL: `nodes` everywhere) are the trees' sizes; nodes from there on
+ * are left alone.  Node i of a request with cached_lengths[r] cached positions
+ * lies in slot cached_lengths[r] + i of its pages and is rotated by position
+ * cached_lengths[r] + depth(i). */
+
+/* masks [batch, nodes, ceil(nodes / 32)]: bit j of node i's mask (word j / 32)
+ * is set where j is i itself or an ancestor; depths [batch, nodes]: its
+ * ancestors' number.  One launch a step, for all layers. */
+int tmc_tree_layout(const int32_t *parents, const int32_t *counts, uint32_t *masks,
+                    int32_t *depths, int64_t batch, int64_t nodes, void *stream);
+
+/* tmc_decode_rope_append for trees: row (r, i) of qkv [batch, nodes, (q_heads +
+ * 2 kv_heads) * head_dim] rotated by row cached_lengths[r] + depths[r, i] of the
+ * tables cosine, sine [positions, head_dim / 2]; the query to q_out [batch,
+ * nodes, q_heads * head_dim], the key and the value to slot cached_lengths[r] + i
+ * of the pools [pool_pages][kv_heads][page_size][head_dim].  The same bits for the
+ * same pair.  Requests >= active_count[0] (NULL: all are active), nodes past the
+ * count, the capacity or the tables are skipped; a token without a page stores
+ * its query alone.  dtype f16 or f32; buffers aligned to two elements (f16 in
+ * 16-byte units where they are aligned to 16 bytes and head_dim is a multiple of
+ * 8, which is faster). */
+int tmc_tree_rope_append(const void *qkv, const float *cosine, const float *sine,
+                         int64_t positions, const int32_t *cached_lengths, const int32_t *depths,
+                         const int32_t *counts, const int32_t *block_tables,
+                         const int32_t *active_count, void *q_out, void *key_pool,
+                         void *value_pool, int dtype, int64_t batch, int64_t nodes,
+                         int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t page_size,
+                         int64_t max_pages, int64_t pool_pages, void *stream);
+
+/* Bytes of device workspace tmc_tree_attention needs for these limits (capacity
+ * = page_size * max_pages; 0 when none is needed), by the rules of
+ * tmc_window_attention_workspace_bytes: one workspace serves launches of both, of
+ * tmc_logprobs and of tmc_sample in turn. */
+size_t tmc_tree_attention_workspace_bytes(int64_t batch, int64_t nodes, int64_t q_heads,
+                                          int64_t kv_heads, int64_t head_dim, int64_t capacity);
+
+/* Attention of every node of every tree: node i of request r (q and out [batch,
+ * nodes, q_heads * head_dim]) attends positions [0, cached_lengths[r]) and slot
+ * cached_lengths[r] + j for every bit j < counts[r] of its mask (as
+ * tmc_tree_layout makes them, or any others); a node that sees nothing gives
+ * zeros.  Geometry, values and limits as tmc_window_decode_attention.  A request
+ * whose cached_lengths[r] + counts[r] positions are not all inside the capacity and
+ * on pages in [0, pool_pages), with a negative length, or >= active_count[0]
+ * (NULL: all are active) leaves its rows untouched, as do nodes past the count. */
+int tmc_tree_attention(const void *q, const void *key_pool, const void *value_pool,
+                       const int32_t *cached_lengths, const uint32_t *masks,
+                       const int32_t *counts, const int32_t *block_tables,
+                       const int32_t *active_count, void *out, int dtype, int64_t batch,
+                       int64_t nodes, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                       int64_t page_size, int64_t max_pages, int64_t pool_pages,
+                       int64_t page_stride, int64_t head_stride, void *workspace,
+                       size_t workspace_bytes, void *stream);
+
+/* Bytes of device workspace tmc_sample needs (0 when none is needed; by the
+ * rules of tmc_window_attention_workspace_bytes). */
+size_t tmc_sample_workspace_bytes(int64_t rows, int64_t vocabulary);
+
+/* A token per row of logits [rows, vocabulary] (f32 or f16, rows row_stride
+ * elements apart), drawn with uniforms[r] in [0, 1).  Each row has settings of its
+ * own, arrays of [rows] or NULL for the neutral value:
+ *   temperature  w_i = exp((x_i - max x) / temperature); 1.  Below 2^-16 (or NaN)
+ *                the row takes its most probable token, as tmc_argmax_f32
+ *   top_k        the k most probable tokens stay; 0 or less: all
+ *   top_p        of those, each before which less than top_p of their sum lies,
+ *                the most probable first; 1 or more: all
+ *   min_p        of those, each with w_i >= min_p; 0 or less: all
+ * Equal logits rank by the lower index; the most probable token always stays.
+ * tokens[r] is the first that stays, in the order of the vocabulary, where the
+ * running sum of w passes uniforms[r] times the sum of all that stay;
+ * probability[r] (may be NULL) its share of that sum, 1 for a row that takes its
+ * most probable token.  Arithmetic in 64 bits.  Never drawn are logits of NaN and
+ * -inf and tokens below 2^-44 of the greatest weight (together less than the
+ * resolution of a 24-bit random number); with logits of +inf the draw is among
+ * them; a row without a logit above -inf gives its most probable token and a
+ * probability of NaN, -1 if all are NaN.  At most 2^20 tokens. */
+int tmc_sample(const void *logits, int dtype, int64_t row_stride, const float *temperature,
+               const int32_t *top_k, const float *top_p, const float *min_p,
+               const float *uniforms, int32_t *tokens, float *probability, int64_t rows,
+               int64_t vocabulary, void *workspace, size_t workspace_bytes, void *stream);
+
+/* The branch that the sampled tokens agree with: from node 0, on to the child
+ * whose drafted token is the one chosen [batch, nodes] at its parent (the lowest of
+ * several), as long as there is one.  accepted[r] is the number of nodes on that
+ * path, at least 1 in an active request with a tree, else 0; path [batch, nodes]
+ * lists them and emitted [batch, nodes] the tokens chosen there, -1 behind; the
+ * last emitted token is node 0 of the next step.  new_lengths[r] (may be NULL) =
+ * cached_lengths[r] + accepted[r].  Nothing overlaps. */
+int tmc_tree_accept(const int32_t *drafted, const int32_t *parents, const int32_t *chosen,
+                    const int32_t *counts, const int32_t *active_count,
+                    const int32_t *cached_lengths, int32_t *path, int32_t *accepted,
+                    int32_t *emitted, int32_t *new_lengths, int64_t batch, int64_t nodes,
+                    void *stream);
+
+/* K and V of the path moved up, in all layers: slot cached_lengths[r] + path[r, s]
+ * is copied to slot cached_lengths[r] + s, bit for bit, for s < accepted[r].
+ * key_pools and value_pools are host arrays of `pools` device pointers as for
+ * tmc_move_pages, block_tables [pools, batch, max_pages].  path increases, as
+ * tmc_tree_accept writes it; where it does not, or leaves [0, nodes), it ends.
+ * Steps whose slots lie past the capacity or on no page are skipped.  No two
+ * requests may share the pages of these slots. */
+int tmc_tree_keep(void *const *key_pools, void *const *value_pools, int64_t pools,
+                  const int32_t *block_tables, const int32_t *cached_lengths, const int32_t *path,
+                  const int32_t *accepted, int dtype, int64_t batch, int64_t nodes, int64_t heads,
+                  int64_t head_dim, int64_t page_size, int64_t max_pages, int64_t pool_pages,
+                  int64_t page_stride, int64_t head_stride, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
