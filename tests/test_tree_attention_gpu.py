@@ -187,3 +187,33 @@ def test_refusals(tmc):
     with pytest.raises(tmc.TmcError):
         f.attend(tmc, t, pool_pages=f.pages + 1)
     assert (t["out"] == 7.0).all()
+
+
+@pytest.mark.parametrize("nodes,qh,kvh,dim", [(3, 4, 4, 64), (9, 2, 1, 128), (16, 8, 2, 64),
+                                              (16, 8, 2, 128), (70, 4, 2, 128), (128, 4, 2, 64)])
+def test_one_long_among_short(tmc, nodes, qh, kvh, dim):
+    """One request has nearly all of the steps, the others one or none."""
+    cached = [3] * 20 + [24000] + [0] * 20
+    f = Forest(15, cached, nodes, qh, kvh, dim, 16, counts=[1 if c < 10 else nodes for c in cached])
+    t = f.device()
+    f.attend(tmc, t)
+    f.check(t, requests=[0, 19, 20, 21, 40])
+
+
+@pytest.mark.parametrize("nodes,qh,kvh,dim", [(2, 2, 1, 64), (40, 2, 1, 64), (40, 2, 1, 128)])
+def test_one_request_one_head(tmc, nodes, qh, kvh, dim):
+    """As many pieces as there can be of one (request, kv head)."""
+    f = Forest(16, [40000], nodes, qh, kvh, dim, 64)
+    t = f.device()
+    f.attend(tmc, t)
+    f.check(t)
+
+
+@pytest.mark.parametrize("batch,nodes,dim", [(300, 2, 64), (70, 20, 128)])
+def test_many_requests(tmc, batch, nodes, dim):
+    rng = random.Random(17)
+    cached = [rng.choice([0, 1, 15, 16, 100, 700]) for _ in range(batch)]
+    f = Forest(17, cached, nodes, 4, 2, dim, 16, counts=[rng.randint(0, nodes) for _ in cached])
+    t = f.device()
+    f.attend(tmc, t)
+    f.check(t)
