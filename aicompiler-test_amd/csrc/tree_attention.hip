@@ -49,6 +49,13 @@ __device__ __forceinline__ bool tree_page_ok(const TreeParams& p, int page) {
   return page >= 0 && page < p.pool_pages;
 }
 
+// A value that the compiler knows nothing of: what follows from it is computed where it is
+// used, not kept in registers around the loops before.
+__device__ __forceinline__ unsigned opaque(unsigned v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
 // ------------------------------------------------------------ any geometry
 // One wave per (node, query head): 64 positions at a time, one per lane for the
 // scores (whole K rows in 16-byte chunks), then lanes over the dims for P V.
@@ -65,7 +72,7 @@ __device__ __forceinline__ void plain_node(const TreeParams& p, int r, const Req
                                            int node, int head, PlainScratch& scratch) {
   constexpr int TILES = (DIM ? DIM : kPlainMaxDim) / kWave;
   constexpr int kAhead = 8;  // chunks of K, rows of V loaded at once
-  const int lane = threadIdx.x & (kWave - 1);
+  const int lane = (int)opaque(threadIdx.x) & (kWave - 1);
   const int32_t* table = p.tables + (size_t)r * p.max_pages;
   const int kvh = head / p.group, d = DIM ? DIM : p.dim;
   const size_t row = (size_t)r * p.nodes + node;
@@ -425,6 +432,7 @@ template <int D, int NV, int COUNT, int THREADS, bool AGENT>
 __device__ __forceinline__ unsigned join(const TreeParams& p, const TreePlan& plan, const Part& at,
                                          int first_vec, int count, char* s_space,
                                          Outputs<COUNT>& s_outputs) {
+  const int thread = (int)opaque(threadIdx.x);
   constexpr int ROW = slot_row<D>();
   constexpr int LANES = THREADS / COUNT < kWave ? THREADS / COUNT : kWave;
   float2* s_factor = reinterpret_cast<float2*>(s_space);  // [pieces][COUNT]: (maximum, sum)
@@ -432,7 +440,7 @@ __device__ __forceinline__ unsigned join(const TreeParams& p, const TreePlan& pl
     return plan.slots + (((size_t)at.slot(piece) * plan.tiles + at.tile) * NV + first_vec) * ROW;
   };
   {
-    const int vec = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+    const int vec = thread / LANES, lane = thread % LANES;
     float top = -INFINITY, sum = 0.0f;
     if (vec < count) {
       for (int b = lane; b < at.pieces; b += LANES) {
@@ -469,7 +477,7 @@ __device__ __forceinline__ unsigned join(const TreeParams& p, const TreePlan& pl
   unsigned again = 0, bit = 1;
   constexpr int kAhead = 4, kTurns = 2;
   const int items = count * (D / 4);
-  for (int i = threadIdx.x; i < items; i += kTurns * THREADS, bit <<= kTurns) {
+  for (int i = thread; i < items; i += kTurns * THREADS, bit <<= kTurns) {
     f4 val[kTurns] = {};
     for (int b = 0; b < at.pieces; b += kAhead) {
       f4 x[kTurns][kAhead];
@@ -509,12 +517,13 @@ __device__ __forceinline__ unsigned join(const TreeParams& p, const TreePlan& pl
 template <int D, int THREADS>
 __device__ __forceinline__ void redo(const TreeParams& p, const Part& at, unsigned again, int first,
                                      char* s_space) {
+  const int thread = (int)opaque(threadIdx.x);
   if (__syncthreads_or(again != 0)) {
-    PlainScratch& scratch = reinterpret_cast<PlainScratch*>(s_space)[threadIdx.x / kWave];
+    PlainScratch& scratch = reinterpret_cast<PlainScratch*>(s_space)[thread / kWave];
     __builtin_amdgcn_s_waitcnt(0);  // the NaNs are stored
     constexpr int SIDE = D / 4;     // lanes of a vector
     static_assert(SIDE < kWave, "a vector is a wave's");
-    first += (int)(threadIdx.x & ~(kWave - 1)) / SIDE;
+    first += (thread & ~(kWave - 1)) / SIDE;
     for (int turn = 0; turn < 32; ++turn) {
       const unsigned long long lanes = __builtin_amdgcn_ballot_w64(again >> turn & 1);
       if (lanes == 0) continue;
@@ -533,6 +542,7 @@ __device__ __forceinline__ void redo(const TreeParams& p, const Part& at, unsign
 template <int D, int NV, int GROUPS, int THREADS>
 __device__ __forceinline__ void finish(const TreeParams& p, const TreePlan& plan, const Part& at,
                                        char* s_space, float* s_max, const float* s_sum, int bad) {
+  const int thread = (int)opaque(threadIdx.x);
   constexpr int ROW = slot_row<D>();
   static_assert(NV <= THREADS && NV * (D / 4) / THREADS <= 32, "a thread a vector, a bit a turn");
   static_assert(sizeof(PlainScratch) * (THREADS / kWave) <= NV * ROW * 4 * GROUPS,
@@ -542,8 +552,8 @@ __device__ __forceinline__ void finish(const TreeParams& p, const TreePlan& plan
   const float* s_out = reinterpret_cast<const float*>(s_space);
   const bool whole = at.pieces == 1;
   float* slot = plan.slots + ((size_t)at.slot(at.piece) * plan.tiles + at.tile) * NV * ROW;
-  if ((int)threadIdx.x < at.vecs) {
-    const int vec = threadIdx.x;
+  if (thread < at.vecs) {
+    const int vec = thread;
     float top = -INFINITY, sum = 0.0f, scale[GROUPS];
 #pragma unroll
     for (int w = 0; w < GROUPS; ++w) top = fmaxf(top, s_max[w * NV + vec]);
@@ -568,7 +578,7 @@ __device__ __forceinline__ void finish(const TreeParams& p, const TreePlan& plan
   }
   __syncthreads();
   unsigned again = 0, bit = 1;
-  for (int i = threadIdx.x; i < at.vecs * (D / 4); i += THREADS, bit <<= 1) {
+  for (int i = thread; i < at.vecs * (D / 4); i += THREADS, bit <<= 1) {
     const int vec = i / (D / 4), d = i % (D / 4) * 4;
     f4 val = {};
 #pragma unroll
@@ -592,12 +602,12 @@ __device__ __forceinline__ void finish(const TreeParams& p, const TreePlan& plan
     int* counter = plan.arrivals + at.unit * kCounterStride;
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    if (threadIdx.x == 0)
+    if (thread == 0)
       s_last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
                at.pieces - 1;
     __syncthreads();
     if (!s_last) return;
-    if (threadIdx.x == 0)
+    if (thread == 0)
       __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     again = join<D, NV, NV, THREADS, true>(p, plan, at, 0, at.vecs, s_space, s_outputs);
     __syncthreads();
@@ -869,11 +879,6 @@ __global__ __launch_bounds__(kTreeWaves * kWave, 1) void tree_ring_kernel(
 // SIMD: one's softmax runs beside the other's products.  K and V go through
 // registers, loaded one stage ahead of the LDS one; one barrier a stage.
 typedef float f16v __attribute__((ext_vector_type(16)));
-
-__device__ __forceinline__ unsigned opaque(unsigned v) {
-  asm volatile("" : "+v"(v));
-  return v;
-}
 
 constexpr int kWideSpan = 64;  // positions a stage
 
