@@ -28,8 +28,8 @@ typedef unsigned long long u64;
 
 // What a block of a shared row leaves to the last of them.
 struct SampleRecord {
-  u64 best;    // greatest rank key
-  double sum;  // of weights, relative to its greatest logit
+  u64 best;  // greatest rank key
+  u64 sum;   // of weights, relative to its greatest logit
 };
 
 struct SampleParams {
@@ -49,6 +49,8 @@ struct SampleParams {
   u64* bins;            // [rows][count][kBins]
   int* arrivals;        // [rows], kCounterStride apart
 };
+
+constexpr int kMostBlocks = 512;  // of a row
 
 // Below it a temperature counts as 0: the most probable token.
 constexpr float kColdest = 1.0f / 65536.0f;
@@ -106,14 +108,19 @@ constexpr int kDigits = 256;
 constexpr int kBinsOctave = 16, kBins = 44 * kBinsOctave;
 static_assert(kFaintest == -44.0, "bins down to the least weight");
 constexpr int kMostKept = 2048, kMostTopK = 1024;  // tokens in the list, top_k that goes by it
-constexpr int kMostGroups = 4096;                  // sums of a wave's loads in a block's part
+constexpr int kMostGroups = 1024;                  // sums of a block's loads
+constexpr int kCoarse = 32;  // bins of a coarse step, and at most steps
+static_assert(kMostTopK <= kMostGroups, "the list's weights fit their place");
+static_assert(kBins % kCoarse == 0 && kBins / kCoarse <= kCoarse, "two steps to a bin");
 
 template <int THREADS> struct SampleScratch {
   u64 hist[kBins > kDigits ? kBins : kDigits];
   u64 keys[kMostKept];
-  double groups[kMostGroups];
-  double wave[THREADS / kWave];
+  u64 groups[kMostGroups];
   u64 words[THREADS / kWave];
+  float highs[kMostBlocks];  // of a row's blocks: the greatest logit,
+  double blocks[kMostBlocks];  // the sum of weights
+  double levels[kCoarse];
   double value;
   u64 found64, below;
   int found, count, last;
@@ -166,13 +173,13 @@ __device__ __forceinline__ double exp2_of(double a) {
 // `target` (at least 1 and at most all of it): digit by digit, a histogram of the
 // costs of the keys that agree so far.
 template <int THREADS, typename EACH>
-__device__ u64 cut_at(u64 target, SampleScratch<THREADS>& s, const EACH& each) {
+__device__ __forceinline__ u64 cut_at(u64 target, SampleScratch<THREADS>& s, const EACH& each) {
   u64 prefix = 0;
   for (int shift = 56; shift >= 0; shift -= 8) {
     __syncthreads();
     for (int d = threadIdx.x; d < kDigits; d += THREADS) s.hist[d] = 0;
     __syncthreads();
-    each([&](u64 key, u64 cost) {
+    each([&](u64 key, u64 cost) TMC_INLINE {
       if (shift == 56 || key >> (shift + 8) == prefix >> (shift + 8))
         atomicAdd(&s.hist[key >> shift & 255], cost);
     });
@@ -195,7 +202,7 @@ __device__ u64 cut_at(u64 target, SampleScratch<THREADS>& s, const EACH& each) {
 // integers, cuts by their digits.  20 to 40 us a pass of a row of 32000, 5 to 25
 // passes.
 template <typename T, int THREADS>
-__device__ void row_by_digits(const SampleParams& p, int row, const Settings& set,
+__device__ __forceinline__ void row_by_digits(const SampleParams& p, int row, const Settings& set,
                               SampleScratch<THREADS>& s) {
   const T* x = static_cast<const T*>(p.logits) + (size_t)row * p.stride;
   // ---- the most probable token
@@ -215,42 +222,42 @@ __device__ void row_by_digits(const SampleParams& p, int row, const Settings& se
     return;
   }
   const double unit = ldexp(1.0, p.scale);
-  auto weight = [&](float v) -> u64 {
+  auto weight = [&](float v) TMC_INLINE -> u64 {
     if (v == top) return (u64)unit;
     if (!(v > -INFINITY) || top == INFINITY) return 0;
     const double a = ((double)v - (double)top) * set.heat;
     return a >= kFaintest ? max((u64)rint(exp2_of(a) * unit), (u64)1) : 0;
   };
   u64 cut = 0;
-  auto kept = [&](float v, int i) -> u64 {
+  auto kept = [&](float v, int i) TMC_INLINE -> u64 {
     const u64 w = weight(v);
     return w && rank_key(v, i) >= cut ? w : 0;
   };
   if (set.most < p.vocab) {
-    auto each = [&](auto&& take) {
+    auto each = [&](auto&& take) TMC_INLINE {
       for (int i = threadIdx.x; i < p.vocab; i += THREADS) {
         const float v = (float)x[i];
         if (weight(v)) take(rank_key(v, i), 1);
       }
     };
     u64 count = 0;
-    each([&](u64, u64 one) { count += one; });
+    each([&](u64, u64 one) TMC_INLINE { count += one; });
     if (block_sum_u64<THREADS>(count, s) > (u64)set.most) cut = cut_at<THREADS>((u64)set.most, s, each);
   }
   if (set.share < 1.0f) {
-    auto each = [&](auto&& take) {
+    auto each = [&](auto&& take) TMC_INLINE {
       for (int i = threadIdx.x; i < p.vocab; i += THREADS) {
         const float v = (float)x[i];
         if (const u64 w = kept(v, i)) take(rank_key(v, i), w);
       }
     };
     u64 sum = 0;
-    each([&](u64, u64 w) { sum += w; });
+    each([&](u64, u64 w) TMC_INLINE { sum += w; });
     sum = block_sum_u64<THREADS>(sum, s);
     const u64 target = max((u64)1, min(sum, (u64)ceil((double)set.share * (double)sum)));
     cut = max(cut, cut_at<THREADS>(target, s, each));
   }
-  auto final_weight = [&](int i) -> u64 {
+  auto final_weight = [&](int i) TMC_INLINE -> u64 {
     const float v = (float)x[i];
     if (v != top && !(((double)v - (double)top) * set.heat >= set.least)) return 0;
     return kept(v, i);
@@ -298,40 +305,45 @@ __device__ void row_by_digits(const SampleParams& p, int row, const Settings& se
 //     are collected and sorted, which gives the cut exactly;
 //   - the sums of the kept weights of every 64 lanes' tokens, and of these the 64 that
 //     hold the number drawn.
-// Bins are of absolute logits, so that those of several blocks fit together.  Sums of
-// bins are of integers, all others are in a fixed order: the result does not depend
-// on which thread comes first.  Rows that this does not fit (more than kMostKept tokens
-// to collect, as in flat rows or with many equals; infinities; a top_k above kMostTopK)
-// go to row_by_digits().
+// A block with its own row takes one 64-bit exponential a token: the bins' weights are of
+// 32 bits, and say only which bins' tokens to sort.  Blocks that share a row cannot
+// come back to it, so their bins are exact.
+//
+// Bins are of absolute logits, so that those of several blocks fit together.  Weights are
+// integers, sums of more blocks 64-bit floats in their order: the result does not
+// depend on which thread comes first.  Rows that this does not fit (more than kMostKept
+// tokens to collect, as in flat rows or with many equals; infinities; a top_k above
+// kMostTopK) go to row_by_digits().
 
 // The thread's EACH consecutive values and their sum.
-template <int EACH, typename VALUE>
-__device__ __forceinline__ double take_values(double (&v)[EACH], const VALUE& value) {
-  double sum = 0.0;
+template <int EACH, typename TYPE, typename VALUE>
+__device__ __forceinline__ TYPE take_values(TYPE (&v)[EACH], const VALUE& value) {
+  TYPE sum = 0;
 #pragma unroll
   for (int e = 0; e < EACH; ++e) sum += v[e] = value((int)threadIdx.x * EACH + e);
   return sum;
 }
 
 // Inclusive and exclusive sums over the block's threads, in their order; `all`: of all.
-template <int THREADS>
-__device__ __forceinline__ double block_scan(double v, SampleScratch<THREADS>& s, double& before,
-                                             double& all) {
+template <int THREADS, typename TYPE>
+__device__ __forceinline__ TYPE block_scan(TYPE v, SampleScratch<THREADS>& s, TYPE& before,
+                                           TYPE& all) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  TYPE* words = reinterpret_cast<TYPE*>(s.words);
 #pragma unroll
   for (int off = 1; off < kWave; off <<= 1) {
-    const double other = __shfl_up(v, off, kWave);
+    const TYPE other = __shfl_up(v, off, kWave);
     if (lane >= off) v += other;
   }
   __syncthreads();
-  if (lane == kWave - 1) s.wave[wave] = v;
+  if (lane == kWave - 1) words[wave] = v;
   __syncthreads();
-  double base = 0.0;
-  all = 0.0;
+  TYPE base = 0;
+  all = 0;
 #pragma unroll
   for (int w = 0; w < THREADS / kWave; ++w) {
     if (w == wave) base = all;
-    all += s.wave[w];
+    all += words[w];
   }
   v += base;
   before = __shfl_up(v, 1, kWave);
@@ -339,27 +351,25 @@ __device__ __forceinline__ double block_scan(double v, SampleScratch<THREADS>& s
   return v;
 }
 
-// Of `count` values, EACH consecutive ones a thread, the first that is not 0 and at which
-// the running sum passes `target` (STRICT) or reaches it, the last that is not 0
-// where none does; `before`: the sum before it.  -1: all are 0.
-template <int THREADS, bool STRICT, int EACH>
-__device__ __forceinline__ int find_in(const double (&v)[EACH], double target, double& before,
+// Of values, EACH consecutive ones a thread, with `base` the sum before the thread's: the
+// first that is not 0 and at which the running sum passes `target` (STRICT) or
+// reaches it, the last that is not 0 where none does; `before`: the sum before it.  -1:
+// all are 0.
+template <int THREADS, bool STRICT, int EACH, typename TYPE>
+__device__ __forceinline__ int find_in(const TYPE (&v)[EACH], TYPE base, TYPE target, TYPE& before,
                                        SampleScratch<THREADS>& s) {
-  double sum = 0.0, base, all;
-#pragma unroll
-  for (int e = 0; e < EACH; ++e) sum += v[e];
-  block_scan<THREADS>(sum, s, base, all);
+  TYPE* value = reinterpret_cast<TYPE*>(&s.value);
   if (threadIdx.x == 0) {
     s.found = 0x7fffffff;
     s.last = -1;
   }
   __syncthreads();
   int mine = 0x7fffffff, last = -1;
-  double run = base, at = 0.0, at_last = 0.0;
+  TYPE run = base, at = 0, at_last = 0;
 #pragma unroll
   for (int e = 0; e < EACH; ++e) {
-    const double next = run + v[e];
-    if (v[e] > 0.0) {
+    const TYPE next = run + v[e];
+    if (v[e] > 0) {
       const int i = (int)threadIdx.x * EACH + e;
       if ((STRICT ? next > target : next >= target) && mine == 0x7fffffff) {
         mine = i;
@@ -375,21 +385,25 @@ __device__ __forceinline__ int find_in(const double (&v)[EACH], double target, d
   __syncthreads();
   const bool some = s.found != 0x7fffffff;
   const int found = some ? s.found : s.last;
-  if (some ? mine == found : last == found && last >= 0) s.value = some ? at : at_last;
+  if (some ? mine == found : last == found && last >= 0) *value = some ? at : at_last;
   __syncthreads();
-  before = s.value;
+  before = *value;
   return found;
 }
 
-// n keys in falling order (0 behind them up to a power of two).
+// n keys in falling order (0 behind them up to a power of two).  Keys up to 64 apart are
+// a wave's own: no barrier between such steps.
 template <int THREADS>
 __device__ __forceinline__ void sort_keys(u64* keys, int n) {
-  int size = 64;
+  int size = 2 * kWave;
   while (size < n) size <<= 1;
   for (int i = n + (int)threadIdx.x; i < size; i += THREADS) keys[i] = 0;
+  bool apart = true;  // the step before was among waves
   for (int span = 2; span <= size; span <<= 1)
     for (int step = span >> 1; step > 0; step >>= 1) {
-      __syncthreads();
+      if (apart || step > kWave) __syncthreads();
+      else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      apart = step > kWave;
       for (int i = threadIdx.x; i < size / 2; i += THREADS) {
         const int low = 2 * i - (i & (step - 1)), high = low + step;
         const u64 a = keys[low], b = keys[high];
@@ -413,39 +427,40 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
   const int split = blockIdx.x % p.count, row = blockIdx.x / p.count;
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const T* x = static_cast<const T*>(p.logits) + (size_t)row * p.stride;
-  const Settings set = settings_of(p, row);
-  const double heat16 = set.heat * kBinsOctave;
   const bool shared = p.count > 1;
 
   // ---- a part of the row: load i of lane l of wave w holds the VEC tokens from
   // ((i WAVES + w) 64 + l) VEC on, so that order is the vocabulary's
+  auto load = [&](int from, int end) TMC_INLINE -> vec {
+    if (from + VEC <= end) return *reinterpret_cast<const unaligned*>(x + from);
+    vec in;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) in[e] = from + e < end ? x[from + e] : (T)__builtin_nanf("");
+    return in;
+  };
   float v[EACH];
-  auto fetch = [&](int at, int end) TMC_INLINE {
+  int held = -1;  // start of the part in v
+  // What a pass computes of each logit it computes anew: kept for the next pass it would
+  // take more registers than there are.
+  float top = 0.0f, first_bin = 0.0f;
+  // take(part's start) for every part of [begin, end), its logits in v
+  auto parts = [&](int begin, int end, auto&& take) TMC_INLINE {
+    for (int at = begin; at < end; at += PART) {
+      if (at != held) {
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int from = at + (i * THREADS + (int)threadIdx.x) * VEC;
-      if (from + VEC <= end) {
-        const vec in = *reinterpret_cast<const unaligned*>(x + from);
+        for (int i = 0; i < LOADS; ++i) {
+          const vec in = load(at + (i * THREADS + (int)threadIdx.x) * VEC, end);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[i * VEC + e] = (float)in[e];
-      } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          v[i * VEC + e] = from + e < end ? (float)x[from + e] : __builtin_nanf("");
+          for (int e = 0; e < VEC; ++e) v[i * VEC + e] = (float)in[e];
+        }
+        held = at;
       }
+      asm volatile("" : "+v"(top), "+v"(first_bin));
+      take(at);
     }
   };
   auto place = [&](int at, int i) TMC_INLINE {
     return at + (i / VEC * THREADS + (int)threadIdx.x) * VEC + i % VEC;
-  };
-  // take(part's start) for every part of [begin, end), its logits in v
-  int held = -1;  // start of the part in v
-  auto parts = [&](int begin, int end, auto&& take) TMC_INLINE {
-    for (int at = begin; at < end; at += PART) {
-      if (at != held) fetch(at, end);
-      held = at;
-      take(at);
-    }
   };
   const int begin = split * p.walk * PART, end = min(p.vocab, begin + p.walk * PART);
 
@@ -455,6 +470,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
 #pragma unroll
     for (int i = 0; i < EACH; ++i) most = fmaxf(most, v[i]);
   });
+  const Settings set = settings_of(p, row);  // (its loads came beside the logits')
   u64 best = 0;
   if (set.heat == 0.0) {  // with its token
     parts(begin, end, [&](int at) TMC_INLINE {
@@ -466,215 +482,108 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
     best = most == -INFINITY ? 0 : rank_key(most, 0);
   }
   best = block_max_u64<THREADS>(best, s);
-  // a row (part) without a logit above -inf, and infinities: by digits
-  float top = best ? key_value(best) : -INFINITY;
-  bool odd = !(fabsf(top) < INFINITY) || (set.most < p.vocab && set.most > kMostTopK);
+  top = best ? key_value(best) : -INFINITY;
+  const float per_bin = (float)(set.heat * kBinsOctave);
+  // parts without a logit above -inf, what has no bins, and long lists: by digits
+  bool odd = !(fabsf(top * per_bin) < INFINITY) || !(fabsf(top) < INFINITY) ||
+             (set.most < p.vocab && set.most > kMostTopK);
 
   // ---- what the row's settings need of it
   enum { kGreedy, kList, kBin, kSum } way =
       set.heat == 0.0 ? kGreedy
       : set.most < p.vocab ? kList
       : set.share < 1.0f || (shared && set.least > kFaintest) ? kBin : kSum;
-  auto bin_of = [&](float x) TMC_INLINE { return floor((double)x * heat16); };
-  double first_bin = bin_of(top);  // of the greatest
-  const double unit = 0x1p43;
+  // A token's bin, counted down from the greatest's (NaN: none).
+  auto level = [&](float x) TMC_INLINE { return floorf(x * per_bin); };
+  first_bin = level(top);
+  auto bin_of = [&](float x) TMC_INLINE { return first_bin - level(x); };
+  auto octaves = [&](float x) TMC_INLINE { return ((double)x - (double)top) * set.heat; };
+  // 2^octaves in multiples of 2^-43: the last bits of that and 512.
+  constexpr double kUnit = 0x1p43;
+  auto integer = [&](double a) TMC_INLINE -> u64 {
+    return __builtin_bit_cast(u64, exp2_of(a) + 512.0) - __builtin_bit_cast(u64, 512.0);
+  };
   if (!odd && (way == kList || way == kBin)) {
     for (int i = threadIdx.x; i < kBins; i += THREADS) s.hist[i] = 0;
     __syncthreads();
-    parts(begin, end, [&](int) TMC_INLINE {
+    if (way == kBin && shared) {
+      parts(begin, end, [&](int) TMC_INLINE {
 #pragma unroll
-      for (int i = 0; i < EACH; ++i) {
-        const double bin = first_bin - bin_of(v[i]);  // (NaN: in none)
-        if (bin < (double)kBins) {
-          u64 cost = 1;
-          if (way == kBin)
-            cost = (u64)rint(exp2_of(fmax(((double)v[i] - (double)top) * set.heat, -60.0)) * unit);
-          atomicAdd(&s.hist[(int)bin], cost);
+        for (int i = 0; i < EACH; ++i) {
+          const float bin = bin_of(v[i]);
+          if (bin < (float)kBins) atomicAdd(&s.hist[(int)bin], integer(fmax(octaves(v[i]), -60.0)));
         }
-      }
-    });
+      });
+    } else {
+      // counts, or weights relative to the bin in 31 bits
+      parts(begin, end, [&](int) TMC_INLINE {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+          const float bin = bin_of(v[i]);
+          if (bin < (float)kBins) {
+            unsigned cost = 1;
+            if (way == kBin)
+              cost = (unsigned)(fast_exp2((v[i] - top) * (per_bin / kBinsOctave) +
+                                          bin * (1.0f / kBinsOctave)) * 0x1p30f);
+            atomicAdd(&s.hist[(int)bin], (u64)cost);
+          }
+        }
+      });
+    }
     __syncthreads();
   }
-  // Weight of a token, 0 for one that is not kept: below the last that counts, or ranked
-  // below `cut`.
+  // Of a token: what it weighs, 0 for one that is not kept: below the last that counts, or
+  // ranked below `cut`.
   const double faintest = fmax(set.least, kFaintest);
   u64 cut = 0;
-  auto weight = [&](float x, int at) TMC_INLINE -> double {
-    const double a = ((double)x - (double)top) * set.heat;
-    return a >= faintest && rank_key(x, at) >= cut ? exp2_of(a) : 0.0;
-  };
-  // the sums of every 64 lanes' loads, in their order, and of all
-  auto sum_groups = [&](int begin, int end) TMC_INLINE {
-    parts(begin, end, [&](int at) TMC_INLINE {
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        double sum = 0.0;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) sum += weight(v[i * VEC + e], place(at, i * VEC + e));
-#pragma unroll
-        for (int off = 1; off < kWave; off <<= 1) sum += __shfl_xor(sum, off, kWave);
-        if (lane == 0) s.groups[((at - begin) / PART * LOADS + i) * WAVES + wave] = sum;
-      }
-    });
-    __syncthreads();
+  auto weight = [&](float x, int at) TMC_INLINE -> u64 {
+    const double a = octaves(x);
+    return a >= faintest && rank_key(x, at) >= cut ? integer(a) : 0;
   };
   auto say = [&](int token, double share) TMC_INLINE {
     p.tokens[row] = token;
     if (p.probability) p.probability[row] = (float)share;
   };
-  // The token of [begin, end) whose weight the running sum, `before` ahead of it, passes
-  // u times the sum `total` with (total < 0: that of these tokens).
-  auto draw = [&](int begin, int end, double before, double total) TMC_INLINE {
-    sum_groups(begin, end);
-    const int groups = (end - begin + PART - 1) / PART * LOADS * WAVES;
-    constexpr int kEach = kMostGroups / THREADS;
-    auto group = [&](int g) TMC_INLINE { return g < groups ? s.groups[g] : 0.0; };
-    double mine[kEach], base, here;
-    block_scan<THREADS>(take_values(mine, group), s, base, here);
-    if (total < 0.0) total = here;
-    double target = set.uniform * total - before;
-    const int g = find_in<THREADS, true>(mine, target, before, s);
-    if (g < 0 || wave != 0) return;  // (the first wave goes on with the group)
-    target -= before;
-    const int at = begin + (g / (LOADS * WAVES)) * PART +
-                   ((g / WAVES % LOADS) * THREADS + g % WAVES * kWave + lane) * VEC;
-    double w[VEC], sum = 0.0;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      w[e] = at + e < end ? weight((float)x[at + e], at + e) : 0.0;
-      sum += w[e];
-    }
-    double run = sum;
-#pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) {
-      const double other = __shfl_up(run, off, kWave);
-      if (lane >= off) run += other;
-    }
-    double ahead = __shfl_up(run, 1, kWave);
-    if (lane == 0) ahead = 0.0;
-    // (the last that is kept where sums of another order fall short)
-    const u64 some = __builtin_amdgcn_ballot_w64(sum > 0.0);
-    const u64 past = __builtin_amdgcn_ballot_w64(sum > 0.0 && run > target);
-    if (some == 0 || lane != (past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some))) return;
-    int token = -1;
-    double share = 0.0;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      if (w[e] > 0.0 && !(token >= 0 && ahead > target)) {
-        token = at + e;
-        share = w[e];
-      }
-      ahead += w[e];
-    }
-    say(token, share / total);
+  auto collect_one = [&](float x, int at) TMC_INLINE {
+    const int slot = atomicAdd(&s.count, 1);
+    if (slot < kMostKept) s.keys[slot] = rank_key(x, at);
   };
-  // The tokens of [begin, end) in bins [from, to] into the list; false: too many.
-  auto collect = [&](int begin, int end, int from, int to) TMC_INLINE -> bool {
-    __syncthreads();
-    if (threadIdx.x == 0) s.count = 0;
+  // What a token of the sorted list weighs.
+  auto listed = [&](int i, int n) TMC_INLINE -> double {
+    const double a = i < n ? octaves(key_value(s.keys[i])) : -INFINITY;
+    return a >= kFaintest ? exp2_of(a) : 0.0;
+  };
+  // The sums of the block's loads of [begin, end), THREADS VEC tokens each: of those that
+  // weight() keeps in bins before `from`; tokens of bins [from, to] into the list.
+  // Returns the sum of all tokens' weights, of this thread.
+  u64* groups = s.groups;
+  auto sum_groups = [&](int begin, int end, float from, float to) TMC_INLINE -> u64 {
+    u64 all = 0;
+    for (int g = threadIdx.x; g < kMostGroups; g += THREADS) groups[g] = 0;
     __syncthreads();
     parts(begin, end, [&](int at) TMC_INLINE {
 #pragma unroll
-      for (int i = 0; i < EACH; ++i) {
-        const double bin = first_bin - bin_of(v[i]);
-        if (bin >= (double)from && bin <= (double)to) {
-          const int slot = atomicAdd(&s.count, 1);
-          if (slot < kMostKept) s.keys[slot] = rank_key(v[i], place(at, i));
+      for (int i = 0; i < LOADS; ++i) {
+        u64 sum = 0;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float logit = v[i * VEC + e], bin = bin_of(logit);
+          const double a = octaves(logit);
+          const u64 w = a >= kFaintest ? integer(a) : 0;
+          all += w;
+          if (bin < from) sum += a >= faintest && rank_key(logit, place(at, i * VEC + e)) >= cut ? w : 0;
+          else if (bin <= to) collect_one(logit, place(at, i * VEC + e));
         }
+#pragma unroll
+        for (int off = 1; off < kWave; off <<= 1) sum += __shfl_xor(sum, off, kWave);
+        if (lane == 0 && sum) atomicAdd(&groups[(at - begin) / PART * LOADS + i], sum);
       }
     });
     __syncthreads();
-    return s.count <= kMostKept;
+    return all;
   };
-  auto listed = [&](int i, int n) TMC_INLINE {  // weight of the list's token i
-    if (i >= n) return 0.0;
-    const double a = ((double)key_value(s.keys[i]) - (double)top) * set.heat;
-    return a >= kFaintest ? exp2_of(a) : 0.0;
-  };
-  // The draw from the sorted list, its first `most` tokens.
-  auto draw_list = [&](int n) TMC_INLINE {
-    n = min(n, set.most);
-    double before, total;
-    double w[KEPT];
-    block_scan<THREADS>(take_values(w, [&](int i) { return listed(i, n); }), s, before, total);
-    // kept: those of which less than the share lies before
-    const double limit = set.share < 1.0f ? (double)set.share * total : INFINITY;
-    int kept = 0;
-#pragma unroll
-    for (int e = 0; e < KEPT; ++e) {
-      const int i = (int)threadIdx.x * KEPT + e;
-      const double a = i < n ? ((double)key_value(s.keys[i]) - (double)top) * set.heat : -INFINITY;
-      kept += i == 0 || (w[e] > 0.0 && before < limit && a >= set.least);
-      before += w[e];
-    }
-    n = (int)block_sum_u64<THREADS>((u64)kept, s);
-    // by index, each with its rank behind
-    u64 index[KEPT];
-#pragma unroll
-    for (int e = 0; e < KEPT; ++e) {
-      const int i = (int)threadIdx.x * KEPT + e;
-      index[e] = i < n ? s.keys[i] & 0xFFFFFFFFull : 0;  // (~index: the lowest first)
-      s.groups[i] = w[e];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < KEPT; ++e) {
-      const int i = (int)threadIdx.x * KEPT + e;
-      if (i < n) s.keys[i] = index[e] << 32 | (unsigned)i;
-    }
-    sort_keys<THREADS>(s.keys, n);
-    auto value = [&](int i) TMC_INLINE { return i < n ? s.groups[(unsigned)s.keys[i]] : 0.0; };
-    block_scan<THREADS>(take_values(w, value), s, before, total);
-    const int i = find_in<THREADS, true>(w, set.uniform * total, before, s);
-    if (threadIdx.x == 0) say((int)~(unsigned)(s.keys[i] >> 32), value(i) / total);
-  };
-  // The bin in which top-p or min-p cuts, of this thread's sums of the bins and their
-  // sum; its tokens decide.  False: too many of them.
-  auto cut_bin = [&](const double (&v)[BINS], double sum, int& bin) -> bool {
-    double before, total, above;
-    block_scan<THREADS>(sum, s, before, total);
-    const double limit = set.share < 1.0f ? (double)set.share * total : INFINITY;
-    bin = find_in<THREADS, false>(v, limit, above, s);
-    // min-p: the bin of the least logit that it keeps, or the one before (a quotient may
-    // be off by its last bit): the tokens of both are looked at
-    const double least = first_bin - bin_of((float)((double)top + faintest / set.heat)) - 1.0;
-    int from = bin, to = bin;
-    if (set.least > kFaintest && least < (double)bin) {
-      from = max((int)least, 0);
-      to = min(bin, (int)least + 2);
-    }
-    if (!collect(0, p.vocab, from, to)) return false;
-    const int n = s.count;
-    sort_keys<THREADS>(s.keys, n);
-    // the sum before the list
-    if (from != bin) {
-      double run = before;
-#pragma unroll
-      for (int e = 0; e < BINS; ++e) {
-        if ((int)threadIdx.x * BINS + e == from) s.value = run;
-        run += v[e];
-      }
-      __syncthreads();
-      above = s.value;
-    }
-    bin = from;
-    double w[KEPT], ahead, all;
-    block_scan<THREADS>(take_values(w, [&](int i) { return listed(i, n); }), s, ahead, all);
-    int kept = 0;
-#pragma unroll
-    for (int e = 0; e < KEPT; ++e) {
-      const int i = (int)threadIdx.x * KEPT + e;
-      const double a = i < n ? ((double)key_value(s.keys[i]) - (double)top) * set.heat : -INFINITY;
-      kept += w[e] > 0.0 && above + ahead < limit && a >= set.least;
-      ahead += w[e];
-    }
-    kept = (int)block_sum_u64<THREADS>((u64)kept, s);
-    if (from == 0) kept = max(kept, 1);  // the most probable token
-    // None kept: the cut is between the list and the bins before it (without a list it is
-    // min-p's, which weight() applies).
-    cut = kept > 0 ? s.keys[kept - 1] : n == 0 ? 0 : s.keys[0] + 1;
-    s.count = kept;
-    return true;
+  auto count_groups = [&](int begin, int end) TMC_INLINE {
+    return (end - begin + PART - 1) / PART * LOADS;
   };
 
   // ---- the row's blocks together: every word at agent scope, completed before the
@@ -687,22 +596,32 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
   };
   SampleRecord* records = p.parts + (size_t)row * p.count;
   u64* bins = p.bins + (size_t)row * p.count * kBins;
+  constexpr int kBlocks = (kMostBlocks + THREADS - 1) / THREADS;  // a thread
   if (shared) {
-    double sum = 0.0;
+    u64 sum = 0;
     if (way == kSum && !odd) {
-      sum_groups(begin, end);
-      const int groups = (end - begin + PART - 1) / PART * LOADS * WAVES;
-      double mine = 0.0, before;
-      for (int g = threadIdx.x; g < groups; g += THREADS) mine += s.groups[g];
+      sum_groups(begin, end, INFINITY, -1.0f);
+      const int n = count_groups(begin, end);
+      u64 mine = 0, before;
+      for (int g = threadIdx.x; g < n; g += THREADS) mine += groups[g];
       block_scan<THREADS>(mine, s, before, sum);
+    }
+    if (!odd && (way == kList || way == kBin)) {
+      // the running sums of its bins
+      u64 mine[BINS], base;
+      const u64 own = take_values(mine, [&](int i) TMC_INLINE { return i < kBins ? s.hist[i] : 0ull; });
+      block_scan<THREADS>(own, s, base, sum);
+#pragma unroll
+      for (int e = 0; e < BINS; ++e) {
+        const int i = (int)threadIdx.x * BINS + e;
+        base += mine[e];
+        if (i < kBins) put(bins + (size_t)split * kBins + i, base);
+      }
     }
     if (threadIdx.x == 0) {
       put(&records[split].best, best);
       put(&records[split].sum, sum);
     }
-    if (!odd && (way == kList || way == kBin))
-      for (int i = threadIdx.x; i < kBins; i += THREADS)
-        put(bins + (size_t)split * kBins + i, s.hist[i]);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     if (threadIdx.x == 0)
@@ -715,134 +634,318 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
     if (threadIdx.x == 0) put(p.arrivals + row * kCounterStride, 0);
     best = 0;
     odd = set.most < p.vocab && set.most > kMostTopK;
-    for (int b = threadIdx.x; b < p.count; b += THREADS) {
+#pragma unroll
+    for (int e = 0; e < kBlocks; ++e) {
+      const int b = e * THREADS + (int)threadIdx.x;
+      if (b >= p.count) continue;
       const u64 other = get(&records[b].best);
+      s.highs[b] = other ? key_value(other) : -INFINITY;
+      s.blocks[b] = (double)get(&records[b].sum);
       best = max(best, other);
-      odd |= other && !(fabsf(key_value(other)) < INFINITY);
+      odd |= other && (!(fabsf(key_value(other)) < INFINITY) ||
+                       !(fabsf(key_value(other) * per_bin) < INFINITY));
     }
     odd = __syncthreads_or(odd);
     best = block_max_u64<THREADS>(best, s);
     top = best ? key_value(best) : -INFINITY;
-    first_bin = bin_of(top);
+    first_bin = level(top);
   }
-  if (way == kGreedy && best) {
-    if (threadIdx.x == 0) say(key_index(best), 1.0);
-    return;
-  }
-  // A block's factor: its greatest weight.  Its bins are so many behind the row's.  (A
-  // block of -inf alone put none, and is passed over.)
-  auto high_of = [&](int b) TMC_INLINE {
-    const u64 other = get(&records[b].best);
-    return other ? key_value(other) : -INFINITY;
-  };
-  auto factor_of = [&](float high) TMC_INLINE {
-    const double a = ((double)high - (double)top) * set.heat;
-    return a >= kFaintest ? exp2_of(a) : 0.0;
-  };
-  bool done = best != 0 && !odd;
-  int bin = 0;
-  if (done && way != kSum) {
-    // the row's bins, block after block
-    double mine[BINS], all = 0.0;
-#pragma unroll
-    for (int e = 0; e < BINS; ++e) mine[e] = 0.0;
-    for (int b = 0; b < p.count; ++b) {
-      const float high = shared ? high_of(b) : top;
-      const double behind = first_bin - bin_of(high);
-      if (!(behind < (double)kBins)) continue;
-      const double scale = way == kBin ? factor_of(high) * (1.0 / unit) : 1.0;
-#pragma unroll
-      for (int e = 0; e < BINS; ++e) {
-        const int i = (int)threadIdx.x * BINS + e - (int)behind;
-        if (i >= 0 && i + (int)behind < kBins)
-          mine[e] += scale * (double)(shared ? get(bins + (size_t)b * kBins + i) : s.hist[i]);
-      }
+  auto by_bins = [&]() TMC_INLINE -> bool {
+    if (way == kGreedy && best) {
+      if (threadIdx.x == 0) say(key_index(best), 1.0);
+      return true;
     }
-#pragma unroll
-    for (int e = 0; e < BINS; ++e) all += mine[e];
-    if (way == kList) {
-      double before;
-      bin = find_in<THREADS, false>(mine, (double)set.most, before, s);
-    } else {
-      done = cut_bin(mine, all, bin);
-    }
-    if (way == kList) {
-      done = collect(0, p.vocab, 0, bin);
-      if (done) {
-        const int n = s.count;
-        sort_keys<THREADS>(s.keys, n);
-        draw_list(n);
-        return;
-      }
-    }
-  }
-  if (!done) {
-    row_by_digits<T, THREADS>(p, row, set, s);
-    return;
-  }
-  int draw_begin = 0, draw_end = p.vocab;
-  double before = 0.0, total = -1.0;
-  if (shared) {
-    // what each block keeps: its bins before the list, and its tokens of the list
-    double* s_block = s.groups;
-    const int kept = s.count, span = p.walk * PART;
-    for (int b = wave; b < p.count; b += WAVES) {
-      const float high = high_of(b);
-      const double behind = first_bin - bin_of(high);
+    // A block's factor: its greatest weight.  (A block of -inf alone put no bins, and is
+    // passed over.)
+    auto factor_of = [&](float high) TMC_INLINE {
+      const double a = octaves(high);
+      return a >= kFaintest ? exp2_of(a) : 0.0;
+    };
+    // The running sum of the row's bins up to bin i: of this thread's share of its blocks,
+    // every `step`-th.
+    auto merged = [&](int i, int first, int step) TMC_INLINE -> double {
+      constexpr int kAhead = 4;  // blocks at once
       double sum = 0.0;
-      if (way == kSum) {
-        sum = lane == 0 ? factor_of(high) * get(&records[b].sum) : 0.0;
-      } else {
-        if (behind < (double)bin) {
-          const double scale = factor_of(high) * (1.0 / unit);
-          for (int i = lane; i + (int)behind < bin; i += kWave)
-            sum += scale * (double)get(bins + (size_t)b * kBins + i);
-        }
-        for (int i = lane; i < kept; i += kWave)
-          if (key_index(s.keys[i]) / span == b) sum += listed(i, kept);
-      }
+      for (int b0 = first; b0 < p.count; b0 += kAhead * step) {
+        u64 in[kAhead];
+        bool here[kAhead];
 #pragma unroll
-      for (int off = 1; off < kWave; off <<= 1) sum += __shfl_xor(sum, off, kWave);
-      if (lane == 0) s_block[b] = sum;
+        for (int u = 0; u < kAhead; ++u) {
+          const int b = min(b0 + u * step, p.count - 1);
+          const float behind = bin_of(s.highs[b]);
+          here[u] = b0 + u * step < p.count && behind <= (float)i;
+          in[u] = get(bins + (size_t)b * kBins + (here[u] ? i - (int)behind : 0));
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const float high = s.highs[min(b0 + u * step, p.count - 1)];
+          if (here[u]) sum += (way == kBin ? factor_of(high) * (1.0 / kUnit) : 1.0) * (double)in[u];
+        }
+      }
+      return sum;
+    };
+    bool done = best != 0 && !odd;
+    int bin = 0;              // the first of the list's
+    double limit = INFINITY;  // top-p: tokens before which less than that lies stay
+    double above = 0.0;       // the sum of the bins before the list
+    if (done && way != kSum) {
+      int from = 0, to = 0;
+      double all = 0.0;
+      if (shared) {
+        // in two steps: the coarse ones' running sums, then those of one's bins
+        double sums = 0.0, base, mine = 0.0;
+#pragma unroll
+        for (int e = 0; e < kBlocks; ++e) {
+          const int b = e * THREADS + (int)threadIdx.x;
+          if (way == kBin && b < p.count) sums += factor_of(s.highs[b]) * (s.blocks[b] * (1.0 / kUnit));
+        }
+        block_scan<THREADS>(sums, s, base, all);
+        if (way == kBin && set.share < 1.0f) limit = (double)set.share * all;
+        const double aim = way == kList ? (double)set.most : limit;
+        constexpr int LANES = THREADS / kCoarse;
+        int first = 0;
+#pragma unroll
+        for (int step = kCoarse; step >= 1; step /= kCoarse) {
+          const int point = (int)threadIdx.x / LANES, i = first + (point + 1) * step - 1;
+          mine = i < kBins ? merged(i, (int)threadIdx.x % LANES, LANES) : 0.0;
+#pragma unroll
+          for (int off = 1; off < LANES; off <<= 1) mine += __shfl_xor(mine, off, kWave);
+          __syncthreads();
+          if (threadIdx.x % LANES == 0) s.levels[point] = i < kBins ? mine : INFINITY;
+          __syncthreads();
+          int at = 0;
+          while (at < kCoarse - 1 && s.levels[at] < aim) ++at;
+          first = min(first + at * step, kBins - step);
+        }
+        bin = first;
+        from = way == kList ? 0 : bin;
+        to = bin;
+      } else {
+        double mine[BINS], sum, base;
+        sum = take_values(mine, [&](int i) TMC_INLINE {
+          const double scale = way == kBin ? exp2_of(-(double)min(i, kBins) / kBinsOctave) : 1.0;
+          return i < kBins ? scale * (double)s.hist[i] : 0.0;
+        });
+        block_scan<THREADS>(sum, s, base, all);
+        if (way == kBin && set.share < 1.0f) limit = (double)set.share * all;
+        bin = find_in<THREADS, false>(mine, base, way == kList ? (double)set.most : limit, above, s);
+        from = way == kList ? 0 : bin;
+        to = bin;
+        if (limit < INFINITY) {  // sums of 32-bit weights: the next bin too where the border is near
+          from = max(0, bin - (limit - above < 1e-5 * all));
+          to = bin + 1;
+        }
+      }
+      // min-p: the bins around the least logit that it keeps
+      const float least = bin_of((float)((double)top + faintest / set.heat)) - 1.0f;
+      if (way == kBin && set.least > kFaintest && least < (float)from) {
+        from = max((int)least, 0);
+        to = min(to, (int)least + 2);
+      }
+      bin = from;
+      if (shared && way == kBin) {
+        double base;
+        block_scan<THREADS>(from > 0 ? merged(from - 1, threadIdx.x, THREADS) : 0.0, s, base, above);
+      }
+      // ---- the list
+      if (threadIdx.x == 0) s.count = 0;
+      __syncthreads();
+      u64 weights = 0;
+      if (shared) {
+        constexpr int AHEAD = 32 / VEC;  // loads in flight
+        for (int at = 0; at < p.vocab; at += AHEAD * THREADS * VEC) {
+          vec in[AHEAD];
+#pragma unroll
+          for (int i = 0; i < AHEAD; ++i)
+            in[i] = load(min(at + (i * THREADS + (int)threadIdx.x) * VEC, p.vocab), p.vocab);
+#pragma unroll
+          for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+              const float bin = bin_of((float)in[i][e]);
+              if (bin >= (float)from && bin <= (float)to)
+                collect_one((float)in[i][e], at + (i * THREADS + (int)threadIdx.x) * VEC + e);
+            }
+        }
+        __syncthreads();
+      } else if (way == kList) {
+        parts(0, p.vocab, [&](int at) TMC_INLINE {
+#pragma unroll
+          for (int i = 0; i < EACH; ++i)
+            if (bin_of(v[i]) <= (float)to) collect_one(v[i], place(at, i));
+        });
+        __syncthreads();
+      } else {
+        weights = sum_groups(0, p.vocab, (float)from, (float)to);
+      }
+      const int n = s.count;
+      done = n <= kMostKept;
+      if (done) {
+        sort_keys<THREADS>(s.keys, n);
+        if (way == kBin && !shared) {
+          // exact sums: of all, and of what lies before the list
+          u64 before, total;
+          block_scan<THREADS>(weights, s, before, total);
+          if (limit < INFINITY) limit = (double)set.share * ((double)total * (1.0 / kUnit));
+          const int groups_here = count_groups(0, p.vocab);
+          u64 ahead = 0;
+          for (int g = threadIdx.x; g < groups_here; g += THREADS) ahead += groups[g];
+          block_scan<THREADS>(ahead, s, before, total);
+          above = (double)total * (1.0 / kUnit);
+        }
+        double w[KEPT], ahead;
+        int kept = 0;
+        const int most = way == kList ? min(n, set.most) : n;
+        block_scan<THREADS>(take_values(w, [&](int i) TMC_INLINE { return listed(i, most); }), s,
+                            ahead, all);
+        if (way == kList && set.share < 1.0f) limit = (double)set.share * all;
+        if (way == kList) above = 0.0;
+        // the bins said that the cut is in the list: its tokens must bear it out
+        if (way == kBin && !shared && limit < INFINITY && from == bin && to > from &&
+            ((from > 0 && above >= limit) || (above + all < limit && !(set.least > kFaintest))))
+          done = false;
+#pragma unroll
+        for (int e = 0; e < KEPT; ++e) {
+          const int i = (int)threadIdx.x * KEPT + e;
+          const double a = i < most ? octaves(key_value(s.keys[i])) : -INFINITY;
+          kept += w[e] > 0.0 && above + ahead < limit && a >= set.least;
+          ahead += w[e];
+        }
+        kept = (int)block_sum_u64<THREADS>((u64)kept, s);
+        if (from == 0) kept = max(kept, 1);  // the most probable token
+        if (way == kList) {
+          // the kept ones in the vocabulary's order, each with its rank behind
+          u64 index[KEPT];
+#pragma unroll
+          for (int e = 0; e < KEPT; ++e) {
+            const int i = (int)threadIdx.x * KEPT + e;
+            index[e] = i < kept ? s.keys[i] & 0xFFFFFFFFull : 0;  // (~index: the lowest first)
+            if (i < kept) groups[i] = __builtin_bit_cast(u64, w[e]);
+          }
+          __syncthreads();
+#pragma unroll
+          for (int e = 0; e < KEPT; ++e) {
+            const int i = (int)threadIdx.x * KEPT + e;
+            if (i < kept) s.keys[i] = index[e] << 32 | (unsigned)i;
+          }
+          sort_keys<THREADS>(s.keys, kept);
+          auto value = [&](int i) TMC_INLINE {
+            return i < kept ? __builtin_bit_cast(double, groups[(unsigned)s.keys[i]]) : 0.0;
+          };
+          double before, total;
+          block_scan<THREADS>(take_values(w, value), s, before, total);
+          const int i = find_in<THREADS, true>(w, before, set.uniform * total, before, s);
+          if (threadIdx.x == 0) say((int)~(unsigned)(s.keys[i] >> 32), value(i) / total);
+          return true;
+        }
+        // None kept: the cut is between the list and the bins before it (without a list it
+        // is min-p's, which weight() applies).
+        cut = kept > 0 ? s.keys[kept - 1] : n == 0 ? 0 : s.keys[0] + 1;
+        s.count = kept;
+        if (!shared) {  // the list's kept tokens to the sums of their groups
+          for (int i = threadIdx.x; i < kept; i += THREADS) {
+            atomicAdd(&groups[key_index(s.keys[i]) / (THREADS * VEC)],
+                      integer(octaves(key_value(s.keys[i]))));
+          }
+        }
+        __syncthreads();
+      }
     }
-    __syncthreads();
-    constexpr int kEach = (kSharedRows + THREADS - 1) / THREADS;  // blocks of a row, at most
-    double mine[kEach], base;
-    const double sum = take_values(mine, [&](int b) { return b < p.count ? s_block[b] : 0.0; });
-    block_scan<THREADS>(sum, s, base, total);
-    const int b = find_in<THREADS, true>(mine, set.uniform * total, before, s);
-    __syncthreads();
-    draw_begin = b * span;
-    draw_end = min(p.vocab, draw_begin + span);
-  }
-  draw(draw_begin, draw_end, before, total);
+    if (!done) return false;
+
+    // ---- the draw
+    int draw_begin = 0, draw_end = p.vocab;
+    double target = -1.0, total = 0.0;  // in units of the greatest weight
+    if (shared) {
+      // what each block keeps: its bins before the list, and its tokens of the list
+      const int kept = s.count, span = p.walk * PART;
+      for (int b = threadIdx.x; b < p.count; b += THREADS) {
+        const float high = s.highs[b], behind = bin_of(high);
+        const double scale = factor_of(high) * (1.0 / kUnit);
+        if (way == kSum) s.blocks[b] *= scale;
+        else s.blocks[b] = behind < (float)bin
+                               ? scale * (double)get(bins + (size_t)b * kBins + bin - 1 - (int)behind)
+                               : 0.0;
+      }
+      __syncthreads();
+      if (way == kBin)  // (a block's tokens one after the other: in their order)
+        for (int b = wave; b < p.count; b += WAVES) {
+          double sum = 0.0;
+          for (int i = lane; i < kept; i += kWave)
+            if (key_index(s.keys[i]) / span == b) sum += listed(i, kept);
+#pragma unroll
+          for (int off = 1; off < kWave; off <<= 1) sum += __shfl_xor(sum, off, kWave);
+          if (lane == 0) s.blocks[b] += sum;
+        }
+      __syncthreads();
+      double mine[kBlocks], base, before;
+      const double sum =
+          take_values(mine, [&](int b) TMC_INLINE { return b < p.count ? s.blocks[b] : 0.0; });
+      block_scan<THREADS>(sum, s, base, total);
+      target = set.uniform * total;
+      const int b = find_in<THREADS, true>(mine, base, target, before, s);
+      target -= before;
+      draw_begin = b * span;
+      draw_end = min(p.vocab, draw_begin + span);
+      held = -1;
+      __syncthreads();
+    }
+    if (shared || way == kSum) sum_groups(draw_begin, draw_end, INFINITY, -1.0f);
+    constexpr int SUMS = kMostGroups / THREADS;  // a thread
+    const int n = count_groups(draw_begin, draw_end);
+    u64 mine[SUMS], base, all, before;
+    const u64 sum = take_values(mine, [&](int g) TMC_INLINE { return g < n ? groups[g] : 0ull; });
+    block_scan<THREADS>(sum, s, base, all);
+    if (!shared) {
+      total = (double)all * (1.0 / kUnit);
+      target = set.uniform * total;
+    }
+    u64 aim = (u64)(fmax(target, 0.0) * kUnit);
+    if (!shared) aim = min(aim, all - 1);
+    const int g = find_in<THREADS, true>(mine, base, aim, before, s);
+    if (g < 0) return false;
+    aim -= min(before, aim);
+    const int at = draw_begin + (g * THREADS + (int)threadIdx.x) * VEC;
+    u64 w[VEC], own = 0;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      w[e] = at + e < draw_end ? weight((float)x[at + e], at + e) : 0;
+      own += w[e];
+    }
+    block_scan<THREADS>(own, s, before, all);
+    // (the last that is kept where sums of several blocks fall short)
+    const int index = find_in<THREADS, true>(w, before, aim, before, s);
+    if (index < 0) return false;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+      if ((int)threadIdx.x * VEC + e == index) say(at + e, (double)w[e] * (1.0 / kUnit) / total);
+    return true;
+  };
+  if (!by_bins()) row_by_digits<T, THREADS>(p, row, set, s);
 }
 
 bool sample_shape(int64_t rows, int64_t vocabulary) {
   return rows > 0 && rows < (1LL << 24) && vocabulary > 0 && vocabulary <= kMostTokens;
 }
 
-// How rows are shared out.  A block of 1024 threads holds a row of up to 32768 in its
-// registers, one of 256 up to 8192.  Where rows are few, blocks of 8192 share one, up to
-// kFill of them together.
-constexpr int64_t kFill = 512, kFewRows = 192;
-static_assert(kFill <= kSharedRows, "every shared row has its counter");
+// How rows are shared out: a block a row, or, where rows are few, blocks of 4096 tokens, up
+// to kFill of them together.
+constexpr int kThreads = 256, kEach = 8;
+constexpr int64_t kFill = 2048, kFewRows = 192;
+static_assert(kFewRows <= kSharedRows, "every shared row has its counter");
+static_assert(kMostTokens / (kThreads * 4) <= kMostGroups, "a sum a load");
 struct SamplePlan {
-  int threads, each, walk, count;
+  int walk, count;
 };
 SamplePlan sample_plan(int64_t rows, int64_t vocabulary) {
-  SamplePlan plan{1024, 32, 1, 1};
-  if (vocabulary <= 8192) {
-    plan.threads = 256;
-  } else if (rows < kFewRows) {
-    const int64_t parts = (vocabulary + 8191) / 8192, blocks = std::min(parts, kFill / rows);
-    plan.each = 8;
-    plan.walk = (int)((parts + blocks - 1) / blocks);
-    plan.count = (int)((parts + plan.walk - 1) / plan.walk);
-    return plan;
-  }
-  const int64_t span = (int64_t)plan.threads * plan.each;
-  plan.walk = (int)((vocabulary + span - 1) / span);
+  const int64_t part = kThreads * kEach, parts = (vocabulary + part - 1) / part;
+  int64_t blocks = 1;
+  if (rows < kFewRows)
+    blocks = std::max<int64_t>(
+        1, std::min({(parts + 1) / 2, kFill / rows, (int64_t)kMostBlocks}));
+  SamplePlan plan;
+  plan.walk = (int)((parts + blocks - 1) / blocks);
+  plan.count = (int)((parts + plan.walk - 1) / plan.walk);
   return plan;
 }
 
@@ -901,18 +1004,9 @@ extern "C" int tmc_sample(const void* logits, int dtype, int64_t row_stride,
   }
   const dim3 grid((unsigned)(rows * plan.count));
   const hipStream_t s = as_stream(stream);
-#define TMC_SAMPLE(TYPE, THREADS, EACH) \
-  hipLaunchKernelGGL((sample_kernel<TYPE, THREADS, EACH>), grid, dim3(THREADS), 0, s, p)
-#define TMC_SAMPLE_PLAN(TYPE)                              \
-  if (plan.threads == 256) TMC_SAMPLE(TYPE, 256, 32);      \
-  else if (plan.each == 32) TMC_SAMPLE(TYPE, 1024, 32);    \
-  else TMC_SAMPLE(TYPE, 1024, 8)
-  if (dtype == TMC_F32) {
-    TMC_SAMPLE_PLAN(float);
-  } else {
-    TMC_SAMPLE_PLAN(half_t);
-  }
-#undef TMC_SAMPLE_PLAN
-#undef TMC_SAMPLE
+  if (dtype == TMC_F32)
+    hipLaunchKernelGGL((sample_kernel<float, kThreads, kEach>), grid, dim3(kThreads), 0, s, p);
+  else
+    hipLaunchKernelGGL((sample_kernel<half_t, kThreads, kEach>), grid, dim3(kThreads), 0, s, p);
   return check_launch("sample_kernel");
 }
