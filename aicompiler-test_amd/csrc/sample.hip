@@ -110,20 +110,20 @@ static_assert(kFaintest == -44.0, "bins down to the least weight");
 constexpr int kMostKept = 2048, kMostTopK = 1024;  // tokens in the list, top_k that goes by it
 constexpr int kMostGroups = 1024;                  // sums of a block's loads
 constexpr int kCoarse = 32;  // bins of a coarse step, and at most steps
-static_assert(kMostTopK <= kMostGroups, "the list's weights fit their place");
+static_assert(kMostBlocks <= kMostGroups, "a sum a block");
 static_assert(kBins % kCoarse == 0 && kBins / kCoarse <= kCoarse, "two steps to a bin");
 
 template <int THREADS> struct SampleScratch {
   u64 hist[kBins > kDigits ? kBins : kDigits];
   u64 keys[kMostKept];
-  u64 groups[kMostGroups];
+  u64 groups[kMostGroups];  // (of a shared row first what its blocks keep of the list)
   u64 words[THREADS / kWave];
   float highs[kMostBlocks];  // of a row's blocks: the greatest logit,
   double blocks[kMostBlocks];  // the sum of weights
   double levels[kCoarse];
-  double value;
+  double value;  // (or an integer)
   u64 found64, below;
-  int found, count, last;
+  int found, count, last, small;
 };
 
 template <int THREADS>
@@ -391,46 +391,82 @@ __device__ __forceinline__ int find_in(const TYPE (&v)[EACH], TYPE base, TYPE ta
   return found;
 }
 
-// n keys in falling order (0 behind them up to a power of two).  Keys up to 64 apart are
-// a wave's own: no barrier between such steps.
-template <int THREADS>
-__device__ __forceinline__ void sort_keys(u64* keys, int n) {
-  int size = 2 * kWave;
-  while (size < n) size <<= 1;
-  for (int i = n + (int)threadIdx.x; i < size; i += THREADS) keys[i] = 0;
-  bool apart = true;  // the step before was among waves
-  for (int span = 2; span <= size; span <<= 1)
-    for (int step = span >> 1; step > 0; step >>= 1) {
-      if (apart || step > kWave) __syncthreads();
-      else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      apart = step > kWave;
-      for (int i = threadIdx.x; i < size / 2; i += THREADS) {
-        const int low = 2 * i - (i & (step - 1)), high = low + step;
-        const u64 a = keys[low], b = keys[high];
-        if ((a < b) == ((low & span) == 0)) {
-          keys[low] = b;
-          keys[high] = a;
-        }
+// The key of the list s.keys[0 ... n), all in [low, high], at which the running cost, from the highest ranked
+// down, reaches `target` (at least 1); 0 where all of it does not.  `cost` gives that of
+// a key.  The list's range of keys is cut into 256, then that of the part with the
+// target, until a wave can take the rest: for logits that are not equal, once.
+template <int THREADS, typename COST>
+__device__ __forceinline__ u64 select_key(int n, u64 low, u64 high, u64 target,
+                                          SampleScratch<THREADS>& s, const COST& cost) {
+  static_assert(THREADS == kDigits, "a digit a thread");
+  const int lane = threadIdx.x & (kWave - 1);
+  u64* hist = s.hist;
+  for (;;) {
+    // the keys in [low, high], by their first eight bits above `low`
+    const int bits = 64 - __clzll((high - low) | 1), shift = max(0, bits - 8);
+    __syncthreads();
+    hist[threadIdx.x] = 0;
+    if (threadIdx.x == 0) s.small = 0;
+    __syncthreads();
+    int here = 0;
+    for (int i = threadIdx.x; i < n; i += THREADS) {
+      const u64 key = s.keys[i];
+      if (key >= low && key <= high) {
+        atomicAdd(&hist[255 - ((key - low) >> shift)], cost(key));
+        ++here;
       }
     }
+    const int left = (int)block_sum_u64<THREADS>((u64)here, s);
+    if (left <= kWave) break;
+    const u64 mine[1] = {hist[threadIdx.x]};
+    u64 base, all, before;
+    block_scan<THREADS>(mine[0], s, base, all);
+    if (all < target) return 0;
+    const int digit = find_in<THREADS, false>(mine, base, target, before, s);
+    target -= before;
+    if (shift == 0) return low + (255 - digit);
+    low += (u64)(255 - digit) << shift;
+    high = min(high, low + (((u64)1 << shift) - 1));
+  }
+  // up to 64 keys: each lane sums what ranks above its own
+  for (int i = threadIdx.x; i < n; i += THREADS) {
+    const u64 key = s.keys[i];
+    if (key < low || key > high) continue;
+    const int slot = atomicAdd(&s.small, 1);
+    hist[slot] = key;
+    hist[kWave + slot] = cost(key);
+  }
+  if (threadIdx.x == 0) s.found64 = 0;
   __syncthreads();
+  const int few = s.small;
+  if ((int)threadIdx.x < few) {
+    const u64 key = hist[lane], own = hist[kWave + lane];
+    u64 run = 0;
+    for (int o = 0; o < few; ++o)
+      if (hist[o] >= key) run += hist[kWave + o];
+    if (run >= target && run - own < target) s.found64 = key;
+  }
+  __syncthreads();
+  const u64 found = s.found64;
+  __syncthreads();
+  return found;
 }
 
 template <typename T, int THREADS, int EACH>
 __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
-  constexpr int WAVES = THREADS / kWave, VEC = 16 / (int)sizeof(T), LOADS = EACH / VEC;
-  constexpr int PART = THREADS * EACH, KEPT = (kMostKept + THREADS - 1) / THREADS;
+  constexpr int VEC = 16 / (int)sizeof(T), LOADS = EACH / VEC;
+  constexpr int PART = THREADS * EACH;
   constexpr int BINS = (kBins + THREADS - 1) / THREADS;  // bins a thread
   typedef T vec __attribute__((ext_vector_type(VEC)));
   typedef vec unaligned __attribute__((aligned(sizeof(T))));  // rows start at any element
   __shared__ SampleScratch<THREADS> s;
   const int split = blockIdx.x % p.count, row = blockIdx.x / p.count;
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int lane = threadIdx.x & (kWave - 1);
   const T* x = static_cast<const T*>(p.logits) + (size_t)row * p.stride;
   const bool shared = p.count > 1;
 
-  // ---- a part of the row: load i of lane l of wave w holds the VEC tokens from
-  // ((i WAVES + w) 64 + l) VEC on, so that order is the vocabulary's
+  // ---- a part of the row: load i of thread t holds the VEC tokens from
+  // (i THREADS + t) VEC on, so that order is the vocabulary's
   auto load = [&](int from, int end) TMC_INLINE -> vec {
     if (from + VEC <= end) return *reinterpret_cast<const unaligned*>(x + from);
     vec in;
@@ -503,19 +539,23 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
   auto integer = [&](double a) TMC_INLINE -> u64 {
     return __builtin_bit_cast(u64, exp2_of(a) + 512.0) - __builtin_bit_cast(u64, 512.0);
   };
+  // (the bins of a block with its own row; a sum of 2^20 tokens fits)
+  unsigned* rough = reinterpret_cast<unsigned*>(s.hist);
   if (!odd && (way == kList || way == kBin)) {
     for (int i = threadIdx.x; i < kBins; i += THREADS) s.hist[i] = 0;
     __syncthreads();
-    if (way == kBin && shared) {
+    if (shared) {
       parts(begin, end, [&](int) TMC_INLINE {
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
           const float bin = bin_of(v[i]);
-          if (bin < (float)kBins) atomicAdd(&s.hist[(int)bin], integer(fmax(octaves(v[i]), -60.0)));
+          if (bin < (float)kBins)
+            atomicAdd(&s.hist[(int)bin],
+                      way == kBin ? integer(fmax(octaves(v[i]), -60.0)) : 1ull);
         }
       });
     } else {
-      // counts, or weights relative to the bin in 31 bits
+      // counts, or weights relative to the bin of 11 bits
       parts(begin, end, [&](int) TMC_INLINE {
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
@@ -523,9 +563,10 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
           if (bin < (float)kBins) {
             unsigned cost = 1;
             if (way == kBin)
-              cost = (unsigned)(fast_exp2((v[i] - top) * (per_bin / kBinsOctave) +
-                                          bin * (1.0f / kBinsOctave)) * 0x1p30f);
-            atomicAdd(&s.hist[(int)bin], (u64)cost);
+              cost = (unsigned)__fmaf_rn(
+                  fast_exp2(__fmaf_rn(v[i] - top, per_bin / kBinsOctave, bin * (1.0f / kBinsOctave))),
+                  0x1p11f, 0.5f);
+            atomicAdd(&rough[(int)bin], cost);
           }
         }
       });
@@ -547,11 +588,6 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
   auto collect_one = [&](float x, int at) TMC_INLINE {
     const int slot = atomicAdd(&s.count, 1);
     if (slot < kMostKept) s.keys[slot] = rank_key(x, at);
-  };
-  // What a token of the sorted list weighs.
-  auto listed = [&](int i, int n) TMC_INLINE -> double {
-    const double a = i < n ? octaves(key_value(s.keys[i])) : -INFINITY;
-    return a >= kFaintest ? exp2_of(a) : 0.0;
   };
   // The sums of the block's loads of [begin, end), THREADS VEC tokens each: of those that
   // weight() keeps in bins before `from`; tokens of bins [from, to] into the list.
@@ -724,15 +760,15 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
         double mine[BINS], sum, base;
         sum = take_values(mine, [&](int i) TMC_INLINE {
           const double scale = way == kBin ? exp2_of(-(double)min(i, kBins) / kBinsOctave) : 1.0;
-          return i < kBins ? scale * (double)s.hist[i] : 0.0;
+          return i < kBins ? scale * (double)rough[i] : 0.0;
         });
         block_scan<THREADS>(sum, s, base, all);
         if (way == kBin && set.share < 1.0f) limit = (double)set.share * all;
         bin = find_in<THREADS, false>(mine, base, way == kList ? (double)set.most : limit, above, s);
         from = way == kList ? 0 : bin;
         to = bin;
-        if (limit < INFINITY) {  // sums of 32-bit weights: the next bin too where the border is near
-          from = max(0, bin - (limit - above < 1e-5 * all));
+        if (limit < INFINITY) {  // rough sums: the next bin too, and the one before where the border is near
+          from = max(0, bin - (limit - above < 3e-4 * all));
           to = bin + 1;
         }
       }
@@ -752,20 +788,31 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
       __syncthreads();
       u64 weights = 0;
       if (shared) {
-        constexpr int AHEAD = 32 / VEC;  // loads in flight
+        constexpr int AHEAD = 16;  // loads in flight
         for (int at = 0; at < p.vocab; at += AHEAD * THREADS * VEC) {
           vec in[AHEAD];
 #pragma unroll
           for (int i = 0; i < AHEAD; ++i)
             in[i] = load(min(at + (i * THREADS + (int)threadIdx.x) * VEC, p.vocab), p.vocab);
 #pragma unroll
-          for (int i = 0; i < AHEAD; ++i)
+          for (int i = 0; i < AHEAD; ++i) {
+            unsigned hits = 0;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
               const float bin = bin_of((float)in[i][e]);
-              if (bin >= (float)from && bin <= (float)to)
-                collect_one((float)in[i][e], at + (i * THREADS + (int)threadIdx.x) * VEC + e);
+              hits |= bin >= (float)from && bin <= (float)to ? 1u << e : 0u;
             }
+            if (hits == 0) continue;
+            int slot = atomicAdd(&s.count, __popc(hits));
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+              if (!(hits >> e & 1)) continue;
+              if (slot < kMostKept)
+                s.keys[slot] = rank_key((float)in[i][e],
+                                        at + (i * THREADS + (int)threadIdx.x) * VEC + e);
+              ++slot;
+            }
+          }
         }
         __syncthreads();
       } else if (way == kList) {
@@ -781,72 +828,67 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
       const int n = s.count;
       done = n <= kMostKept;
       if (done) {
-        sort_keys<THREADS>(s.keys, n);
+        __syncthreads();
+        auto cost = [&](u64 key) TMC_INLINE -> u64 {
+          const double a = octaves(key_value(key));
+          return a >= kFaintest ? max(integer(a), (u64)1) : 0;
+        };
+        auto list_sum = [&](u64 from) TMC_INLINE -> u64 {  // of its keys from there on
+          u64 sum = 0, before, all;
+          for (int i = threadIdx.x; i < n; i += THREADS)
+            if (s.keys[i] >= from) sum += cost(s.keys[i]);
+          block_scan<THREADS>(sum, s, before, all);
+          return all;
+        };
+        u64 low = ~0ull, high = 0;  // of the list's keys
+        for (int i = threadIdx.x; i < n; i += THREADS) {
+          low = min(low, s.keys[i]);
+          high = max(high, s.keys[i]);
+        }
+        high = block_max_u64<THREADS>(high, s);
+        low = ~block_max_u64<THREADS>(~low, s);
+        u64 ahead = 0, all = 0;  // what lies before the list; of the list
         if (way == kBin && !shared) {
           // exact sums: of all, and of what lies before the list
           u64 before, total;
           block_scan<THREADS>(weights, s, before, total);
           if (limit < INFINITY) limit = (double)set.share * ((double)total * (1.0 / kUnit));
-          const int groups_here = count_groups(0, p.vocab);
-          u64 ahead = 0;
-          for (int g = threadIdx.x; g < groups_here; g += THREADS) ahead += groups[g];
-          block_scan<THREADS>(ahead, s, before, total);
-          above = (double)total * (1.0 / kUnit);
+          u64 mine = 0;
+          for (int g = threadIdx.x; g < count_groups(0, p.vocab); g += THREADS) mine += groups[g];
+          block_scan<THREADS>(mine, s, before, ahead);
+          above = (double)ahead * (1.0 / kUnit);
         }
-        double w[KEPT], ahead;
-        int kept = 0;
-        const int most = way == kList ? min(n, set.most) : n;
-        block_scan<THREADS>(take_values(w, [&](int i) TMC_INLINE { return listed(i, most); }), s,
-                            ahead, all);
-        if (way == kList && set.share < 1.0f) limit = (double)set.share * all;
         if (way == kList) above = 0.0;
+        if (n > 0 && (way == kList || limit < INFINITY)) {
+          cut = low;  // (nothing behind the list)
+          if (way == kList && n > set.most)
+            cut = select_key<THREADS>(n, low, high, (u64)set.most, s, [](u64) { return 1ull; });
+          all = list_sum(cut);
+        }
+        if (way == kList && set.share < 1.0f)
+          limit = (double)set.share * ((double)all * (1.0 / kUnit));
         // the bins said that the cut is in the list: its tokens must bear it out
-        if (way == kBin && !shared && limit < INFINITY && from == bin && to > from &&
-            ((from > 0 && above >= limit) || (above + all < limit && !(set.least > kFaintest))))
+        if (way == kBin && !shared && limit < INFINITY && !(set.least > kFaintest) &&
+            ((from > 0 && above >= limit) || above + (double)all * (1.0 / kUnit) < limit))
           done = false;
-#pragma unroll
-        for (int e = 0; e < KEPT; ++e) {
-          const int i = (int)threadIdx.x * KEPT + e;
-          const double a = i < most ? octaves(key_value(s.keys[i])) : -INFINITY;
-          kept += w[e] > 0.0 && above + ahead < limit && a >= set.least;
-          ahead += w[e];
+        if (n > 0 && limit < INFINITY && done) {
+          // (none kept: only what lies before the list; but the most probable token stays)
+          const double room = ceil((limit - above) * kUnit);
+          cut = !(room >= 1.0) && from > 0
+                    ? high + 1
+                    : max(cut, select_key<THREADS>(n, low, high, (u64)fmax(room, 1.0), s, cost));
         }
-        kept = (int)block_sum_u64<THREADS>((u64)kept, s);
-        if (from == 0) kept = max(kept, 1);  // the most probable token
-        if (way == kList) {
-          // the kept ones in the vocabulary's order, each with its rank behind
-          u64 index[KEPT];
-#pragma unroll
-          for (int e = 0; e < KEPT; ++e) {
-            const int i = (int)threadIdx.x * KEPT + e;
-            index[e] = i < kept ? s.keys[i] & 0xFFFFFFFFull : 0;  // (~index: the lowest first)
-            if (i < kept) groups[i] = __builtin_bit_cast(u64, w[e]);
-          }
-          __syncthreads();
-#pragma unroll
-          for (int e = 0; e < KEPT; ++e) {
-            const int i = (int)threadIdx.x * KEPT + e;
-            if (i < kept) s.keys[i] = index[e] << 32 | (unsigned)i;
-          }
-          sort_keys<THREADS>(s.keys, kept);
-          auto value = [&](int i) TMC_INLINE {
-            return i < kept ? __builtin_bit_cast(double, groups[(unsigned)s.keys[i]]) : 0.0;
-          };
-          double before, total;
-          block_scan<THREADS>(take_values(w, value), s, before, total);
-          const int i = find_in<THREADS, true>(w, before, set.uniform * total, before, s);
-          if (threadIdx.x == 0) say((int)~(unsigned)(s.keys[i] >> 32), value(i) / total);
-          return true;
-        }
-        // None kept: the cut is between the list and the bins before it (without a list it
-        // is min-p's, which weight() applies).
-        cut = kept > 0 ? s.keys[kept - 1] : n == 0 ? 0 : s.keys[0] + 1;
-        s.count = kept;
-        if (!shared) {  // the list's kept tokens to the sums of their groups
-          for (int i = threadIdx.x; i < kept; i += THREADS) {
-            atomicAdd(&groups[key_index(s.keys[i]) / (THREADS * VEC)],
-                      integer(octaves(key_value(s.keys[i]))));
-          }
+        // the list's kept tokens to the sums of their loads, or blocks
+        const int span = p.walk * PART;
+        if (shared || way == kList)
+          for (int g = threadIdx.x; g < kMostGroups; g += THREADS) groups[g] = 0;
+        __syncthreads();
+        for (int i = threadIdx.x; i < n; i += THREADS) {
+          const u64 key = s.keys[i];
+          const double a = octaves(key_value(key));
+          if (key < cut || !(a >= faintest)) continue;
+          const int token = key_index(key);
+          atomicAdd(&groups[token / (shared && way == kBin ? span : THREADS * VEC)], integer(a));
         }
         __syncthreads();
       }
@@ -856,27 +898,19 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
     // ---- the draw
     int draw_begin = 0, draw_end = p.vocab;
     double target = -1.0, total = 0.0;  // in units of the greatest weight
-    if (shared) {
+    if (shared && way != kList) {
       // what each block keeps: its bins before the list, and its tokens of the list
-      const int kept = s.count, span = p.walk * PART;
+      const int span = p.walk * PART;
       for (int b = threadIdx.x; b < p.count; b += THREADS) {
         const float high = s.highs[b], behind = bin_of(high);
         const double scale = factor_of(high) * (1.0 / kUnit);
         if (way == kSum) s.blocks[b] *= scale;
-        else s.blocks[b] = behind < (float)bin
-                               ? scale * (double)get(bins + (size_t)b * kBins + bin - 1 - (int)behind)
-                               : 0.0;
+        else s.blocks[b] =
+                 (double)groups[b] * (1.0 / kUnit) +
+                 (behind < (float)bin
+                      ? scale * (double)get(bins + (size_t)b * kBins + bin - 1 - (int)behind)
+                      : 0.0);
       }
-      __syncthreads();
-      if (way == kBin)  // (a block's tokens one after the other: in their order)
-        for (int b = wave; b < p.count; b += WAVES) {
-          double sum = 0.0;
-          for (int i = lane; i < kept; i += kWave)
-            if (key_index(s.keys[i]) / span == b) sum += listed(i, kept);
-#pragma unroll
-          for (int off = 1; off < kWave; off <<= 1) sum += __shfl_xor(sum, off, kWave);
-          if (lane == 0) s.blocks[b] += sum;
-        }
       __syncthreads();
       double mine[kBlocks], base, before;
       const double sum =
@@ -890,18 +924,19 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
       held = -1;
       __syncthreads();
     }
-    if (shared || way == kSum) sum_groups(draw_begin, draw_end, INFINITY, -1.0f);
+    if (way == kSum || (shared && way == kBin)) sum_groups(draw_begin, draw_end, INFINITY, -1.0f);
     constexpr int SUMS = kMostGroups / THREADS;  // a thread
     const int n = count_groups(draw_begin, draw_end);
     u64 mine[SUMS], base, all, before;
     const u64 sum = take_values(mine, [&](int g) TMC_INLINE { return g < n ? groups[g] : 0ull; });
     block_scan<THREADS>(sum, s, base, all);
-    if (!shared) {
+    const bool whole = !shared || way == kList;
+    if (whole) {
       total = (double)all * (1.0 / kUnit);
       target = set.uniform * total;
     }
     u64 aim = (u64)(fmax(target, 0.0) * kUnit);
-    if (!shared) aim = min(aim, all - 1);
+    if (whole) aim = min(aim, all - 1);
     const int g = find_in<THREADS, true>(mine, base, aim, before, s);
     if (g < 0) return false;
     aim -= min(before, aim);
