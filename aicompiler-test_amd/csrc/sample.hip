@@ -17,6 +17,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 // (a lambda that is not inlined keeps what it refers to in memory)
 #define TMC_INLINE __attribute__((always_inline))
@@ -96,10 +97,26 @@ __device__ __forceinline__ Settings settings_of(const SampleParams& p, int row) 
 }
 
 // ------------------------------------------------------------ shared by both ways
-__device__ __forceinline__ u64 wave_sum_u64(u64 v) {
-#pragma unroll
-  for (int off = 1; off < kWave; off <<= 1) v += __shfl_xor(v, off, kWave);
+// v of the lane that the row operation CTRL names, 0 where it names none.
+template <int CTRL, int ROWS, typename TYPE> __device__ __forceinline__ TYPE lane_move(TYPE v) {
+  const u64 b = __builtin_bit_cast(u64, v);
+  const unsigned low = __builtin_amdgcn_update_dpp(0, (int)b, CTRL, ROWS, 0xf, false);
+  const unsigned high = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROWS, 0xf, false);
+  return __builtin_bit_cast(TYPE, (u64)high << 32 | low);
+}
+// Running sums (or maxima) over the lanes: of rows of 16, then of all.
+template <typename TYPE, typename JOIN>
+__device__ __forceinline__ TYPE wave_scan(TYPE v, const JOIN& join) {
+  v = join(v, lane_move<0x111, 0xf>(v));  // the lane 1, 2, 4 and 8 before
+  v = join(v, lane_move<0x112, 0xf>(v));
+  v = join(v, lane_move<0x114, 0xf>(v));
+  v = join(v, lane_move<0x118, 0xf>(v));
+  v = join(v, lane_move<0x142, 0xa>(v));  // the last of the row before, in every other row
+  v = join(v, lane_move<0x143, 0xc>(v));  // the last of the lower half, in the upper
   return v;
+}
+template <typename TYPE> __device__ __forceinline__ TYPE wave_scan(TYPE v) {
+  return wave_scan(v, [](TYPE a, TYPE b) TMC_INLINE { return a + b; });
 }
 
 constexpr int kDigits = 256;
@@ -108,7 +125,7 @@ constexpr int kDigits = 256;
 constexpr int kBinsOctave = 16, kBins = 44 * kBinsOctave;
 static_assert(kFaintest == -44.0, "bins down to the least weight");
 constexpr int kMostKept = 2048, kMostTopK = 1024;  // tokens in the list, top_k that goes by it
-constexpr int kMostGroups = 1024;                  // sums of a block's loads
+constexpr int kMostGroups = 512;                   // sums of a block's parts
 constexpr int kCoarse = 32;  // bins of a coarse step, and at most steps
 static_assert(kMostBlocks <= kMostGroups, "a sum a block");
 static_assert(kBins % kCoarse == 0 && kBins / kCoarse <= kCoarse, "two steps to a bin");
@@ -118,19 +135,17 @@ template <int THREADS> struct SampleScratch {
   u64 keys[kMostKept];
   u64 groups[kMostGroups];  // (of a shared row first what its blocks keep of the list)
   u64 words[THREADS / kWave];
-  float highs[kMostBlocks];  // of a row's blocks: the greatest logit,
-  double blocks[kMostBlocks];  // the sum of weights
   double levels[kCoarse];
   double value;  // (or an integer)
   u64 found64, below;
-  int found, count, last, small;
+  int found, last, small;
 };
 
 template <int THREADS>
 __device__ __forceinline__ u64 block_sum_u64(u64 v, SampleScratch<THREADS>& s) {
-  v = wave_sum_u64(v);
+  v = wave_scan(v);
   __syncthreads();
-  if ((threadIdx.x & (kWave - 1)) == 0) s.words[threadIdx.x / kWave] = v;
+  if ((threadIdx.x & (kWave - 1)) == kWave - 1) s.words[threadIdx.x / kWave] = v;
   __syncthreads();
   u64 sum = 0;
 #pragma unroll
@@ -139,11 +154,11 @@ __device__ __forceinline__ u64 block_sum_u64(u64 v, SampleScratch<THREADS>& s) {
 }
 template <int THREADS>
 __device__ __forceinline__ u64 block_max_u64(u64 v, SampleScratch<THREADS>& s) {
-#pragma unroll
-  for (int off = 1; off < kWave; off <<= 1) v = max(v, (u64)__shfl_xor(v, off, kWave));
+  v = wave_scan(v, [](u64 a, u64 b) TMC_INLINE { return max(a, b); });
   __syncthreads();
-  if ((threadIdx.x & (kWave - 1)) == 0) s.words[threadIdx.x / kWave] = v;
+  if ((threadIdx.x & (kWave - 1)) == kWave - 1) s.words[threadIdx.x / kWave] = v;
   __syncthreads();
+  v = 0;
 #pragma unroll
   for (int w = 0; w < THREADS / kWave; ++w) v = max(v, s.words[w]);
   return v;
@@ -330,11 +345,7 @@ __device__ __forceinline__ TYPE block_scan(TYPE v, SampleScratch<THREADS>& s, TY
                                            TYPE& all) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   TYPE* words = reinterpret_cast<TYPE*>(s.words);
-#pragma unroll
-  for (int off = 1; off < kWave; off <<= 1) {
-    const TYPE other = __shfl_up(v, off, kWave);
-    if (lane >= off) v += other;
-  }
+  v = wave_scan(v);
   __syncthreads();
   if (lane == kWave - 1) words[wave] = v;
   __syncthreads();
@@ -345,10 +356,8 @@ __device__ __forceinline__ TYPE block_scan(TYPE v, SampleScratch<THREADS>& s, TY
     if (w == wave) base = all;
     all += words[w];
   }
-  v += base;
-  before = __shfl_up(v, 1, kWave);
-  if (lane == 0) before = base;
-  return v;
+  before = base + lane_move<0x138, 0xf>(v);  // the lane before
+  return base + v;
 }
 
 // Of values, EACH consecutive ones a thread, with `base` the sum before the thread's: the
@@ -452,7 +461,7 @@ __device__ __forceinline__ u64 select_key(int n, u64 low, u64 high, u64 target,
   return found;
 }
 
-template <typename T, int THREADS, int EACH>
+template <typename T, int THREADS, int EACH, bool SHARED>
 __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
   constexpr int VEC = 16 / (int)sizeof(T), LOADS = EACH / VEC;
   constexpr int PART = THREADS * EACH;
@@ -460,13 +469,15 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
   typedef T vec __attribute__((ext_vector_type(VEC)));
   typedef vec unaligned __attribute__((aligned(sizeof(T))));  // rows start at any element
   __shared__ SampleScratch<THREADS> s;
+  __shared__ double factors[SHARED ? kMostBlocks : 1];  // of a row's blocks: the greatest weight,
+  __shared__ double blocks[SHARED ? kMostBlocks : 1];   // the sum of weights,
+  __shared__ float highs[SHARED ? kMostBlocks : 1];     // the greatest logit
   const int split = blockIdx.x % p.count, row = blockIdx.x / p.count;
   const int lane = threadIdx.x & (kWave - 1);
   const T* x = static_cast<const T*>(p.logits) + (size_t)row * p.stride;
-  const bool shared = p.count > 1;
+  constexpr bool shared = SHARED;
 
-  // ---- a part of the row: load i of thread t holds the VEC tokens from
-  // (i THREADS + t) VEC on, so that order is the vocabulary's
+  // ---- a part of the row, EACH tokens a thread, so that order is the vocabulary's
   auto load = [&](int from, int end) TMC_INLINE -> vec {
     if (from + VEC <= end) return *reinterpret_cast<const unaligned*>(x + from);
     vec in;
@@ -483,12 +494,18 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
   auto parts = [&](int begin, int end, auto&& take) TMC_INLINE {
     for (int at = begin; at < end; at += PART) {
       if (at != held) {
+        vec in[LOADS];
+        const int from = at + (int)threadIdx.x * EACH;
+        if (at + PART <= end) {  // (for all threads: the loads are in flight together)
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-          const vec in = load(at + (i * THREADS + (int)threadIdx.x) * VEC, end);
+          for (int i = 0; i < LOADS; ++i)
+            in[i] = *reinterpret_cast<const unaligned*>(x + from + i * VEC);
+        } else {
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) v[i * VEC + e] = (float)in[e];
+          for (int i = 0; i < LOADS; ++i) in[i] = load(from + i * VEC, end);
         }
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) v[i] = (float)in[i / VEC][i % VEC];
         held = at;
       }
       asm volatile("" : "+v"(top), "+v"(first_bin));
@@ -496,7 +513,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
     }
   };
   auto place = [&](int at, int i) TMC_INLINE {
-    return at + (i / VEC * THREADS + (int)threadIdx.x) * VEC + i % VEC;
+    return at + (int)threadIdx.x * EACH + i;
   };
   const int begin = split * p.walk * PART, end = min(p.vocab, begin + p.walk * PART);
 
@@ -585,41 +602,96 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
     p.tokens[row] = token;
     if (p.probability) p.probability[row] = (float)share;
   };
-  auto collect_one = [&](float x, int at) TMC_INLINE {
-    const int slot = atomicAdd(&s.count, 1);
-    if (slot < kMostKept) s.keys[slot] = rank_key(x, at);
+  // The least logit of a level from `low` on: 64 of the remaining floats at a time, in
+  // their order, from -inf (which has none) up.
+  auto least_of = [&](float low) TMC_INLINE -> float {
+    constexpr u64 kFirst = 0x007FFFFFull, kLast = 0xFF800000ull;  // keys of -inf and inf
+    u64 below = kFirst;
+#pragma unroll
+    for (int shift = 30; shift >= 0; shift -= 6) {
+      const u64 at = below + ((u64)lane << shift);
+      const bool less = at <= kLast && !(level(key_value(at << 32)) >= low);
+      below += (u64)max(__popcll(__ballot(less)) - 1, 0) << shift;
+    }
+    return key_value((below + 1) << 32);
   };
-  // The sums of the block's loads of [begin, end), THREADS VEC tokens each: of those that
-  // weight() keeps in bins before `from`; tokens of bins [from, to] into the list.
-  // Returns the sum of all tokens' weights, of this thread.
+  // Tokens into the list: each wave its own, by index, then all of them together.
+  constexpr int WAVES = THREADS / kWave, OWN = 2 * kMostKept / WAVES;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  unsigned* queue = reinterpret_cast<unsigned*>(s.keys) + wave * OWN;
+  int queued = 0;  // of this wave
+  auto collect = [&](bool take, int token) TMC_INLINE {
+    const u64 takes = __ballot(take);
+    if (takes == 0) return;
+    const int slot = queued + __builtin_amdgcn_mbcnt_hi((unsigned)(takes >> 32),
+                                                        __builtin_amdgcn_mbcnt_lo((unsigned)takes, 0));
+    if (take && slot < OWN) queue[slot] = (unsigned)token;
+    queued += __popcll(takes);
+  };
+  // Returns how many there are, above kMostKept where they are too many.
+  auto collected = [&]() TMC_INLINE -> int {
+    constexpr int KEPT = kMostKept / THREADS;
+    int* counts = reinterpret_cast<int*>(s.words);
+    __syncthreads();
+    if (lane == 0) counts[wave] = queued;
+    __syncthreads();
+    int n = 0, ends[WAVES];
+    bool fits = true;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      fits &= counts[w] <= OWN;
+      ends[w] = n += counts[w];
+    }
+    if (!fits || n > kMostKept) return kMostKept + 1;
+    u64 keys[KEPT];
+#pragma unroll
+    for (int e = 0; e < KEPT; ++e) {
+      const int i = e * THREADS + (int)threadIdx.x;
+      keys[e] = 0;
+      if (i >= n) continue;
+      int slot = i;
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w)
+        if (i >= ends[w - 1]) slot = w * OWN + i - ends[w - 1];
+      const int token = (int)reinterpret_cast<const unsigned*>(s.keys)[slot];
+      keys[e] = rank_key((float)x[token], token);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < KEPT; ++e) {
+      const int i = e * THREADS + (int)threadIdx.x;
+      if (i < n) s.keys[i] = keys[e];
+    }
+    __syncthreads();
+    return n;
+  };
+  // The sums of the block's parts of [begin, end): of the tokens from the logit `high` on
+  // that weight() keeps; those from `low` on and below `high` into the list.  Returns the
+  // sum of all tokens' weights, of this thread.
   u64* groups = s.groups;
-  auto sum_groups = [&](int begin, int end, float from, float to) TMC_INLINE -> u64 {
+  auto sum_groups = [&](int begin, int end, auto lists, float low, float high) TMC_INLINE -> u64 {
     u64 all = 0;
     for (int g = threadIdx.x; g < kMostGroups; g += THREADS) groups[g] = 0;
     __syncthreads();
     parts(begin, end, [&](int at) TMC_INLINE {
+      u64 sum = 0;
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        u64 sum = 0;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float logit = v[i * VEC + e], bin = bin_of(logit);
-          const double a = octaves(logit);
-          const u64 w = a >= kFaintest ? integer(a) : 0;
-          all += w;
-          if (bin < from) sum += a >= faintest && rank_key(logit, place(at, i * VEC + e)) >= cut ? w : 0;
-          else if (bin <= to) collect_one(logit, place(at, i * VEC + e));
-        }
-#pragma unroll
-        for (int off = 1; off < kWave; off <<= 1) sum += __shfl_xor(sum, off, kWave);
-        if (lane == 0 && sum) atomicAdd(&groups[(at - begin) / PART * LOADS + i], sum);
+      for (int i = 0; i < EACH; ++i) {
+        const double a = octaves(v[i]);
+        const u64 w = a >= kFaintest ? integer(a) : 0;
+        all += w;
+        if ((!lists || v[i] >= high) && a >= faintest && rank_key(v[i], place(at, i)) >= cut)
+          sum += w;
+        if (lists) collect(v[i] >= low && v[i] < high, place(at, i));
       }
+      sum = wave_scan(sum);
+      if (lane == kWave - 1 && sum) atomicAdd(&groups[(at - begin) / PART], sum);
     });
     __syncthreads();
     return all;
   };
   auto count_groups = [&](int begin, int end) TMC_INLINE {
-    return (end - begin + PART - 1) / PART * LOADS;
+    return (end - begin + PART - 1) / PART;
   };
 
   // ---- the row's blocks together: every word at agent scope, completed before the
@@ -636,7 +708,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
   if (shared) {
     u64 sum = 0;
     if (way == kSum && !odd) {
-      sum_groups(begin, end, INFINITY, -1.0f);
+      sum_groups(begin, end, std::false_type(), 0.0f, 0.0f);
       const int n = count_groups(begin, end);
       u64 mine = 0, before;
       for (int g = threadIdx.x; g < n; g += THREADS) mine += groups[g];
@@ -670,13 +742,11 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
     if (threadIdx.x == 0) put(p.arrivals + row * kCounterStride, 0);
     best = 0;
     odd = set.most < p.vocab && set.most > kMostTopK;
-#pragma unroll
-    for (int e = 0; e < kBlocks; ++e) {
-      const int b = e * THREADS + (int)threadIdx.x;
-      if (b >= p.count) continue;
+#pragma unroll 1
+    for (int b = threadIdx.x; b < p.count; b += THREADS) {
       const u64 other = get(&records[b].best);
-      s.highs[b] = other ? key_value(other) : -INFINITY;
-      s.blocks[b] = (double)get(&records[b].sum);
+      highs[b] = other ? key_value(other) : -INFINITY;
+      blocks[b] = (double)get(&records[b].sum);
       best = max(best, other);
       odd |= other && (!(fabsf(key_value(other)) < INFINITY) ||
                        !(fabsf(key_value(other) * per_bin) < INFINITY));
@@ -691,12 +761,16 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
       if (threadIdx.x == 0) say(key_index(best), 1.0);
       return true;
     }
-    // A block's factor: its greatest weight.  (A block of -inf alone put no bins, and is
-    // passed over.)
-    auto factor_of = [&](float high) TMC_INLINE {
-      const double a = octaves(high);
-      return a >= kFaintest ? exp2_of(a) : 0.0;
-    };
+    // (A block of -inf alone put no bins, and is passed over.)
+    if (shared) {
+#pragma unroll 1
+      for (int b = threadIdx.x; b < p.count; b += THREADS) {
+        const double a = octaves(highs[b]);
+        factors[b] = a >= kFaintest ? exp2_of(a) * (1.0 / kUnit) : 0.0;
+        blocks[b] *= factors[b];
+      }
+      __syncthreads();
+    }
     // The running sum of the row's bins up to bin i: of this thread's share of its blocks,
     // every `step`-th.
     auto merged = [&](int i, int first, int step) TMC_INLINE -> double {
@@ -708,14 +782,14 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
           const int b = min(b0 + u * step, p.count - 1);
-          const float behind = bin_of(s.highs[b]);
+          const float behind = bin_of(highs[b]);
           here[u] = b0 + u * step < p.count && behind <= (float)i;
           in[u] = get(bins + (size_t)b * kBins + (here[u] ? i - (int)behind : 0));
         }
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-          const float high = s.highs[min(b0 + u * step, p.count - 1)];
-          if (here[u]) sum += (way == kBin ? factor_of(high) * (1.0 / kUnit) : 1.0) * (double)in[u];
+          const double factor = way == kBin ? factors[min(b0 + u * step, p.count - 1)] : 1.0;
+          if (here[u]) sum += factor * (double)in[u];
         }
       }
       return sum;
@@ -733,14 +807,14 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
 #pragma unroll
         for (int e = 0; e < kBlocks; ++e) {
           const int b = e * THREADS + (int)threadIdx.x;
-          if (way == kBin && b < p.count) sums += factor_of(s.highs[b]) * (s.blocks[b] * (1.0 / kUnit));
+          if (b < p.count) sums += blocks[b];
         }
         block_scan<THREADS>(sums, s, base, all);
         if (way == kBin && set.share < 1.0f) limit = (double)set.share * all;
         const double aim = way == kList ? (double)set.most : limit;
         constexpr int LANES = THREADS / kCoarse;
         int first = 0;
-#pragma unroll
+#pragma unroll 1
         for (int step = kCoarse; step >= 1; step /= kCoarse) {
           const int point = (int)threadIdx.x / LANES, i = first + (point + 1) * step - 1;
           mine = i < kBins ? merged(i, (int)threadIdx.x % LANES, LANES) : 0.0;
@@ -784,61 +858,55 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
         block_scan<THREADS>(from > 0 ? merged(from - 1, threadIdx.x, THREADS) : 0.0, s, base, above);
       }
       // ---- the list
-      if (threadIdx.x == 0) s.count = 0;
-      __syncthreads();
+      const float low = least_of(first_bin - (float)to);
+      const float high = from > 0 ? least_of(first_bin - (float)from + 1.0f) : INFINITY;
       u64 weights = 0;
       if (shared) {
-        constexpr int AHEAD = 16;  // loads in flight
-        for (int at = 0; at < p.vocab; at += AHEAD * THREADS * VEC) {
-          vec in[AHEAD];
+        // (short loops: code that runs once waits for its fetch)
+        constexpr int AHEAD = 4 / LOADS;  // parts at once, the next on their way meanwhile
+        vec in[AHEAD][LOADS], next[AHEAD][LOADS];
+        auto fetch = [&](int at) TMC_INLINE {
+          const int from = at + (int)threadIdx.x * EACH;
+          if (at + AHEAD * PART <= p.vocab) {
 #pragma unroll
-          for (int i = 0; i < AHEAD; ++i)
-            in[i] = load(min(at + (i * THREADS + (int)threadIdx.x) * VEC, p.vocab), p.vocab);
+            for (int u = 0; u < AHEAD * LOADS; ++u)
+              next[u / LOADS][u % LOADS] = *reinterpret_cast<const unaligned*>(
+                  x + from + u / LOADS * PART + u % LOADS * VEC);
+          } else {
 #pragma unroll
-          for (int i = 0; i < AHEAD; ++i) {
-            unsigned hits = 0;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-              const float bin = bin_of((float)in[i][e]);
-              hits |= bin >= (float)from && bin <= (float)to ? 1u << e : 0u;
-            }
-            if (hits == 0) continue;
-            int slot = atomicAdd(&s.count, __popc(hits));
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-              if (!(hits >> e & 1)) continue;
-              if (slot < kMostKept)
-                s.keys[slot] = rank_key((float)in[i][e],
-                                        at + (i * THREADS + (int)threadIdx.x) * VEC + e);
-              ++slot;
-            }
+            for (int u = 0; u < AHEAD * LOADS; ++u)
+              next[u / LOADS][u % LOADS] = load(from + u / LOADS * PART + u % LOADS * VEC, p.vocab);
           }
+        };
+        fetch(0);
+#pragma unroll 1
+        for (int at = 0; at < p.vocab; at += AHEAD * PART) {
+#pragma unroll
+          for (int u = 0; u < AHEAD * LOADS; ++u) in[u / LOADS][u % LOADS] = next[u / LOADS][u % LOADS];
+          if (at + AHEAD * PART < p.vocab) fetch(at + AHEAD * PART);
+#pragma unroll
+          for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+              const float logit = (float)in[u][i / VEC][i % VEC];
+              collect(logit >= low && logit < high, place(at + u * PART, i));
+            }
         }
-        __syncthreads();
       } else if (way == kList) {
         parts(0, p.vocab, [&](int at) TMC_INLINE {
 #pragma unroll
-          for (int i = 0; i < EACH; ++i)
-            if (bin_of(v[i]) <= (float)to) collect_one(v[i], place(at, i));
+          for (int i = 0; i < EACH; ++i) collect(v[i] >= low, place(at, i));
         });
-        __syncthreads();
       } else {
-        weights = sum_groups(0, p.vocab, (float)from, (float)to);
+        weights = sum_groups(0, p.vocab, std::true_type(), low, high);
       }
-      const int n = s.count;
+      const int n = collected();
       done = n <= kMostKept;
       if (done) {
         __syncthreads();
-        auto cost = [&](u64 key) TMC_INLINE -> u64 {
+        auto cost_of = [&](u64 key) TMC_INLINE -> u64 {
           const double a = octaves(key_value(key));
           return a >= kFaintest ? max(integer(a), (u64)1) : 0;
-        };
-        auto list_sum = [&](u64 from) TMC_INLINE -> u64 {  // of its keys from there on
-          u64 sum = 0, before, all;
-          for (int i = threadIdx.x; i < n; i += THREADS)
-            if (s.keys[i] >= from) sum += cost(s.keys[i]);
-          block_scan<THREADS>(sum, s, before, all);
-          return all;
         };
         u64 low = ~0ull, high = 0;  // of the list's keys
         for (int i = threadIdx.x; i < n; i += THREADS) {
@@ -847,36 +915,48 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
         }
         high = block_max_u64<THREADS>(high, s);
         low = ~block_max_u64<THREADS>(~low, s);
-        u64 ahead = 0, all = 0;  // what lies before the list; of the list
         if (way == kBin && !shared) {
           // exact sums: of all, and of what lies before the list
-          u64 before, total;
+          u64 before, total, ahead;
           block_scan<THREADS>(weights, s, before, total);
           if (limit < INFINITY) limit = (double)set.share * ((double)total * (1.0 / kUnit));
           u64 mine = 0;
-          for (int g = threadIdx.x; g < count_groups(0, p.vocab); g += THREADS) mine += groups[g];
+          for (int g = threadIdx.x; g < count_groups(0, p.vocab); g += THREADS)
+            mine += groups[g];
           block_scan<THREADS>(mine, s, before, ahead);
           above = (double)ahead * (1.0 / kUnit);
         }
+        // top-k, then top-p: (in a loop, for one copy of its code)
         if (way == kList) above = 0.0;
-        if (n > 0 && (way == kList || limit < INFINITY)) {
-          cut = low;  // (nothing behind the list)
-          if (way == kList && n > set.most)
-            cut = select_key<THREADS>(n, low, high, (u64)set.most, s, [](u64) { return 1ull; });
-          all = list_sum(cut);
-        }
-        if (way == kList && set.share < 1.0f)
-          limit = (double)set.share * ((double)all * (1.0 / kUnit));
-        // the bins said that the cut is in the list: its tokens must bear it out
-        if (way == kBin && !shared && limit < INFINITY && !(set.least > kFaintest) &&
-            ((from > 0 && above >= limit) || above + (double)all * (1.0 / kUnit) < limit))
-          done = false;
-        if (n > 0 && limit < INFINITY && done) {
-          // (none kept: only what lies before the list; but the most probable token stays)
-          const double room = ceil((limit - above) * kUnit);
-          cut = !(room >= 1.0) && from > 0
-                    ? high + 1
-                    : max(cut, select_key<THREADS>(n, low, high, (u64)fmax(room, 1.0), s, cost));
+#pragma unroll 1
+        for (int step = way == kList ? 0 : 1; step < 2 && n > 0 && done; ++step) {
+          u64 target = (u64)set.most;
+          if (step == 0) {
+            cut = low;  // (nothing behind the list)
+            if (n <= set.most) continue;
+          } else {
+            if (set.share == 1.0f) break;
+            cut = max(cut, low);
+            u64 sum = 0, before, all;  // of the list
+            for (int i = threadIdx.x; i < n; i += THREADS)
+              if (s.keys[i] >= cut) sum += cost_of(s.keys[i]);
+            block_scan<THREADS>(sum, s, before, all);
+            const double listed = (double)all * (1.0 / kUnit);
+            if (way == kList) limit = (double)set.share * listed;
+            // the bins said that the cut is in the list: its tokens must bear it out
+            else if (!shared && !(set.least > kFaintest) &&
+                     ((from > 0 && above >= limit) || above + listed < limit))
+              done = false;
+            const double room = ceil((limit - above) * kUnit);
+            if (!(room >= 1.0) && from > 0) {  // only what lies before the list
+              cut = high + 1;
+              break;
+            }
+            target = (u64)fmax(room, 1.0);  // (the most probable token stays)
+          }
+          cut = max(cut, select_key<THREADS>(n, low, high, target, s, [&](u64 key) TMC_INLINE {
+                      return step == 0 ? (u64)1 : cost_of(key);
+                    }));
         }
         // the list's kept tokens to the sums of their loads, or blocks
         const int span = p.walk * PART;
@@ -888,7 +968,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
           const double a = octaves(key_value(key));
           if (key < cut || !(a >= faintest)) continue;
           const int token = key_index(key);
-          atomicAdd(&groups[token / (shared && way == kBin ? span : THREADS * VEC)], integer(a));
+          atomicAdd(&groups[token / (shared && way == kBin ? span : PART)], integer(a));
         }
         __syncthreads();
       }
@@ -902,19 +982,16 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
       // what each block keeps: its bins before the list, and its tokens of the list
       const int span = p.walk * PART;
       for (int b = threadIdx.x; b < p.count; b += THREADS) {
-        const float high = s.highs[b], behind = bin_of(high);
-        const double scale = factor_of(high) * (1.0 / kUnit);
-        if (way == kSum) s.blocks[b] *= scale;
-        else s.blocks[b] =
-                 (double)groups[b] * (1.0 / kUnit) +
-                 (behind < (float)bin
-                      ? scale * (double)get(bins + (size_t)b * kBins + bin - 1 - (int)behind)
-                      : 0.0);
+        if (way == kSum) break;
+        const float behind = bin_of(highs[b]);
+        blocks[b] = (double)groups[b] * (1.0 / kUnit);
+        if (behind < (float)bin)
+          blocks[b] += factors[b] * (double)get(bins + (size_t)b * kBins + bin - 1 - (int)behind);
       }
       __syncthreads();
       double mine[kBlocks], base, before;
       const double sum =
-          take_values(mine, [&](int b) TMC_INLINE { return b < p.count ? s.blocks[b] : 0.0; });
+          take_values(mine, [&](int b) TMC_INLINE { return b < p.count ? blocks[b] : 0.0; });
       block_scan<THREADS>(sum, s, base, total);
       target = set.uniform * total;
       const int b = find_in<THREADS, true>(mine, base, target, before, s);
@@ -924,7 +1001,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
       held = -1;
       __syncthreads();
     }
-    if (way == kSum || (shared && way == kBin)) sum_groups(draw_begin, draw_end, INFINITY, -1.0f);
+    if (way == kSum || (shared && way == kBin)) sum_groups(draw_begin, draw_end, std::false_type(), 0.0f, 0.0f);
     constexpr int SUMS = kMostGroups / THREADS;  // a thread
     const int n = count_groups(draw_begin, draw_end);
     u64 mine[SUMS], base, all, before;
@@ -940,20 +1017,19 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
     const int g = find_in<THREADS, true>(mine, base, aim, before, s);
     if (g < 0) return false;
     aim -= min(before, aim);
-    const int at = draw_begin + (g * THREADS + (int)threadIdx.x) * VEC;
-    u64 w[VEC], own = 0;
+    u64 w[EACH], own = 0;
+    parts(draw_begin + g * PART, min(draw_end, draw_begin + (g + 1) * PART), [&](int at) TMC_INLINE {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      w[e] = at + e < draw_end ? weight((float)x[at + e], at + e) : 0;
-      own += w[e];
-    }
+      for (int i = 0; i < EACH; ++i) own += w[i] = weight(v[i], place(at, i));
+    });
     block_scan<THREADS>(own, s, before, all);
     // (the last that is kept where sums of several blocks fall short)
     const int index = find_in<THREADS, true>(w, before, aim, before, s);
     if (index < 0) return false;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e)
-      if ((int)threadIdx.x * VEC + e == index) say(at + e, (double)w[e] * (1.0 / kUnit) / total);
+    for (int i = 0; i < EACH; ++i)
+      if ((int)threadIdx.x * EACH + i == index)
+        say(draw_begin + g * PART + index, (double)w[i] * (1.0 / kUnit) / total);
     return true;
   };
   if (!by_bins()) row_by_digits<T, THREADS>(p, row, set, s);
@@ -968,7 +1044,7 @@ bool sample_shape(int64_t rows, int64_t vocabulary) {
 constexpr int kThreads = 256, kEach = 8;
 constexpr int64_t kFill = 2048, kFewRows = 192;
 static_assert(kFewRows <= kSharedRows, "every shared row has its counter");
-static_assert(kMostTokens / (kThreads * 4) <= kMostGroups, "a sum a load");
+static_assert(kMostTokens / (kThreads * kEach) <= kMostGroups, "a sum a part");
 struct SamplePlan {
   int walk, count;
 };
@@ -1037,11 +1113,11 @@ extern "C" int tmc_sample(const void* logits, int dtype, int64_t row_stride,
     p.parts = reinterpret_cast<SampleRecord*>(static_cast<char*>(workspace) + kCounterBytes);
     p.bins = reinterpret_cast<u64*>(p.parts + rows * plan.count);
   }
-  const dim3 grid((unsigned)(rows * plan.count));
-  const hipStream_t s = as_stream(stream);
-  if (dtype == TMC_F32)
-    hipLaunchKernelGGL((sample_kernel<float, kThreads, kEach>), grid, dim3(kThreads), 0, s, p);
-  else
-    hipLaunchKernelGGL((sample_kernel<half_t, kThreads, kEach>), grid, dim3(kThreads), 0, s, p);
+  auto kernel = plan.count > 1 ? (dtype == TMC_F32 ? sample_kernel<float, kThreads, kEach, true>
+                                                   : sample_kernel<half_t, kThreads, kEach, true>)
+                               : (dtype == TMC_F32 ? sample_kernel<float, kThreads, kEach, false>
+                                                   : sample_kernel<half_t, kThreads, kEach, false>);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * plan.count)), dim3(kThreads), 0,
+                     as_stream(stream), p);
   return check_launch("sample_kernel");
 }
