@@ -27,10 +27,12 @@ namespace {
 
 typedef unsigned long long u64;
 
-// What a block of a shared row leaves to the last of them.
-struct SampleRecord {
-  u64 best;  // greatest rank key
-  u64 sum;   // of weights, relative to its greatest logit
+// What the blocks of a shared row find out together in the first launch.
+struct SampleRow {
+  u64 best;         // greatest rank key
+  float low, high;  // the logits in the list: from low on, below high
+  int odd;          // to be done by digits
+  int listed;       // in the second launch: tokens in the list so far
 };
 
 struct SampleParams {
@@ -46,8 +48,12 @@ struct SampleParams {
   int rows, vocab;
   int scale;            // integer weights are multiples of 2^-scale
   int count, walk;      // blocks a row, parts of a row that each takes
-  SampleRecord* parts;  // of shared rows: [rows][count]
-  u64* bins;            // [rows][count][kBins]
+  // of shared rows
+  SampleRow* records;   // [rows]
+  u64* blocks;          // [rows][count]: greatest rank keys, then sums of weights
+  u64* sums;            // [rows][count][walk]: the kept weights of every part
+  u64* lists;           // [rows][kMostKept]
+  float* bins;          // [rows][count][kBins]: their running sums
   int* arrivals;        // [rows], kCounterStride apart
 };
 
@@ -131,7 +137,7 @@ static_assert(kMostBlocks <= kMostGroups, "a sum a block");
 static_assert(kBins % kCoarse == 0 && kBins / kCoarse <= kCoarse, "two steps to a bin");
 
 template <int THREADS> struct SampleScratch {
-  u64 hist[kBins > kDigits ? kBins : kDigits];
+  u64 hist[kBins > 2 * kDigits ? (kBins + 1) / 2 : kDigits];  // (bins: of 32 bits)
   u64 keys[kMostKept];
   u64 groups[kMostGroups];  // (of a shared row first what its blocks keep of the list)
   u64 words[THREADS / kWave];
@@ -312,23 +318,26 @@ __device__ __forceinline__ void row_by_digits(const SampleParams& p, int row, co
 }
 
 // ------------------------------------------------------------ rows in registers
-// A block takes a row, or, where rows are few, a part of one; the last of a row's blocks
-// to arrive goes on with the row.  With the part's logits in registers:
+// With a part of the row at a time in registers:
 //   - the maximum;
 //   - for top-k and top-p, the tokens' number or weight in each bin, in LDS, and from
-//     these the bin in which the cut falls: its tokens (for top-k those above it too)
-//     are collected and sorted, which gives the cut exactly;
-//   - the sums of the kept weights of every 64 lanes' tokens, and of these the 64 that
-//     hold the number drawn.
-// A block with its own row takes one 64-bit exponential a token: the bins' weights are of
-// 32 bits, and say only which bins' tokens to sort.  Blocks that share a row cannot
-// come back to it, so their bins are exact.
+//     these the bins in which the cut falls;
+//   - the tokens of these bins (for top-k those above too) into a list, and the sums of
+//     the weights before them, of every part; in the list the cut is found exactly;
+//   - the part that holds the number drawn, and in it the token.
+// One 64-bit exponential a token: the bins' weights are of 32 bits, and say only which
+// tokens to list.
+//
+// Where rows are few, several blocks share one, in two launches: the first ends with the
+// bins, of which the last of a row's blocks to arrive finds the list's bounds; in the
+// second each block sums and lists its own tokens, and the last goes on with the row.
+// (In one launch the last block would have to read the whole row again by itself: 40 us
+// of 90 for rows of 128000.)
 //
 // Bins are of absolute logits, so that those of several blocks fit together.  Weights are
-// integers, sums of more blocks 64-bit floats in their order: the result does not
-// depend on which thread comes first.  Rows that this does not fit (more than kMostKept
-// tokens to collect, as in flat rows or with many equals; infinities; a top_k above
-// kMostTopK) go to row_by_digits().
+// integers: the result does not depend on which thread comes first.  Rows that this does
+// not fit (more than kMostKept tokens to list, as in flat rows or with many equals;
+// infinities; a top_k above kMostTopK) go to row_by_digits().
 
 // The thread's EACH consecutive values and their sum.
 template <int EACH, typename TYPE, typename VALUE>
@@ -461,21 +470,21 @@ __device__ __forceinline__ u64 select_key(int n, u64 low, u64 high, u64 target,
   return found;
 }
 
-template <typename T, int THREADS, int EACH, bool SHARED>
+// STAGE: 0 for a row of one block, 1 and 2 for the launches of shared rows.
+template <typename T, int THREADS, int EACH, int STAGE>
 __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
   constexpr int VEC = 16 / (int)sizeof(T), LOADS = EACH / VEC;
   constexpr int PART = THREADS * EACH;
   constexpr int BINS = (kBins + THREADS - 1) / THREADS;  // bins a thread
+  constexpr bool SHARED = STAGE > 0;
   typedef T vec __attribute__((ext_vector_type(VEC)));
   typedef vec unaligned __attribute__((aligned(sizeof(T))));  // rows start at any element
   __shared__ SampleScratch<THREADS> s;
-  __shared__ double factors[SHARED ? kMostBlocks : 1];  // of a row's blocks: the greatest weight,
-  __shared__ double blocks[SHARED ? kMostBlocks : 1];   // the sum of weights,
-  __shared__ float highs[SHARED ? kMostBlocks : 1];     // the greatest logit
-  const int split = blockIdx.x % p.count, row = blockIdx.x / p.count;
+  __shared__ double factors[STAGE == 1 ? kMostBlocks : 1];  // of a row's blocks: the greatest weight,
+  __shared__ float highs[STAGE == 1 ? kMostBlocks : 1];     // the greatest logit
+  const int split = SHARED ? blockIdx.x % p.count : 0, row = SHARED ? blockIdx.x / p.count : blockIdx.x;
   const int lane = threadIdx.x & (kWave - 1);
   const T* x = static_cast<const T*>(p.logits) + (size_t)row * p.stride;
-  constexpr bool shared = SHARED;
 
   // ---- a part of the row, EACH tokens a thread, so that order is the vocabulary's
   auto load = [&](int from, int end) TMC_INLINE -> vec {
@@ -487,27 +496,29 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
   };
   float v[EACH];
   int held = -1;  // start of the part in v
+  auto fetch = [&](int at, int end) TMC_INLINE {
+    if (at == held) return;
+    vec in[LOADS];
+    const int from = at + (int)threadIdx.x * EACH;
+    if (at + PART <= end) {  // (for all threads: the loads are in flight together)
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i)
+        in[i] = *reinterpret_cast<const unaligned*>(x + from + i * VEC);
+    } else {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) in[i] = load(from + i * VEC, end);
+    }
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) v[i] = (float)in[i / VEC][i % VEC];
+    held = at;
+  };
   // What a pass computes of each logit it computes anew: kept for the next pass it would
   // take more registers than there are.
   float top = 0.0f, first_bin = 0.0f;
   // take(part's start) for every part of [begin, end), its logits in v
   auto parts = [&](int begin, int end, auto&& take) TMC_INLINE {
     for (int at = begin; at < end; at += PART) {
-      if (at != held) {
-        vec in[LOADS];
-        const int from = at + (int)threadIdx.x * EACH;
-        if (at + PART <= end) {  // (for all threads: the loads are in flight together)
-#pragma unroll
-          for (int i = 0; i < LOADS; ++i)
-            in[i] = *reinterpret_cast<const unaligned*>(x + from + i * VEC);
-        } else {
-#pragma unroll
-          for (int i = 0; i < LOADS; ++i) in[i] = load(from + i * VEC, end);
-        }
-#pragma unroll
-        for (int i = 0; i < EACH; ++i) v[i] = (float)in[i / VEC][i % VEC];
-        held = at;
-      }
+      fetch(at, end);
       asm volatile("" : "+v"(top), "+v"(first_bin));
       take(at);
     }
@@ -515,37 +526,46 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
   auto place = [&](int at, int i) TMC_INLINE {
     return at + (int)threadIdx.x * EACH + i;
   };
-  const int begin = split * p.walk * PART, end = min(p.vocab, begin + p.walk * PART);
+  const int span = p.walk * PART;  // of a block
+  const int begin = split * span, end = SHARED ? min(p.vocab, begin + span) : p.vocab;
+  SampleRow* record = p.records + row;
 
-  // ---- the block's greatest
-  float most = -INFINITY;  // (NaN left out)
-  parts(begin, end, [&](int) TMC_INLINE {
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) most = fmaxf(most, v[i]);
-  });
-  const Settings set = settings_of(p, row);  // (its loads came beside the logits')
+  // ---- the greatest, of the block or (known already) of the row
   u64 best = 0;
-  if (set.heat == 0.0) {  // with its token
-    parts(begin, end, [&](int at) TMC_INLINE {
-#pragma unroll
-      for (int i = 0; i < EACH; ++i)
-        if (v[i] == most) best = max(best, rank_key(v[i], place(at, i)));
-    });
+  fetch(begin, end);
+  const Settings set = settings_of(p, row);
+  if (STAGE == 2) {
+    best = record->best;
   } else {
-    best = most == -INFINITY ? 0 : rank_key(most, 0);
+    float most = -INFINITY;  // (NaN left out)
+    parts(begin, end, [&](int) TMC_INLINE {
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) most = fmaxf(most, v[i]);
+    });
+    if (set.heat == 0.0) {  // with its token
+      parts(begin, end, [&](int at) TMC_INLINE {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i)
+          if (v[i] == most) best = max(best, rank_key(v[i], place(at, i)));
+      });
+    } else {
+      best = most == -INFINITY ? 0 : rank_key(most, 0);
+    }
+    best = block_max_u64<THREADS>(best, s);
   }
-  best = block_max_u64<THREADS>(best, s);
   top = best ? key_value(best) : -INFINITY;
   const float per_bin = (float)(set.heat * kBinsOctave);
-  // parts without a logit above -inf, what has no bins, and long lists: by digits
-  bool odd = !(fabsf(top * per_bin) < INFINITY) || !(fabsf(top) < INFINITY) ||
-             (set.most < p.vocab && set.most > kMostTopK);
+  // what has no bins, and long lists: by digits
+  auto is_odd = [&](float top) TMC_INLINE {
+    return !(fabsf(top * per_bin) < INFINITY) || !(fabsf(top) < INFINITY);
+  };
+  bool odd = STAGE == 2 ? record->odd : is_odd(top) || (set.most < p.vocab && set.most > kMostTopK);
 
   // ---- what the row's settings need of it
-  enum { kGreedy, kList, kBin, kSum } way =
-      set.heat == 0.0 ? kGreedy
-      : set.most < p.vocab ? kList
-      : set.share < 1.0f || (shared && set.least > kFaintest) ? kBin : kSum;
+  enum { kGreedy, kList, kBin, kSum } way = set.heat == 0.0         ? kGreedy
+                                            : set.most < p.vocab    ? kList
+                                            : set.share < 1.0f      ? kBin
+                                                                    : kSum;
   // A token's bin, counted down from the greatest's (NaN: none).
   auto level = [&](float x) TMC_INLINE { return floorf(x * per_bin); };
   first_bin = level(top);
@@ -556,40 +576,35 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
   auto integer = [&](double a) TMC_INLINE -> u64 {
     return __builtin_bit_cast(u64, exp2_of(a) + 512.0) - __builtin_bit_cast(u64, 512.0);
   };
-  // (the bins of a block with its own row; a sum of 2^20 tokens fits)
+  // counts, or weights relative to the bin in units of 2^-11 (a sum of 2^20 tokens fits)
   unsigned* rough = reinterpret_cast<unsigned*>(s.hist);
-  if (!odd && (way == kList || way == kBin)) {
-    for (int i = threadIdx.x; i < kBins; i += THREADS) s.hist[i] = 0;
+  if (STAGE < 2 && !odd && (way == kList || way == kBin)) {
+    for (int i = threadIdx.x; i < kBins; i += THREADS) rough[i] = 0;
     __syncthreads();
-    if (shared) {
-      parts(begin, end, [&](int) TMC_INLINE {
+    parts(begin, end, [&](int) TMC_INLINE {
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-          const float bin = bin_of(v[i]);
-          if (bin < (float)kBins)
-            atomicAdd(&s.hist[(int)bin],
-                      way == kBin ? integer(fmax(octaves(v[i]), -60.0)) : 1ull);
+      for (int i = 0; i < EACH; ++i) {
+        const float bin = bin_of(v[i]);
+        if (bin < (float)kBins) {
+          unsigned cost = 1;
+          if (way == kBin)
+            cost = (unsigned)__fmaf_rn(
+                fast_exp2(__fmaf_rn(v[i] - top, per_bin / kBinsOctave, bin * (1.0f / kBinsOctave))),
+                0x1p11f, 0.5f);
+          atomicAdd(&rough[(int)bin], cost);
         }
-      });
-    } else {
-      // counts, or weights relative to the bin of 11 bits
-      parts(begin, end, [&](int) TMC_INLINE {
-#pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-          const float bin = bin_of(v[i]);
-          if (bin < (float)kBins) {
-            unsigned cost = 1;
-            if (way == kBin)
-              cost = (unsigned)__fmaf_rn(
-                  fast_exp2(__fmaf_rn(v[i] - top, per_bin / kBinsOctave, bin * (1.0f / kBinsOctave))),
-                  0x1p11f, 0.5f);
-            atomicAdd(&rough[(int)bin], cost);
-          }
-        }
-      });
-    }
+      }
+    });
     __syncthreads();
   }
+  // The thread's bins, and the sum of all before them.
+  auto take_bins = [&](double (&mine)[BINS], double& base, double& all) TMC_INLINE {
+    const double sum = take_values(mine, [&](int i) TMC_INLINE {
+      const double scale = way == kBin ? (double)fast_exp2((float)-i / kBinsOctave) : 1.0;
+      return i < kBins ? scale * (double)rough[i] : 0.0;
+    });
+    block_scan<THREADS>(sum, s, base, all);
+  };
   // Of a token: what it weighs, 0 for one that is not kept: below the last that counts, or
   // ranked below `cut`.
   const double faintest = fmax(set.least, kFaintest);
@@ -665,11 +680,12 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
     __syncthreads();
     return n;
   };
-  // The sums of the block's parts of [begin, end): of the tokens from the logit `high` on
-  // that weight() keeps; those from `low` on and below `high` into the list.  Returns the
-  // sum of all tokens' weights, of this thread.
+  float low = 0.0f, high = 0.0f;  // the list's logits: from low on, below high
+  // The sums of the block's parts: of the tokens from the logit `high` on (all, where none
+  // are listed) that min-p keeps; those from `low` on and below `high` into the list.
+  // Returns the sum of all tokens' weights, of this thread.
   u64* groups = s.groups;
-  auto sum_groups = [&](int begin, int end, auto lists, float low, float high) TMC_INLINE -> u64 {
+  auto sum_groups = [&](auto lists) TMC_INLINE -> u64 {
     u64 all = 0;
     for (int g = threadIdx.x; g < kMostGroups; g += THREADS) groups[g] = 0;
     __syncthreads();
@@ -680,8 +696,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
         const double a = octaves(v[i]);
         const u64 w = a >= kFaintest ? integer(a) : 0;
         all += w;
-        if ((!lists || v[i] >= high) && a >= faintest && rank_key(v[i], place(at, i)) >= cut)
-          sum += w;
+        if ((!lists || v[i] >= high) && a >= faintest) sum += w;
         if (lists) collect(v[i] >= low && v[i] < high, place(at, i));
       }
       sum = wave_scan(sum);
@@ -690,8 +705,26 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
     __syncthreads();
     return all;
   };
-  auto count_groups = [&](int begin, int end) TMC_INLINE {
-    return (end - begin + PART - 1) / PART;
+  auto count_groups = [&](int tokens) TMC_INLINE { return (tokens + PART - 1) / PART; };
+
+  // The bins [from, to] that are listed: that in which the running sum, `above` before it and
+  // `reached` with it, reaches its aim, and its neighbours where the border is nearer than
+  // rough sums are exact (half a unit of a token's 2^11 and more, and as much of the aim).
+  auto bounds = [&](int bin, double above, double reached, double aim, double all) TMC_INLINE {
+    int from = 0, to = bin;
+    if (way == kBin) {
+      const double near = 6e-4 * all;
+      from = max(0, bin - (aim - above < near));
+      to = bin + (reached - aim < near);
+      // min-p: the bins around the least logit that it keeps
+      const float least = bin_of((float)((double)top + faintest / set.heat)) - 1.0f;
+      if (set.least > kFaintest && least < (float)from) {
+        from = max((int)least, 0);
+        to = min(to, (int)least + 2);
+      }
+    }
+    low = least_of(first_bin - (float)to);
+    high = from > 0 ? least_of(first_bin - (float)from + 1.0f) : INFINITY;
   };
 
   // ---- the row's blocks together: every word at agent scope, completed before the
@@ -702,207 +735,170 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
   auto get = [](const auto* from) TMC_INLINE {
     return __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   };
-  SampleRecord* records = p.parts + (size_t)row * p.count;
-  u64* bins = p.bins + (size_t)row * p.count * kBins;
-  constexpr int kBlocks = (kMostBlocks + THREADS - 1) / THREADS;  // a thread
-  if (shared) {
-    u64 sum = 0;
-    if (way == kSum && !odd) {
-      sum_groups(begin, end, std::false_type(), 0.0f, 0.0f);
-      const int n = count_groups(begin, end);
-      u64 mine = 0, before;
-      for (int g = threadIdx.x; g < n; g += THREADS) mine += groups[g];
-      block_scan<THREADS>(mine, s, before, sum);
+  auto arrive = [&]() TMC_INLINE -> bool {
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      int* count = p.arrivals + row * kCounterStride;
+      s.last = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+               p.count - 1;
+      if (s.last) put(count, 0);
     }
+    __syncthreads();
+    const bool last = s.last;
+    __syncthreads();
+    return last;
+  };
+  u64* blocks = p.blocks + (size_t)row * p.count;
+  if constexpr (STAGE == 1) {
+    float* bins = p.bins + (size_t)row * p.count * kBins;
     if (!odd && (way == kList || way == kBin)) {
-      // the running sums of its bins
-      u64 mine[BINS], base;
-      const u64 own = take_values(mine, [&](int i) TMC_INLINE { return i < kBins ? s.hist[i] : 0ull; });
-      block_scan<THREADS>(own, s, base, sum);
+      double mine[BINS], base, all;
+      take_bins(mine, base, all);
 #pragma unroll
       for (int e = 0; e < BINS; ++e) {
         const int i = (int)threadIdx.x * BINS + e;
         base += mine[e];
-        if (i < kBins) put(bins + (size_t)split * kBins + i, base);
+        if (i < kBins) put(bins + (size_t)split * kBins + i, (float)base);
       }
     }
-    if (threadIdx.x == 0) {
-      put(&records[split].best, best);
-      put(&records[split].sum, sum);
-    }
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    if (threadIdx.x == 0)
-      s.last = __hip_atomic_fetch_add(p.arrivals + row * kCounterStride, 1, __ATOMIC_RELAXED,
-                                      __HIP_MEMORY_SCOPE_AGENT) == p.count - 1;
-    __syncthreads();
-    const bool last = s.last;
-    __syncthreads();
-    if (!last) return;
-    if (threadIdx.x == 0) put(p.arrivals + row * kCounterStride, 0);
+    if (threadIdx.x == 0) put(blocks + split, best);
+    if (!arrive()) return;
     best = 0;
     odd = set.most < p.vocab && set.most > kMostTopK;
-#pragma unroll 1
     for (int b = threadIdx.x; b < p.count; b += THREADS) {
-      const u64 other = get(&records[b].best);
-      highs[b] = other ? key_value(other) : -INFINITY;
-      blocks[b] = (double)get(&records[b].sum);
+      const u64 other = get(blocks + b);
+      highs[b] = other ? key_value(other) : -INFINITY;  // (of -inf alone: no bins, passed over)
       best = max(best, other);
-      odd |= other && (!(fabsf(key_value(other)) < INFINITY) ||
-                       !(fabsf(key_value(other) * per_bin) < INFINITY));
+      odd |= other && is_odd(highs[b]);
     }
     odd = __syncthreads_or(odd);
     best = block_max_u64<THREADS>(best, s);
+    odd |= best == 0;
     top = best ? key_value(best) : -INFINITY;
     first_bin = level(top);
+    if (way == kGreedy && best) {
+      odd = false;
+      if (threadIdx.x == 0) say(key_index(best), 1.0);
+    }
+    if (!odd && (way == kList || way == kBin)) {
+      double sum = 0.0, base, all;
+      for (int b = threadIdx.x; b < p.count; b += THREADS) {
+        const double a = octaves(highs[b]);
+        factors[b] = way == kList ? 1.0 : a >= kFaintest ? exp2_of(a) : 0.0;
+        sum += highs[b] > -INFINITY ? factors[b] * (double)get(bins + (size_t)b * kBins + kBins - 1) : 0.0;
+      }
+      block_scan<THREADS>(sum, s, base, all);
+      // The running sum of the row's bins up to bin i: of this thread's share of its blocks,
+      // every `step`-th.
+      auto merged = [&](int i, int first, int step) TMC_INLINE -> double {
+        constexpr int kAhead = 4;  // blocks at once
+        double sum = 0.0;
+        for (int b0 = first; b0 < p.count; b0 += kAhead * step) {
+          float in[kAhead];
+          double factor[kAhead];
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) {
+            const int b = min(b0 + u * step, p.count - 1);
+            const float behind = bin_of(highs[b]);
+            const bool here = b0 + u * step < p.count && behind <= (float)i;
+            in[u] = get(bins + (size_t)(here ? b : split) * kBins + (here ? i - (int)behind : 0));
+            factor[u] = here ? factors[b] : 0.0;
+          }
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u)
+            if (factor[u] > 0.0) sum += factor[u] * (double)in[u];
+        }
+        return sum;
+      };
+      // in two steps: the coarse ones' running sums, then those of one's bins
+      const double aim = way == kList ? (double)set.most : (double)set.share * all;
+      constexpr int LANES = THREADS / kCoarse;
+      int first = 0;
+      double above = 0.0, reached = 0.0;
+#pragma unroll 1
+      for (int step = kCoarse; step >= 1; step /= kCoarse) {
+        const int point = (int)threadIdx.x / LANES, i = first + (point + 1) * step - 1;
+        double mine = i < kBins ? merged(i, (int)threadIdx.x % LANES, LANES) : 0.0;
+#pragma unroll
+        for (int off = 1; off < LANES; off <<= 1) mine += __shfl_xor(mine, off, kWave);
+        __syncthreads();
+        if (threadIdx.x % LANES == 0) s.levels[point] = i < kBins ? mine : INFINITY;
+        __syncthreads();
+        int at = 0;
+        while (at < kCoarse - 1 && s.levels[at] < aim) ++at;
+        if (at > 0) above = s.levels[at - 1];
+        reached = s.levels[at];
+        first = min(first + at * step, kBins - step);
+      }
+      bounds(first, above, reached, aim, all);
+    }
+    if (threadIdx.x == 0) *record = {best, low, high, odd, 0};
+    return;
+  }
+  if (STAGE == 2) {
+    if (odd && split > 0) return;
+    if (!odd && way == kGreedy) return;
+    low = record->low;
+    high = record->high;
   }
   auto by_bins = [&]() TMC_INLINE -> bool {
+    bool done = best != 0 && !odd;
     if (way == kGreedy && best) {
       if (threadIdx.x == 0) say(key_index(best), 1.0);
       return true;
     }
-    // (A block of -inf alone put no bins, and is passed over.)
-    if (shared) {
-#pragma unroll 1
-      for (int b = threadIdx.x; b < p.count; b += THREADS) {
-        const double a = octaves(highs[b]);
-        factors[b] = a >= kFaintest ? exp2_of(a) * (1.0 / kUnit) : 0.0;
-        blocks[b] *= factors[b];
+    u64 weights = 0;  // of all tokens, this thread's
+    if (done) {
+      if (STAGE == 0 && way != kSum) {
+        double mine[BINS], base, all, above;
+        take_bins(mine, base, all);
+        const double aim = way == kList ? (double)set.most : (double)set.share * all;
+        const int bin = find_in<THREADS, false>(mine, base, aim, above, s);
+        const double here = bin >= 0 ? (way == kBin ? exp2_of(-(double)bin / kBinsOctave) : 1.0) * rough[bin] : 0.0;
+        bounds(bin, above, above + here, aim, all);
       }
-      __syncthreads();
-    }
-    // The running sum of the row's bins up to bin i: of this thread's share of its blocks,
-    // every `step`-th.
-    auto merged = [&](int i, int first, int step) TMC_INLINE -> double {
-      constexpr int kAhead = 4;  // blocks at once
-      double sum = 0.0;
-      for (int b0 = first; b0 < p.count; b0 += kAhead * step) {
-        u64 in[kAhead];
-        bool here[kAhead];
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-          const int b = min(b0 + u * step, p.count - 1);
-          const float behind = bin_of(highs[b]);
-          here[u] = b0 + u * step < p.count && behind <= (float)i;
-          in[u] = get(bins + (size_t)b * kBins + (here[u] ? i - (int)behind : 0));
-        }
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-          const double factor = way == kBin ? factors[min(b0 + u * step, p.count - 1)] : 1.0;
-          if (here[u]) sum += factor * (double)in[u];
-        }
-      }
-      return sum;
-    };
-    bool done = best != 0 && !odd;
-    int bin = 0;              // the first of the list's
-    double limit = INFINITY;  // top-p: tokens before which less than that lies stay
-    double above = 0.0;       // the sum of the bins before the list
-    if (done && way != kSum) {
-      int from = 0, to = 0;
-      double all = 0.0;
-      if (shared) {
-        // in two steps: the coarse ones' running sums, then those of one's bins
-        double sums = 0.0, base, mine = 0.0;
-#pragma unroll
-        for (int e = 0; e < kBlocks; ++e) {
-          const int b = e * THREADS + (int)threadIdx.x;
-          if (b < p.count) sums += blocks[b];
-        }
-        block_scan<THREADS>(sums, s, base, all);
-        if (way == kBin && set.share < 1.0f) limit = (double)set.share * all;
-        const double aim = way == kList ? (double)set.most : limit;
-        constexpr int LANES = THREADS / kCoarse;
-        int first = 0;
-#pragma unroll 1
-        for (int step = kCoarse; step >= 1; step /= kCoarse) {
-          const int point = (int)threadIdx.x / LANES, i = first + (point + 1) * step - 1;
-          mine = i < kBins ? merged(i, (int)threadIdx.x % LANES, LANES) : 0.0;
-#pragma unroll
-          for (int off = 1; off < LANES; off <<= 1) mine += __shfl_xor(mine, off, kWave);
-          __syncthreads();
-          if (threadIdx.x % LANES == 0) s.levels[point] = i < kBins ? mine : INFINITY;
-          __syncthreads();
-          int at = 0;
-          while (at < kCoarse - 1 && s.levels[at] < aim) ++at;
-          first = min(first + at * step, kBins - step);
-        }
-        bin = first;
-        from = way == kList ? 0 : bin;
-        to = bin;
-      } else {
-        double mine[BINS], sum, base;
-        sum = take_values(mine, [&](int i) TMC_INLINE {
-          const double scale = way == kBin ? exp2_of(-(double)min(i, kBins) / kBinsOctave) : 1.0;
-          return i < kBins ? scale * (double)rough[i] : 0.0;
-        });
-        block_scan<THREADS>(sum, s, base, all);
-        if (way == kBin && set.share < 1.0f) limit = (double)set.share * all;
-        bin = find_in<THREADS, false>(mine, base, way == kList ? (double)set.most : limit, above, s);
-        from = way == kList ? 0 : bin;
-        to = bin;
-        if (limit < INFINITY) {  // rough sums: the next bin too, and the one before where the border is near
-          from = max(0, bin - (limit - above < 3e-4 * all));
-          to = bin + 1;
-        }
-      }
-      // min-p: the bins around the least logit that it keeps
-      const float least = bin_of((float)((double)top + faintest / set.heat)) - 1.0f;
-      if (way == kBin && set.least > kFaintest && least < (float)from) {
-        from = max((int)least, 0);
-        to = min(to, (int)least + 2);
-      }
-      bin = from;
-      if (shared && way == kBin) {
-        double base;
-        block_scan<THREADS>(from > 0 ? merged(from - 1, threadIdx.x, THREADS) : 0.0, s, base, above);
-      }
-      // ---- the list
-      const float low = least_of(first_bin - (float)to);
-      const float high = from > 0 ? least_of(first_bin - (float)from + 1.0f) : INFINITY;
-      u64 weights = 0;
-      if (shared) {
-        // (short loops: code that runs once waits for its fetch)
-        constexpr int AHEAD = 4 / LOADS;  // parts at once, the next on their way meanwhile
-        vec in[AHEAD][LOADS], next[AHEAD][LOADS];
-        auto fetch = [&](int at) TMC_INLINE {
-          const int from = at + (int)threadIdx.x * EACH;
-          if (at + AHEAD * PART <= p.vocab) {
-#pragma unroll
-            for (int u = 0; u < AHEAD * LOADS; ++u)
-              next[u / LOADS][u % LOADS] = *reinterpret_cast<const unaligned*>(
-                  x + from + u / LOADS * PART + u % LOADS * VEC);
-          } else {
-#pragma unroll
-            for (int u = 0; u < AHEAD * LOADS; ++u)
-              next[u / LOADS][u % LOADS] = load(from + u / LOADS * PART + u % LOADS * VEC, p.vocab);
-          }
-        };
-        fetch(0);
-#pragma unroll 1
-        for (int at = 0; at < p.vocab; at += AHEAD * PART) {
-#pragma unroll
-          for (int u = 0; u < AHEAD * LOADS; ++u) in[u / LOADS][u % LOADS] = next[u / LOADS][u % LOADS];
-          if (at + AHEAD * PART < p.vocab) fetch(at + AHEAD * PART);
-#pragma unroll
-          for (int u = 0; u < AHEAD; ++u)
-#pragma unroll
-            for (int i = 0; i < EACH; ++i) {
-              const float logit = (float)in[u][i / VEC][i % VEC];
-              collect(logit >= low && logit < high, place(at + u * PART, i));
-            }
-        }
-      } else if (way == kList) {
-        parts(0, p.vocab, [&](int at) TMC_INLINE {
+      if (way == kList) {
+        parts(begin, end, [&](int at) TMC_INLINE {
 #pragma unroll
           for (int i = 0; i < EACH; ++i) collect(v[i] >= low, place(at, i));
         });
+      } else if (way == kBin) {
+        weights = sum_groups(std::true_type());
       } else {
-        weights = sum_groups(0, p.vocab, std::true_type(), low, high);
+        sum_groups(std::false_type());
       }
-      const int n = collected();
+      int n = way == kSum ? 0 : collected();
+      if constexpr (STAGE == 2) {
+        // its tokens and sums to the row's
+        u64* list = p.lists + (size_t)row * kMostKept;
+        u64* sums = p.sums + (size_t)row * p.count * p.walk;
+        if (n > 0) {
+          if (threadIdx.x == 0)
+            s.found = __hip_atomic_fetch_add(&record->listed, n, __ATOMIC_RELAXED,
+                                             __HIP_MEMORY_SCOPE_AGENT);
+          __syncthreads();
+          const int first = s.found;
+          for (int i = threadIdx.x; i < n && n <= kMostKept && first + i < kMostKept; i += THREADS)
+            put(list + first + i, s.keys[i]);
+        }
+        if (way != kList)
+          for (int g = threadIdx.x; g < p.walk; g += THREADS) put(sums + split * p.walk + g, groups[g]);
+        weights = block_sum_u64<THREADS>(weights, s);
+        if (threadIdx.x == 0) put(blocks + split, weights);
+        if (!arrive()) return true;
+        n = get(&record->listed);
+        weights = 0;
+        for (int b = threadIdx.x; b < p.count; b += THREADS) weights += get(blocks + b);
+        if (way != kList)
+          for (int g = threadIdx.x; g < count_groups(p.vocab); g += THREADS) groups[g] = get(sums + g);
+        for (int i = threadIdx.x; i < min(n, kMostKept); i += THREADS) s.keys[i] = get(list + i);
+        __syncthreads();
+      }
       done = n <= kMostKept;
-      if (done) {
+      double limit = INFINITY;  // top-p: tokens before which less than that lies stay
+      double above = 0.0;       // the sum before the list
+      if (done && way != kSum) {
         __syncthreads();
         auto cost_of = [&](u64 key) TMC_INLINE -> u64 {
           const double a = octaves(key_value(key));
@@ -915,19 +911,17 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
         }
         high = block_max_u64<THREADS>(high, s);
         low = ~block_max_u64<THREADS>(~low, s);
-        if (way == kBin && !shared) {
+        if (way == kBin) {
           // exact sums: of all, and of what lies before the list
           u64 before, total, ahead;
           block_scan<THREADS>(weights, s, before, total);
-          if (limit < INFINITY) limit = (double)set.share * ((double)total * (1.0 / kUnit));
+          limit = (double)set.share * ((double)total * (1.0 / kUnit));
           u64 mine = 0;
-          for (int g = threadIdx.x; g < count_groups(0, p.vocab); g += THREADS)
-            mine += groups[g];
+          for (int g = threadIdx.x; g < count_groups(p.vocab); g += THREADS) mine += groups[g];
           block_scan<THREADS>(mine, s, before, ahead);
           above = (double)ahead * (1.0 / kUnit);
         }
         // top-k, then top-p: (in a loop, for one copy of its code)
-        if (way == kList) above = 0.0;
 #pragma unroll 1
         for (int step = way == kList ? 0 : 1; step < 2 && n > 0 && done; ++step) {
           u64 target = (u64)set.most;
@@ -944,11 +938,11 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
             const double listed = (double)all * (1.0 / kUnit);
             if (way == kList) limit = (double)set.share * listed;
             // the bins said that the cut is in the list: its tokens must bear it out
-            else if (!shared && !(set.least > kFaintest) &&
-                     ((from > 0 && above >= limit) || above + listed < limit))
+            else if (!(set.least > kFaintest) &&
+                     ((above > 0.0 && above >= limit) || above + listed < limit))
               done = false;
             const double room = ceil((limit - above) * kUnit);
-            if (!(room >= 1.0) && from > 0) {  // only what lies before the list
+            if (!(room >= 1.0) && above > 0.0) {  // only what lies before the list
               cut = high + 1;
               break;
             }
@@ -958,17 +952,14 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
                       return step == 0 ? (u64)1 : cost_of(key);
                     }));
         }
-        // the list's kept tokens to the sums of their loads, or blocks
-        const int span = p.walk * PART;
-        if (shared || way == kList)
+        // the list's kept tokens to the sums of their parts
+        if (way == kList)
           for (int g = threadIdx.x; g < kMostGroups; g += THREADS) groups[g] = 0;
         __syncthreads();
         for (int i = threadIdx.x; i < n; i += THREADS) {
           const u64 key = s.keys[i];
           const double a = octaves(key_value(key));
-          if (key < cut || !(a >= faintest)) continue;
-          const int token = key_index(key);
-          atomicAdd(&groups[token / (shared && way == kBin ? span : PART)], integer(a));
+          if (key >= cut && a >= faintest) atomicAdd(&groups[key_index(key) / PART], integer(a));
         }
         __syncthreads();
       }
@@ -976,60 +967,27 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
     if (!done) return false;
 
     // ---- the draw
-    int draw_begin = 0, draw_end = p.vocab;
-    double target = -1.0, total = 0.0;  // in units of the greatest weight
-    if (shared && way != kList) {
-      // what each block keeps: its bins before the list, and its tokens of the list
-      const int span = p.walk * PART;
-      for (int b = threadIdx.x; b < p.count; b += THREADS) {
-        if (way == kSum) break;
-        const float behind = bin_of(highs[b]);
-        blocks[b] = (double)groups[b] * (1.0 / kUnit);
-        if (behind < (float)bin)
-          blocks[b] += factors[b] * (double)get(bins + (size_t)b * kBins + bin - 1 - (int)behind);
-      }
-      __syncthreads();
-      double mine[kBlocks], base, before;
-      const double sum =
-          take_values(mine, [&](int b) TMC_INLINE { return b < p.count ? blocks[b] : 0.0; });
-      block_scan<THREADS>(sum, s, base, total);
-      target = set.uniform * total;
-      const int b = find_in<THREADS, true>(mine, base, target, before, s);
-      target -= before;
-      draw_begin = b * span;
-      draw_end = min(p.vocab, draw_begin + span);
-      held = -1;
-      __syncthreads();
-    }
-    if (way == kSum || (shared && way == kBin)) sum_groups(draw_begin, draw_end, std::false_type(), 0.0f, 0.0f);
     constexpr int SUMS = kMostGroups / THREADS;  // a thread
-    const int n = count_groups(draw_begin, draw_end);
+    const int n = count_groups(p.vocab);
     u64 mine[SUMS], base, all, before;
     const u64 sum = take_values(mine, [&](int g) TMC_INLINE { return g < n ? groups[g] : 0ull; });
     block_scan<THREADS>(sum, s, base, all);
-    const bool whole = !shared || way == kList;
-    if (whole) {
-      total = (double)all * (1.0 / kUnit);
-      target = set.uniform * total;
-    }
-    u64 aim = (u64)(fmax(target, 0.0) * kUnit);
-    if (whole) aim = min(aim, all - 1);
+    if (all == 0) return false;
+    u64 aim = min((u64)(set.uniform * (double)all), all - 1);
     const int g = find_in<THREADS, true>(mine, base, aim, before, s);
     if (g < 0) return false;
-    aim -= min(before, aim);
-    u64 w[EACH], own = 0;
-    parts(draw_begin + g * PART, min(draw_end, draw_begin + (g + 1) * PART), [&](int at) TMC_INLINE {
+    aim -= before;
+    u64 w[EACH], own = 0, part;
+    parts(g * PART, min(p.vocab, (g + 1) * PART), [&](int at) TMC_INLINE {
 #pragma unroll
       for (int i = 0; i < EACH; ++i) own += w[i] = weight(v[i], place(at, i));
     });
-    block_scan<THREADS>(own, s, before, all);
-    // (the last that is kept where sums of several blocks fall short)
+    block_scan<THREADS>(own, s, before, part);
     const int index = find_in<THREADS, true>(w, before, aim, before, s);
     if (index < 0) return false;
 #pragma unroll
     for (int i = 0; i < EACH; ++i)
-      if ((int)threadIdx.x * EACH + i == index)
-        say(draw_begin + g * PART + index, (double)w[i] * (1.0 / kUnit) / total);
+      if ((int)threadIdx.x * EACH + i == index) say(g * PART + index, (double)w[i] / (double)all);
     return true;
   };
   if (!by_bins()) row_by_digits<T, THREADS>(p, row, set, s);
@@ -1042,7 +1000,7 @@ bool sample_shape(int64_t rows, int64_t vocabulary) {
 // How rows are shared out: a block a row, or, where rows are few, blocks of 4096 tokens, up
 // to kFill of them together.
 constexpr int kThreads = 256, kEach = 8;
-constexpr int64_t kFill = 2048, kFewRows = 192;
+constexpr int64_t kFill = 1024, kFewRows = 192;
 static_assert(kFewRows <= kSharedRows, "every shared row has its counter");
 static_assert(kMostTokens / (kThreads * kEach) <= kMostGroups, "a sum a part");
 struct SamplePlan {
@@ -1067,10 +1025,11 @@ using namespace tmc;
 
 extern "C" size_t tmc_sample_workspace_bytes(int64_t rows, int64_t vocabulary) {
   if (!sample_shape(rows, vocabulary)) return 0;
-  const int64_t count = sample_plan(rows, vocabulary).count;
-  return count == 1 ? 0
-                    : kCounterBytes + (size_t)(rows * count) *
-                                          (sizeof(SampleRecord) + kBins * sizeof(u64));
+  const SamplePlan plan = sample_plan(rows, vocabulary);
+  const size_t block = sizeof(u64) * (1 + plan.walk) + sizeof(float) * kBins;
+  return plan.count == 1 ? 0
+                         : kCounterBytes + (size_t)rows * (sizeof(SampleRow) + plan.count * block +
+                                                           kMostKept * sizeof(u64));
 }
 
 extern "C" int tmc_sample(const void* logits, int dtype, int64_t row_stride,
@@ -1110,14 +1069,22 @@ extern "C" int tmc_sample(const void* logits, int dtype, int64_t row_stride,
   p.count = plan.count;
   if (need) {
     p.arrivals = static_cast<int*>(workspace);
-    p.parts = reinterpret_cast<SampleRecord*>(static_cast<char*>(workspace) + kCounterBytes);
-    p.bins = reinterpret_cast<u64*>(p.parts + rows * plan.count);
+    p.records = reinterpret_cast<SampleRow*>(static_cast<char*>(workspace) + kCounterBytes);
+    p.lists = reinterpret_cast<u64*>(p.records + rows);
+    p.blocks = p.lists + rows * kMostKept;
+    p.sums = p.blocks + rows * plan.count;
+    p.bins = reinterpret_cast<float*>(p.sums + rows * plan.count * plan.walk);
   }
-  auto kernel = plan.count > 1 ? (dtype == TMC_F32 ? sample_kernel<float, kThreads, kEach, true>
-                                                   : sample_kernel<half_t, kThreads, kEach, true>)
-                               : (dtype == TMC_F32 ? sample_kernel<float, kThreads, kEach, false>
-                                                   : sample_kernel<half_t, kThreads, kEach, false>);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * plan.count)), dim3(kThreads), 0,
-                     as_stream(stream), p);
+  const bool full = dtype == TMC_F32;
+  auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * plan.count)), dim3(kThreads), 0,
+                       as_stream(stream), p);
+  };
+  if (plan.count == 1) {
+    launch(full ? sample_kernel<float, kThreads, kEach, 0> : sample_kernel<half_t, kThreads, kEach, 0>);
+  } else {
+    launch(full ? sample_kernel<float, kThreads, kEach, 1> : sample_kernel<half_t, kThreads, kEach, 1>);
+    launch(full ? sample_kernel<float, kThreads, kEach, 2> : sample_kernel<half_t, kThreads, kEach, 2>);
+  }
   return check_launch("sample_kernel");
 }
