@@ -409,10 +409,11 @@ __device__ __forceinline__ int find_in(const TYPE (&v)[EACH], TYPE base, TYPE ta
   return found;
 }
 
-// The key of the list s.keys[0 ... n), all in [low, high], at which the running cost, from the highest ranked
-// down, reaches `target` (at least 1); 0 where all of it does not.  `cost` gives that of
-// a key.  The list's range of keys is cut into 256, then that of the part with the
-// target, until a wave can take the rest: for logits that are not equal, once.
+// The key of the list s.keys[0 ... n), all in [low, high], at which the running cost, from
+// the highest ranked down, reaches `target` (at least 1); 0 where all of it does not.
+// `cost` gives that of a key.  The list's range of keys is cut into 256, then that of the
+// part with the target, until a wave can take the rest: for logits that are not equal,
+// once or twice.
 template <int THREADS, typename COST>
 __device__ __forceinline__ u64 select_key(int n, u64 low, u64 high, u64 target,
                                           SampleScratch<THREADS>& s, const COST& cost) {
@@ -683,7 +684,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
   float low = 0.0f, high = 0.0f;  // the list's logits: from low on, below high
   // The sums of the block's parts: of the tokens from the logit `high` on (all, where none
   // are listed) that min-p keeps; those from `low` on and below `high` into the list.
-  // Returns the sum of all tokens' weights, of this thread.
+  // Returns the sum of all tokens' weights, of this thread (0 where none are listed).
   u64* groups = s.groups;
   auto sum_groups = [&](auto lists) TMC_INLINE -> u64 {
     u64 all = 0;
@@ -695,7 +696,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
       for (int i = 0; i < EACH; ++i) {
         const double a = octaves(v[i]);
         const u64 w = a >= kFaintest ? integer(a) : 0;
-        all += w;
+        if (lists) all += w;
         if ((!lists || v[i] >= high) && a >= faintest) sum += w;
         if (lists) collect(v[i] >= low && v[i] < high, place(at, i));
       }
