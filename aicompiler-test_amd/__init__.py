@@ -214,6 +214,28 @@ def open_variant(name: str) -> C.CDLL:
 
 
 _host = None
+_tensors = None
+
+
+def _open_module(name):
+    import importlib.util
+    import sysconfig
+    lib()  # loads torch's HIP runtime and libtmc_hip.so first
+    path = os.path.join(HERE, name + sysconfig.get_config_var("EXT_SUFFIX"))
+    if not os.path.exists(path):
+        raise TmcError(f"{path} is missing; run aicompiler-test_amd/build.py")
+    spec = importlib.util.spec_from_file_location(name, path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    return mod
+
+
+def _open_tensors():
+    """The checks of torch tensors (_tmc_tensors, built next to this file)."""
+    global _tensors
+    if _tensors is None:
+        _tensors = _open_module("_tmc_tensors")
+    return _tensors
 
 
 def host():
@@ -221,16 +243,7 @@ def host():
     file).  torch is imported first so one HIP runtime serves the process."""
     global _host
     if _host is None:
-        import importlib.util
-        import sysconfig
-        lib()  # loads torch's HIP runtime and libtmc_hip.so first
-        path = os.path.join(HERE, "_tmc_host" + sysconfig.get_config_var("EXT_SUFFIX"))
-        if not os.path.exists(path):
-            raise TmcError(f"{path} is missing; run aicompiler-test_amd/build.py")
-        spec = importlib.util.spec_from_file_location("_tmc_host", path)
-        mod = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(mod)
-        _host = mod
+        _host = _open_module("_tmc_host")
     return _host
 
 
@@ -796,10 +809,10 @@ def _address(what, device, dtype, name, t, count):
     type, gaps between elements, fewer than `count` of them."""
     if t is None:
         return None
-    if t.get_device() != device or t.dtype is not dtype or not t.is_contiguous() or \
-            t.numel() < count:
+    address = (_tensors or _open_tensors()).address(t, device, dtype, count)
+    if address is False:
         _refuse(what, device, dtype, name, t, count)
-    return t.data_ptr()
+    return address
 
 
 def _workspace(what, device, t):
@@ -905,17 +918,20 @@ def page_moves(moves, pools, pool_pages, page_size):
 
 
 def _pool_list(torch, what, device, k_pools, v_pools):
-    """K pools and V pools in one list, and their type, after a refusal of what is
-    not on the current GPU, whole and of one type."""
-    pools, tensor, dtype = [*k_pools, *v_pools], torch.Tensor, k_pools[0].dtype
+    """Addresses of the K pools, then of the V pools, and the elements that the
+    least of them holds, after a refusal of what is not on the current GPU, whole
+    and of one type."""
+    pools, dtype = [*k_pools, *v_pools], k_pools[0].dtype
     if dtype not in (torch.float16, torch.bfloat16, torch.float32):
         raise TmcError(f"{what}: pools must be float16, bfloat16 or float32, not {dtype}")
-    if set(map(tensor.get_device, pools)) != {device} or \
-            not all(map(tensor.is_contiguous, pools)) or {t.dtype for t in pools} != {dtype}:
+    addresses = array.array("Q", bytes(8 * len(pools)))
+    least = (_tensors or _open_tensors()).addresses(pools, device, dtype, addresses)
+    if least is False:
         for i, t in enumerate(pools):
             if t.get_device() != device or t.dtype is not dtype or not t.is_contiguous():
                 _refuse(what, device, dtype, f"pool {i}", t, 0)
-    return pools, dtype
+        raise TmcError(f"{what}: pools must be strided tensors")
+    return addresses, least
 
 
 def move_pages(k_pools, v_pools, moves, heads, page_size, head_dim, page_stride=None,
@@ -936,12 +952,10 @@ def move_pages(k_pools, v_pools, moves, heads, page_size, head_dim, page_stride=
         raise TmcError(f"{what}: moves must be [count, 4]")
     device = torch.cuda.current_device()
     move_list = _address(what, device, torch.int32, "moves", moves, 0)
-    pools, _ = _pool_list(torch, what, device, k_pools, v_pools)
-    tensor = torch.Tensor
+    addresses, least = _pool_list(torch, what, device, k_pools, v_pools)
     if moves.shape[0] == 0:
         return
-    pool_pages = min(map(tensor.numel, pools)) // page_stride
-    addresses = array.array("Q", map(tensor.data_ptr, pools))
+    pool_pages = least // page_stride
     first, size = addresses.buffer_info()[0], addresses.itemsize
     check(lib().tmc_move_pages(first, first + count * size, count,
                                move_list, moves.shape[0], _dtype_code(k_pools[0]), pool_pages,
@@ -1182,9 +1196,8 @@ def tree_keep(k_pools, v_pools, tables, cached_lengths, path, accepted, heads, p
     if tables.dim() != 3 or tables.shape[0] != count or tables.shape[1] != batch:
         raise TmcError(f"{what}: tables must be [layers, batch, max_pages]")
     device, i32 = torch.cuda.current_device(), torch.int32
-    pools, dtype = _pool_list(torch, what, device, k_pools, v_pools)
-    pool_pages = min(map(torch.Tensor.numel, pools)) // page_stride
-    addresses = array.array("Q", map(torch.Tensor.data_ptr, pools))
+    addresses, least = _pool_list(torch, what, device, k_pools, v_pools)
+    pool_pages = least // page_stride
     first, size = addresses.buffer_info()[0], addresses.itemsize
     check(lib().tmc_tree_keep(
         first, first + count * size, count,

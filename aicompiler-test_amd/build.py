@@ -4,7 +4,8 @@
                   (the C ABI of include/tmc_hip.h);
   libtmc_host.so  the C++ host layer under host/ (HipRuntime, KV pools and
                   states, decoder executors, serving loop) over that ABI;
-  _tmc_host*.so   its Python module (pybind11), for tests and bench.py.
+  _tmc_host*.so   its Python module (pybind11), for tests and bench.py;
+  _tmc_tensors*.so  the Python wrappers' checks of torch tensors.
 
   libtmc_hip_merge_launch.so  the same ABI built with TMC_ATTN_MERGE_LAUNCH=1
                   (every split-attention merge in a launch of its own, no
@@ -14,7 +15,7 @@
                   tmc_attention_timeline; profiling.py timeline).
 
 Objects go under _build/ (git-ignored); the libraries land next to this file
-so they travel with the source tree to the GPU box.
+so they travel with the source tree.
 
 Usage: python aicompiler-test_amd/build.py
 """
@@ -63,10 +64,10 @@ FLAGS = [
 ]
 
 
-# Per-source additions.  prefill.hip, window.hip, tree_attention.hip: keep MFMA accumulators in VGPRs (the
-# online-softmax rescale multiplies them every block; from AGPRs each one is
-# a read, a multiply and a write back).
-SOURCE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"] 
+# Per-source additions.  prefill.hip, window.hip, tree_attention.hip: keep MFMA
+# accumulators in VGPRs (the online-softmax rescale multiplies them every block;
+# from AGPRs each one is a read, a multiply and a write back).
+SOURCE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"]
                 for name in ("prefill.hip", "window.hip", "tree_attention.hip")}
 
 
@@ -117,6 +118,20 @@ def _build_module() -> str:
     return out
 
 
+def _build_tensors() -> str:
+    import sysconfig
+    import torch
+    base = os.path.dirname(torch.__file__)
+    abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    out = os.path.join(HERE, "_tmc_tensors" + sysconfig.get_config_var("EXT_SUFFIX"))
+    _run([CXX, "-std=c++17", "-O2", "-fPIC", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+          f"-I{base}/include", f"-I{sysconfig.get_paths()['include']}", "-fvisibility=hidden",
+          "-shared", "-o", out + ".tmp", os.path.join(HOST, "tensors.cpp"), f"-L{base}/lib",
+          "-ltorch_python", "-ltorch_cpu", "-lc10"], "g++ tensors.cpp")
+    shutil.move(out + ".tmp", out)
+    return out
+
+
 def _link_hip(objs: list, out: str) -> None:
     tmp = out + ".tmp"
     cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", tmp, *objs, f"-L{ROCM_LIB}",
@@ -133,10 +148,12 @@ def build(jobs: int = 4) -> str:
         merge_launch = pool.submit(_compile, "attention.hip", "_merge_launch",
                                    ("-DTMC_ATTN_MERGE_LAUNCH=1",))
         timeline = pool.submit(_compile, "attention.hip", "_timeline", ("-DTMC_ATTN_TIMELINE=1",))
+        tensors = pool.submit(_build_tensors)
         objs = list(pool.map(_compile, SOURCES))
         host_objs = list(pool.map(_compile_host, HOST_SOURCES))
         merge_launch_obj = merge_launch.result()
         timeline_obj = timeline.result()
+        tensors.result()
     _link_hip(objs, OUT)
     attention = os.path.join(BUILD, "attention.o")
     _link_hip([merge_launch_obj if o == attention else o for o in objs], MERGE_LAUNCH_OUT)

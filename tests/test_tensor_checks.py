@@ -1,0 +1,59 @@
+"""The native checks of tensors behind the Python wrappers (host/tensors.cpp)."""
+import array
+import importlib
+
+import pytest
+import torch
+
+tmc = importlib.import_module("aicompiler-test_amd")
+HOST = -1  # the device number of host tensors
+
+
+@pytest.fixture(scope="module")
+def checks():
+    return tmc._open_tensors()
+
+
+def test_address(checks):
+    x = torch.zeros(4, 6)
+    assert checks.address(x, HOST, torch.float32, 24) == x.data_ptr()
+    assert checks.address(x[1:], HOST, torch.float32, 18) == x.data_ptr() + 24
+    assert checks.address(torch.zeros(0), HOST, torch.float32, 0) == 0
+
+
+@pytest.mark.parametrize("t, device, dtype, count", [
+    (torch.zeros(4), HOST, torch.float32, 5),
+    (torch.zeros(4), 0, torch.float32, 1),
+    (torch.zeros(4), HOST, torch.float16, 1),
+    (torch.zeros(4, 4).t(), HOST, torch.float32, 1),
+    (torch.zeros(8)[::2], HOST, torch.float32, 1),
+    (torch.zeros(4).expand(2, 4), HOST, torch.float32, 1),
+    (torch.zeros(4).to_sparse(), HOST, torch.float32, 1),
+])
+def test_address_refuses(checks, t, device, dtype, count):
+    assert checks.address(t, device, dtype, count) is False
+
+
+@pytest.mark.parametrize("args", [
+    (), (torch.zeros(1),), (3, HOST, torch.float32, 1), (None, HOST, torch.float32, 1),
+    (torch.zeros(1), HOST, "float32", 1), (torch.zeros(1), "0", torch.float32, 1),
+    (torch.zeros(1), HOST, torch.float32, None)])
+def test_address_of_other_objects(checks, args):
+    with pytest.raises(TypeError):
+        checks.address(*args)
+
+
+def test_addresses(checks):
+    pools = [torch.zeros(n, dtype=torch.float16) for n in (7, 5, 9)]
+    words = array.array("Q", bytes(24))
+    assert checks.addresses(pools, HOST, torch.float16, words) == 5
+    assert list(words) == [t.data_ptr() for t in pools]
+    assert checks.addresses(pools + pools[:0], 0, torch.float16, words) is False
+    assert checks.addresses(pools, HOST, torch.float32, words) is False
+    assert checks.addresses([pools[0], None], HOST, torch.float16, words) is False
+    assert checks.addresses([pools[0], pools[1][::2]], HOST, torch.float16, words) is False
+    for bad in ((pools * 2, HOST, torch.float16, words), (tuple(pools), HOST, torch.float16, words)):
+        with pytest.raises(TypeError):
+            checks.addresses(*bad)
+    with pytest.raises((TypeError, BufferError)):
+        checks.addresses(pools, HOST, torch.float16, bytes(24))
