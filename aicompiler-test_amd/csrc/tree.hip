@@ -72,6 +72,7 @@ struct TreeAppend {
   const int32_t* active;    // or null
   int batch, nodes, q_heads, kv_heads, head_dim, page_size, max_pages, pool_pages;
   long positions;
+  PageDivide by_row, by_nodes, by_head, by_page;  // by a row's units, and so on
 };
 
 // EACH adjacent elements of one head a thread: 8 in 16-byte loads and stores, else
@@ -83,12 +84,10 @@ __global__ __launch_bounds__(256) void tree_append_kernel(const T* __restrict__ 
                                                           T* __restrict__ v_pool, TreeAppend p) {
   typedef T vec __attribute__((ext_vector_type(EACH)));
   const int width = (p.q_heads + 2 * p.kv_heads) * p.head_dim;
-  const unsigned row_units = (unsigned)(width / EACH);
-  const unsigned id = blockIdx.x * 256u + threadIdx.x;
-  const unsigned node = id / row_units;
-  if (node >= (unsigned)(p.batch * p.nodes)) return;
-  const int request = (int)(node / (unsigned)p.nodes), i = (int)node - request * p.nodes;
-  const int column = EACH * (int)(id - node * row_units);
+  const int id = (int)(blockIdx.x * 256u + threadIdx.x), node = p.by_row(id);
+  if (node >= p.batch * p.nodes) return;
+  const int request = p.by_nodes(node), i = node - request * p.nodes;
+  const int column = EACH * id - node * width;
   // everything that depends on nothing, in flight at once
   const int active = p.active ? p.active[0] : p.batch;
   const int cached = p.cached[request], depth = p.depths[node];
@@ -101,12 +100,15 @@ __global__ __launch_bounds__(256) void tree_append_kernel(const T* __restrict__ 
   const int q_width = p.q_heads * p.head_dim, kv_width = p.kv_heads * p.head_dim;
   vec y = x;
   if (column < q_width + kv_width) {
-    const size_t at = (size_t)position * (p.head_dim / 2) + column % p.head_dim / 2;
+    const int feature = column - p.by_head(column) * p.head_dim;
+    const size_t at = (size_t)position * (p.head_dim / 2) + feature / 2;
+    typedef float angles __attribute__((ext_vector_type(EACH / 2), aligned(4)));
+    const angles cosine = *reinterpret_cast<const angles*>(p.cosine + at);
+    const angles sine = *reinterpret_cast<const angles*>(p.sine + at);
 #pragma unroll
     for (int e = 0; e < EACH; e += 2) {
       float even, odd;
-      rotate_pair(to_float<T>(x[e]), to_float<T>(x[e + 1]), p.cosine[at + e / 2],
-                  p.sine[at + e / 2], even, odd);
+      rotate_pair(to_float<T>(x[e]), to_float<T>(x[e + 1]), cosine[e / 2], sine[e / 2], even, odd);
       // fp32 first, then the storage type, as the other rotations round
       asm volatile("" : "+v"(even), "+v"(odd));
       y[e] = from_float<T>(even);
@@ -117,11 +119,11 @@ __global__ __launch_bounds__(256) void tree_append_kernel(const T* __restrict__ 
     *reinterpret_cast<vec*>(q_out + (size_t)node * q_width + column) = y;
     return;
   }
-  const int index = (int)slot / p.page_size;
+  const int index = p.by_page((int)slot);
   const int page = p.tables[(size_t)request * p.max_pages + index];
   if (page < 0 || page >= p.pool_pages) return;
   const bool key = column < q_width + kv_width;
-  const int feature = column - q_width - (key ? 0 : kv_width), head = feature / p.head_dim;
+  const int feature = column - q_width - (key ? 0 : kv_width), head = p.by_head(feature);
   *reinterpret_cast<vec*>((key ? k_pool : v_pool) +
                           (((size_t)page * p.kv_heads + head) * p.page_size +
                            ((int)slot - index * p.page_size)) * p.head_dim +
@@ -200,6 +202,7 @@ __global__ __launch_bounds__(kWave) void tree_accept_kernel(TreeAccept p) {
 // the first with path[s] != s have nothing to move.  A thread owns a unit of a
 // (layer, K or V, head) and takes the steps in order, kKeepAhead loads before
 // their stores, so that nobody else is waited for.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kKeepPools = 128;  // pool pairs per launch (kernel arguments)
 constexpr int kKeepAhead = 8, kKeepThreads = 128;
 
@@ -212,13 +215,14 @@ struct TreeKeep {
   const int32_t* accepted;  // [batch]
   int batch, nodes, heads, page_size, max_pages, pool_pages, row_units;
   long page_stride, head_stride;  // units
+  PageDivide by_row, by_page;
 };
 
 template <typename UNIT>
 __global__ __launch_bounds__(kKeepThreads) void tree_keep_kernel(TreeKeep p) {
   const int request = blockIdx.x, pool = blockIdx.y;
   const int column = (int)(blockIdx.z >> 1) * kKeepThreads + threadIdx.x;
-  const int head = column / p.row_units;
+  const int head = p.by_row(column);
   const int32_t* path = p.path + (size_t)request * p.nodes;
   const int taken = min(p.accepted[request], p.nodes), cached = p.cached[request];
   if (head >= p.heads || cached < 0) return;
@@ -226,35 +230,40 @@ __global__ __launch_bounds__(kKeepThreads) void tree_keep_kernel(TreeKeep p) {
   const long capacity = (long)p.page_size * p.max_pages;
   UNIT* base = static_cast<UNIT*>(blockIdx.z & 1 ? p.value[pool] : p.key[pool]) +
                (size_t)head * p.head_stride + (column - head * p.row_units);
-  auto place = [&](int node) -> UNIT* {
-    const long slot = (long)cached + node;
-    if (slot >= capacity) return nullptr;
-    const int index = (int)slot / p.page_size, page = table[index];
-    if (page < 0 || page >= p.pool_pages) return nullptr;
-    return base + (size_t)page * p.page_stride +
-           (size_t)((int)slot - index * p.page_size) * p.row_units;
-  };
   int last = -1;  // node of the step before
   for (int s0 = 0; s0 < taken; s0 += kKeepAhead) {
+    // (every load of a stage in flight at once: those of steps that move nothing from a
+    // place that is there)
+    int node[kKeepAhead], row[2][kKeepAhead], page[2][kKeepAhead];
+    bool moves[kKeepAhead];
     UNIT held[kKeepAhead];
-    UNIT* to[kKeepAhead];
+#pragma unroll
+    for (int a = 0; a < kKeepAhead; ++a) node[a] = path[min(s0 + a, p.nodes - 1)];
 #pragma unroll
     for (int a = 0; a < kKeepAhead; ++a) {
-      const int s = s0 + a, node = s < taken ? path[s] : -1;
-      to[a] = nullptr;
+      const int s = s0 + a;
       // (a list that does not increase ends where it does not)
-      if (node <= last || node >= p.nodes) last = p.nodes;
-      else last = node;
-      if (last == p.nodes || node == s) continue;
-      const UNIT* from = place(node);
-      UNIT* target = place(s);
-      if (!from || !target) continue;
-      held[a] = *from;
-      to[a] = target;
+      last = s < taken && node[a] > last && node[a] < p.nodes ? node[a] : p.nodes;
+      moves[a] = last != p.nodes && node[a] != s && (long)cached + node[a] < capacity;
+#pragma unroll
+      for (int side = 0; side < 2; ++side) {
+        const int slot = moves[a] ? cached + (side ? s : node[a]) : 0, index = p.by_page(slot);
+        row[side][a] = slot - index * p.page_size;
+        page[side][a] = table[index];
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < kKeepAhead; ++a) {
+#pragma unroll
+      for (int side = 0; side < 2; ++side)
+        moves[a] = moves[a] && page[side][a] >= 0 && page[side][a] < p.pool_pages;
+      held[a] = base[moves[a] ? (size_t)page[0][a] * p.page_stride + (size_t)row[0][a] * p.row_units
+                              : 0];
     }
 #pragma unroll
     for (int a = 0; a < kKeepAhead; ++a)
-      if (to[a]) *to[a] = held[a];
+      if (moves[a])
+        base[(size_t)page[1][a] * p.page_stride + (size_t)row[1][a] * p.row_units] = held[a];
   }
 }
 
@@ -307,9 +316,11 @@ extern "C" int tmc_tree_rope_append(const void* qkv, const float* cosine, const 
                          reinterpret_cast<uintptr_t>(key_pool) |
                          reinterpret_cast<uintptr_t>(value_pool);
   TMC_REQUIRE(bits % (2 * size) == 0, "Tree append: buffers must be aligned to two elements.");
+  const int each = dtype == TMC_F16 && head_dim % 8 == 0 && bits % 16 == 0 ? 8 : 2;
   TreeAppend p{cosine,     sine,         cached_lengths, depths,        counts,         block_tables,
                active_count, (int)batch, (int)nodes,     (int)q_heads,  (int)kv_heads,  (int)head_dim,
-               (int)page_size, (int)max_pages, (int)pool_pages, (long)positions};
+               (int)page_size, (int)max_pages, (int)pool_pages, (long)positions,
+               PageDivide::by(width / each), PageDivide::by(nodes), PageDivide::by(head_dim), PageDivide::by(page_size)};
 #define TMC_TREE_APPEND(TYPE, EACH)                                                             \
   hipLaunchKernelGGL((tree_append_kernel<TYPE, EACH>),                                          \
                      dim3((unsigned)((batch * nodes * (width / EACH) + 255) / 256)), dim3(256), \
@@ -317,7 +328,7 @@ extern "C" int tmc_tree_rope_append(const void* qkv, const float* cosine, const 
                      static_cast<TYPE*>(q_out), static_cast<TYPE*>(key_pool),                   \
                      static_cast<TYPE*>(value_pool), p)
   if (dtype == TMC_F32) TMC_TREE_APPEND(float, 2);
-  else if (head_dim % 8 == 0 && bits % 16 == 0) TMC_TREE_APPEND(half_t, 8);
+  else if (each == 8) TMC_TREE_APPEND(half_t, 8);
   else TMC_TREE_APPEND(half_t, 2);
 #undef TMC_TREE_APPEND
   return check_launch("tree_append_kernel");
@@ -393,12 +404,14 @@ extern "C" int tmc_tree_keep(void* const* key_pools, void* const* value_pools, i
     p.max_pages = (int)max_pages;
     p.pool_pages = (int)pool_pages;
     p.row_units = (int)(head_dim * size / unit);
+    p.by_row = PageDivide::by(p.row_units);
+    p.by_page = PageDivide::by(page_size);
     p.page_stride = (long)page_stride * size / unit;
     p.head_stride = (long)head_stride * size / unit;
     const dim3 grid((unsigned)batch, (unsigned)here, (unsigned)(2 * parts));
     const hipStream_t s = as_stream(stream);
     if (unit == 16)
-      hipLaunchKernelGGL((tree_keep_kernel<uint4>), grid, dim3(kKeepThreads), 0, s, p);
+      hipLaunchKernelGGL((tree_keep_kernel<u32x4>), grid, dim3(kKeepThreads), 0, s, p);
     else if (unit == 4)
       hipLaunchKernelGGL((tree_keep_kernel<uint32_t>), grid, dim3(kKeepThreads), 0, s, p);
     else
