@@ -200,7 +200,7 @@ __global__ __launch_bounds__(kWave) void tree_accept_kernel(TreeAccept p) {
 // Slot cached + path[s] to slot cached + s, for every step s.  Paths increase, so
 // path[s] >= s, no later step reads what an earlier one wrote, and steps before
 // the first with path[s] != s have nothing to move.  A thread owns a unit of a
-// (layer, K or V, head) and takes the steps in order, kKeepAhead loads before
+// (layer, head), of K and of V, and takes the steps in order, kKeepAhead loads before
 // their stores, so that nobody else is waited for.
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kKeepPools = 128;  // pool pairs per launch (kernel arguments)
@@ -221,22 +221,23 @@ struct TreeKeep {
 template <typename UNIT>
 __global__ __launch_bounds__(kKeepThreads) void tree_keep_kernel(TreeKeep p) {
   const int request = blockIdx.x, pool = blockIdx.y;
-  const int column = (int)(blockIdx.z >> 1) * kKeepThreads + threadIdx.x;
+  const int column = (int)blockIdx.z * kKeepThreads + threadIdx.x;
   const int head = p.by_row(column);
   const int32_t* path = p.path + (size_t)request * p.nodes;
   const int taken = min(p.accepted[request], p.nodes), cached = p.cached[request];
   if (head >= p.heads || cached < 0) return;
   const int32_t* table = p.tables + ((size_t)pool * p.batch + request) * p.max_pages;
   const long capacity = (long)p.page_size * p.max_pages;
-  UNIT* base = static_cast<UNIT*>(blockIdx.z & 1 ? p.value[pool] : p.key[pool]) +
-               (size_t)head * p.head_stride + (column - head * p.row_units);
+  const size_t own = (size_t)head * p.head_stride + (column - head * p.row_units);
+  UNIT* const base[2] = {static_cast<UNIT*>(p.key[pool]) + own,
+                         static_cast<UNIT*>(p.value[pool]) + own};
   int last = -1;  // node of the step before
   for (int s0 = 0; s0 < taken; s0 += kKeepAhead) {
     // (every load of a stage in flight at once: those of steps that move nothing from a
     // place that is there)
     int node[kKeepAhead], row[2][kKeepAhead], page[2][kKeepAhead];
     bool moves[kKeepAhead];
-    UNIT held[kKeepAhead];
+    UNIT held[2][kKeepAhead];
 #pragma unroll
     for (int a = 0; a < kKeepAhead; ++a) node[a] = path[min(s0 + a, p.nodes - 1)];
 #pragma unroll
@@ -257,13 +258,19 @@ __global__ __launch_bounds__(kKeepThreads) void tree_keep_kernel(TreeKeep p) {
 #pragma unroll
       for (int side = 0; side < 2; ++side)
         moves[a] = moves[a] && page[side][a] >= 0 && page[side][a] < p.pool_pages;
-      held[a] = base[moves[a] ? (size_t)page[0][a] * p.page_stride + (size_t)row[0][a] * p.row_units
-                              : 0];
+      const size_t from = moves[a] ? (size_t)page[0][a] * p.page_stride +
+                                         (size_t)row[0][a] * p.row_units
+                                   : 0;
+      held[0][a] = base[0][from];
+      held[1][a] = base[1][from];
     }
 #pragma unroll
-    for (int a = 0; a < kKeepAhead; ++a)
-      if (moves[a])
-        base[(size_t)page[1][a] * p.page_stride + (size_t)row[1][a] * p.row_units] = held[a];
+    for (int a = 0; a < kKeepAhead; ++a) {
+      if (!moves[a]) continue;
+      const size_t to = (size_t)page[1][a] * p.page_stride + (size_t)row[1][a] * p.row_units;
+      base[0][to] = held[0][a];
+      base[1][to] = held[1][a];
+    }
   }
 }
 
@@ -385,7 +392,7 @@ extern "C" int tmc_tree_keep(void* const* key_pools, void* const* value_pools, i
   const int unit = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 2;
   const int64_t columns = heads * head_dim * size / unit;
   const int64_t parts = (columns + kKeepThreads - 1) / kKeepThreads;
-  TMC_REQUIRE(2 * parts < 65536, "Tree keep: too many heads.");
+  TMC_REQUIRE(parts < 65536, "Tree keep: too many heads.");
   for (int64_t first = 0; first < pools; first += kKeepPools) {
     const int here = (int)std::min<int64_t>(kKeepPools, pools - first);
     TreeKeep p{};
@@ -408,7 +415,7 @@ extern "C" int tmc_tree_keep(void* const* key_pools, void* const* value_pools, i
     p.by_page = PageDivide::by(page_size);
     p.page_stride = (long)page_stride * size / unit;
     p.head_stride = (long)head_stride * size / unit;
-    const dim3 grid((unsigned)batch, (unsigned)here, (unsigned)(2 * parts));
+    const dim3 grid((unsigned)batch, (unsigned)here, (unsigned)parts);
     const hipStream_t s = as_stream(stream);
     if (unit == 16)
       hipLaunchKernelGGL((tree_keep_kernel<u32x4>), grid, dim3(kKeepThreads), 0, s, p);
