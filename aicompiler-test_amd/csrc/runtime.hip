@@ -1162,6 +1162,170 @@ bool make_spec(const std::string& name, const Params& p, KernelSpec& s) {
     };
     return true;
   }
+  if (name == "tree_layout") {
+    // Inputs the parents (, counts with counts=1); outputs masks and depths.
+    const int64_t b = param_int(p, "batch"), n = param_int(p, "nodes");
+    const bool counts = param_int(p, "counts", 0) != 0;
+    NEED(b > 0 && n > 0, "tree_layout needs batch and nodes.");
+    s.inputs.assign(counts ? 2 : 1, TMC_I32);
+    s.outputs = {TMC_I32, TMC_I32};
+    s.counts = {(size_t)(b * n)};
+    if (counts) s.counts.push_back((size_t)b);
+    s.counts.insert(s.counts.end(), {(size_t)(b * n * ((n + 31) / 32)), (size_t)(b * n)});
+    const int o = counts ? 2 : 1;
+    s.launch = [=](const LaunchContext& c) {
+      return tmc_tree_layout(static_cast<const int32_t*>(c.ptrs[0]),
+                             counts ? static_cast<const int32_t*>(c.ptrs[1]) : nullptr,
+                             static_cast<uint32_t*>(c.ptrs[o]),
+                             static_cast<int32_t*>(c.ptrs[o + 1]), b, n, c.stream);
+    };
+    return true;
+  }
+  if (name == "tree_rope_append" || name == "tree_attention") {
+    // Inputs qkv, cosine, sine, cached lengths, depths, or q, the pools, cached lengths, masks;
+    // then tables, active (, counts with counts=1); outputs q and the pools, or the result.
+    const bool append = name == "tree_rope_append";
+    const int64_t b = param_int(p, "batch"), n = param_int(p, "nodes"),
+                  qh = param_int(p, "q_heads"), kvh = param_int(p, "kv_heads", qh),
+                  d = param_int(p, "head_dim"), ps = param_int(p, "page_size"),
+                  mp = param_int(p, "max_pages"), positions = param_int(p, "positions", 0);
+    const bool counts = param_int(p, "counts", 0) != 0;
+    NEED(b > 0 && n > 0 && qh > 0 && kvh > 0 && d > 0 && ps > 0 && mp > 0,
+         name + " needs batch, nodes, q_heads, head_dim, page_size and max_pages.");
+    NEED(append ? positions > 0 : dt == TMC_F16,
+         append ? "tree_rope_append needs positions." : "tree_attention needs dtype=f16.");
+    const int64_t head_stride = append ? ps * d : param_int(p, "head_stride", ps * d);
+    const int64_t page_stride = append ? kvh * ps * d : param_int(p, "page_stride", kvh * ps * d);
+    NEED(page_stride > 0, name + ": page_stride must be positive.");
+    const size_t rows = (size_t)(b * n), tables = (size_t)(b * mp);
+    if (append) {
+      s.inputs = {dt, TMC_F32, TMC_F32, TMC_I32, TMC_I32, TMC_I32, TMC_I32};
+      s.outputs = {dt, dt, dt};
+      const size_t angles = (size_t)(positions * (d / 2));
+      s.counts = {rows * (size_t)((qh + 2 * kvh) * d), angles, angles, (size_t)b, rows, tables, 1};
+    } else {
+      s.inputs = {dt, dt, dt, TMC_I32, TMC_I32, TMC_I32, TMC_I32};
+      s.outputs = {dt};
+      s.counts = {rows * (size_t)(qh * d), 0, 0, (size_t)b, rows * (size_t)((n + 31) / 32), tables,
+                  1};
+      s.workspace_bytes = tmc_tree_attention_workspace_bytes(b, n, qh, kvh, d, ps * mp);
+    }
+    if (counts) {
+      s.inputs.push_back(TMC_I32);
+      s.counts.push_back((size_t)b);
+    }
+    s.counts.push_back(rows * (size_t)(qh * d));
+    if (append) s.counts.insert(s.counts.end(), 2, 0);
+    const int o = counts ? 8 : 7, pool = append ? o + 1 : 1;  // the first output, the K pool
+    s.launch = [=](const LaunchContext& c) {
+      const auto i32 = [&](int i) { return static_cast<const int32_t*>(c.ptrs[i]); };
+      const int64_t pool_pages =
+          (int64_t)(std::min(c.counts[pool], c.counts[pool + 1]) / (size_t)page_stride);
+      const int32_t* count = counts ? i32(7) : nullptr;
+      if (append)
+        return tmc_tree_rope_append(c.ptrs[0], static_cast<const float*>(c.ptrs[1]),
+                                    static_cast<const float*>(c.ptrs[2]), positions, i32(3),
+                                    i32(4), count, i32(5), i32(6), c.ptrs[o], c.ptrs[o + 1],
+                                    c.ptrs[o + 2], dt, b, n, qh, kvh, d, ps, mp, pool_pages,
+                                    c.stream);
+      return tmc_tree_attention(c.ptrs[0], c.ptrs[1], c.ptrs[2], i32(3),
+                                static_cast<const uint32_t*>(c.ptrs[4]), count, i32(5), i32(6),
+                                c.ptrs[o], dt, b, n, qh, kvh, d, ps, mp, pool_pages, page_stride,
+                                head_stride, c.workspace, c.workspace_bytes, c.stream);
+    };
+    return true;
+  }
+  if (name == "sample") {
+    // Inputs logits, uniforms (, temperature) (, top_k) (, top_p) (, min_p), each with its
+    // name=1; outputs tokens and their probabilities.
+    const int64_t rows = param_int(p, "rows"), v = param_int(p, "vocab");
+    const int type = param_dtype(p, "dtype", TMC_F32);
+    const bool heat = param_int(p, "temperature", 0) != 0, most = param_int(p, "top_k", 0) != 0,
+               share = param_int(p, "top_p", 0) != 0, least = param_int(p, "min_p", 0) != 0;
+    NEED(rows > 0 && v > 0 && (type == TMC_F32 || type == TMC_F16),
+         "sample needs rows, vocab and dtype f32|f16.");
+    s.inputs = {type, TMC_F32};
+    if (heat) s.inputs.push_back(TMC_F32);
+    if (most) s.inputs.push_back(TMC_I32);
+    if (share) s.inputs.push_back(TMC_F32);
+    if (least) s.inputs.push_back(TMC_F32);
+    s.outputs = {TMC_I32, TMC_F32};
+    s.counts.assign(s.inputs.size() + 2, (size_t)rows);
+    s.counts[0] = (size_t)(rows * v);
+    s.workspace_bytes = tmc_sample_workspace_bytes(rows, v);
+    s.groups = (size_t)rows;
+    s.launch = [=](const LaunchContext& c) {
+      int next = 2;
+      const auto take = [&](bool here) { return here ? c.ptrs[next++] : nullptr; };
+      const float* t = static_cast<const float*>(take(heat));
+      const int32_t* k = static_cast<const int32_t*>(take(most));
+      const float* top = static_cast<const float*>(take(share));
+      const float* low = static_cast<const float*>(take(least));
+      int32_t* tokens = static_cast<int32_t*>(take(true));
+      return tmc_sample(c.ptrs[0], type, v, t, k, top, low, static_cast<const float*>(c.ptrs[1]),
+                        tokens, static_cast<float*>(take(true)), rows, v, c.workspace,
+                        c.workspace_bytes, c.stream);
+    };
+    return true;
+  }
+  if (name == "tree_accept") {
+    // Inputs drafted, parents and chosen tokens, active (, counts with counts=1) (, cached
+    // lengths with lengths=1); outputs path, accepted, emitted (, new lengths).
+    const int64_t b = param_int(p, "batch"), n = param_int(p, "nodes");
+    const bool counts = param_int(p, "counts", 0) != 0, lengths = param_int(p, "lengths", 0) != 0;
+    NEED(b > 0 && n > 0, "tree_accept needs batch and nodes.");
+    const size_t rows = (size_t)(b * n);
+    s.counts = {rows, rows, rows, 1};
+    if (counts) s.counts.push_back((size_t)b);
+    if (lengths) s.counts.push_back((size_t)b);
+    s.inputs.assign(s.counts.size(), TMC_I32);
+    s.outputs.assign(lengths ? 4 : 3, TMC_I32);
+    s.counts.insert(s.counts.end(), {rows, (size_t)b, rows});
+    if (lengths) s.counts.push_back((size_t)b);
+    s.launch = [=](const LaunchContext& c) {
+      int next = 0;
+      const auto take = [&](bool here) {
+        return here ? static_cast<int32_t*>(c.ptrs[next++]) : nullptr;
+      };
+      const int32_t *drafted = take(true), *parents = take(true), *chosen = take(true),
+                    *active = take(true), *count = take(counts), *cached = take(lengths);
+      int32_t *path = take(true), *accepted = take(true), *emitted = take(true),
+              *longer = take(lengths);
+      return tmc_tree_accept(drafted, parents, chosen, count, active, cached, path, accepted,
+                             emitted, longer, b, n, c.stream);
+    };
+    return true;
+  }
+  if (name == "tree_keep") {
+    // Inputs tables [pools, batch, max_pages], cached lengths, path, accepted; outputs the K
+    // pools, then the V pools.
+    const int64_t b = param_int(p, "batch"), n = param_int(p, "nodes"),
+                  pools = param_int(p, "pools", 1), h = param_int(p, "heads"),
+                  d = param_int(p, "head_dim"), ps = param_int(p, "page_size"),
+                  mp = param_int(p, "max_pages");
+    NEED(b > 0 && n > 0 && h > 0 && d > 0 && ps > 0 && mp > 0,
+         "tree_keep needs batch, nodes, heads, head_dim, page_size and max_pages.");
+    NEED(pools > 0 && pools <= 14, "tree_keep: 1 to 14 pools (32 bindings).");
+    const int64_t head_stride = param_int(p, "head_stride", ps * d);
+    const int64_t page_stride = param_int(p, "page_stride", h * ps * d);
+    NEED(page_stride > 0, "tree_keep: page_stride must be positive.");
+    s.inputs.assign(4, TMC_I32);
+    s.outputs.assign((size_t)(2 * pools), dt);
+    s.counts.assign((size_t)(4 + 2 * pools), 0);
+    s.counts[0] = (size_t)(pools * b * mp);
+    s.counts[1] = s.counts[3] = (size_t)b;
+    s.counts[2] = (size_t)(b * n);
+    s.launch = [=](const LaunchContext& c) {
+      size_t least = c.counts[4];
+      for (int64_t i = 5; i < 4 + 2 * pools; ++i) least = std::min(least, c.counts[i]);
+      const auto i32 = [&](int i) { return static_cast<const int32_t*>(c.ptrs[i]); };
+      return tmc_tree_keep(c.ptrs.data() + 4, c.ptrs.data() + 4 + pools, pools, i32(0), i32(1),
+                           i32(2), i32(3), dt, b, n, h, d, ps, mp,
+                           (int64_t)(least / (size_t)page_stride), page_stride, head_stride,
+                           c.stream);
+    };
+    return true;
+  }
   if (name == "argmax") {
     const int64_t rows = param_int(p, "rows"), v = param_int(p, "vocab");
     NEED(rows > 0 && v > 0, "argmax needs rows and vocab.");

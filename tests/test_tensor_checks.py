@@ -1,16 +1,14 @@
 """The native checks of tensors behind the Python wrappers (host/tensors.cpp)."""
 import array
-import importlib
 
 import pytest
 import torch
 
-tmc = importlib.import_module("aicompiler-test_amd")
 HOST = -1  # the device number of host tensors
 
 
 @pytest.fixture(scope="module")
-def checks():
+def checks(tmc):
     return tmc._open_tensors()
 
 
