@@ -267,10 +267,15 @@ def _stream(stream=None):
     return C.c_void_p(s.cuda_stream)
 
 
+_codes = {}
+
+
 def _dtype_code(t) -> int:
-    import torch
-    return {torch.float16: F16, torch.float32: F32, torch.bfloat16: BF16,
-            torch.int32: I32}[t.dtype]
+    if not _codes:
+        import torch
+        _codes.update({torch.float16: F16, torch.float32: F32, torch.bfloat16: BF16,
+                       torch.int32: I32})
+    return _codes[t.dtype]
 
 
 def gemv(x, w, y, stream=None):

@@ -1001,7 +1001,7 @@ bool sample_shape(int64_t rows, int64_t vocabulary) {
 // How rows are shared out: a block a row, or, where rows are few, blocks of 4096 tokens, up
 // to kFill of them together.
 constexpr int kThreads = 256, kEach = 8;
-constexpr int64_t kFill = 1024, kFewRows = 192;
+constexpr int64_t kFill = 1024, kFewRows = 512;
 static_assert(kFewRows <= kSharedRows, "every shared row has its counter");
 static_assert(kMostTokens / (kThreads * kEach) <= kMostGroups, "a sum a part");
 struct SamplePlan {
