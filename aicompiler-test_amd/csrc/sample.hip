@@ -189,134 +189,6 @@ __device__ __forceinline__ double exp2_of(double a) {
   return ldexp(s, (int)n);
 }
 
-// ------------------------------------------------------------ any row
-// The key at which the running cost, from the highest ranked down, reaches
-// `target` (at least 1 and at most all of it): digit by digit, a histogram of the
-// costs of the keys that agree so far.
-template <int THREADS, typename EACH>
-__device__ __forceinline__ u64 cut_at(u64 target, SampleScratch<THREADS>& s, const EACH& each) {
-  u64 prefix = 0;
-  for (int shift = 56; shift >= 0; shift -= 8) {
-    __syncthreads();
-    for (int d = threadIdx.x; d < kDigits; d += THREADS) s.hist[d] = 0;
-    __syncthreads();
-    each([&](u64 key, u64 cost) TMC_INLINE {
-      if (shift == 56 || key >> (shift + 8) == prefix >> (shift + 8))
-        atomicAdd(&s.hist[key >> shift & 255], cost);
-    });
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      u64 above = 0;
-      int d = kDigits - 1;
-      while (d > 0 && above + s.hist[d] < target) above += s.hist[d--];
-      s.found64 = d;
-      s.below = target - above;
-    }
-    __syncthreads();
-    prefix |= s.found64 << shift;
-    target = s.below;
-  }
-  return prefix;
-}
-
-// A row by one block, whatever it holds, pass after pass over memory: weights as
-// integers, cuts by their digits.  20 to 40 us a pass of a row of 32000, 5 to 25
-// passes.
-template <typename T, int THREADS>
-__device__ __forceinline__ void row_by_digits(const SampleParams& p, int row, const Settings& set,
-                              SampleScratch<THREADS>& s) {
-  const T* x = static_cast<const T*>(p.logits) + (size_t)row * p.stride;
-  // ---- the most probable token
-  u64 best = 0;
-  for (int i = threadIdx.x; i < p.vocab; i += THREADS) {
-    const float v = (float)x[i];
-    if (v == v) best = max(best, rank_key(v, i));
-  }
-  best = block_max_u64<THREADS>(best, s);
-  const float top = key_value(best);
-  if (set.heat == 0.0 || best == 0 || top == -INFINITY) {
-    if (threadIdx.x == 0) {
-      p.tokens[row] = best ? key_index(best) : -1;
-      if (p.probability)
-        p.probability[row] = set.heat == 0.0 && best ? 1.0f : __builtin_nanf("");
-    }
-    return;
-  }
-  const double unit = ldexp(1.0, p.scale);
-  auto weight = [&](float v) TMC_INLINE -> u64 {
-    if (v == top) return (u64)unit;
-    if (!(v > -INFINITY) || top == INFINITY) return 0;
-    const double a = ((double)v - (double)top) * set.heat;
-    return a >= kFaintest ? max((u64)rint(exp2_of(a) * unit), (u64)1) : 0;
-  };
-  u64 cut = 0;
-  auto kept = [&](float v, int i) TMC_INLINE -> u64 {
-    const u64 w = weight(v);
-    return w && rank_key(v, i) >= cut ? w : 0;
-  };
-  if (set.most < p.vocab) {
-    auto each = [&](auto&& take) TMC_INLINE {
-      for (int i = threadIdx.x; i < p.vocab; i += THREADS) {
-        const float v = (float)x[i];
-        if (weight(v)) take(rank_key(v, i), 1);
-      }
-    };
-    u64 count = 0;
-    each([&](u64, u64 one) TMC_INLINE { count += one; });
-    if (block_sum_u64<THREADS>(count, s) > (u64)set.most) cut = cut_at<THREADS>((u64)set.most, s, each);
-  }
-  if (set.share < 1.0f) {
-    auto each = [&](auto&& take) TMC_INLINE {
-      for (int i = threadIdx.x; i < p.vocab; i += THREADS) {
-        const float v = (float)x[i];
-        if (const u64 w = kept(v, i)) take(rank_key(v, i), w);
-      }
-    };
-    u64 sum = 0;
-    each([&](u64, u64 w) TMC_INLINE { sum += w; });
-    sum = block_sum_u64<THREADS>(sum, s);
-    const u64 target = max((u64)1, min(sum, (u64)ceil((double)set.share * (double)sum)));
-    cut = max(cut, cut_at<THREADS>(target, s, each));
-  }
-  auto final_weight = [&](int i) TMC_INLINE -> u64 {
-    const float v = (float)x[i];
-    if (v != top && !(((double)v - (double)top) * set.heat >= set.least)) return 0;
-    return kept(v, i);
-  };
-  u64 sum = 0;
-  for (int i = threadIdx.x; i < p.vocab; i += THREADS) sum += final_weight(i);
-  sum = block_sum_u64<THREADS>(sum, s);
-  const u64 target = min(sum - 1, (u64)(set.uniform * (double)sum));
-  // ---- the first kept token at which the running sum passes the target
-  u64 before = 0;
-  for (int at = 0;; at += THREADS) {
-    const int i = at + threadIdx.x, lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    const u64 w = i < p.vocab ? final_weight(i) : 0;
-    u64 run = w;
-#pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) {
-      const u64 other = __shfl_up(run, off, kWave);
-      if (lane >= off) run += other;
-    }
-    __syncthreads();
-    if (lane == kWave - 1) s.words[wave] = run;
-    __syncthreads();
-    u64 all = 0;
-    run += before;
-#pragma unroll
-    for (int v = 0; v < THREADS / kWave; ++v) {
-      if (v < wave) run += s.words[v];
-      all += s.words[v];
-    }
-    if (w && run > target && run - w <= target) {
-      p.tokens[row] = i;
-      if (p.probability) p.probability[row] = (float)((double)w / (double)sum);
-    }
-    before += all;
-    if (before > target) break;
-  }
-}
-
 // ------------------------------------------------------------ rows in registers
 // With a part of the row at a time in registers:
 //   - the maximum;
@@ -471,9 +343,139 @@ __device__ __forceinline__ u64 select_key(int n, u64 low, u64 high, u64 target,
   return found;
 }
 
+// ------------------------------------------------------------ any row
+// The key at which the running cost, from the highest ranked down, reaches
+// `target` (at least 1 and at most all of it): digit by digit, a histogram of the
+// costs of the keys that agree so far.
+template <int THREADS, typename EACH>
+__device__ __forceinline__ u64 cut_at(u64 target, SampleScratch<THREADS>& s, const EACH& each) {
+  static_assert(THREADS == kDigits, "a digit a thread");
+  u64 prefix = 0;
+#pragma unroll 1
+  for (int shift = 56; shift >= 0; shift -= 8) {
+    __syncthreads();
+    s.hist[threadIdx.x] = 0;
+    __syncthreads();
+    each([&](u64 key, u64 cost) TMC_INLINE {
+      if (shift < 56 && key >> (shift + 8) != prefix >> (shift + 8)) return;
+      // (rows of equals: one lane for all that are alike)
+      const unsigned digit = (unsigned)(key >> shift) & 255u;
+      const u64 here = __ballot(true);
+      const bool alike = digit == (unsigned)__builtin_amdgcn_readfirstlane(digit) &&
+                         cost == ((u64)(unsigned)__builtin_amdgcn_readfirstlane((int)(cost >> 32)) << 32 |
+                                  (unsigned)__builtin_amdgcn_readfirstlane((int)cost));
+      if (__ballot(alike) != here) atomicAdd(&s.hist[digit], cost);
+      else if ((threadIdx.x & (kWave - 1)) == __builtin_ctzll(here))
+        atomicAdd(&s.hist[digit], cost * __popcll(here));
+    });
+    __syncthreads();
+    const u64 mine[1] = {s.hist[kDigits - 1 - threadIdx.x]};
+    u64 base, all, before;
+    block_scan<THREADS>(mine[0], s, base, all);
+    const int digit = kDigits - 1 - find_in<THREADS, false>(mine, base, target, before, s);
+    prefix |= (u64)digit << shift;
+    target -= before;
+  }
+  return prefix;
+}
+
+// A row by one block, whatever it holds, pass after pass over memory: weights as
+// integers, cuts by their digits, up to 20 passes.
+template <typename T, int THREADS>
+__device__ __forceinline__ void row_by_digits(const SampleParams& p, int row, const Settings& set,
+                                              SampleScratch<THREADS>& s) {
+  constexpr int AHEAD = 4;  // loads in flight
+  const T* x = static_cast<const T*>(p.logits) + (size_t)row * p.stride;
+  // take(logit, index) of the tokens of [begin, end); NaN behind them
+  auto tokens = [&](int begin, int end, auto&& take) TMC_INLINE {
+#pragma unroll 1
+    for (int at = begin + (int)threadIdx.x; at - (int)threadIdx.x < end; at += AHEAD * THREADS) {
+      float v[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j)
+        v[j] = at + j * THREADS < end ? (float)x[at + j * THREADS] : __builtin_nanf("");
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) take(v[j], at + j * THREADS);
+    }
+  };
+  // ---- the most probable token
+  u64 best = 0;
+  tokens(0, p.vocab, [&](float v, int i) TMC_INLINE {
+    if (v == v) best = max(best, rank_key(v, i));
+  });
+  best = block_max_u64<THREADS>(best, s);
+  const float top = key_value(best);
+  if (set.heat == 0.0 || best == 0 || top == -INFINITY) {
+    if (threadIdx.x == 0) {
+      p.tokens[row] = best ? key_index(best) : -1;
+      if (p.probability)
+        p.probability[row] = set.heat == 0.0 && best ? 1.0f : __builtin_nanf("");
+    }
+    return;
+  }
+  const double unit = ldexp(1.0, p.scale);
+  auto weight = [&](float v) TMC_INLINE -> u64 {
+    if (v == top) return (u64)unit;
+    if (!(v > -INFINITY) || top == INFINITY) return 0;
+    const double a = ((double)v - (double)top) * set.heat;
+    return a >= kFaintest ? max((u64)rint(exp2_of(a) * unit), (u64)1) : 0;
+  };
+  u64 cut = 0;
+  // top-k, then top-p
+#pragma unroll 1
+  for (int step = set.most < p.vocab ? 0 : 1; step < (set.share < 1.0f ? 2 : 1); ++step) {
+    auto each = [&](auto&& take) TMC_INLINE {
+      tokens(0, p.vocab, [&](float v, int i) TMC_INLINE {
+        const u64 w = weight(v), key = rank_key(v, i);
+        if (w && key >= cut) take(key, step == 0 ? (u64)1 : w);
+      });
+    };
+    u64 sum = 0;
+    each([&](u64, u64 cost) TMC_INLINE { sum += cost; });
+    sum = block_sum_u64<THREADS>(sum, s);
+    u64 target = (u64)set.most;
+    if (step == 1) target = max((u64)1, min(sum, (u64)ceil((double)set.share * (double)sum)));
+    else if (sum <= target) continue;
+    cut = max(cut, cut_at<THREADS>(target, s, each));
+  }
+  auto kept = [&](float v, int i) TMC_INLINE -> u64 {
+    if (v != top && !(((double)v - (double)top) * set.heat >= set.least)) return 0;
+    const u64 w = weight(v);
+    return w && rank_key(v, i) >= cut ? w : 0;
+  };
+  u64 sum = 0;
+  tokens(0, p.vocab, [&](float v, int i) TMC_INLINE { sum += kept(v, i); });
+  sum = block_sum_u64<THREADS>(sum, s);
+  const u64 target = min(sum - 1, (u64)(set.uniform * (double)sum));
+  // ---- the first kept token at which the running sum passes the target: among 16 loads a
+  // thread, then among one
+  u64 before = 0;
+  int begin = 0;
+#pragma unroll 1
+  for (int span = 16 * THREADS; span >= THREADS; span /= 16)
+#pragma unroll 1
+    for (;; begin += span) {
+      u64 own = 0;
+      tokens(begin, min(p.vocab, begin + span), [&](float v, int i) TMC_INLINE { own += kept(v, i); });
+      own = block_sum_u64<THREADS>(own, s);
+      if (before + own > target || begin + span >= p.vocab) break;
+      before += own;
+    }
+  const int at = begin + (int)threadIdx.x;
+  const u64 w[1] = {at < p.vocab ? kept((float)x[at], at) : 0};
+  u64 base, all, ahead;
+  block_scan<THREADS>(w[0], s, base, all);
+  const int index = find_in<THREADS, true>(w, base, target - before, ahead, s);
+  if ((int)threadIdx.x == index) {
+    p.tokens[row] = at;
+    if (p.probability) p.probability[row] = (float)((double)w[0] / (double)sum);
+  }
+}
+
+// ------------------------------------------------------------ the kernel
 // STAGE: 0 for a row of one block, 1 and 2 for the launches of shared rows.
 template <typename T, int THREADS, int EACH, int STAGE>
-__global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
+__global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleParams p) {
   constexpr int VEC = 16 / (int)sizeof(T), LOADS = EACH / VEC;
   constexpr int PART = THREADS * EACH;
   constexpr int BINS = (kBins + THREADS - 1) / THREADS;  // bins a thread
@@ -528,7 +530,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
     return at + (int)threadIdx.x * EACH + i;
   };
   const int span = p.walk * PART;  // of a block
-  const int begin = split * span, end = SHARED ? min(p.vocab, begin + span) : p.vocab;
+  int begin = split * span, end = SHARED ? min(p.vocab, begin + span) : p.vocab;
   SampleRow* record = p.records + row;
 
   // ---- the greatest, of the block or (known already) of the row
@@ -555,7 +557,8 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
     best = block_max_u64<THREADS>(best, s);
   }
   top = best ? key_value(best) : -INFINITY;
-  const float per_bin = (float)(set.heat * kBinsOctave);
+  const float heat = (float)set.heat;
+  float octave = kBinsOctave, per_bin = heat * octave;  // bins an octave, and a logit
   // what has no bins, and long lists: by digits
   auto is_odd = [&](float top) TMC_INLINE {
     return !(fabsf(top * per_bin) < INFINITY) || !(fabsf(top) < INFINITY);
@@ -568,40 +571,46 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
                                             : set.share < 1.0f      ? kBin
                                                                     : kSum;
   // A token's bin, counted down from the greatest's (NaN: none).
-  auto level = [&](float x) TMC_INLINE { return floorf(x * per_bin); };
-  first_bin = level(top);
-  auto bin_of = [&](float x) TMC_INLINE { return first_bin - level(x); };
+  auto level_of = [&](float x) TMC_INLINE { return floorf(x * per_bin); };
+  first_bin = level_of(top);
+  auto bin_of = [&](float x) TMC_INLINE { return first_bin - level_of(x); };
   auto octaves = [&](float x) TMC_INLINE { return ((double)x - (double)top) * set.heat; };
   // 2^octaves in multiples of 2^-43: the last bits of that and 512.
   constexpr double kUnit = 0x1p43;
   auto integer = [&](double a) TMC_INLINE -> u64 {
     return __builtin_bit_cast(u64, exp2_of(a) + 512.0) - __builtin_bit_cast(u64, 512.0);
   };
-  // counts, or weights relative to the bin in units of 2^-11 (a sum of 2^20 tokens fits)
+  // The tokens of [low, roof) in bins counted from that of `ref`: numbers, or weights
+  // relative to the bin's in units of 2^-11 (a sum of 2^20 tokens fits).  Returns how many of
+  // the thread's are above.
   unsigned* rough = reinterpret_cast<unsigned*>(s.hist);
-  if (STAGE < 2 && !odd && (way == kList || way == kBin)) {
+  float low = -INFINITY, roof = INFINITY, ref = top;
+  auto fill_bins = [&]() TMC_INLINE -> int {
     for (int i = threadIdx.x; i < kBins; i += THREADS) rough[i] = 0;
     __syncthreads();
+    int above = 0;
     parts(begin, end, [&](int) TMC_INLINE {
 #pragma unroll
       for (int i = 0; i < EACH; ++i) {
         const float bin = bin_of(v[i]);
-        if (bin < (float)kBins) {
+        if (v[i] >= roof) ++above;
+        else if (v[i] >= low && bin < (float)kBins) {
           unsigned cost = 1;
           if (way == kBin)
-            cost = (unsigned)__fmaf_rn(
-                fast_exp2(__fmaf_rn(v[i] - top, per_bin / kBinsOctave, bin * (1.0f / kBinsOctave))),
-                0x1p11f, 0.5f);
+            cost = (unsigned)__fmaf_rn(fast_exp2(__fmaf_rn(v[i] - ref, heat, bin / octave)), 0x1p11f,
+                                       0.5f);
           atomicAdd(&rough[(int)bin], cost);
         }
       }
     });
     __syncthreads();
-  }
+    return above;
+  };
+  if (STAGE < 2 && !odd && (way == kList || way == kBin)) fill_bins();
   // The thread's bins, and the sum of all before them.
   auto take_bins = [&](double (&mine)[BINS], double& base, double& all) TMC_INLINE {
     const double sum = take_values(mine, [&](int i) TMC_INLINE {
-      const double scale = way == kBin ? (double)fast_exp2((float)-i / kBinsOctave) : 1.0;
+      const double scale = way == kBin ? (double)fast_exp2((float)-i / octave) : 1.0;
       return i < kBins ? scale * (double)rough[i] : 0.0;
     });
     block_scan<THREADS>(sum, s, base, all);
@@ -626,7 +635,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
 #pragma unroll
     for (int shift = 30; shift >= 0; shift -= 6) {
       const u64 at = below + ((u64)lane << shift);
-      const bool less = at <= kLast && !(level(key_value(at << 32)) >= low);
+      const bool less = at <= kLast && !(level_of(key_value(at << 32)) >= low);
       below += (u64)max(__popcll(__ballot(less)) - 1, 0) << shift;
     }
     return key_value((below + 1) << 32);
@@ -681,7 +690,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
     __syncthreads();
     return n;
   };
-  float low = 0.0f, high = 0.0f;  // the list's logits: from low on, below high
+  float high = 0.0f;  // the list's logits: from low on, below high
   // The sums of the block's parts: of the tokens from the logit `high` on (all, where none
   // are listed) that min-p keeps; those from `low` on and below `high` into the list.
   // Returns the sum of all tokens' weights, of this thread (0 where none are listed).
@@ -725,7 +734,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
       }
     }
     low = least_of(first_bin - (float)to);
-    high = from > 0 ? least_of(first_bin - (float)from + 1.0f) : INFINITY;
+    high = from > 0 ? least_of(first_bin - (float)from + 1.0f) : roof;
   };
 
   // ---- the row's blocks together: every word at agent scope, completed before the
@@ -777,7 +786,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
     best = block_max_u64<THREADS>(best, s);
     odd |= best == 0;
     top = best ? key_value(best) : -INFINITY;
-    first_bin = level(top);
+    first_bin = level_of(top);
     if (way == kGreedy && best) {
       odd = false;
       if (threadIdx.x == 0) say(key_index(best), 1.0);
@@ -851,14 +860,17 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
     }
     u64 weights = 0;  // of all tokens, this thread's
     if (done) {
-      if (STAGE == 0 && way != kSum) {
+      // the bins' running sum reaches `aim`: the list's bounds
+      auto find_bounds = [&](double aim, bool share) TMC_INLINE {
         double mine[BINS], base, all, above;
         take_bins(mine, base, all);
-        const double aim = way == kList ? (double)set.most : (double)set.share * all;
-        const int bin = find_in<THREADS, false>(mine, base, aim, above, s);
-        const double here = bin >= 0 ? (way == kBin ? exp2_of(-(double)bin / kBinsOctave) : 1.0) * rough[bin] : 0.0;
-        bounds(bin, above, above + here, aim, all);
-      }
+        if (share) aim *= all;
+        const int bin = max(find_in<THREADS, false>(mine, base, aim, above, s), 0);
+        const double scale = way == kBin ? (double)fast_exp2((float)-bin / octave) : 1.0;
+        bounds(bin, above, above + scale * rough[bin], aim, all);
+      };
+      if (STAGE == 0 && way != kSum)
+        find_bounds(way == kList ? (double)set.most : (double)set.share, way == kBin);
       if (way == kList) {
         parts(begin, end, [&](int at) TMC_INLINE {
 #pragma unroll
@@ -895,6 +907,39 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleParams p) {
           for (int g = threadIdx.x; g < count_groups(p.vocab); g += THREADS) groups[g] = get(sums + g);
         for (int i = threadIdx.x; i < min(n, kMostKept); i += THREADS) s.keys[i] = get(list + i);
         __syncthreads();
+      }
+      // too many: those bins in 64 finer ones each, as long as that tells tokens apart
+#pragma unroll 1
+      for (int level = 0; level < 3 && n > kMostKept && !(set.least > kFaintest); ++level) {
+        double aim = 0.0;
+        roof = way == kBin ? high : least_of(level_of(low) + 1.0f);
+        ref = fminf(roof, top);
+        if (way == kBin) {
+          u64 mine = 0;
+          for (int g = threadIdx.x; g < count_groups(p.vocab); g += THREADS) mine += groups[g];
+          const u64 total = block_sum_u64<THREADS>(weights, s), ahead = block_sum_u64<THREADS>(mine, s);
+          aim = ((double)set.share * (double)total - (double)ahead) * (0x1p11 / kUnit) /
+                exp2_of(octaves(ref));
+        }
+        octave *= 64.0f;
+        per_bin = heat * octave;
+        if (is_odd(top)) break;
+        first_bin = level_of(ref);
+        begin = 0;
+        end = p.vocab;
+        queued = 0;
+        const int above = fill_bins();
+        if (way == kList) aim = (double)set.most - (double)block_sum_u64<THREADS>((u64)above, s);
+        find_bounds(aim, false);
+        if (way == kList) {
+          parts(begin, end, [&](int at) TMC_INLINE {
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) collect(v[i] >= low, place(at, i));
+          });
+        } else {
+          weights = sum_groups(std::true_type());
+        }
+        n = collected();
       }
       done = n <= kMostKept;
       double limit = INFINITY;  // top-p: tokens before which less than that lies stay

@@ -93,6 +93,17 @@ def test_flat_and_steep_rows(tmc, style, spread):
     check(tmc, logits.cuda(), numbers(len(kinds), 3), kinds)
 
 
+@pytest.mark.parametrize("rows,vocab", [(520, 9001), (3, 131072)])
+@pytest.mark.parametrize("spread", [3e-6, 1e-3, 0.05, 0.5])
+def test_cuts_among_many(tmc, rows, vocab, spread):
+    """More tokens near the cut than a list holds, in rows of one block and of several."""
+    kinds = [dict(top_p=0.9), dict(top_k=900, top_p=0.7), dict(top_p=0.3, min_p=0.2),
+             dict(top_k=1000), dict(top_p=0.999), dict(top_k=1500, top_p=0.5)]
+    gen = torch.Generator().manual_seed(11)
+    logits = torch.randn(rows, vocab, generator=gen) * spread - 1.0
+    check(tmc, logits.cuda(), numbers(rows, 12), [kinds[r % len(kinds)] for r in range(rows)])
+
+
 @pytest.mark.parametrize("style", ["temperature", "top_k", "top_p", "min_p", "all", "greedy"])
 def test_equal_logits(tmc, style):
     """Few different values: every cut falls inside a run of equals."""
