@@ -327,7 +327,8 @@ extern "C" int tmc_tree_rope_append(const void* qkv, const float* cosine, const 
   TreeAppend p{cosine,     sine,         cached_lengths, depths,        counts,         block_tables,
                active_count, (int)batch, (int)nodes,     (int)q_heads,  (int)kv_heads,  (int)head_dim,
                (int)page_size, (int)max_pages, (int)pool_pages, (long)positions,
-               PageDivide::by(width / each), PageDivide::by(nodes), PageDivide::by(head_dim), PageDivide::by(page_size)};
+               PageDivide::by(width / each), PageDivide::by(nodes), PageDivide::by(head_dim),
+               PageDivide::by(page_size)};
 #define TMC_TREE_APPEND(TYPE, EACH)                                                             \
   hipLaunchKernelGGL((tree_append_kernel<TYPE, EACH>),                                          \
                      dim3((unsigned)((batch * nodes * (width / EACH) + 255) / 256)), dim3(256), \

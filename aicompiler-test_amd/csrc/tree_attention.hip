@@ -1230,8 +1230,8 @@ struct TreeLayout {
 TreeLayout tree_layout(int64_t batch, int64_t nodes, int64_t q_heads, int64_t kv_heads,
                        int64_t head_dim, int64_t capacity) {
   TreeLayout l{};
-  const int64_t vectors = nodes * (q_heads / kv_heads);
-  int resident;  // blocks that the card holds at once
+  const int64_t vectors = nodes * (q_heads / kv_heads), pairs = batch * kv_heads;
+  int resident;  // blocks that share the steps
   if (vectors <= 32) {
     l.vectors = vectors <= 16 ? 16 : 32;
     l.least = 8;
@@ -1239,22 +1239,39 @@ TreeLayout tree_layout(int64_t batch, int64_t nodes, int64_t q_heads, int64_t kv
     l.lead = 12;
     resident = kTreeCus;
   } else {
-    // wide blocks do the same work in less time, but not on vectors that are not there
+    // Shared out, a block's partials cost as much as some steps: few blocks, and for
+    // head dim 128 one tile of up to 256 vectors, reading K and V once (16 requests of up to
+    // 4096 positions with 96, 192 and 256 vectors 54, 80 and 95 us, tiles of 64: 57, 75
+    // and 90; one of 100000 with 256: 158 and 198).  For head dim 64, with half the
+    // work a vector, tiles of 64 (31, 44 and 53 us, of 256: 53, 74 and 84; 116 and 123).
+    // One tile of 64 on one block a CU: 47 us with 64 vectors, on two 55.
+    const bool one = vectors <= 64;
+    l.vectors = one || head_dim == 64 ? 64 : 256;
+    l.least = 4;
+    l.alone = one ? 24 : 6;
+    l.lead = 8;
+    resident = one || l.vectors == 256 ? kTreeCus : 2 * kTreeCus;
+  }
+  const auto share = [&]() {
+    const int step = l.vectors <= 32 ? kTreeStep : kWideSpan;
+    const int64_t steps = (capacity + step - 1) / step;
+    l.tiles = (int)((vectors + l.vectors - 1) / l.vectors);
+    return batch <= kTreeSurvey && pairs * l.tiles <= kSharedRows && steps > l.alone &&
+           pairs * (steps + l.lead) < (1LL << 30);
+  };
+  l.split = share();
+  if (vectors > 64 && (!l.split || pairs >= 2 * kTreeCus)) {
+    // mostly whole units: wide blocks do the same work in less time, but not on vectors that
+    // are not there (64 requests of 1000 positions with 128 vectors: tiles of 64 87 us, of
+    // 128 70, of 256 83; with 256 vectors 156, 123 and 118)
     const int64_t cost64 = (vectors + 63) / 64 * 64 * 7, cost128 = (vectors + 127) / 128 * 128 * 6,
                   cost256 = (vectors + 255) / 256 * 256 * 5;
     l.vectors = cost64 < std::min(cost128, cost256) ? 64 : cost128 < cost256 ? 128 : 256;
-    l.least = 4;
-    l.alone = 6;
-    l.lead = 8;
     resident = l.vectors == 256 && head_dim == 128 ? kTreeCus : 2 * kTreeCus;
+    l.split = share();
   }
-  const int step = l.vectors <= 32 ? kTreeStep : kWideSpan;
-  l.tiles = (int)((vectors + l.vectors - 1) / l.vectors);
-  const int64_t pairs = batch * kv_heads, steps = (capacity + step - 1) / step;
-  l.split = batch <= kTreeSurvey && pairs * l.tiles <= kSharedRows && steps > l.alone &&
-            pairs * (steps + l.lead) < (1LL << 30);
-  const int64_t blocks = l.split ? std::max(resident / l.tiles, 8) : pairs;
-  l.blocks = (int)((blocks + 7) / 8 * 8);
+  // a multiple of the XCDs, no more than are resident
+  l.blocks = (int)(l.split ? std::max(resident / l.tiles / 8 * 8, 8) : (pairs + 7) / 8 * 8);
   l.arrivals = l.vectors <= 32 || l.blocks <= 6 * pairs;
   return l;
 }
@@ -1324,7 +1341,7 @@ extern "C" int tmc_tree_attention(const void* q, const void* key_pool, const voi
   do {                                                                                      \
     hipLaunchKernelGGL((tree_wide_kernel<DIM, VG, PG>), dim3((unsigned)blocks),             \
                        dim3(VG * PG * kWave), 0, s, p, plan);                               \
-    if (l.split && !l.arrivals && !check_launch("tree_wide_kernel"))                                       \
+    if (l.split && !l.arrivals && !check_launch("tree_wide_kernel"))                        \
       hipLaunchKernelGGL((tree_join_kernel<DIM, 32 * VG>),                                  \
                          dim3((unsigned)(batch * kv_heads * l.tiles * (32 * VG) * (DIM / 4) / \
                                          kJoinThreads)),                                    \
