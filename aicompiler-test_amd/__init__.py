@@ -183,6 +183,7 @@ def _declare(l):
         fn = getattr(l, name)
         fn.restype = res
         fn.argtypes = args
+        fn.address = C.cast(fn, vp).value
 
 
 def lib() -> C.CDLL:
@@ -1036,6 +1037,17 @@ def logprobs(logits, tokens, logprob, entropy=None, top_tokens=None, top_logprob
 
 
 # ---------------------------------------------------------------- speculative decoding
+def _call(what, device, function, names, *args):
+    """function(*args) of the library, a tensor's argument followed by the dtype and
+    the number of elements that it must have; `names` are those of the tensors."""
+    result = (_tensors or _open_tensors()).call(function.address, device, *args)
+    if result < 0:
+        tensors = [args[i:i + 3] for i, t in enumerate(args) if t is None or hasattr(t, "numel")]
+        t, dtype, count = tensors[-1 - result]
+        _refuse(what, device, dtype, names[-1 - result], t, count)
+    check(result, what)
+
+
 def _tree_shape(what, parents):
     if parents.dim() != 2:
         raise TmcError(f"{what}: trees must be [batch, nodes]")
@@ -1049,12 +1061,9 @@ def tree_layout(parents, masks, depths, counts=None, stream=None):
     what = "tmc_tree_layout"
     device, i32 = torch.cuda.current_device(), torch.int32
     batch, nodes = _tree_shape(what, parents)
-    check(lib().tmc_tree_layout(
-        _address(what, device, i32, "parents", parents, 0),
-        _address(what, device, i32, "counts", counts, batch),
-        _address(what, device, i32, "masks", masks, batch * nodes * ((nodes + 31) // 32)),
-        _address(what, device, i32, "depths", depths, batch * nodes), batch, nodes,
-        _launch_stream(torch, what, device, stream)), what)
+    _call(what, device, lib().tmc_tree_layout, ("parents", "counts", "masks", "depths"),
+          parents, i32, 0, counts, i32, batch, masks, i32, batch * nodes * ((nodes + 31) // 32),
+          depths, i32, batch * nodes, batch, nodes, _launch_stream(torch, what, device, stream))
 
 
 def tree_rope_append(qkv, cosine, sine, cached_lengths, depths, counts, tables, active, q_out,
@@ -1075,20 +1084,15 @@ def tree_rope_append(qkv, cosine, sine, cached_lengths, depths, counts, tables, 
     pairs = head_dim // 2
     positions = min(cosine.numel(), sine.numel()) // max(pairs, 1)
     f32, i32, rows = torch.float32, torch.int32, batch * nodes
-    check(lib().tmc_tree_rope_append(
-        _address(what, device, dtype, "qkv", qkv, rows * (q_heads + 2 * kv_heads) * head_dim),
-        _address(what, device, f32, "cosine", cosine, 0),
-        _address(what, device, f32, "sine", sine, 0), positions,
-        _address(what, device, i32, "cached_lengths", cached_lengths, batch),
-        _address(what, device, i32, "depths", depths, rows),
-        _address(what, device, i32, "counts", counts, batch),
-        _address(what, device, i32, "tables", tables, batch * max_pages),
-        _address(what, device, i32, "active", active, 1),
-        _address(what, device, dtype, "q_out", q_out, rows * q_heads * head_dim),
-        _address(what, device, dtype, "k_pool", k_pool, 0),
-        _address(what, device, dtype, "v_pool", v_pool, 0), _dtype_code(qkv), batch, nodes,
-        q_heads, kv_heads, head_dim, page_size, max_pages, pool_pages,
-        _launch_stream(torch, what, device, stream)), what)
+    _call(what, device, lib().tmc_tree_rope_append,
+          ("qkv", "cosine", "sine", "cached_lengths", "depths", "counts", "tables", "active",
+           "q_out", "k_pool", "v_pool"),
+          qkv, dtype, rows * (q_heads + 2 * kv_heads) * head_dim, cosine, f32, 0, sine, f32, 0,
+          positions, cached_lengths, i32, batch, depths, i32, rows, counts, i32, batch,
+          tables, i32, batch * max_pages, active, i32, 1,
+          q_out, dtype, rows * q_heads * head_dim, k_pool, dtype, 0, v_pool, dtype, 0,
+          F16 if dtype is torch.float16 else F32, batch, nodes, q_heads, kv_heads, head_dim,
+          page_size, max_pages, pool_pages, _launch_stream(torch, what, device, stream))
 
 
 def tree_attention_workspace_bytes(batch, nodes, q_heads, kv_heads, head_dim, capacity) -> int:
@@ -1111,19 +1115,14 @@ def tree_attention(q, k_pool, v_pool, cached_lengths, masks, counts, tables, act
         raise TmcError(f"{what}: nodes must be positive")
     f16, i32, rows = torch.float16, torch.int32, batch * nodes
     space, space_bytes = _workspace(what, device, workspace)
-    check(lib().tmc_tree_attention(
-        _address(what, device, f16, "q", q, rows * q_heads * head_dim),
-        _address(what, device, f16, "k_pool", k_pool, 0),
-        _address(what, device, f16, "v_pool", v_pool, 0),
-        _address(what, device, i32, "cached_lengths", cached_lengths, batch),
-        _address(what, device, i32, "masks", masks, rows * ((nodes + 31) // 32)),
-        _address(what, device, i32, "counts", counts, batch),
-        _address(what, device, i32, "tables", tables, batch * max_pages),
-        _address(what, device, i32, "active", active, 1),
-        _address(what, device, f16, "out", out, rows * q_heads * head_dim),
-        F16, batch, nodes, q_heads, kv_heads, head_dim, page_size, max_pages, pool_pages,
-        page_stride, head_stride, space, space_bytes,
-        _launch_stream(torch, what, device, stream)), what)
+    _call(what, device, lib().tmc_tree_attention,
+          ("q", "k_pool", "v_pool", "cached_lengths", "masks", "counts", "tables", "active", "out"),
+          q, f16, rows * q_heads * head_dim, k_pool, f16, 0, v_pool, f16, 0,
+          cached_lengths, i32, batch, masks, i32, rows * ((nodes + 31) // 32), counts, i32, batch,
+          tables, i32, batch * max_pages, active, i32, 1, out, f16, rows * q_heads * head_dim,
+          F16, batch, nodes, q_heads, kv_heads, head_dim, page_size, max_pages, pool_pages,
+          page_stride, head_stride, space or 0, space_bytes,
+          _launch_stream(torch, what, device, stream))
 
 
 def sample_workspace_bytes(rows, vocabulary) -> int:
@@ -1149,16 +1148,12 @@ def sample(logits, uniforms, tokens, temperature=None, top_k=None, top_p=None, m
     rows, vocabulary = logits.shape
     f32, i32 = torch.float32, torch.int32
     space, space_bytes = _workspace(what, device, workspace)
-    check(lib().tmc_sample(
-        logits.data_ptr(), F32 if dtype is f32 else F16, strides[0] if rows > 1 else vocabulary,
-        _address(what, device, f32, "temperature", temperature, rows),
-        _address(what, device, i32, "top_k", top_k, rows),
-        _address(what, device, f32, "top_p", top_p, rows),
-        _address(what, device, f32, "min_p", min_p, rows),
-        _address(what, device, f32, "uniforms", uniforms, rows),
-        _address(what, device, i32, "tokens", tokens, rows),
-        _address(what, device, f32, "probability", probability, rows), rows, vocabulary, space,
-        space_bytes, _launch_stream(torch, what, device, stream)), what)
+    _call(what, device, lib().tmc_sample,
+          ("temperature", "top_k", "top_p", "min_p", "uniforms", "tokens", "probability"),
+          logits.data_ptr(), F32 if dtype is f32 else F16, strides[0] if rows > 1 else vocabulary,
+          temperature, f32, rows, top_k, i32, rows, top_p, f32, rows, min_p, f32, rows,
+          uniforms, f32, rows, tokens, i32, rows, probability, f32, rows, rows, vocabulary,
+          space or 0, space_bytes, _launch_stream(torch, what, device, stream))
 
 
 def tree_accept(drafted, parents, chosen, path, accepted, emitted, counts=None, active=None,
@@ -1170,18 +1165,13 @@ def tree_accept(drafted, parents, chosen, path, accepted, emitted, counts=None, 
     device, i32 = torch.cuda.current_device(), torch.int32
     batch, nodes = _tree_shape(what, parents)
     rows = batch * nodes
-    check(lib().tmc_tree_accept(
-        _address(what, device, i32, "drafted", drafted, rows),
-        _address(what, device, i32, "parents", parents, rows),
-        _address(what, device, i32, "chosen", chosen, rows),
-        _address(what, device, i32, "counts", counts, batch),
-        _address(what, device, i32, "active", active, 1),
-        _address(what, device, i32, "cached_lengths", cached_lengths, batch),
-        _address(what, device, i32, "path", path, rows),
-        _address(what, device, i32, "accepted", accepted, batch),
-        _address(what, device, i32, "emitted", emitted, rows),
-        _address(what, device, i32, "new_lengths", new_lengths, batch), batch, nodes,
-        _launch_stream(torch, what, device, stream)), what)
+    _call(what, device, lib().tmc_tree_accept,
+          ("drafted", "parents", "chosen", "counts", "active", "cached_lengths", "path",
+           "accepted", "emitted", "new_lengths"),
+          drafted, i32, rows, parents, i32, rows, chosen, i32, rows, counts, i32, batch,
+          active, i32, 1, cached_lengths, i32, batch, path, i32, rows, accepted, i32, batch,
+          emitted, i32, rows, new_lengths, i32, batch, batch, nodes,
+          _launch_stream(torch, what, device, stream))
 
 
 def tree_keep(k_pools, v_pools, tables, cached_lengths, path, accepted, heads, page_size, head_dim,
@@ -1204,14 +1194,11 @@ def tree_keep(k_pools, v_pools, tables, cached_lengths, path, accepted, heads, p
     addresses, least = _pool_list(torch, what, device, k_pools, v_pools)
     pool_pages = least // page_stride
     first, size = addresses.buffer_info()[0], addresses.itemsize
-    check(lib().tmc_tree_keep(
-        first, first + count * size, count,
-        _address(what, device, i32, "tables", tables, 0),
-        _address(what, device, i32, "cached_lengths", cached_lengths, batch),
-        _address(what, device, i32, "path", path, 0),
-        _address(what, device, i32, "accepted", accepted, batch), _dtype_code(k_pools[0]), batch,
-        nodes, heads, head_dim, page_size, tables.shape[2], pool_pages, page_stride, head_stride,
-        _launch_stream(torch, what, device, stream)), what)
+    _call(what, device, lib().tmc_tree_keep, ("tables", "cached_lengths", "path", "accepted"),
+          first, first + count * size, count, tables, i32, 0, cached_lengths, i32, batch,
+          path, i32, 0, accepted, i32, batch, _dtype_code(k_pools[0]), batch, nodes, heads,
+          head_dim, page_size, tables.shape[2], pool_pages, page_stride, head_stride,
+          _launch_stream(torch, what, device, stream))
 
 
 def fill_normal(t, seed, mean=0.0, std=1.0, stream=None):

@@ -60,7 +60,7 @@ __device__ __forceinline__ unsigned opaque(unsigned v) {
 // One wave per (node, query head): 64 positions at a time, one per lane for the
 // scores (whole K rows in 16-byte chunks), then lanes over the dims for P V.  Every node
 // reads all of K and V: 8 requests of up to 2000 positions with 24 nodes, 32 heads and
-// head dim 96 550 us, where the kernels below take 40 us for head dim 128.
+// head dim 96 550 us, where the kernels below take 32 us for head dim 128.
 constexpr int kPlainMaxDim = 256;
 
 struct PlainScratch {  // of one wave

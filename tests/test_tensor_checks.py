@@ -55,3 +55,41 @@ def test_addresses(checks):
             checks.addresses(*bad)
     with pytest.raises((TypeError, BufferError)):
         checks.addresses(pools, HOST, torch.float16, bytes(24))
+
+
+def sum_of_words():
+    """A C function of 24 words: the sum of i times word i, as an int."""
+    import ctypes as C
+    kind = C.CFUNCTYPE(C.c_int, *[C.c_int64] * 24)
+    return kind(lambda *w: sum(i * v for i, v in enumerate(w, 1)))
+
+
+def test_call(checks):
+    import ctypes as C
+    f = sum_of_words()
+    at = C.cast(f, C.c_void_p).value
+    t = torch.zeros(4)
+    assert checks.call(at, HOST) == 0
+    assert checks.call(at, HOST, *range(24)) == sum(i * v for i, v in enumerate(range(24), 1))
+    assert checks.call(at, HOST, 5, None, torch.int32, 3, -7) == 5 - 3 * 7
+    seen = []
+    g = C.CFUNCTYPE(C.c_int, C.c_int64, C.c_void_p, C.c_int64)(lambda *w: seen.append(w) or 1)
+    assert checks.call(C.cast(g, C.c_void_p).value, HOST, 3, t, torch.float32, 4, 1 << 40) == 1
+    assert seen == [(3, t.data_ptr(), 1 << 40)]
+
+
+def test_call_refuses(checks):
+    import ctypes as C
+    f = sum_of_words()
+    at = C.cast(f, C.c_void_p).value
+    t = torch.zeros(4)
+    assert checks.call(at, HOST, 1, None, torch.int32, 3, t, torch.float32, 5) == -2
+    assert checks.call(at, 0, t, torch.float32, 4) == -1
+    assert checks.call(at, HOST, t, torch.int32, 4) == -1
+    for bad in ((), (at,), (at, HOST, 1.5), (at, HOST, t), (at, HOST, t, torch.float32),
+                (at, HOST, None, 3, 4), (at, HOST, "x", torch.float32, 1), (None, HOST),
+                (0, HOST), (at, HOST, *range(25)), (at, "0", 1)):
+        with pytest.raises(TypeError):
+            checks.call(*bad)
+    with pytest.raises(OverflowError):
+        checks.call(at, HOST, 1 << 70)
