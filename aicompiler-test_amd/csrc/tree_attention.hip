@@ -1245,10 +1245,15 @@ TreeLayout tree_layout(int64_t batch, int64_t nodes, int64_t q_heads, int64_t kv
   TreeLayout l{};
   const int64_t vectors = nodes * (q_heads / kv_heads), pairs = batch * kv_heads;
   int resident;  // blocks that share the steps
+  // Sharing costs some 10 us of lookups and joins: requests up to `alone` steps go whole, up
+  // to so many positions that half the CUs take as long.  Whole and shared: 4 requests of 400
+  // positions with 32 vectors 12.5 and 15.6 us, of 1400 23.6 and 19.2; 24 requests 16.2 and
+  // 27.6, 33.0 and 41.7; with 256 vectors 4 of 1400 54 and 32, 24 of 1400 67 and 97.
+  const bool many = pairs >= kTreeCus / 2;
   if (vectors <= 32) {
     l.vectors = vectors <= 16 ? 16 : 32;
     l.least = 8;
-    l.alone = 10;
+    l.alone = many ? 48 : 20;
     l.lead = 12;
     resident = kTreeCus;
   } else {
@@ -1261,7 +1266,7 @@ TreeLayout tree_layout(int64_t batch, int64_t nodes, int64_t q_heads, int64_t kv
     const bool one = vectors <= 64;
     l.vectors = one || head_dim == 64 ? 64 : 256;
     l.least = 4;
-    l.alone = one ? 24 : 6;
+    l.alone = many ? 24 : one ? 9 : 7;
     l.lead = 8;
     resident = one || l.vectors == 256 ? kTreeCus : 2 * kTreeCus;
   }
