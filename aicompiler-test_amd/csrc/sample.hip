@@ -130,7 +130,7 @@ constexpr int kDigits = 256;
 // kFaintest.
 constexpr int kBinsOctave = 16, kBins = 44 * kBinsOctave;
 static_assert(kFaintest == -44.0, "bins down to the least weight");
-// Tokens in the list (of 3584: 64 us for 60 where rows are shared), top_k that goes by it.
+// Tokens in the list, as many as let four blocks into LDS, and the top_k that goes by it.
 constexpr int kMostKept = 2048, kMostTopK = 1024;
 constexpr int kMostGroups = 512;                   // sums of a block's parts
 constexpr int kCoarse = 32;  // bins of a coarse step, and at most steps
@@ -206,13 +206,13 @@ __device__ __forceinline__ double exp2_of(double a) {
 // bins, of which the last of a row's blocks to arrive finds the list's bounds; in the
 // second each block sums and lists its own tokens, and the last goes on with the row.
 // (In one launch the last block has to read the whole row again by itself: 30 us of 91
-// for 64 rows of 128000, in two launches 60 us.)
+// for 64 rows of 128000, in two launches 60.)
 //
 // Measured (32-bit logits, top-k and top-p, warm caches): one row of 32000 30 us, a
 // chain of some thirty steps that each wait for the one before; 1024 rows of 32003 with
-// mixed settings 108 us, 1.2 TB/s: 32 us the maximum, which reads the logits from memory,
-// 10 us the bins, 45 us the exponentials (some 40 64-bit operations a token), 20 us the
-// list and the draw.  64 rows of 128000 fp16 tokens 60 us: 17 us the first launch.
+// mixed settings 100 us, 1.3 TB/s: 32 us the maximum, which reads the logits from memory,
+// 10 us the bins, 38 us the exponentials (some 35 64-bit operations a token), 20 us the
+// list and the draw.  64 rows of 128000 fp16 tokens 57 us: 17 us the first launch.
 //
 // Bins are of absolute logits, so that those of several blocks fit together.  Weights are
 // integers: the result does not depend on which thread comes first.  Rows that this does
@@ -291,7 +291,7 @@ __device__ __forceinline__ int find_in(const TYPE (&v)[EACH], TYPE base, TYPE ta
 
 // The key of the list s.keys[0 ... n), all in [low, high], at which the running cost, from
 // the highest ranked down, reaches `target` (at least 1); 0 where all of it does not.
-// `cost` gives that of a key.  The list's range of keys is cut into 256, then that of the
+// `cost` gives that of a place.  The list's range of keys is cut into 256, then that of the
 // part with the target, until a wave can take the rest: for logits that are not equal,
 // once or twice.
 template <int THREADS, typename COST>
@@ -311,7 +311,7 @@ __device__ __forceinline__ u64 select_key(int n, u64 low, u64 high, u64 target,
     for (int i = threadIdx.x; i < n; i += THREADS) {
       const u64 key = s.keys[i];
       if (key >= low && key <= high) {
-        atomicAdd(&hist[255 - ((key - low) >> shift)], cost(key));
+        atomicAdd(&hist[255 - ((key - low) >> shift)], cost(i));
         ++here;
       }
     }
@@ -333,7 +333,7 @@ __device__ __forceinline__ u64 select_key(int n, u64 low, u64 high, u64 target,
     if (key < low || key > high) continue;
     const int slot = atomicAdd(&s.small, 1);
     hist[slot] = key;
-    hist[kWave + slot] = cost(key);
+    hist[kWave + slot] = cost(i);
   }
   if (threadIdx.x == 0) s.found64 = 0;
   __syncthreads();
@@ -482,8 +482,8 @@ __device__ __forceinline__ void row_by_digits(const SampleParams& p, int row, co
 
 // ------------------------------------------------------------ the kernel
 // STAGE: 0 for a row of one block, 1 and 2 for the launches of shared rows.  Four blocks a
-// CU: without the bound the loop over finer bins costs registers (1024 rows 121 us for
-// 108; a bound of five spills, 110).
+// CU, as many as LDS holds: without the bound the loop over finer bins takes registers
+// from them (1024 rows 121 us for 108).
 template <typename T, int THREADS, int EACH, int STAGE>
 __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleParams p) {
   constexpr int VEC = 16 / (int)sizeof(T), LOADS = EACH / VEC;
@@ -494,6 +494,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleParams p) {
   typedef vec unaligned __attribute__((aligned(sizeof(T))));  // rows start at any element
   __shared__ SampleScratch<THREADS> s;
   __shared__ double factors[STAGE == 1 ? kMostBlocks : 1];  // of a row's blocks: the greatest weight,
+  __shared__ u64 costs[STAGE == 1 ? 1 : kMostKept];         // of the list's keys
   __shared__ float highs[STAGE == 1 ? kMostBlocks : 1];     // the greatest logit
   const int split = SHARED ? blockIdx.x % p.count : 0, row = SHARED ? blockIdx.x / p.count : blockIdx.x;
   const int lane = threadIdx.x & (kWave - 1);
@@ -714,7 +715,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleParams p) {
 #pragma unroll
       for (int i = 0; i < EACH; ++i) {
         const double a = octaves(v[i]);
-        const u64 w = a >= kFaintest ? integer(a) : 0;
+        const u64 w = integer(fmax(a, -60.0));  // (below 2^-44, and of NaN: 0)
         if (lists) all += w;
         if ((!lists || v[i] >= high) && a >= faintest) sum += w;
         if (lists) collect(v[i] >= low && v[i] < high, place(at, i));
@@ -956,14 +957,13 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleParams p) {
       double above = 0.0;       // the sum before the list
       if (done && way != kSum) {
         __syncthreads();
-        auto cost_of = [&](u64 key) TMC_INLINE -> u64 {
-          const double a = octaves(key_value(key));
-          return a >= kFaintest ? max(integer(a), (u64)1) : 0;
-        };
         u64 low = ~0ull, high = 0;  // of the list's keys
         for (int i = threadIdx.x; i < n; i += THREADS) {
-          low = min(low, s.keys[i]);
-          high = max(high, s.keys[i]);
+          const u64 key = s.keys[i];
+          low = min(low, key);
+          high = max(high, key);
+          const double a = octaves(key_value(key));
+          costs[i] = a >= kFaintest ? integer(a) : 0;
         }
         high = block_max_u64<THREADS>(high, s);
         low = ~block_max_u64<THREADS>(~low, s);
@@ -989,7 +989,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleParams p) {
             cut = max(cut, low);
             u64 sum = 0, before, all;  // of the list
             for (int i = threadIdx.x; i < n; i += THREADS)
-              if (s.keys[i] >= cut) sum += cost_of(s.keys[i]);
+              if (s.keys[i] >= cut) sum += costs[i];
             block_scan<THREADS>(sum, s, before, all);
             const double listed = (double)all * (1.0 / kUnit);
             if (way == kList) limit = (double)set.share * listed;
@@ -1004,8 +1004,8 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleParams p) {
             }
             target = (u64)fmax(room, 1.0);  // (the most probable token stays)
           }
-          cut = max(cut, select_key<THREADS>(n, low, high, target, s, [&](u64 key) TMC_INLINE {
-                      return step == 0 ? (u64)1 : cost_of(key);
+          cut = max(cut, select_key<THREADS>(n, low, high, target, s, [&](int i) TMC_INLINE {
+                      return step == 0 ? (u64)1 : costs[i];
                     }));
         }
         // the list's kept tokens to the sums of their parts
@@ -1015,7 +1015,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleParams p) {
         for (int i = threadIdx.x; i < n; i += THREADS) {
           const u64 key = s.keys[i];
           const double a = octaves(key_value(key));
-          if (key >= cut && a >= faintest) atomicAdd(&groups[key_index(key) / PART], integer(a));
+          if (key >= cut && a >= faintest) atomicAdd(&groups[key_index(key) / PART], costs[i]);
         }
         __syncthreads();
       }
