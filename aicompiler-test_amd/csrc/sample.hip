@@ -599,6 +599,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleParams p) {
   auto fill_bins = [&]() TMC_INLINE -> int {
     for (int i = threadIdx.x; i < kBins; i += THREADS) rough[i] = 0;
     __syncthreads();
+    const float width = 1.0f / octave;  // (a power of two)
     int above = 0;
     parts(begin, end, [&](int) TMC_INLINE {
 #pragma unroll
@@ -608,7 +609,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleParams p) {
         else if (v[i] >= low && bin < (float)kBins) {
           unsigned cost = 1;
           if (way == kBin)
-            cost = (unsigned)__fmaf_rn(fast_exp2(__fmaf_rn(v[i] - ref, heat, bin / octave)), 0x1p11f,
+            cost = (unsigned)__fmaf_rn(fast_exp2(__fmaf_rn(v[i] - ref, heat, bin * width)), 0x1p11f,
                                        0.5f);
           atomicAdd(&rough[(int)bin], cost);
         }
