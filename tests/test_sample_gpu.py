@@ -246,3 +246,28 @@ def test_refusals(tmc):
         with pytest.raises(tmc.TmcError):
             tmc.sample(args.pop("logits"), args.pop("u"), args.pop("tokens"), **args)
     assert (tokens == -7).all()
+
+
+def test_two_at_once(tmc):
+    """On two streams with a workspace each, neither waiting for the other."""
+    rows, vocab, kinds = 9, 50000, STYLES["all"]
+    settings = [kinds[r % len(kinds)] for r in range(rows)]
+    logits = [torch.randn(rows, vocab, generator=torch.Generator().manual_seed(30 + i)) * 3
+              for i in range(2)]
+    u = [numbers(rows, 40 + i) for i in range(2)]
+    want = [run(tmc, x.cuda(), n, settings) for x, n in zip(logits, u)]
+    f32 = lambda n: torch.tensor([{**NEUTRAL, **s}[n] for s in settings], device="cuda")  # noqa: E731
+    heat, share, least = (f32(n).float() for n in ("temperature", "top_p", "min_p"))
+    k = f32("top_k").int()
+    sides = [dict(x=x.cuda(), u=torch.from_numpy(n).cuda(), stream=torch.cuda.Stream(),
+                  tokens=torch.full((rows,), -5, dtype=torch.int32, device="cuda"),
+                  space=torch.zeros(tmc.sample_workspace_bytes(rows, vocab) // 4 + 4, device="cuda"))
+             for x, n in zip(logits, u)]
+    torch.cuda.synchronize()
+    for _ in range(6):
+        for s in sides:
+            tmc.sample(s["x"], s["u"], s["tokens"], temperature=heat, top_k=k, top_p=share,
+                       min_p=least, workspace=s["space"], stream=s["stream"])
+    torch.cuda.synchronize()
+    for s, (tokens, _) in zip(sides, want):
+        assert torch.equal(s["tokens"], tokens)

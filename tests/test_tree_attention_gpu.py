@@ -217,3 +217,46 @@ def test_many_requests(tmc, batch, nodes, dim):
     t = f.device()
     f.attend(tmc, t)
     f.check(t)
+
+
+@pytest.mark.parametrize("batch,nodes,qh,kvh,dim,most,longest", [
+    (40, 4, 16, 4, 128, 300, 1400),    # many pairs, up to 32 vectors: whole, the longest's steps
+    (40, 4, 16, 4, 128, 300, 2500),    # shared out
+    (2, 8, 8, 2, 64, 500, 700),        # few pairs, whole and shared
+    (2, 8, 8, 2, 64, 500, 600),
+    (40, 16, 16, 4, 128, 200, 1400),   # one tile of 64, many pairs
+    (40, 16, 16, 4, 64, 200, 2000),
+    (3, 16, 8, 2, 128, 300, 550),      # few
+    (3, 16, 8, 2, 128, 300, 900),
+    (3, 25, 8, 1, 128, 200, 3000),     # one tile of 256
+    (40, 25, 32, 4, 128, 100, 1400),
+    (3, 25, 8, 1, 64, 200, 3000),      # tiles of 64
+    (70, 25, 16, 2, 64, 60, 600),      # more tiles than there are counters
+    (66, 32, 32, 8, 128, 30, 500),     # tiles of 128, shared and whole
+    (66, 32, 32, 8, 128, 30, 200),
+    (66, 60, 32, 8, 128, 20, 500),     # tiles of 256 of many pairs
+])
+def test_ways_of_sharing(tmc, batch, nodes, qh, kvh, dim, most, longest):
+    rng = random.Random(19)
+    cached = [rng.randint(0, most) for _ in range(batch)]
+    at = batch // 2
+    cached[at] = longest - nodes
+    f = Forest(19, cached, nodes, qh, kvh, dim, 16)
+    t = f.device()
+    f.attend(tmc, t)
+    f.check(t, requests=sorted({0, at, batch - 1, rng.randrange(batch)}))
+
+
+@pytest.mark.parametrize("nodes", [6, 16, 70])
+def test_two_at_once(tmc, nodes):
+    """On two streams with a workspace each, neither waiting for the other."""
+    pair = [Forest(20 + i, [900 * (i + 1), 20, 3000], nodes, 8, 2, 128, 16) for i in range(2)]
+    ts, spaces = [f.device() for f in pair], [f.workspace(tmc) for f in pair]
+    streams = [torch.cuda.Stream() for _ in pair]
+    torch.cuda.synchronize()
+    for _ in range(6):
+        for f, t, space, stream in zip(pair, ts, spaces, streams):
+            f.attend(tmc, t, workspace=space, stream=stream)
+    torch.cuda.synchronize()
+    for f, t in zip(pair, ts):
+        f.check(t)
