@@ -483,7 +483,7 @@ __device__ __forceinline__ unsigned join(const TreeParams& p, const TreePlan& pl
   }
   __syncthreads();
   unsigned again = 0, bit = 1;
-  constexpr int kAhead = 4, kTurns = 2;
+  constexpr int kTurns = COUNT * (D / 4) > THREADS ? 2 : 1, kAhead = kTurns > 1 ? 4 : 12;
   const int items = count * (D / 4);
   for (int i = thread; i < items; i += kTurns * THREADS, bit <<= kTurns) {
     f4 val[kTurns] = {};
@@ -1290,6 +1290,7 @@ TreeLayout tree_layout(int64_t batch, int64_t nodes, int64_t q_heads, int64_t kv
   }
   // a multiple of the XCDs, no more than are resident
   l.blocks = (int)(l.split ? std::max(resident / l.tiles / 8 * 8, 8) : (pairs + 7) / 8 * 8);
+  // (tiles of 128, and of 256 for head dim 64, only where pairs are many)
   l.arrivals = l.vectors <= 32 || l.blocks <= 6 * pairs;
   return l;
 }
@@ -1355,16 +1356,13 @@ extern "C" int tmc_tree_attention(const void* q, const void* key_pool, const voi
 #define TMC_TREE_RING(DIM, C)                                                               \
   hipLaunchKernelGGL((tree_ring_kernel<DIM, C>), dim3((unsigned)blocks),                    \
                      dim3(kTreeWaves * kWave), 0, s, p, plan)
-#define TMC_TREE_WIDE(DIM, VG, PG)                                                          \
-  do {                                                                                      \
-    hipLaunchKernelGGL((tree_wide_kernel<DIM, VG, PG>), dim3((unsigned)blocks),             \
-                       dim3(VG * PG * kWave), 0, s, p, plan);                               \
-    if (l.split && !l.arrivals && !check_launch("tree_wide_kernel"))                        \
-      hipLaunchKernelGGL((tree_join_kernel<DIM, 32 * VG>),                                  \
-                         dim3((unsigned)(batch * kv_heads * l.tiles * (32 * VG) * (DIM / 4) / \
-                                         kJoinThreads)),                                    \
-                         dim3(kJoinThreads), 0, s, p, plan);                                \
-  } while (0)
+#define TMC_TREE_WIDE(DIM, VG, PG)                                               \
+  hipLaunchKernelGGL((tree_wide_kernel<DIM, VG, PG>), dim3((unsigned)blocks),    \
+                     dim3(VG * PG * kWave), 0, s, p, plan)
+#define TMC_TREE_JOIN(DIM, NV)                                                   \
+  hipLaunchKernelGGL((tree_join_kernel<DIM, NV>),                                \
+                     dim3((unsigned)(batch * kv_heads * l.tiles * NV * (DIM / 4) / kJoinThreads)), \
+                     dim3(kJoinThreads), 0, s, p, plan)
 #define TMC_TREE_VECTORS(DIM)                        \
   if (l.vectors == 16) TMC_TREE_RING(DIM, 1);        \
   else if (l.vectors == 32) TMC_TREE_RING(DIM, 2);   \
@@ -1379,5 +1377,12 @@ extern "C" int tmc_tree_attention(const void* q, const void* key_pool, const voi
 #undef TMC_TREE_VECTORS
 #undef TMC_TREE_WIDE
 #undef TMC_TREE_RING
-  return check_launch("tree_attention_kernel");
+  if (check_launch("tree_attention_kernel")) return 1;
+  if (!l.split || l.arrivals) return 0;
+  // (few pairs: tiles of 64, or for head dim 128 one of 256)
+  if (head_dim == 64) TMC_TREE_JOIN(64, 64);
+  else if (l.vectors == 64) TMC_TREE_JOIN(128, 64);
+  else TMC_TREE_JOIN(128, 256);
+#undef TMC_TREE_JOIN
+  return check_launch("tree_join_kernel");
 }
