@@ -1257,16 +1257,18 @@ TreeLayout tree_layout(int64_t batch, int64_t nodes, int64_t q_heads, int64_t kv
     l.lead = 12;
     resident = kTreeCus;
   } else {
-    // Shared out, a block's partials cost as much as some steps: few blocks, and for
-    // head dim 128 one tile of up to 256 vectors, reading K and V once (16 requests of up to
-    // 4096 positions with 96, 192 and 256 vectors 54, 80 and 95 us, tiles of 64: 57, 75
-    // and 90; one of 100000 with 256: 158 and 198).  For head dim 64, with half the
-    // work a vector, tiles of 64 (31, 44 and 53 us, of 256: 53, 74 and 84; 116 and 123).
+    // Shared out, a block's partials cost as much as some steps, and tiles of 64 vectors have
+    // the fewest.  For head dim 128 and much to read, one tile of up to 256 vectors reads K
+    // and V once: 4 requests of 1400 and 8000 positions with 256 vectors 32 and 64 us, in
+    // tiles of 64 32 and 78; 12 of up to 3000 64 and 60; one of 100000 with 240 146 and 194.
+    // Head dim 64 has half the work a vector: 16 requests of up to 4096 with 256 vectors 53
+    // us in tiles of 64, 84 in one of 256; one of 100000 116 and 123.
     // One tile of 64 on one block a CU: 47 us with 64 vectors, on two 55.
     const bool one = vectors <= 64;
-    l.vectors = one || head_dim == 64 ? 64 : 256;
+    l.vectors = one || head_dim == 64 || pairs * ((capacity + kWideSpan - 1) / kWideSpan) <= 12 * kTreeCus
+                    ? 64 : 256;
     l.least = 4;
-    l.alone = many ? 24 : one ? 9 : 7;
+    l.alone = !many ? (one ? 9 : 7) : one || head_dim == 128 ? 24 : 16;
     l.lead = 8;
     resident = one || l.vectors == 256 ? kTreeCus : 2 * kTreeCus;
   }
@@ -1290,8 +1292,10 @@ TreeLayout tree_layout(int64_t batch, int64_t nodes, int64_t q_heads, int64_t kv
   }
   // a multiple of the XCDs, no more than are resident
   l.blocks = (int)(l.split ? std::max(resident / l.tiles / 8 * 8, 8) : (pairs + 7) / 8 * 8);
-  // (tiles of 128, and of 256 for head dim 64, only where pairs are many)
-  l.arrivals = l.vectors <= 32 || l.blocks <= 6 * pairs;
+  // A unit's last block joins two pieces sooner than another launch does, but not more (8
+  // requests of 8000 positions with 256 vectors 132 and 113 us, 16 of them 205 and 210).
+  // (Tiles of 128, and of 256 for head dim 64, have many pairs.)
+  l.arrivals = l.vectors <= 32 || l.blocks <= 2 * pairs;
   return l;
 }
 }  // namespace
