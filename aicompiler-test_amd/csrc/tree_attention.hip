@@ -889,7 +889,7 @@ __global__ __launch_bounds__(kTreeWaves * kWave, 1) void tree_ring_kernel(
 //
 // 8 requests of 1000 to 8000 positions with 64 nodes and 32 K/V heads of 128 dims 137 us,
 // 4.4 TB/s: the loads.  One of 100000 positions with 240 vectors for each of 8 K/V heads
-// 158 us, 640 TFLOP/s of products (a large library product reaches 1300) at 2.7 TB/s:
+// 150 us, 660 TFLOP/s of products (a large library product reaches 1300) at 2.7 TB/s:
 // bound by the waves' issue, of which softmax has as much as the products.
 typedef float f16v __attribute__((ext_vector_type(16)));
 
