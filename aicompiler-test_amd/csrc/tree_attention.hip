@@ -1294,8 +1294,10 @@ TreeLayout tree_layout(int64_t batch, int64_t nodes, int64_t q_heads, int64_t kv
   l.blocks = (int)(l.split ? std::max(resident / l.tiles / 8 * 8, 8) : (pairs + 7) / 8 * 8);
   // A unit's last block joins two pieces sooner than another launch does, but not more (8
   // requests of 8000 positions with 256 vectors 132 and 113 us, 16 of them 205 and 210).
-  // (Tiles of 128, and of 256 for head dim 64, have many pairs.)
-  l.arrivals = l.vectors <= 32 || l.blocks <= 2 * pairs;
+  // Tiles of 128, and of 256 for head dim 64, are for many pairs or many tiles, and have no
+  // other launch.
+  l.arrivals = l.vectors <= 32 || l.vectors == 128 || (l.vectors == 256 && head_dim == 64) ||
+               l.blocks <= 2 * pairs;
   return l;
 }
 }  // namespace
@@ -1383,7 +1385,7 @@ extern "C" int tmc_tree_attention(const void* q, const void* key_pool, const voi
 #undef TMC_TREE_RING
   if (check_launch("tree_attention_kernel")) return 1;
   if (!l.split || l.arrivals) return 0;
-  // (few pairs: tiles of 64, or for head dim 128 one of 256)
+  // (tiles of 64, or of 256 for head dim 128)
   if (head_dim == 64) TMC_TREE_JOIN(64, 64);
   else if (l.vectors == 64) TMC_TREE_JOIN(128, 64);
   else TMC_TREE_JOIN(128, 256);

@@ -232,6 +232,10 @@ def test_many_requests(tmc, batch, nodes, dim):
     (40, 25, 32, 4, 128, 100, 1400),
     (3, 25, 8, 1, 64, 200, 3000),      # tiles of 64
     (70, 25, 16, 2, 64, 60, 600),      # more tiles than there are counters
+    (5, 128, 64, 8, 64, 60, 700),      # tiles of 256 of few pairs
+    (5, 128, 64, 8, 128, 60, 700),
+    (22, 96, 16, 4, 128, 20, 600),     # tiles of 128
+    (22, 96, 16, 4, 64, 20, 600),
     (66, 32, 32, 8, 128, 30, 500),     # tiles of 128, shared and whole
     (66, 32, 32, 8, 128, 30, 200),
     (66, 60, 32, 8, 128, 20, 500),     # tiles of 256 of many pairs
