@@ -129,6 +129,8 @@ constexpr int kDigits = 256;
 // A row's tokens are looked at bin by bin: 1/16 octave of the weight each, down to
 // kFaintest.
 constexpr int kBinsOctave = 16, kBins = 44 * kBinsOctave;
+// Bins are numbered in fp32: below this number, and kBins further down, exactly.
+constexpr float kMostLevel = 0x1p23f;
 static_assert(kFaintest == -44.0, "bins down to the least weight");
 // Tokens in the list, as many as let four blocks into LDS, and the top_k that goes by it.
 constexpr int kMostKept = 2048, kMostTopK = 1024;
@@ -570,19 +572,25 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleParams p) {
   top = best ? key_value(best) : -INFINITY;
   const float heat = (float)set.heat;
   float octave = kBinsOctave, per_bin = heat * octave;  // bins an octave, and a logit
-  // what has no bins, and long lists: by digits
-  auto is_odd = [&](float top) TMC_INLINE {
-    return !(fabsf(top * per_bin) < INFINITY) || !(fabsf(top) < INFINITY);
+  // what has no bins, and long lists: by digits.  (A block of a shared row whose logits are
+  // far below the row's is passed over: its bins need a number, no exact one.)
+  auto is_odd = [&](float top, float most) TMC_INLINE {
+    return !(fabsf(top * per_bin) < most) || !(fabsf(top) < INFINITY);
   };
-  bool odd = STAGE == 2 ? record->odd : is_odd(top) || (set.most < p.vocab && set.most > kMostTopK);
+  bool odd = STAGE == 2 ? record->odd
+                        : is_odd(top, SHARED ? INFINITY : kMostLevel) ||
+                              (set.most < p.vocab && set.most > kMostTopK);
 
   // ---- what the row's settings need of it
   enum { kGreedy, kList, kBin, kSum } way = set.heat == 0.0         ? kGreedy
                                             : set.most < p.vocab    ? kList
                                             : set.share < 1.0f      ? kBin
                                                                     : kSum;
-  // A token's bin, counted down from the greatest's (NaN: none).
-  auto level_of = [&](float x) TMC_INLINE { return floorf(x * per_bin); };
+  // A token's bin, counted down from the greatest's (NaN: none).  Levels are of logits less
+  // `origin`: 0, or in finer bins the logit that these begin with, so that they are exact for
+  // logits of any size.
+  float origin = 0.0f;
+  auto level_of = [&](float x) TMC_INLINE { return floorf((x - origin) * per_bin); };
   first_bin = level_of(top);
   auto bin_of = [&](float x) TMC_INLINE { return first_bin - level_of(x); };
   auto octaves = [&](float x) TMC_INLINE { return ((double)x - (double)top) * set.heat; };
@@ -792,12 +800,13 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleParams p) {
       const u64 other = get(blocks + b);
       highs[b] = other ? key_value(other) : -INFINITY;  // (of -inf alone: no bins, passed over)
       best = max(best, other);
-      odd |= other && is_odd(highs[b]);
+      odd |= other && is_odd(highs[b], INFINITY);
     }
     odd = __syncthreads_or(odd);
     best = block_max_u64<THREADS>(best, s);
     odd |= best == 0;
     top = best ? key_value(best) : -INFINITY;
+    odd |= is_odd(top, kMostLevel);
     first_bin = level_of(top);
     if (way == kGreedy && best) {
       odd = false;
@@ -935,7 +944,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleParams p) {
         }
         octave *= 64.0f;
         per_bin = heat * octave;
-        if (is_odd(top)) break;
+        origin = ref;
         first_bin = level_of(ref);
         begin = 0;
         end = p.vocab;
@@ -977,6 +986,13 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleParams p) {
           for (int g = threadIdx.x; g < count_groups(p.vocab); g += THREADS) mine += groups[g];
           block_scan<THREADS>(mine, s, before, ahead);
           above = (double)ahead * (1.0 / kUnit);
+          // the bins said that the cut is in the list: its tokens must bear it out
+          u64 sum = 0, all;
+          for (int i = threadIdx.x; i < n; i += THREADS) sum += costs[i];
+          block_scan<THREADS>(sum, s, before, all);
+          const double listed = (double)all * (1.0 / kUnit);
+          if (!(set.least > kFaintest))
+            done = n > 0 && (above == 0.0 || above < limit) && above + listed >= limit;
         }
         // top-k, then top-p: (in a loop, for one copy of its code)
 #pragma unroll 1
@@ -988,16 +1004,13 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleParams p) {
           } else {
             if (set.share == 1.0f) break;
             cut = max(cut, low);
-            u64 sum = 0, before, all;  // of the list
-            for (int i = threadIdx.x; i < n; i += THREADS)
-              if (s.keys[i] >= cut) sum += costs[i];
-            block_scan<THREADS>(sum, s, before, all);
-            const double listed = (double)all * (1.0 / kUnit);
-            if (way == kList) limit = (double)set.share * listed;
-            // the bins said that the cut is in the list: its tokens must bear it out
-            else if (!(set.least > kFaintest) &&
-                     ((above > 0.0 && above >= limit) || above + listed < limit))
-              done = false;
+            if (way == kList) {
+              u64 sum = 0, before, all;
+              for (int i = threadIdx.x; i < n; i += THREADS)
+                if (s.keys[i] >= cut) sum += costs[i];
+              block_scan<THREADS>(sum, s, before, all);
+              limit = (double)set.share * ((double)all * (1.0 / kUnit));
+            }
             const double room = ceil((limit - above) * kUnit);
             if (!(room >= 1.0) && above > 0.0) {  // only what lies before the list
               cut = high + 1;

@@ -1,0 +1,83 @@
+"""Sampling where a cut is hard to find: long runs of equal logits, logits that are great
+next to the temperature.  Rows hold the same logits and settings and differ in their random
+numbers, so that draws reach all that stays."""
+import numpy as np
+import pytest
+import torch
+
+from sample_helpers import kept_weights, single
+
+pytestmark = pytest.mark.gpu
+
+
+def check_draws(tmc, row, rows, seed, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """Tokens exactly; probabilities as in test_sample_gpu.check()."""
+    weight = kept_weights(row.float().numpy(), temperature, top_k, top_p, min_p)
+    sums = np.cumsum(weight)
+    u = np.random.default_rng(seed).random(rows).astype(np.float32)
+    u[0] = 0.0
+    u[-1] = np.float32(1.0 - 2.0 ** -24)
+    want = np.searchsorted(sums, u.astype(np.float64) * sums[-1], side="right")
+    logits = row.cuda().expand(rows, -1).contiguous()
+    full = lambda v, t: torch.full((rows,), v, dtype=t, device="cuda")  # noqa: E731
+    tokens, shares = full(-7, torch.int32), full(-7.0, torch.float32)
+    space = torch.zeros(tmc.sample_workspace_bytes(rows, len(row)) // 4 + 4, device="cuda")
+    tmc.sample(logits, torch.from_numpy(u).cuda(), tokens, full(temperature, torch.float32),
+               full(top_k, torch.int32), full(top_p, torch.float32), full(min_p, torch.float32),
+               probability=shares, workspace=space)
+    got = tokens.cpu().numpy()
+    assert (got == want).all(), f"{(got != want).sum()} of {rows} differ, " \
+        f"{(weight[np.clip(got, 0, len(row) - 1)] == 0).sum()} are cut off"
+    share = weight[want] / sums[-1]
+    off = np.abs(shares.cpu().numpy() - share)
+    assert (off <= 2.0 ** -23 * share + 2.0 ** -34).all()
+    assert single(share[0]) > 0
+
+
+def noise(vocab, seed, spread, offset, dtype):
+    gen = torch.Generator().manual_seed(seed)
+    return (torch.randn(vocab, generator=gen) * spread + offset).to(dtype)
+
+
+# (rows of one block each, and of several)
+ROWS = [512, 40]
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("vocab,spread,offset,dtype,top_p", [
+    (128000, 0.1, 10.0, torch.float16, 0.5),
+    (128000, 0.05, 5.0, torch.float16, 0.5),
+    (128000, 0.1, -300.0, torch.float16, 0.7),
+    (40000, 0.01, 1000.0, torch.float32, 0.9),
+    (40000, 0.3, 1e6, torch.float32, 0.5),
+    (40000, 0.3, -2e6, torch.float32, 0.8),
+    (40000, 0.0, 7.0, torch.float32, 0.3),
+])
+def test_alike_far_from_zero(tmc, rows, vocab, spread, offset, dtype, top_p):
+    """Thousands of equal logits at the cut, whose bins' numbers grow with the offset."""
+    row = noise(vocab, 21, spread, offset, dtype)
+    check_draws(tmc, row, rows, 22, top_p=top_p)
+    check_draws(tmc, row, rows, 23, top_k=700, top_p=top_p)
+    check_draws(tmc, row, rows, 24, temperature=0.25, top_p=top_p)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("top_p", [0.1, 0.5, 0.9, 0.999])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_few_great_values(tmc, rows, top_p, dtype):
+    gen = torch.Generator().manual_seed(25)
+    row = torch.randint(3, 8, (30011,), generator=gen).to(dtype)
+    check_draws(tmc, row, rows, 26, top_p=top_p)
+    check_draws(tmc, row, rows, 27, temperature=3.0, top_p=top_p)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("settings", [dict(top_p=0.9), dict(top_k=50, top_p=0.9), dict(top_k=900),
+                                      dict(min_p=0.01), dict()])
+def test_forbidden_blocks(tmc, rows, settings):
+    """A third of the vocabulary forbidden by a great negative number, whole blocks of it."""
+    for least in (-1e4, -1e9, -1e30, torch.finfo(torch.float32).min):
+        row = noise(30011, 28, 2.0, 0.0, torch.float32)
+        row[4000:14000] = least
+        check_draws(tmc, row, rows, 29, **settings)
+        check_draws(tmc, row, rows, 30, temperature=0.1, **settings)
