@@ -934,7 +934,9 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleParams p) {
       for (int level = 0; level < 3 && n > kMostKept && !(set.least > kFaintest); ++level) {
         double aim = 0.0;
         roof = way == kBin ? high : least_of(level_of(low) + 1.0f);
-        ref = fminf(roof, top);
+        // (the greatest logit below the roof: where logits are far apart next to the bins' width
+        // the roof itself is many bins away)
+        ref = fminf(key_value(rank_key(roof, 0) - (1ull << 32)), top);
         if (way == kBin) {
           u64 mine = 0;
           for (int g = threadIdx.x; g < count_groups(p.vocab); g += THREADS) mine += groups[g];

@@ -81,3 +81,21 @@ def test_forbidden_blocks(tmc, rows, settings):
         row[4000:14000] = least
         check_draws(tmc, row, rows, 29, **settings)
         check_draws(tmc, row, rows, 30, temperature=0.1, **settings)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("vocab,spread,offset,dtype", [
+    (46060, 1.2, 1203.0, torch.float16),     # steps of 1 between logits
+    (46060, 12.0, -1e4, torch.float16),
+    (112000, 0.008, -37300.0, torch.float32),
+    (112000, 0.008, 5e4, torch.float32),
+    (30011, 0.5, 3e5, torch.float32),
+])
+@pytest.mark.parametrize("top_k", [300, 1000, 1024])
+def test_top_k_among_equals_far_from_zero(tmc, rows, vocab, spread, offset, dtype, top_k):
+    """The cut by number inside a run of more equals than a list holds, at logits whose
+    neighbouring floats lie many finer bins apart."""
+    row = noise(vocab, 31, spread, offset, dtype)
+    check_draws(tmc, row, rows, 32, top_k=top_k)
+    check_draws(tmc, row, rows, 33, top_k=top_k, top_p=0.6)
+    check_draws(tmc, row, rows, 34, temperature=0.5, top_k=top_k, min_p=1e-4)
