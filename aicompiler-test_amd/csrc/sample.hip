@@ -32,6 +32,7 @@ struct SampleRow {
   u64 best;         // greatest rank key
   float low, high;  // the logits in the list: from low on, below high
   int odd;          // to be done by digits
+  int least;        // the list is where min-p cuts, see bounds()
   int listed;       // in the second launch: tokens in the list so far
 };
 
@@ -739,16 +740,18 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleParams p) {
 
   // The bins [from, to] that are listed: that in which the running sum, `above` before it and
   // `reached` with it, reaches its aim, and its neighbours where the border is nearer than
-  // rough sums are exact (half a unit of a token's 2^11 and more, and as much of the aim).
+  // rough sums are exact (half a unit of a token's 2^11 and more, and as much of the aim); or,
+  // where min-p ends before them, the bins around the least logit that it keeps.
+  bool by_least = false;  // the latter
   auto bounds = [&](int bin, double above, double reached, double aim, double all) TMC_INLINE {
     int from = 0, to = bin;
     if (way == kBin) {
       const double near = 6e-4 * all;
       from = max(0, bin - (aim - above < near));
       to = bin + (reached - aim < near);
-      // min-p: the bins around the least logit that it keeps
       const float least = bin_of((float)((double)top + faintest / set.heat)) - 1.0f;
-      if (set.least > kFaintest && least < (float)from) {
+      by_least = set.least > kFaintest && least < (float)from;
+      if (by_least) {
         from = max((int)least, 0);
         to = min(to, (int)least + 2);
       }
@@ -864,7 +867,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleParams p) {
       }
       bounds(first, above, reached, aim, all);
     }
-    if (threadIdx.x == 0) *record = {best, low, high, odd, 0};
+    if (threadIdx.x == 0) *record = {best, low, high, odd, by_least, 0};
     return;
   }
   if (STAGE == 2) {
@@ -872,6 +875,7 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleParams p) {
     if (!odd && way == kGreedy) return;
     low = record->low;
     high = record->high;
+    by_least = record->least;
   }
   auto by_bins = [&]() TMC_INLINE -> bool {
     bool done = best != 0 && !odd;
@@ -988,13 +992,14 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleParams p) {
           for (int g = threadIdx.x; g < count_groups(p.vocab); g += THREADS) mine += groups[g];
           block_scan<THREADS>(mine, s, before, ahead);
           above = (double)ahead * (1.0 / kUnit);
-          // the bins said that the cut is in the list: its tokens must bear it out
+          // the bins said that the cut is in the list (or, where min-p ends before it, in it or
+          // behind it): the tokens must bear it out
           u64 sum = 0, all;
           for (int i = threadIdx.x; i < n; i += THREADS) sum += costs[i];
           block_scan<THREADS>(sum, s, before, all);
           const double listed = (double)all * (1.0 / kUnit);
-          if (!(set.least > kFaintest))
-            done = n > 0 && (above == 0.0 || above < limit) && above + listed >= limit;
+          done = (above == 0.0 || above < limit) &&
+                 (by_least || (n > 0 && above + listed >= limit));
         }
         // top-k, then top-p: (in a loop, for one copy of its code)
 #pragma unroll 1
@@ -1013,12 +1018,8 @@ __global__ __launch_bounds__(THREADS, 4) void sample_kernel(SampleParams p) {
               block_scan<THREADS>(sum, s, before, all);
               limit = (double)set.share * ((double)all * (1.0 / kUnit));
             }
-            const double room = ceil((limit - above) * kUnit);
-            if (!(room >= 1.0) && above > 0.0) {  // only what lies before the list
-              cut = high + 1;
-              break;
-            }
-            target = (u64)fmax(room, 1.0);  // (the most probable token stays)
+            // (the most probable token stays)
+            target = (u64)fmax(ceil((limit - above) * kUnit), 1.0);
           }
           cut = max(cut, select_key<THREADS>(n, low, high, target, s, [&](int i) TMC_INLINE {
                       return step == 0 ? (u64)1 : costs[i];

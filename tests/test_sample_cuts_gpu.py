@@ -99,3 +99,39 @@ def test_top_k_among_equals_far_from_zero(tmc, rows, vocab, spread, offset, dtyp
     check_draws(tmc, row, rows, 32, top_k=top_k)
     check_draws(tmc, row, rows, 33, top_k=top_k, top_p=0.6)
     check_draws(tmc, row, rows, 34, temperature=0.5, top_k=top_k, min_p=1e-4)
+
+
+PLATEAUS = [(1, 0.0), (20000, -0.64523), (617, -0.90103), (40000, -1.37627)]
+
+
+def plateaus(shuffled):
+    row = torch.cat([torch.full((n,), v) for n, v in PLATEAUS])
+    return row[torch.randperm(len(row), generator=torch.Generator().manual_seed(35))] if shuffled else row
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("edge", [1, 2, 3])
+@pytest.mark.parametrize("min_p", [0.0, 0.01, 0.3, 0.45, 0.52])
+def test_cuts_next_to_gaps(tmc, rows, edge, min_p):
+    """top_p just before and behind the end of a run of equals with nothing for many bins
+    behind it, alone and where min_p is far behind, in the gaps or before the cut."""
+    row = plateaus(shuffled=edge == 3)
+    weight = np.exp(np.array([single(v) for _, v in PLATEAUS])) * [n for n, _ in PLATEAUS]
+    at = weight[:edge].sum() / weight.sum()
+    for off in np.geomspace(2e-6, 6e-4, 24):
+        for top_p in (at - off, at + off):
+            if 0 < top_p < 1:
+                check_draws(tmc, row, rows, 36, top_p=top_p, min_p=min_p)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+def test_top_p_with_min_p_next_to_a_gap(tmc, rows):
+    """Three tokens behind the cut stayed, and 14000 was drawn for 13998 with 0.7."""
+    row = plateaus(shuffled=False)
+    check_draws(tmc, row, rows, 37, top_p=0.50328, min_p=0.01)
+    tokens = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    full = lambda v: torch.full((rows,), v, device="cuda")  # noqa: E731
+    space = torch.zeros(tmc.sample_workspace_bytes(rows, len(row)) // 4 + 4, device="cuda")
+    tmc.sample(row.cuda().expand(rows, -1).contiguous(), full(0.7), tokens, top_p=full(0.50328),
+               min_p=full(0.01), workspace=space)
+    assert (tokens == 13998).all()
