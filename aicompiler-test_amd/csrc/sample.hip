@@ -96,8 +96,11 @@ __device__ __forceinline__ Settings settings_of(const SampleParams& p, int row) 
   const double u = p.uniforms[row];
   s.uniform = u > 0.0 ? fmin(u, 1.0) : 0.0;  // (NaN: 0)
   s.heat = t >= kColdest ? 1.4426950408889634 / (double)t : 0.0;
-  if (t == INFINITY) s.heat = 0x1p-1000;  // equal weights
   s.least = least > 0.0f ? log2((double)fminf(least, 1.0f)) : -INFINITY;
+  if (t == INFINITY) {  // equal weights, of which min-p takes none
+    s.heat = 0x1p-1000;
+    s.least = -INFINITY;
+  }
   s.share = share < 1.0f ? fmaxf(share, 0.0f) : 1.0f;
   s.most = k > 0 && k < p.vocab ? k : p.vocab;
   return s;

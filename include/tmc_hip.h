@@ -981,11 +981,13 @@ size_t tmc_sample_workspace_bytes(int64_t rows, int64_t vocabulary);
  * elements apart), drawn with uniforms[r] in [0, 1).  Each row has settings of its
  * own, arrays of [rows] or NULL for the neutral value:
  *   temperature  w_i = exp((x_i - max x) / temperature); 1.  Below 2^-16 (or NaN)
- *                the row takes its most probable token, as tmc_argmax_f32
+ *                the row takes its most probable token, as tmc_argmax_f32; +inf:
+ *                all above -inf weigh the same
  *   top_k        the k most probable tokens stay; 0 or less: all
  *   top_p        of those, each before which less than top_p of their sum lies,
  *                the most probable first; 1 or more: all
- *   min_p        of those, each with w_i >= min_p; 0 or less: all
+ *   min_p        of those, each with w_i >= min_p; 0 or less: all; 1 or more: those
+ *                that equal the greatest
  * Equal logits rank by the lower index; the most probable token always stays.
  * tokens[r] is the first that stays, in the order of the vocabulary, where the
  * running sum of w passes uniforms[r] times the sum of all that stay;

@@ -135,3 +135,14 @@ def test_top_p_with_min_p_next_to_a_gap(tmc, rows):
     tmc.sample(row.cuda().expand(rows, -1).contiguous(), full(0.7), tokens, top_p=full(0.50328),
                min_p=full(0.01), workspace=space)
     assert (tokens == 13998).all()
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("min_p", [0.5, 1.0, 3.0])
+@pytest.mark.parametrize("vocab", [50, 9001])
+def test_infinite_temperature_with_min_p(tmc, rows, min_p, vocab):
+    """All weights are 1, and min-p keeps them all."""
+    row = noise(vocab, 38, 2.0, 1.0, torch.float32)
+    row[::3] = float("-inf")
+    for more in (dict(), dict(top_k=7), dict(top_p=0.613), dict(top_k=1500, top_p=0.8)):
+        check_draws(tmc, row, rows, 39, temperature=float("inf"), min_p=min_p, **more)
