@@ -11,7 +11,11 @@ pytestmark = pytest.mark.gpu
 
 
 def check_draws(tmc, row, rows, seed, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
-    """Tokens exactly; probabilities as in test_sample_gpu.check()."""
+    """Tokens, either of two neighbours where a number lies on their border: n running sums of 64
+    bits are off by n 2^-53 of the whole, the kernel's weights by 2^-44 of the greatest each,
+    which is 2^-44 n / n' of the whole for n' of at least half the greatest, here 2^-42 at most
+    (2^20 tokens of alike weights have borders on multiples of 2^-20, as the numbers).
+    Probabilities as in test_sample_gpu.check()."""
     weight = kept_weights(row.float().numpy(), temperature, top_k, top_p, min_p)
     sums = np.cumsum(weight)
     u = np.random.default_rng(seed).random(rows).astype(np.float32)
@@ -26,9 +30,14 @@ def check_draws(tmc, row, rows, seed, temperature=1.0, top_k=0, top_p=1.0, min_p
                full(top_k, torch.int32), full(top_p, torch.float32), full(min_p, torch.float32),
                probability=shares, workspace=space)
     got = tokens.cpu().numpy()
-    assert (got == want).all(), f"{(got != want).sum()} of {rows} differ, " \
-        f"{(weight[np.clip(got, 0, len(row) - 1)] == 0).sum()} are cut off"
-    share = weight[want] / sums[-1]
+    assert ((got >= 0) & (got < len(row))).all()
+    kept = np.cumsum(weight > 0)
+    low, high = np.minimum(got, want), np.maximum(got, want)
+    on_border = (np.abs(u * sums[-1] - sums[low]) <= (len(row) * 2.0 ** -53 + 2.0 ** -42) * sums[-1]) \
+        & (kept[high] - kept[low] == 1) & (weight[got] > 0)
+    bad = (got != want) & ~on_border
+    assert not bad.any(), f"{bad.sum()} of {rows} differ, {(weight[got] == 0).sum()} are cut off"
+    share = weight[got] / sums[-1]
     off = np.abs(shares.cpu().numpy() - share)
     assert (off <= 2.0 ** -23 * share + 2.0 ** -34).all()
     assert single(share[0]) > 0
