@@ -87,10 +87,11 @@ __global__ __launch_bounds__(256) void tree_append_kernel(const T* __restrict__ 
                                                           T* __restrict__ v_pool, TreeAppend p) {
   typedef T vec __attribute__((ext_vector_type(EACH)));
   const int width = (p.q_heads + 2 * p.kv_heads) * p.head_dim;
-  const int id = (int)(blockIdx.x * 256u + threadIdx.x), node = p.by_row(id);
+  const unsigned id = blockIdx.x * 256u + threadIdx.x;  // below 2^31; of elements, below 2^32
+  const int node = p.by_row((int)id);
   if (node >= p.batch * p.nodes) return;
   const int request = p.by_nodes(node), i = node - request * p.nodes;
-  const int column = EACH * id - node * width;
+  const int column = (int)(EACH * id - (unsigned)node * (unsigned)width);
   // everything that depends on nothing, in flight at once
   const int active = p.active ? p.active[0] : p.batch;
   const int cached = p.cached[request], depth = p.depths[node];
