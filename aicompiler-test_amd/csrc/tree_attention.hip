@@ -1234,6 +1234,11 @@ namespace {
 // The shapes tree_attention_kernel takes; the others run tree_plain_kernel.
 bool tree_shape(int64_t head_dim) { return head_dim == 64 || head_dim == 128; }
 
+// The tiles whose pieces tree_join_kernel joins; of the others a unit's last block does.
+bool has_join(int64_t head_dim, int vectors) {
+  return vectors == 64 || (vectors == 256 && head_dim == 128);
+}
+
 // How a launch is shared out: query vectors a block, tiles of so many of a (request,
 // kv head), blocks a tile, and whether steps are shared out.
 struct TreeLayout {
@@ -1295,9 +1300,8 @@ TreeLayout tree_layout(int64_t batch, int64_t nodes, int64_t q_heads, int64_t kv
   // A unit's last block joins two pieces sooner than another launch does, but not more (8
   // requests of 8000 positions with 256 vectors 132 and 113 us, 16 of them 205 and 210).
   // Tiles of 128, and of 256 for head dim 64, are for many pairs or many tiles, and have no
-  // other launch.
-  l.arrivals = l.vectors <= 32 || l.vectors == 128 || (l.vectors == 256 && head_dim == 64) ||
-               l.blocks <= 2 * pairs;
+  // other launch, nor have those of up to 32.
+  l.arrivals = !has_join(head_dim, l.vectors) || l.blocks <= 2 * pairs;
   return l;
 }
 }  // namespace
@@ -1340,6 +1344,8 @@ extern "C" int tmc_tree_attention(const void* q, const void* key_pool, const voi
   const hipStream_t s = as_stream(stream);
   const TreeLayout l =
       tree_layout(batch, nodes, q_heads, kv_heads, head_dim, page_size * max_pages);
+  TMC_REQUIRE(!l.split || l.arrivals || has_join(head_dim, l.vectors),
+              "Tree attention: no kernel joins these tiles.");
   const int64_t blocks = (int64_t)l.blocks * l.tiles;
   // 16-byte units of the pools are counted in 32 bits: below 64 GiB each
   if (!tree_shape(head_dim) || (uint64_t)pool_pages * (uint64_t)page_stride / 8 >= 0xFFFFFFFFull ||
@@ -1385,7 +1391,7 @@ extern "C" int tmc_tree_attention(const void* q, const void* key_pool, const voi
 #undef TMC_TREE_RING
   if (check_launch("tree_attention_kernel")) return 1;
   if (!l.split || l.arrivals) return 0;
-  // (tiles of 64, or of 256 for head dim 128)
+  // has_join()
   if (head_dim == 64) TMC_TREE_JOIN(64, 64);
   else if (l.vectors == 64) TMC_TREE_JOIN(128, 64);
   else TMC_TREE_JOIN(128, 256);
