@@ -1231,7 +1231,7 @@ using namespace tmc;
 
 namespace tmc {
 namespace {
-// The shapes tree_attention_kernel takes; the others run tree_plain_kernel.
+// The shapes tree_ring_kernel and tree_wide_kernel take; the others run tree_plain_kernel.
 bool tree_shape(int64_t head_dim) { return head_dim == 64 || head_dim == 128; }
 
 // The tiles whose pieces tree_join_kernel joins; of the others a unit's last block does.
@@ -1389,7 +1389,7 @@ extern "C" int tmc_tree_attention(const void* q, const void* key_pool, const voi
 #undef TMC_TREE_VECTORS
 #undef TMC_TREE_WIDE
 #undef TMC_TREE_RING
-  if (check_launch("tree_attention_kernel")) return 1;
+  if (check_launch(l.vectors <= 32 ? "tree_ring_kernel" : "tree_wide_kernel")) return 1;
   if (!l.split || l.arrivals) return 0;
   // has_join()
   if (head_dim == 64) TMC_TREE_JOIN(64, 64);
