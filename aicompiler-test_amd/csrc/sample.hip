@@ -46,7 +46,7 @@ struct SampleParams {
   int32_t* tokens;
   float* probability;  // or null
   long stride;
-  int rows, vocab;
+  int vocab;
   int scale;            // integer weights are multiples of 2^-scale
   int count, walk;      // blocks a row, parts of a row that each takes
   // of shared rows
@@ -150,7 +150,7 @@ template <int THREADS> struct SampleScratch {
   u64 words[THREADS / kWave];
   double levels[kCoarse];
   double value;  // (or an integer)
-  u64 found64, below;
+  u64 found64;
   int found, last, small;
 };
 
@@ -1137,7 +1137,6 @@ extern "C" int tmc_sample(const void* logits, int dtype, int64_t row_stride,
   p.tokens = tokens;
   p.probability = probability;
   p.stride = (long)row_stride;
-  p.rows = (int)rows;
   p.vocab = (int)vocabulary;
   // a sum of `vocabulary` weights fits 64 bits
   int bits = 0;

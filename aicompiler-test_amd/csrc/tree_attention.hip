@@ -242,10 +242,8 @@ __device__ __forceinline__ void read_step_values(const unsigned (&at)[8], h4 (&v
 
 // The products of N tiles, see settle(): one wait for all.
 template <int N> __device__ __forceinline__ void settle_all(f4 (&sc)[N]) {
-  static_assert(N == 1 || N == 2 || N == 4, "the operands of one instruction");
-  if constexpr (N == 1)
-    settle(sc[0]);
-  else if constexpr (N == 2)
+  static_assert(N == 2 || N == 4, "the operands of one instruction");
+  if constexpr (N == 2)
     asm volatile("s_nop 15" : "+v"(sc[0]), "+v"(sc[1]));
   else
     asm volatile("s_nop 15" : "+v"(sc[0]), "+v"(sc[1]), "+v"(sc[2]), "+v"(sc[3]));
@@ -628,6 +626,7 @@ __global__ __launch_bounds__(kTreeWaves * kWave, 1) void tree_ring_kernel(
     TreeParams p, TreePlan plan) {
   constexpr int STEP = kTreeStep, STAGES = D == 128 ? 2 : 4, WAVES = kTreeWaves, NV = 16 * C;
   constexpr int KS = D / 32, DT = D / 16, CH = D / 8, TILES = STEP / 16;
+  static_assert(TILES == 2, "a step is the depth of one product with V");
   constexpr int RPL = kWave / CH, LOADS = STEP / RPL;  // rows a load, loads of K (of V) a step
   constexpr int STAGE = 2 * STEP * D;                  // halves
   constexpr int THREADS = WAVES * kWave;
@@ -803,14 +802,10 @@ __global__ __launch_bounds__(kTreeWaves * kWave, 1) void tree_ring_kernel(
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        if constexpr (TILES == 2)
-          o[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              __builtin_shufflevector(v[0][t], v[1][t], 0, 1, 2, 3, 4, 5, 6, 7),
-              __builtin_shufflevector(w[c][0], w[c][1], 0, 1, 2, 3, 4, 5, 6, 7), o[c][t], 0, 0, 0);
-        else
-          o[c][t] = __builtin_amdgcn_mfma_f32_16x16x16f16(v[0][t], w[c][0], o[c][t], 0, 0, 0);
-      }
+      for (int c = 0; c < C; ++c)
+        o[c][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+            __builtin_shufflevector(v[0][t], v[1][t], 0, 1, 2, 3, 4, 5, 6, 7),
+            __builtin_shufflevector(w[c][0], w[c][1], 0, 1, 2, 3, 4, 5, 6, 7), o[c][t], 0, 0, 0);
   };
 
   // ---- the wave's steps: every WAVES-th of the piece
