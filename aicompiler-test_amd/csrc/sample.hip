@@ -64,7 +64,7 @@ constexpr int kMostBlocks = 512;  // of a row
 constexpr float kColdest = 1.0f / 65536.0f;
 
 // log2 of the least weight that counts: what lies below it, of 2^20 tokens, is less
-// than half the distance of two 24-bit random numbers near 1.
+// than the distance of two 24-bit random numbers near 1.
 constexpr double kFaintest = -44.0;
 constexpr int64_t kMostTokens = 1 << 20;
 
@@ -178,7 +178,7 @@ __device__ __forceinline__ u64 block_max_u64(u64 v, SampleScratch<THREADS>& s) {
 }
 
 // 2^a for a <= 0: Taylor's series of e^z, |z| <= ln 2 / 2, up to z^11: its rest is below
-// 2^-47 of it.
+// 2^-46.6 of it.
 __device__ __forceinline__ double exp2_of(double a) {
   const double n = rint(a), z = (a - n) * 0.6931471805599453;
   double s = 1.0 / 39916800.0;
@@ -394,7 +394,7 @@ __device__ __forceinline__ u64 cut_at(u64 target, SampleScratch<THREADS>& s, con
 }
 
 // A row by one block, whatever it holds, pass after pass over memory: weights as
-// integers, cuts by their digits, up to 20 passes.
+// integers, cuts by their digits, up to 21 passes.
 template <typename T, int THREADS>
 __device__ __forceinline__ void row_by_digits(const SampleParams& p, int row, const Settings& set,
                                               SampleScratch<THREADS>& s) {
