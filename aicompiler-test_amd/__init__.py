@@ -184,6 +184,7 @@ def _declare(l):
         fn.restype = res
         fn.argtypes = args
         fn.address = C.cast(fn, vp).value
+        fn.checked = False  # by _check_words()
 
 
 def lib() -> C.CDLL:
@@ -1037,9 +1038,27 @@ def logprobs(logits, tokens, logprob, entropy=None, top_tokens=None, top_logprob
 
 
 # ---------------------------------------------------------------- speculative decoding
+def _check_words(what, function, names, args):
+    """Refuse arguments that are not the function's: their number, and tensors
+    where it takes no pointer.  The native call passes words as they come."""
+    kinds, i = [], 0
+    while i < len(args):
+        tensor = args[i] is None or hasattr(args[i], "numel")
+        kinds.append(tensor)
+        i += 3 if tensor else 1
+    takes = function.argtypes
+    whole = (C.c_void_p, C.c_int32, C.c_int64, C.c_size_t)
+    if len(kinds) != len(takes) or sum(kinds) != len(names) or function.restype is not C.c_int32 or \
+            any(t not in whole or (k and t is not C.c_void_p) for k, t in zip(kinds, takes)):
+        raise TmcError(f"{what}: the wrapper's arguments are not those of the library's function")
+    function.checked = True
+
+
 def _call(what, device, function, names, *args):
     """function(*args) of the library, a tensor's argument followed by the dtype and
     the number of elements that it must have; `names` are those of the tensors."""
+    if not function.checked:
+        _check_words(what, function, names, args)
     result = (_tensors or _open_tensors()).call(function.address, device, *args)
     if result < 0:
         tensors = [args[i:i + 3] for i, t in enumerate(args) if t is None or hasattr(t, "numel")]

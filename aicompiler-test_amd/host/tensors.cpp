@@ -118,8 +118,13 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
     return nullptr;
   }
-  // The x86-64 convention passes integers and pointers alike, an int in the low half of its
-  // word, and the caller takes back words that the function does not look at.
+  // The x86-64 System V convention passes integers and pointers alike, an int in the low half
+  // of its word, and the caller takes back words that the function does not look at.  That the
+  // words are the function's own is the caller's to check (_check_words() of the wrappers,
+  // against the declared types, which the tests compare with the header).
+#if !defined(__x86_64__) || !defined(__linux__)
+#error "call() relies on the x86-64 System V convention"
+#endif
   using Function = int (*)(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t,
                            int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t,
                            int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t);
