@@ -206,7 +206,7 @@ __device__ __forceinline__ double exp2_of(double a) {
 //   - the part that holds the number drawn, and in it the token.
 // One 64-bit exponential a token: the bins' weights are of 32 bits, and say only which
 // tokens to list.  Where these are more than kMostKept, their bins are cut into 64 each and
-// the last two steps are done again.
+// the last two steps are done again (not with min-p, whose cut may be another bin's).
 //
 // Where rows are few, several blocks share one, in two launches: the first ends with the
 // bins, of which the last of a row's blocks to arrive finds the list's bounds; in the
@@ -218,12 +218,17 @@ __device__ __forceinline__ double exp2_of(double a) {
 // chain of some thirty steps that each wait for the one before; 1024 rows of 32003 with
 // mixed settings 100 us, 1.3 TB/s: 32 us the maximum, which reads the logits from memory,
 // 10 us the bins, 38 us the exponentials (some 35 64-bit operations a token), 20 us the
-// list and the draw.  64 rows of 128000 fp16 tokens 57 us: 17 us the first launch.
+// list and the draw.  64 rows of 128000 fp16 tokens 57 us: 18 us the first launch.
 //
-// Bins are of absolute logits, so that those of several blocks fit together.  Weights are
-// integers: the result does not depend on which thread comes first.  Rows that this does
-// not fit (long runs of equals at the cut; infinities; a top_k above kMostTopK) go to
-// row_by_digits(): 0.4 to 0.5 ms a row of 32000.
+// Bins are of absolute logits, so that those of several blocks fit together; finer ones of
+// logits less the greatest of theirs.  Weights are integers: the result does not depend on
+// which thread comes first.  Rows that this does not fit go to row_by_digits(), 0.5 ms a
+// row of 32000 and 1.8 to 2.1 ms one of 128000, 3.5 to 4.1 ms 64 of these:
+//   - long runs of equals at the cut, infinities, a top_k above kMostTopK;
+//   - more than kMostKept tokens in the cut's bins, with a min-p;
+//   - a greatest logit of 3.6e5 temperatures and more (kMostLevel bins);
+//   - a run of equals so close to top-p's border that the bins took the wrong one, which the
+//     exact sums of the listed tokens tell.
 
 // The thread's EACH consecutive values and their sum.
 template <int EACH, typename TYPE, typename VALUE>
@@ -1075,9 +1080,9 @@ bool sample_shape(int64_t rows, int64_t vocabulary) {
 
 // How rows are shared out: a block a row, or, below kFewRows rows, blocks of 4096 tokens, up
 // to kFill of them together.  fp16 rows of 32000 and of 128000 tokens, shared and not:
-// 16 rows 34 and 58, 43 and 164 us; 256 rows 54 and 63, 121 and 196 us; 511 rows 75 and
-// 77, 207 and 245 us.  kFill 512: 61 us for 64 rows of 128000 for 58, 2048: 63 us for 256
-// rows of 32000 for 54.
+// 16 rows 33 and 54, 42 and 150 us; 256 rows 52 and 59, 112 and 180 us; 511 rows 71 and
+// 72, 190 and 224 us.  kFill 512: 134 us for 256 rows of 128000 for 112, 2048: 68 us for 256
+// rows of 32000 for 52.
 constexpr int kThreads = 256, kEach = 8;
 constexpr int64_t kFill = 1024, kFewRows = 512;
 static_assert(kFewRows <= kSharedRows, "every shared row has its counter");

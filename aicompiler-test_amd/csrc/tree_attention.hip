@@ -60,7 +60,7 @@ __device__ __forceinline__ unsigned opaque(unsigned v) {
 // One wave per (node, query head): 64 positions at a time, one per lane for the
 // scores (whole K rows in 16-byte chunks), then lanes over the dims for P V.  Every node
 // reads all of K and V: 8 requests of up to 2000 positions with 24 nodes, 32 heads and
-// head dim 96 550 us, where the kernels below take 32 us for head dim 128.
+// head dim 96 543 us, where the kernels below take 28 us for head dim 128.
 constexpr int kPlainMaxDim = 256;
 
 struct PlainScratch {  // of one wave
@@ -177,8 +177,8 @@ __global__ __launch_bounds__(kWave) void tree_plain_kernel(TreeParams p) {
 // positions.
 //
 // Bound by the loads of K and V: 32 requests of 2048 positions with 8 nodes, 8 K/V heads of
-// 128 dims and 32 vectors each 58 us, 4.6 TB/s; 16 requests of 65 to 4096 positions with
-// 16 and 32 vectors 36 and 42 us (26 of loads at the rate of a large copy, the rest
+// 128 dims and 32 vectors each 56 us, 4.8 TB/s; 16 requests of 65 to 4096 positions with
+// 16 and 32 vectors 37 and 42 us (26 of loads at the rate of a large copy, the rest
 // beginnings and joins).  One request of 300: 11 us of latencies, with one vector a
 // head 8.
 constexpr int kTreeStep = 32, kTreeWaves = 4;
@@ -1247,8 +1247,9 @@ TreeLayout tree_layout(int64_t batch, int64_t nodes, int64_t q_heads, int64_t kv
   int resident;  // blocks that share the steps
   // Sharing costs some 10 us of lookups and joins: requests up to `alone` steps go whole, up
   // to so many positions that half the CUs take as long.  Whole and shared: 4 requests of 400
-  // positions with 32 vectors 12.5 and 15.6 us, of 1400 23.6 and 19.2; 24 requests 16.2 and
-  // 27.6, 33.0 and 41.7; with 256 vectors 4 of 1400 54 and 32, 24 of 1400 67 and 97.
+  // positions with 32 vectors 12.6 and 15.6 us, of 1400 23.5 and 19.1; 24 requests 16.5 and
+  // 27.6, 33.2 and 42.1; with 256 vectors 4 of 1400 54 and 32, 24 of 1400 62 and 94
+  // (but 16 of 1400, which go whole, 59 and 51).
   const bool many = pairs >= kTreeCus / 2;
   if (vectors <= 32) {
     l.vectors = vectors <= 16 ? 16 : 32;
@@ -1260,10 +1261,12 @@ TreeLayout tree_layout(int64_t batch, int64_t nodes, int64_t q_heads, int64_t kv
     // Shared out, a block's partials cost as much as some steps, and tiles of 64 vectors have
     // the fewest.  For head dim 128 and much to read, one tile of up to 256 vectors reads K
     // and V once: 4 requests of 1400 and 8000 positions with 256 vectors 32 and 64 us, in
-    // tiles of 64 32 and 78; 12 of up to 3000 64 and 60; one of 100000 with 240 146 and 194.
-    // Head dim 64 has half the work a vector: 16 requests of up to 4096 with 256 vectors 53
-    // us in tiles of 64, 84 in one of 256; one of 100000 116 and 123.
-    // One tile of 64 on one block a CU: 47 us with 64 vectors, on two 55.
+    // tiles of 64 32 and 79; 12 of up to 3000 65 and 62; one of 100000 with 240 153 and 195
+    // (but 4 of 1400 with 256 vectors for each of 32 K/V heads 81 and 59).
+    // Head dim 64 has half the work a vector: 16 requests of up to 4096 with 256 vectors 52
+    // us in tiles of 64, 55 in one of 256; one of 100000 113 and 146.
+    // One tile of 64 on one block a CU: 16 requests of up to 4096 with 64 vectors 47 us, on two
+    // 48; 24 of up to 2000 with head dim 64 25 and 30.
     const bool one = vectors <= 64;
     l.vectors = one || head_dim == 64 || pairs * ((capacity + kWideSpan - 1) / kWideSpan) <= 12 * kTreeCus
                     ? 64 : 256;
@@ -1282,8 +1285,8 @@ TreeLayout tree_layout(int64_t batch, int64_t nodes, int64_t q_heads, int64_t kv
   l.split = share();
   if (vectors > 64 && (!l.split || pairs >= 2 * kTreeCus)) {
     // mostly whole units: wide blocks do the same work in less time, but not on vectors that
-    // are not there (64 requests of 1000 positions with 128 vectors: tiles of 64 87 us, of
-    // 128 70, of 256 83; with 256 vectors 156, 123 and 118)
+    // are not there (64 requests of 1000 positions with 128 vectors: tiles of 64 85 us, of
+    // 128 69, of 256 82; with 256 vectors 152, 124 and 117)
     const int64_t cost64 = (vectors + 63) / 64 * 64 * 7, cost128 = (vectors + 127) / 128 * 128 * 6,
                   cost256 = (vectors + 255) / 256 * 256 * 5;
     l.vectors = cost64 < std::min(cost128, cost256) ? 64 : cost128 < cost256 ? 128 : 256;
@@ -1293,7 +1296,7 @@ TreeLayout tree_layout(int64_t batch, int64_t nodes, int64_t q_heads, int64_t kv
   // a multiple of the XCDs, no more than are resident
   l.blocks = (int)(l.split ? std::max(resident / l.tiles / 8 * 8, 8) : (pairs + 7) / 8 * 8);
   // A unit's last block joins two pieces sooner than another launch does, but not more (8
-  // requests of 8000 positions with 256 vectors 132 and 113 us, 16 of them 205 and 210).
+  // requests of 8000 positions with 256 vectors 135 and 115 us, 16 of them 205 and 207).
   // Tiles of 128, and of 256 for head dim 64, are for many pairs or many tiles, and have no
   // other launch, nor have those of up to 32.
   l.arrivals = !has_join(head_dim, l.vectors) || l.blocks <= 2 * pairs;

@@ -67,7 +67,8 @@ def kernel_summary(db: str, title: str, command: str) -> str:
         meta[key] = (vgpr, agpr, lds)
     out = [f"# {title}", "", "Command (repo root, MI355X box):", "", f"    {command}", "",
            "Durations in microseconds from the kernel trace (`kernels` view of the rocpd "
-           "database).", "",
+           "database); VGPR as there, on gfx950 half of the vector registers a wave has been "
+           "given.", "",
            "| kernel | grid (threads) | block | VGPR | AGPR | LDS B | calls | avg | median | min | max |",
            "|---|---|---|---|---|---|---|---|---|---|---|"]
     for key, d in sorted(agg.items(), key=lambda kv: -sum(kv[1])):
